@@ -431,6 +431,56 @@ int qr_batch_decode_f16(void* o, const void* q, const void* kv_data, const void*
                         int head_dim, int64_t batch_size, void* stream);
 
 /*
+ * Attention of new tokens over the paged cache (no counterpart in the reference, whose kernels attend with one query per
+ * sequence and key head): sequence b brings the tokens seqlen_indptr[b] .. seqlen_indptr[b + 1] - 1 of q (NULL: token b,
+ * one per sequence, tokens == batch_size), which are the LAST positions that its page tables count, and whose keys and
+ * values are in the pages already (qr_kv_append_i4, qr_kv_quant_append_f16_i4, qr_kv_append_f16 with the same bounds):
+ *   o[t, h, :] = sum_j softmax_j( q[t, h, :] . k[j, h / G] / sqrt(128) ) v[j, h / G],   G = num_q_heads / num_heads,
+ *   over the positions j <= P, P the token's own; with window > 0 only those with P - j < window or j < sinks.
+ *   A row that sees no position is zero (a sequence without pages, more new tokens than the sequence holds); rows of q and
+ *   o behind the last sequence are neither read nor written.  Positions on page numbers outside [0, num_pages) are skipped.
+ * qr_batch_chunk_i4: int4 pages, k_j[i] = code * scale_j - zero_j (codes enter the products as they are, weights are rounded to
+ *   fp16 once, everything else is in 32 bits).  qr_batch_chunk_f16: fp16 pages, kv_param is not read.
+ *   q, o fp16, a token's num_q_heads * 128 halves contiguous, q_stride / o_stride halves from one token to the next (multiples
+ *   of 8; 16-byte aligned); num_q_heads a multiple of num_heads.  q_had_mode 1: q through H_128 / sqrt(128) first, rounded to
+ *   fp16, as matmul_had_cuda gives it.
+ *   max_new_len, max_seq_len: the largest number of new tokens and of positions of a sequence if the caller knows them, else
+ *   0; they size the launch and may be wrong at the cost of time only.  With a workspace of qr_batch_chunk_workspace_bytes
+ *   bytes (16-byte aligned, contents arbitrary) few rows are split along the positions, and a second launch merges.
+ */
+size_t qr_batch_chunk_workspace_bytes(int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
+                                      int64_t max_seq_len, int64_t window, int64_t sinks);
+int qr_batch_chunk_i4(void* o, int64_t o_stride, const void* q, int64_t q_stride, int q_had_mode,
+                      const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,
+                      const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                      int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim,
+                      int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
+                      void* workspace, size_t workspace_bytes, void* stream);
+int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_stride, int q_had_mode,
+                       const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,
+                       const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                       int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim,
+                       int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Page tables of sequences of unequal lengths, from lengths on the device (qr_page_tables is for one common length):
+ *   lengths int32 [batch_size], the tokens every sequence holds (negative: none; more than max_pages * page_size: that many);
+ *   block_table_or_null int32 [batch_size, >= max_pages], rows table_stride apart: the pages of every sequence (NULL: page i of
+ *   sequence b is page number i * batch_size + b).
+ *   kv_indptr int32 [batch_size + 1], kv_indices int32 [batch_size * max_pages] (the lists one behind the other, -1 behind the
+ *   last one), last_page_offset int32 [batch_size] (0: no pages).
+ *   new_lengths_or_null int32 [batch_size]: how many of the tokens are new, the last ones.  Then seqlen_indptr int32 [batch_size + 1]
+ *   gets their bounds, and positions, slots int64 [tokens] every new token's position and its place page * page_size + entry
+ *   (-1: none, because the sequence is shorter than its new tokens, or the block table has a negative page there); both are -1
+ *   behind the last new token, and new tokens beyond `tokens` are left out.
+ */
+int qr_build_page_tables(const void* lengths, const void* new_lengths_or_null, int64_t batch_size, int page_size,
+                         int64_t max_pages, const void* block_table_or_null, int64_t table_stride, int64_t tokens,
+                         void* kv_indptr, void* kv_indices, void* last_page_offset, void* seqlen_indptr, void* positions,
+                         void* slots, void* stream);
+
+/*
  * Measurement aids.  NO counterpart in the reference and no caller in the product path: kernels whose
  * work is known exactly, run by bench.py next to the workloads to calibrate the rooflines.
  *

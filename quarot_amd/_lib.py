@@ -14,6 +14,9 @@ LIB_PATH = _PKG / "libquarot_hip.so"
 _c = ctypes
 _i64, _int, _f32, _ptr = _c.c_int64, _c.c_int, _c.c_float, _c.c_void_p
 
+_CHUNK = (_ptr, _i64, _ptr, _i64, _int, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int, _i64, _i64, _i64, _i64,
+          _i64, _ptr, _c.c_size_t, _ptr)
+
 # name -> (restype, argtypes); mirrors include/quarot_hip.h one to one
 SIGNATURES = {
     "qr_version": (_int, ()),
@@ -56,6 +59,10 @@ SIGNATURES = {
     "qr_kv_append_f16": (_int, (_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int,
                                 _i64, _ptr)),
     "qr_batch_decode_f16": (_int, (_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int, _i64, _ptr)),
+    "qr_batch_chunk_workspace_bytes": (_c.c_size_t, (_i64, _int, _int, _i64, _i64, _i64, _i64, _i64)),
+    "qr_batch_chunk_i4": (_int, _CHUNK),
+    "qr_batch_chunk_f16": (_int, _CHUNK),
+    "qr_build_page_tables": (_int, (_ptr, _ptr, _i64, _int, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr)),
     "qr_calib_mfma_i8": (_int, (_int, _int, _int, _ptr, _ptr)),
     "qr_calib_copy": (_int, (_ptr, _ptr, _i64, _ptr)),
 }

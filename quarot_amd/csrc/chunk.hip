@@ -1,0 +1,555 @@
+// Attention of new tokens over the paged KV cache: every sequence brings any number of them, each sees the cached positions up to its own
+// (all of them, or the last `window` and the first `sinks`), and several query heads may share a key head.
+//
+//   o[t, h] = sum_j softmax_j( q[t, h] . k[j, h / G] / sqrt(128) ) v[j, h / G]      over j <= P(t) and (P(t) - j < window or j < sinks)
+//
+// with P(t) = (tokens the sequence holds) - (its new tokens) + (which of them t is).  A row that sees no position is zero.
+//
+// Int4 pages hold x = code * scale - zero.  Both products run on the codes themselves, c = code - 8, which fp16 holds exactly, so that no
+// cached value is rounded:
+//   q . k_j = scale_j (q . c_j) - (zero_j - 8 scale_j) sum(q)                       (the last factor once per row)
+//   sum_j p_j v_j = sum_j (p_j f_j) (2^e_j c_j) - sum_j p_j (zero_j - 8 scale_j)    with scale_j = f_j 2^e_j
+// Only p_j f_j is rounded to fp16, the matrix instruction's type (2^-11 of each weight at most, as any fp16 weight would be); f_j lies in
+// [1, 2), so weights of large and of tiny scales have the same range.  Maxima, sums and outputs are held in 32 bits.
+#include "qr_paged.h"
+
+namespace {
+
+// What a launch works on.  Rows of a (sequence, key head): row r is new token r / group, query head kv_head * group + r % group.
+struct Chunk {
+    PagedKV c;
+    const f16* q;
+    f16* o;
+    const int32_t* starts;            // nullptr: one new token per sequence
+    float* part;                      // splits > 1: 132 floats per row and split: maximum, sum, -, -, 128 outputs
+    int64_t q_stride, o_stride;       // halves from a token to the next
+    int tokens, group, tiles, splits, window, sinks;      // window 0: none
+    int q_had;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kScale = 0.08838834764831845f;             // 1 / sqrt(128)
+constexpr float kEmpty = -1e30f;                           // the running maximum of a row that has seen nothing
+constexpr float kGrow = 8.f;                               // a maximum is raised when a logit (base 2) is this far above it
+
+template <int MASK>
+__device__ __forceinline__ u32x2 both_halves(u32 w) {      // the words of this lane and of lane ^ MASK, the lower lane's first
+    if constexpr (MASK == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+        return u32x2{(u32)r[0], (u32)r[1]};
+    } else {
+        const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+        return u32x2{(u32)r[0], (u32)r[1]};
+    }
+}
+__device__ __forceinline__ float as_f32(u32 w) { return __builtin_bit_cast(float, w); }
+__device__ __forceinline__ u32 as_u32(float v) { return __builtin_bit_cast(u32, v); }
+// over the four lanes that hold a query row's quarters
+__device__ __forceinline__ float quarters_sum(float v) {
+    const u32x2 a = both_halves<16>(as_u32(v));
+    v = as_f32(a.x) + as_f32(a.y);
+    const u32x2 b = both_halves<32>(as_u32(v));
+    return as_f32(b.x) + as_f32(b.y);
+}
+__device__ __forceinline__ float quarters_max(float v) {
+    const u32x2 a = both_halves<16>(as_u32(v));
+    v = __builtin_fmaxf(as_f32(a.x), as_f32(a.y));
+    const u32x2 b = both_halves<32>(as_u32(v));
+    return __builtin_fmaxf(as_f32(b.x), as_f32(b.y));
+}
+
+// Four pairs of codes of a word, each less eight, as fp16: codes (0, 4), (1, 5), (2, 6), (3, 7).  A nibble under the exponent of 1024 (64 for
+// the upper nibble of a byte) is 1024 + code (64 + code); taking 1032 (72) off is exact.
+__device__ __forceinline__ u32 less(u32 w, float by) { return __builtin_bit_cast(u32, as_f16x2(w) - f16x2{(f16)by, (f16)by}); }
+__device__ __forceinline__ u32x4 centred(u32 w) {
+    const u32 w8 = w >> 8;
+    return u32x4{less((w & 0x000F000Fu) | 0x64006400u, 1032.f), less((w & 0x00F000F0u) | 0x54005400u, 72.f),
+                 less((w8 & 0x000F000Fu) | 0x64006400u, 1032.f), less((w8 & 0x00F000F0u) | 0x54005400u, 72.f)};
+}
+// scale = f 2^e: the power of two as fp16 bits, 2^-14 .. 2^14 (a smaller scale has a smaller f, a larger one a larger)
+__device__ __forceinline__ u32 power_bits(u32 scale) {
+    const u32 e = scale & 0x7C00u;
+    return e < 0x0400u ? 0x0400u : e > 0x7400u ? 0x7400u : e;
+}
+
+// The positions that the rows of a tile see, in steps of 32: steps [0, near) hold the sinks, then [far, far + rest).
+struct Steps {
+    int near, far, all;
+    __device__ int at(int s) const { return s < near ? s : s - near + far; }
+};
+__device__ __forceinline__ Steps steps_of(const Chunk& a, int lowest, int highest) {        // positions of the tile's first and last row
+    Steps s{0, 0, 0};
+    if (highest < 0) return s;
+    int from = 0;
+    if (a.window > 0 && lowest - a.window + 1 > 0) {
+        from = lowest - a.window + 1;
+        const int sinks = a.sinks < from ? a.sinks : from;
+        s.near = (sinks + 31) >> 5;
+    }
+    s.far = from >> 5;
+    if (s.far < s.near) s.far = s.near;
+    const int end = (highest >> 5) + 1;
+    s.all = s.near + (end > s.far ? end - s.far : 0);
+    return s;
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------------------------------------
+// A workgroup of four waves takes 16 NB rows of a (sequence, key head); its waves (and those of the other splits) take the steps of 32
+// positions in turn, so a cached vector is read once per tile of rows.  A wave works on transposed tiles, positions x rows: the first product's
+// result has a row in every lane and positions in its registers, which is what the second product takes as its right operand, with no exchange
+// between lanes.  The contraction's order is free, so a position's codes are used as they lie: lane (n, g) of the first product takes bytes 16 g ..
+// of key n, the word s of them in step s; lane (m, g) of the second takes word m of the eight keys 4 g .. 4 g + 3 and 16 + 4 g .. of a step,
+// whose nibble b is row m of its block b of outputs.
+template <bool F16>
+struct Fetched {                       // the step that is on its way
+    u32x4 k[F16 ? 8 : 2], kp[F16 ? 1 : 2], vp[F16 ? 1 : 2];
+    u32x4 v4[F16 ? 8 : 1];
+    u32 v[F16 ? 1 : 8];
+    u32 ok;                            // bit 4 kb + i: position 16 kb + 4 g + i is there
+};
+
+template <int NB, bool F16, bool ALIGNED>
+__global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
+    __shared__ f32x4 st4[4 * 16 * 33];                     // per wave and row: maximum, sum, -, -, 128 outputs
+    const PagedKV& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    int id = blockIdx.x;
+    const int split = id % a.splits;
+    id /= a.splits;
+    const int first_tile = id % a.tiles;
+    id /= a.tiles;
+    const int h = id % c.num_heads, b = id / c.num_heads;
+
+    int start = b, fresh = 1;
+    if (a.starts) {                                        // (kept inside q and o, whatever the bounds say)
+        start = a.starts[b];
+        int end = a.starts[b + 1];
+        start = start < 0 ? 0 : start;
+        end = end > a.tokens ? a.tokens : end;
+        fresh = end > start ? end - start : 0;
+    }
+    const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
+    const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
+    const int rows = fresh * a.group;
+    const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
+    const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
+    const int64_t kv_slots = (int64_t)c.num_heads * c.page_size;
+    constexpr int VEC = F16 ? 16 : 4;                      // 16-byte pieces of a vector
+    const u32x4* const data = (const u32x4*)c.data;
+
+    for (int tile = first_tile; tile * 16 * NB < rows; tile += a.tiles) {
+        const int r0 = tile * 16 * NB, r1 = r0 + 16 * NB < rows ? r0 + 16 * NB : rows;
+        const int lowest = len - fresh + r0 / a.group, highest = len - fresh + (r1 - 1) / a.group;
+        const Steps steps = steps_of(a, lowest, highest);
+
+        // the queries: lane (n, g) holds dimensions 32 g .. 32 g + 31 of row n of every block
+        u32x4 qf[NB][4];
+        float qsum[NB];                                    // -log2(e) / sqrt(128) times the row's sum
+        int place[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = r0 + 16 * nb + n;
+            const bool in = r < rows;
+            const int t = (in ? r : r0) / a.group, head = h * a.group + (in ? r : r0) - t * a.group;
+            place[nb] = in ? len - fresh + t : -1;
+            const u32x4* src = (const u32x4*)(a.q + (int64_t)(start + t) * a.q_stride + (int64_t)head * 128) + 4 * g;
+            u32x4 w[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) w[s] = in ? src[s] : u32x4{0, 0, 0, 0};
+            if (a.q_had) {
+                // the Hadamard transform over the head dimension in 32 bits: index bits 0 .. 4 within the lane, 5 and 6 across the quarters;
+                // rounded to fp16 like the transform's own entry point
+                float t32[32];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const f16x2 p = as_f16x2(w[i >> 2][i & 3]);
+                    t32[2 * i] = (float)p[0], t32[2 * i + 1] = (float)p[1];
+                }
+#pragma unroll
+                for (int bit = 1; bit < 32; bit *= 2)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!(i & bit)) {
+                            const float x = t32[i], y = t32[i | bit];
+                            t32[i] = x + y, t32[i | bit] = x - y;
+                        }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    u32x2 e = both_halves<16>(as_u32(t32[i]));
+                    float v = (lane & 16) ? as_f32(e.x) - as_f32(e.y) : as_f32(e.x) + as_f32(e.y);
+                    e = both_halves<32>(as_u32(v));
+                    t32[i] = (lane & 32) ? as_f32(e.x) - as_f32(e.y) : as_f32(e.x) + as_f32(e.y);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i >> 2][i & 3] = narrow_f16x2(t32[2 * i] * kScale, t32[2 * i + 1] * kScale);
+            }
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const f16x2 p = as_f16x2(w[i >> 2][i & 3]);
+                sum += (float)p[0] + (float)p[1];
+            }
+            qsum[nb] = quarters_sum(sum) * -(kLog2e * kScale);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                qf[nb][s] = F16 ? w[s]
+                                : u32x4{__builtin_amdgcn_perm(w[s][2], w[s][0], 0x05040100u), __builtin_amdgcn_perm(w[s][2], w[s][0], 0x07060302u),
+                                        __builtin_amdgcn_perm(w[s][3], w[s][1], 0x05040100u), __builtin_amdgcn_perm(w[s][3], w[s][1], 0x07060302u)};
+        }
+
+        float m[NB], d[NB], pz[NB];
+        f32x4 acc[NB][8];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            m[nb] = kEmpty, d[nb] = 0.f, pz[nb] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[nb][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
+        // Loads are unconditional: a position that is not there reads the first entries of page 0 and is masked.
+        auto fetch = [&](Fetched<F16>& f, int s) {
+            const int at = steps.at(s) * 32;
+            f.ok = 0;
+            int64_t mine = 0;
+            bool mine_ok = false;
+            if (!ALIGNED) {
+                const int pos = at + (lane & 31), it = pos / c.page_size;
+                const bool in = pos < len && it < npages;
+                const int page = npages > 0 ? c.indices[p0 + (in ? it : 0)] : -1;
+                mine_ok = in && page >= 0 && page < c.num_pages;
+                mine = mine_ok ? page * page_slots + head_slots + (pos - it * c.page_size) : head_slots;
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                if (ALIGNED) {
+                    const int pos = at + 16 * kb, it = pos / c.page_size;
+                    const bool in = it < npages;
+                    const int page = npages > 0 ? c.indices[p0 + (in ? it : 0)] : -1;
+                    const bool there = in && page >= 0 && page < c.num_pages;
+                    const int64_t slot = there ? page * page_slots + head_slots + (pos - it * c.page_size) : head_slots;
+                    const int64_t ks = slot + n, vs = slot + kv_slots + 4 * g;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f.ok |= (there && pos + 4 * g + i < len ? 1u : 0u) << (4 * kb + i);
+                    if (F16) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f.k[4 * kb + i] = data[ks * VEC + 4 * g + i];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f.v4[4 * kb + i] = data[(vs + i) * VEC + n];
+                    } else {
+                        f.k[kb] = data[ks * VEC + g];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f.v[4 * kb + i] = ((const u32*)c.data)[(vs + i) * 16 + n];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f.kp[kb][i] = c.param[slot + 4 * g + i], f.vp[kb][i] = c.param[vs + i];
+                    }
+                } else {
+                    const int64_t ks = __shfl(mine, 16 * kb + n, 64);
+                    if (F16) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f.k[4 * kb + i] = data[ks * VEC + 4 * g + i];
+                    } else {
+                        f.k[kb] = data[ks * VEC + g];
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t slot = __shfl(mine, 16 * kb + 4 * g + i, 64);
+                        f.ok |= (u32)__shfl((int)mine_ok, 16 * kb + 4 * g + i, 64) << (4 * kb + i);
+                        if (F16) {
+                            f.v4[4 * kb + i] = data[(slot + kv_slots) * VEC + n];
+                        } else {
+                            f.v[4 * kb + i] = ((const u32*)c.data)[(slot + kv_slots) * 16 + n];
+                            f.kp[kb][i] = c.param[slot], f.vp[kb][i] = c.param[slot + kv_slots];
+                        }
+                    }
+                }
+            }
+        };
+
+        auto consume = [&](Fetched<F16>& f, int s) {
+            const int at = steps.at(s) * 32;
+            const bool whole = at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks) &&
+                               __builtin_amdgcn_ballot_w64(f.ok != 0xFFu) == 0;
+            // a position that is not there may hold anything: its value counts as zero (its weight is)
+            u32x4 vp[2];
+            if (!F16) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) vp[k >> 2][k & 3] = (f.ok >> k & 1) ? f.vp[k >> 2][k & 3] : 0u;
+            }
+            f32x4 x[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) x[nb][0] = x[nb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f16x8 k = __builtin_bit_cast(f16x8, F16 ? f.k[4 * kb + i] : centred(f.k[kb][i]));
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+                        x[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(f16x8, qf[nb][i]), x[nb][kb], 0, 0, 0);
+                }
+            float ka[8], kz[8], vf[8], vz[8];
+            u32 power[4];
+            if (!F16) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const f16x2 kp = as_f16x2(f.kp[k >> 2][k & 3]), vq = as_f16x2(vp[k >> 2][k & 3]);
+                    ka[k] = (float)kp[0] * (kLog2e * kScale);
+                    kz[k] = __builtin_fmaf(-8.f, (float)kp[0], (float)kp[1]);
+                    vz[k] = __builtin_fmaf(-8.f, (float)vq[0], (float)vq[1]);
+                    const u32 bits = power_bits(vp[k >> 2][k & 3]);
+                    vf[k] = (float)vq[0] * (float)as_f16x2(0x7800u - bits)[0];
+                    power[k >> 1] = k & 1 ? power[k >> 1] | bits << 16 : bits;
+                }
+            }
+            f16x8 p[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                float y[8], top = -__builtin_inff();
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    y[k] = F16 ? x[nb][k >> 2][k & 3] * (kLog2e * kScale) : __builtin_fmaf(x[nb][k >> 2][k & 3], ka[k], kz[k] * qsum[nb]);
+                if (!whole) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int pos = at + 16 * (k >> 2) + 4 * g + (k & 3);
+                        const bool sees = pos <= place[nb] && (a.window == 0 || pos > place[nb] - a.window || pos < a.sinks) && (f.ok >> k & 1);
+                        y[k] = sees ? y[k] : -__builtin_inff();
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = __builtin_fmaxf(top, y[k]);
+                if (__builtin_amdgcn_ballot_w64(top > m[nb] + kGrow)) {
+                    const float now = __builtin_fmaxf(m[nb], quarters_max(top)), keep = __builtin_amdgcn_exp2f(m[nb] - now);
+                    m[nb] = now;
+                    d[nb] *= keep, pz[nb] *= keep;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) acc[nb][k] *= keep;
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float w = __builtin_amdgcn_exp2f(y[k] - m[nb]);
+                    d[nb] += w;
+                    if (!F16) pz[nb] = __builtin_fmaf(w, vz[k], pz[nb]);
+                    p[nb][k] = (f16)(F16 ? w : w * vf[k]);
+                }
+            }
+            // the values: row m of block b is dimension 8 m + b
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {         // nibbles (words of a piece) 4 half .. 4 half + 3
+                u32x4 v[4];                                // [block][pair of keys]
+                if (F16) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool ok0 = f.ok >> (2 * k) & 1, ok1 = f.ok >> (2 * k + 1) & 1;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const u32 w0 = ok0 ? f.v4[2 * k][2 * half + i] : 0u, w1 = ok1 ? f.v4[2 * k + 1][2 * half + i] : 0u;
+                            v[2 * i][k] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+                            v[2 * i + 1][k] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const u32 w = __builtin_amdgcn_perm(f.v[2 * k + 1], f.v[2 * k], half ? 0x07060302u : 0x05040100u);
+                        const u32x4 codes = centred(w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i][k] = __builtin_bit_cast(u32, as_f16x2(codes[i]) * as_f16x2(power[k]));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+                        acc[nb][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v[i]), p[nb], acc[nb][4 * half + i], 0, 0, 0);
+            }
+        };
+
+        const int stride = 4 * a.splits;
+        int s = split * 4 + wave;
+        Fetched<F16> f;
+        if (s < steps.all) fetch(f, s);
+        for (; s < steps.all; s += stride) {
+            Fetched<F16> now = f;
+            const int next = s + stride < steps.all ? s + stride : s;
+            fetch(f, next);
+            consume(now, s);
+        }
+
+        // ---- merge: a wave's states are those of its rows; the four waves' through LDS, one block of 16 rows at a time
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const float dd = quarters_sum(d[nb]), zz = F16 ? 0.f : quarters_sum(pz[nb]);
+            __syncthreads();
+            f32x4* const mine = st4 + (wave * 16 + n) * 33;
+            if (g == 0) mine[0] = f32x4{m[nb], dd, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                  // dimensions 8 (4 g + i) + block
+                mine[1 + 8 * g + 2 * i] = f32x4{acc[nb][0][i] - zz, acc[nb][1][i] - zz, acc[nb][2][i] - zz, acc[nb][3][i] - zz};
+                mine[2 + 8 * g + 2 * i] = f32x4{acc[nb][4][i] - zz, acc[nb][5][i] - zz, acc[nb][6][i] - zz, acc[nb][7][i] - zz};
+            }
+            __syncthreads();
+            const int row = threadIdx.x >> 4, l = threadIdx.x & 15, r = r0 + 16 * nb + row;
+            if (r < rows) {
+                float M = kEmpty, D = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, st4[(w * 16 + row) * 33][0]);
+                f32x4 O[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const f32x4* src = st4 + (w * 16 + row) * 33;
+                    const float keep = __builtin_amdgcn_exp2f(src[0][0] - M);
+                    D = __builtin_fmaf(src[0][1], keep, D);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        O[0][i] = __builtin_fmaf(src[1 + 2 * l][i], keep, O[0][i]);
+                        O[1][i] = __builtin_fmaf(src[2 + 2 * l][i], keep, O[1][i]);
+                    }
+                }
+                const int t = r / a.group, head = h * a.group + r - t * a.group;
+                if (a.splits == 1) {
+                    const float inv = D == 0.f ? 0.f : 1.f / D;                 // (a row that sees nothing is zero)
+                    u32x4 out;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[i] = cvt_f16x2(O[i >> 1][2 * i & 2] * inv, O[i >> 1][(2 * i & 2) + 1] * inv);
+                    *((u32x4*)(a.o + (int64_t)(start + t) * a.o_stride + (int64_t)head * 128) + l) = out;
+                } else {
+                    float* dst = a.part + (((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.splits + split) * 132;
+                    if (l == 0) dst[0] = M, dst[1] = D;
+                    *((f32x4*)dst + 1 + 2 * l) = O[0];
+                    *((f32x4*)dst + 2 + 2 * l) = O[1];
+                }
+            }
+        }
+    }
+}
+
+// the partial states of every row -> its output: sixteen lanes per row, eight dimensions each
+__global__ __launch_bounds__(256) void chunk_merge_kernel(const float* __restrict__ part, const int32_t* __restrict__ starts, int batch, int tokens,
+                                                          int heads, int splits, f16* __restrict__ o, int64_t o_stride) {
+    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int l = threadIdx.x & 15;
+    const int64_t token = row / heads;
+    const int head = (int)(row - token * heads);
+    // (rows that belong to no sequence have no states and are left as they are)
+    if (token >= tokens || (starts && (token < starts[0] || token >= starts[batch]))) return;
+    const f32x4* src = (const f32x4*)(part + row * splits * 132);
+    float M = kEmpty, D = 0.f;
+    for (int s = 0; s < splits; ++s) M = __builtin_fmaxf(M, src[s * 33][0]);
+    f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    for (int s = 0; s < splits; ++s) {
+        const f32x4 head4 = src[s * 33], x = src[s * 33 + 1 + 2 * l], y = src[s * 33 + 2 + 2 * l];
+        const float keep = __builtin_amdgcn_exp2f(head4[0] - M);
+        D = __builtin_fmaf(head4[1], keep, D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = __builtin_fmaf(x[i], keep, a[i]), b[i] = __builtin_fmaf(y[i], keep, b[i]);
+    }
+    const float inv = D == 0.f ? 0.f : 1.f / D;
+    *((u32x4*)(o + token * o_stride + (int64_t)head * 128) + l) =
+        u32x4{cvt_f16x2(a[0] * inv, a[1] * inv), cvt_f16x2(a[2] * inv, a[3] * inv), cvt_f16x2(b[0] * inv, b[1] * inv), cvt_f16x2(b[2] * inv, b[3] * inv)};
+}
+
+// How a call is cut: column blocks per workgroup, tiles of rows per (sequence, key head), splits of the positions.
+struct ChunkPlan {
+    int nb, tiles, splits;
+};
+ChunkPlan chunk_plan(int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
+    if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
+    const int64_t rows = max_new_len * group, cus = qr_device().cus;
+    ChunkPlan p;
+    p.nb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const int64_t tiles = (rows + 16 * p.nb - 1) / (16 * p.nb);
+    p.tiles = (int)(tiles > 4096 ? 4096 : tiles);          // (a workgroup goes on to the next tile behind them)
+    int64_t seen = max_seq_len > 0 ? max_seq_len : 0;
+    if (window > 0 && seen > window + max_new_len + sinks + 64) seen = window + max_new_len + sinks + 64;
+    const int64_t groups = batch * num_heads * p.tiles, steps = (seen + 31) / 32;
+    int64_t splits = (2 * cus + groups - 1) / groups;
+    if (splits > steps / 8) splits = steps / 8;            // (two steps per wave at least)
+    if (splits > 32) splits = 32;
+    p.splits = splits < 1 ? 1 : (int)splits;
+    return p;
+}
+
+size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? (size_t)tokens * q_heads * splits * 132 * sizeof(float) : 0; }
+
+int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_stride, int q_had_mode, const void* seqlen_indptr_or_null, int64_t tokens,
+                int num_q_heads, const void* kv_data, const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim, int64_t batch_size, int64_t max_new_len,
+                int64_t max_seq_len, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = qr_internal_check_paged_cache(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,
+                                                 page_size, head_dim, batch_size);
+    if (rc != QR_OK) return rc;
+    if (q_had_mode != 0 && q_had_mode != 1) return QR_E_DTYPE;
+    if (tokens < 0 || num_q_heads <= 0 || num_q_heads % num_heads || window < 0 || sinks < 0 || max_new_len < 0 || max_seq_len < 0) return QR_E_SHAPE;
+    if (tokens == 0 || batch_size == 0) return QR_OK;
+    if (!seqlen_indptr_or_null && tokens != batch_size) return QR_E_SHAPE;       // one new token per sequence
+    if (!o || !q) return QR_E_NULL;
+    if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || q_stride % 8 || o_stride % 8) return QR_E_ALIGN;
+    const int64_t width = (int64_t)num_q_heads * 128;
+    if (q_stride < width || o_stride < width || tokens * num_q_heads > 0x7fffffff || num_q_heads / num_heads > 1024) return QR_E_SHAPE;
+    const ChunkPlan plan = chunk_plan(tokens, num_q_heads / num_heads, num_heads, batch_size, seqlen_indptr_or_null ? max_new_len : 1, max_seq_len, window, sinks);
+    Chunk a;
+    a.c = qr_internal_paged_kv((void*)kv_data, (void*)kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,
+                               page_size, batch_size);
+    a.q = (const f16*)q;
+    a.o = (f16*)o;
+    a.starts = (const int32_t*)seqlen_indptr_or_null;
+    a.q_stride = q_stride, a.o_stride = o_stride;
+    a.tokens = (int)tokens;
+    a.group = num_q_heads / num_heads;
+    a.tiles = plan.tiles;
+    a.window = (int)(window > 0x3fffffff ? 0 : window);    // (longer than any sequence)
+    a.sinks = (int)(sinks > 0x3fffffff ? 0x3fffffff : sinks);
+    a.q_had = q_had_mode;
+    a.splits = plan.splits;
+    if (a.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < chunk_part_bytes(tokens, num_q_heads, a.splits))) a.splits = 1;
+    a.part = (float*)workspace;
+    const int64_t groups = batch_size * num_heads * plan.tiles * a.splits;
+    if (groups > 0x7fffffff) return QR_E_SHAPE;
+    hipStream_t st = (hipStream_t)stream;
+    const bool aligned = page_size % 16 == 0;
+#define QR_CHUNK(NB, F, AL) chunk_rows_kernel<NB, F, AL><<<dim3((unsigned)groups), dim3(256), 0, st>>>(a)
+#define QR_CHUNK_NB(F, AL)                                                              \
+    do {                                                                                \
+        if (plan.nb == 1) QR_CHUNK(1, F, AL);                                           \
+        else if (plan.nb == 2) QR_CHUNK(2, F, AL);                                      \
+        else QR_CHUNK(4, F, AL);                                                        \
+    } while (0)
+    if (fp16) {
+        if (aligned) QR_CHUNK_NB(true, true);
+        else QR_CHUNK_NB(true, false);
+    } else {
+        if (aligned) QR_CHUNK_NB(false, true);
+        else QR_CHUNK_NB(false, false);
+    }
+#undef QR_CHUNK_NB
+#undef QR_CHUNK
+    const int lrc = qr_launch_status();
+    if (lrc != QR_OK || a.splits == 1) return lrc;
+    chunk_merge_kernel<<<dim3((unsigned)((tokens * num_q_heads + 15) / 16)), dim3(256), 0, st>>>(a.part, a.starts, (int)batch_size, (int)tokens, num_q_heads,
+                                                                                              a.splits, a.o, o_stride);
+    return qr_launch_status();
+}
+
+}  // namespace
+
+extern "C" size_t qr_batch_chunk_workspace_bytes(int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
+                                                 int64_t max_seq_len, int64_t window, int64_t sinks) {
+    if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0) return 0;
+    const int splits = chunk_plan(tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, max_seq_len, window, sinks).splits;
+    return chunk_part_bytes(tokens, num_q_heads, splits);
+}
+
+#define QR_CHUNK_ENTRY(NAME, FP16)                                                                                                                \
+    extern "C" int NAME(void* o, int64_t o_stride, const void* q, int64_t q_stride, int q_had_mode, const void* seqlen_indptr_or_null,            \
+                        int64_t tokens, int num_q_heads, const void* kv_data, const void* kv_param, const void* kv_indptr,                         \
+                        const void* kv_indices, const void* last_page_offset, int64_t num_pages, int num_layers, int layer_idx, int num_heads,     \
+                        int page_size, int head_dim, int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,  \
+                        void* workspace, size_t workspace_bytes, void* stream) {                                                                  \
+        return batch_chunk(FP16, o, o_stride, q, q_stride, q_had_mode, seqlen_indptr_or_null, tokens, num_q_heads, kv_data, kv_param, kv_indptr,    \
+                           kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size, head_dim, batch_size,           \
+                           max_new_len, max_seq_len, window, sinks, workspace, workspace_bytes, stream);                                          \
+    }
+QR_CHUNK_ENTRY(qr_batch_chunk_i4, false)
+QR_CHUNK_ENTRY(qr_batch_chunk_f16, true)

@@ -289,6 +289,139 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
             None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev)))
 
 
+def _chunk(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
+           window, sinks, q_hadamard, workspace):
+    pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
+    dev, batch = kv_data.device, last_page_offset.shape[0]
+    for name, t in (("o", o), ("q", q)):
+        if not (t.is_cuda and t.dim() == 3 and t.dtype == torch.float16):
+            raise RuntimeError(f"{fn}: {name} must be a 3D fp16 CUDA tensor")
+        if not (t.shape[2] == head_dim and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == head_dim)):
+            raise RuntimeError(f"{fn}: {name} must be [tokens, heads, {head_dim}] with contiguous heads")
+        if t.shape[0] > 1 and not (t.stride(0) >= t.shape[1] * head_dim and t.stride(0) % 8 == 0):
+            raise RuntimeError(f"{fn}: {name}'s tokens must not overlap and start at multiples of 8 elements")
+    if not (o.shape == q.shape):
+        raise RuntimeError(f"{fn}: o.size() != q.size()")
+    tokens, q_heads = q.shape[0], q.shape[1]
+    if not (q_heads > 0 and q_heads % heads == 0):
+        raise RuntimeError(f"{fn}: q's heads must be a multiple of the cache's {heads}")
+    if not (kv_indptr.shape[0] == batch + 1):
+        raise RuntimeError(f"{fn}: CHECK_EQ(kv_indptr.size(0), batch_size + 1) failed")
+    if seqlen_indptr is None:
+        if not (tokens == batch):
+            raise RuntimeError(f"{fn}: one token per sequence expected")
+    elif not (seqlen_indptr.is_cuda and seqlen_indptr.is_contiguous() and seqlen_indptr.dtype == torch.int32
+              and tuple(seqlen_indptr.shape) == (batch + 1,)):
+        raise RuntimeError(f"{fn}: seqlen_indptr must be int32 [batch_size + 1]")
+    for name, t in (("o", o), ("q", q), ("kv_param", kv_param), ("kv_indptr", kv_indptr), ("kv_indicies", kv_indices),
+                    ("last_page_offset", last_page_offset), ("seqlen_indptr", seqlen_indptr)):
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{fn}: expected all tensors on {dev}, but {name} is on {t.device}")
+    window, sinks, max_new_len, max_seq_len = int(window), int(sinks), int(max_new_len), int(max_seq_len)
+    if window < 0 or sinks < 0 or max_new_len < 0 or max_seq_len < 0:
+        raise RuntimeError(f"{fn}: window, sinks and the lengths must not be negative")
+    with _lib.on_device(dev):
+        ws_bytes = _lib.lib().qr_batch_chunk_workspace_bytes(tokens, q_heads, heads, batch, 1 if seqlen_indptr is None else max_new_len,
+                                                             max_seq_len, window, sinks)
+        ws = None
+        if ws_bytes:
+            fits = (workspace is not None and workspace.device == dev and workspace.dtype == torch.uint8
+                    and workspace.is_contiguous() and workspace.numel() >= ws_bytes)
+            ws = workspace if fits else torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+        entry = _lib.lib().qr_batch_chunk_f16 if f16 else _lib.lib().qr_batch_chunk_i4
+        row = q_heads * head_dim
+        _lib.check(entry(
+            o.data_ptr(), o.stride(0) if tokens > 1 else row, q.data_ptr(), q.stride(0) if tokens > 1 else row, 1 if q_hadamard else 0,
+            None if seqlen_indptr is None else seqlen_indptr.data_ptr(), tokens, q_heads, kv_data.data_ptr(), kv_param.data_ptr(),
+            kv_indptr.data_ptr(), kv_indices.data_ptr(), last_page_offset.data_ptr(), pages, layers, int(layer_idx), heads, page_size,
+            head_dim, batch, max_new_len, max_seq_len, window, sinks, None if ws is None else ws.data_ptr(), ws_bytes,
+            _lib.stream_ptr(dev)))
+
+
+def batch_chunk_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
+                   max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None):
+    """Attention of several new tokens per sequence over the int4 cache: q, o fp16 [tokens, q_heads, 128], the tokens of sequence b
+    being seqlen_indptr[b] .. seqlen_indptr[b + 1] - 1 (None: token b, one per sequence), its LAST positions, whose keys and values
+    quantize_append_kv_i4 or init_kv_i4 has stored with the same bounds.
+
+        o[t, h] = softmax(q[t, h] . K^T / sqrt(128)) . V   over the positions up to the token's own
+
+    q_heads may be a multiple of the cache's heads: query heads h G .. h G + G - 1 share key head h.  window > 0: a token sees the last
+    `window` positions, its own among them, and the first `sinks` of the sequence.  A row that sees nothing is zero; rows of `o`
+    outside seqlen_indptr's bounds are left as they are.  q and o may be slices of wider rows (a fused projection), each token's heads
+    contiguous.  max_new_len, max_seq_len (optional): the largest counts of new tokens and of positions; they size the launch, and the
+    latter lets few rows be split along the positions.  q_hadamard: the kernel applies matmul_had_cuda(q, torch.float16) first.
+    workspace: as batch_decode_i4's, with arbitrary contents.  Writes into `o` and returns None."""
+    _chunk("batch_chunk_i4", False, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
+           max_seq_len, window, sinks, q_hadamard, workspace)
+
+
+def batch_chunk_f16(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
+                    max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None):
+    """batch_chunk_i4 for the cache with fp16 pages (kv_data fp16 [pages, layers, 2, heads, page_size, 128])."""
+    _chunk("batch_chunk_f16", True, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
+           max_seq_len, window, sinks, q_hadamard, workspace)
+
+
+def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_lengths=None, tokens=0):
+    """Page tables of sequences of unequal lengths, from lengths on the GPU, by one launch and without waiting for it.
+
+    lengths int32 [batch]: the tokens every sequence holds, this step's included.  block_table int32 [batch, >= max_pages]: every
+    sequence's pages; without one, page i of sequence b is page number i * batch + b, as in MultiLayerPagedKVCache4Bit.  max_pages
+    (default: the block table's width) bounds the pages of a sequence; a longer length counts as max_pages * page_size.
+    Returns a dict with kv_indptr [batch + 1], kv_indices [batch * max_pages] (-1 behind the last list) and last_page_offset
+    [batch], all int32: the arguments of the cache's other functions.  With new_lengths int32 [batch], how many of the tokens are new
+    (the last ones), and `tokens`, their number, also seqlen_indptr int32 [batch + 1], and for every new token int64 positions and
+    slots (page * page_size + entry, -1 where it has no place)."""
+    fn = "build_page_tables"
+    page_size, tokens = int(page_size), int(tokens)
+    if not (lengths.is_cuda and lengths.is_contiguous() and lengths.dim() == 1 and lengths.dtype == torch.int32):
+        raise RuntimeError(f"{fn}: lengths must be a contiguous 1D int32 CUDA tensor")
+    dev, batch = lengths.device, lengths.shape[0]
+    stride = 0
+    if block_table is not None:
+        if not (block_table.is_cuda and block_table.device == dev and block_table.dim() == 2 and block_table.dtype == torch.int32
+                and block_table.shape[0] == batch and (block_table.shape[1] <= 1 or block_table.stride(1) == 1)):
+            raise RuntimeError(f"{fn}: block_table must be int32 [batch_size, max_pages] on {dev} with contiguous rows")
+        max_pages = block_table.shape[1] if max_pages is None else max_pages
+        if not (int(max_pages) <= block_table.shape[1]):
+            raise RuntimeError(f"{fn}: block_table has fewer than max_pages columns")
+        stride = block_table.stride(0) if batch > 1 else block_table.shape[1]
+        if stride < int(max_pages):
+            raise RuntimeError(f"{fn}: block_table's rows must not overlap")
+    if max_pages is None:
+        raise RuntimeError(f"{fn}: max_pages or a block_table is needed")
+    max_pages = int(max_pages)
+    if not (page_size > 0 and max_pages > 0 and tokens >= 0):
+        raise RuntimeError(f"{fn}: page_size and max_pages must be positive, tokens not negative")
+    if new_lengths is None:
+        if tokens:
+            raise RuntimeError(f"{fn}: tokens without new_lengths")
+    elif not (new_lengths.is_cuda and new_lengths.device == dev and new_lengths.is_contiguous() and new_lengths.dtype == torch.int32
+              and tuple(new_lengths.shape) == (batch,)):
+        raise RuntimeError(f"{fn}: new_lengths must be int32 [batch_size] on {dev}")
+    new = functools.partial(torch.empty, dtype=torch.int32, device=dev)
+    tables = {"kv_indptr": new((batch + 1,)), "kv_indices": new((batch * max_pages,)), "last_page_offset": new((batch,))}
+    if new_lengths is not None:
+        tables["seqlen_indptr"] = new((batch + 1,))
+        tables["positions"], tables["slots"] = (torch.empty((tokens,), dtype=torch.int64, device=dev) for _ in range(2))
+    ptr = lambda name: tables[name].data_ptr() if name in tables else None
+    with _lib.on_device(dev):
+        if batch == 0:                               # no launch: the empty batch's bounds
+            for name in ("kv_indptr", "seqlen_indptr"):
+                if name in tables:
+                    tables[name].zero_()
+            for name in ("positions", "slots"):
+                if name in tables:
+                    tables[name].fill_(-1)
+            return tables
+        _lib.check(_lib.lib().qr_build_page_tables(
+            lengths.data_ptr(), None if new_lengths is None else new_lengths.data_ptr(), batch, page_size, max_pages,
+            None if block_table is None else block_table.data_ptr(), stride, tokens, ptr("kv_indptr"), ptr("kv_indices"),
+            ptr("last_page_offset"), ptr("seqlen_indptr"), ptr("positions"), ptr("slots"), _lib.stream_ptr(dev)))
+    return tables
+
+
 class _AttentionStub(object):
     """What MultiLayerPagedKVCache4Bit.update hands back for a decode step (kv_cache.py:104-129): called
     with the query states it runs attention over the cache."""
