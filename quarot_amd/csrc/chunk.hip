@@ -5,93 +5,16 @@
 //
 // with P(t) = (tokens the sequence holds) - (its new tokens) + (which of them t is).  A row that sees no position is zero.
 //
-// Int4 pages hold x = code * scale - zero.  Both products run on the codes themselves, c = code - 8, which fp16 holds exactly, so that no
-// cached value is rounded:
-//   q . k_j = scale_j (q . c_j) - (zero_j - 8 scale_j) sum(q)                       (the last factor once per row)
-//   sum_j p_j v_j = sum_j (p_j f_j) (2^e_j c_j) - sum_j p_j (zero_j - 8 scale_j)    with scale_j = f_j 2^e_j
-// Only p_j f_j is rounded to fp16, the matrix instruction's type (2^-11 of each weight at most, as any fp16 weight would be); f_j lies in
-// [1, 2), so weights of large and of tiny scales have the same range.  Maxima, sums and outputs are held in 32 bits.
-#include "qr_paged.h"
+// Int4 pages hold x = code * scale - zero.  Both products run on the codes themselves, which fp16 holds exactly, so that no cached value is
+// rounded:
+//   q . k_j = scale_j (q . code_j) - zero_j sum(q)                                 (the last factor once per row)
+//   sum_j p_j v_j = sum_j (p_j f_j) (2^e_j code_j) - sum_j p_j zero_j              with scale_j = f_j 2^e_j
+// Only p_j f_j is rounded to fp16, the matrix instruction's type; f_j lies in [1, 2), so weights of large and of tiny scales have the same range.
+// The rounded number over f_j is the weight in every sum, so a rounding (2^-11 at most) changes a weight and nothing else.  Maxima, sums and
+// outputs are held in 32 bits.
+#include "qr_chunk.h"
 
 namespace {
-
-// What a launch works on.  Rows of a (sequence, key head): row r is new token r / group, query head kv_head * group + r % group.
-struct Chunk {
-    PagedKV c;
-    const f16* q;
-    f16* o;
-    const int32_t* starts;            // nullptr: one new token per sequence
-    float* part;                      // splits > 1: 132 floats per row and split: maximum, sum, -, -, 128 outputs
-    int64_t q_stride, o_stride;       // halves from a token to the next
-    int tokens, group, tiles, splits, window, sinks;      // window 0: none
-    int q_had;
-};
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kScale = 0.08838834764831845f;             // 1 / sqrt(128)
-constexpr float kEmpty = -1e30f;                           // the running maximum of a row that has seen nothing
-constexpr float kGrow = 8.f;                               // a maximum is raised when a logit (base 2) is this far above it
-
-template <int MASK>
-__device__ __forceinline__ u32x2 both_halves(u32 w) {      // the words of this lane and of lane ^ MASK, the lower lane's first
-    if constexpr (MASK == 32) {
-        const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-        return u32x2{(u32)r[0], (u32)r[1]};
-    } else {
-        const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-        return u32x2{(u32)r[0], (u32)r[1]};
-    }
-}
-__device__ __forceinline__ float as_f32(u32 w) { return __builtin_bit_cast(float, w); }
-__device__ __forceinline__ u32 as_u32(float v) { return __builtin_bit_cast(u32, v); }
-// over the four lanes that hold a query row's quarters
-__device__ __forceinline__ float quarters_sum(float v) {
-    const u32x2 a = both_halves<16>(as_u32(v));
-    v = as_f32(a.x) + as_f32(a.y);
-    const u32x2 b = both_halves<32>(as_u32(v));
-    return as_f32(b.x) + as_f32(b.y);
-}
-__device__ __forceinline__ float quarters_max(float v) {
-    const u32x2 a = both_halves<16>(as_u32(v));
-    v = __builtin_fmaxf(as_f32(a.x), as_f32(a.y));
-    const u32x2 b = both_halves<32>(as_u32(v));
-    return __builtin_fmaxf(as_f32(b.x), as_f32(b.y));
-}
-
-// Four pairs of codes of a word, each less eight, as fp16: codes (0, 4), (1, 5), (2, 6), (3, 7).  A nibble under the exponent of 1024 (64 for
-// the upper nibble of a byte) is 1024 + code (64 + code); taking 1032 (72) off is exact.
-__device__ __forceinline__ u32 less(u32 w, float by) { return __builtin_bit_cast(u32, as_f16x2(w) - f16x2{(f16)by, (f16)by}); }
-__device__ __forceinline__ u32x4 centred(u32 w) {
-    const u32 w8 = w >> 8;
-    return u32x4{less((w & 0x000F000Fu) | 0x64006400u, 1032.f), less((w & 0x00F000F0u) | 0x54005400u, 72.f),
-                 less((w8 & 0x000F000Fu) | 0x64006400u, 1032.f), less((w8 & 0x00F000F0u) | 0x54005400u, 72.f)};
-}
-// scale = f 2^e: the power of two as fp16 bits, 2^-14 .. 2^14 (a smaller scale has a smaller f, a larger one a larger)
-__device__ __forceinline__ u32 power_bits(u32 scale) {
-    const u32 e = scale & 0x7C00u;
-    return e < 0x0400u ? 0x0400u : e > 0x7400u ? 0x7400u : e;
-}
-
-// The positions that the rows of a tile see, in steps of 32: steps [0, near) hold the sinks, then [far, far + rest).
-struct Steps {
-    int near, far, all;
-    __device__ int at(int s) const { return s < near ? s : s - near + far; }
-};
-__device__ __forceinline__ Steps steps_of(const Chunk& a, int lowest, int highest) {        // positions of the tile's first and last row
-    Steps s{0, 0, 0};
-    if (highest < 0) return s;
-    int from = 0;
-    if (a.window > 0 && lowest - a.window + 1 > 0) {
-        from = lowest - a.window + 1;
-        const int sinks = a.sinks < from ? a.sinks : from;
-        s.near = (sinks + 31) >> 5;
-    }
-    s.far = from >> 5;
-    if (s.far < s.near) s.far = s.near;
-    const int end = (highest >> 5) + 1;
-    s.all = s.near + (end > s.far ? end - s.far : 0);
-    return s;
-}
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
 // A workgroup of four waves takes 16 NB rows of a (sequence, key head); its waves (and those of the other splits) take the steps of 32
@@ -109,7 +32,7 @@ struct Fetched {                       // the step that is on its way
 };
 
 template <int NB, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
+__global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk a) {
     __shared__ f32x4 st4[4 * 16 * 33];                     // per wave and row: maximum, sum, -, -, 128 outputs
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -121,14 +44,8 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
     id /= a.tiles;
     const int h = id % c.num_heads, b = id / c.num_heads;
 
-    int start = b, fresh = 1;
-    if (a.starts) {                                        // (kept inside q and o, whatever the bounds say)
-        start = a.starts[b];
-        int end = a.starts[b + 1];
-        start = start < 0 ? 0 : start;
-        end = end > a.tokens ? a.tokens : end;
-        fresh = end > start ? end - start : 0;
-    }
+    const Fresh mine_tokens = fresh_of(a, b);
+    const int start = mine_tokens.start, fresh = mine_tokens.count;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
     const int rows = fresh * a.group;
@@ -141,7 +58,7 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
     for (int tile = first_tile; tile * 16 * NB < rows; tile += a.tiles) {
         const int r0 = tile * 16 * NB, r1 = r0 + 16 * NB < rows ? r0 + 16 * NB : rows;
         const int lowest = len - fresh + r0 / a.group, highest = len - fresh + (r1 - 1) / a.group;
-        const Steps steps = steps_of(a, lowest, highest);
+        const Steps steps = steps_of<5>(a, lowest, highest);
 
         // the queries: lane (n, g) holds dimensions 32 g .. 32 g + 31 of row n of every block
         u32x4 qf[NB][4];
@@ -192,10 +109,7 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
             }
             qsum[nb] = quarters_sum(sum) * -(kLog2e * kScale);
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-                qf[nb][s] = F16 ? w[s]
-                                : u32x4{__builtin_amdgcn_perm(w[s][2], w[s][0], 0x05040100u), __builtin_amdgcn_perm(w[s][2], w[s][0], 0x07060302u),
-                                        __builtin_amdgcn_perm(w[s][3], w[s][1], 0x05040100u), __builtin_amdgcn_perm(w[s][3], w[s][1], 0x07060302u)};
+            for (int s = 0; s < 4; ++s) qf[nb][s] = F16 ? w[s] : query_for_codes(w[s]);
         }
 
         float m[NB], d[NB], pz[NB];
@@ -270,11 +184,11 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
             const int at = steps.at(s) * 32;
             const bool whole = at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks) &&
                                __builtin_amdgcn_ballot_w64(f.ok != 0xFFu) == 0;
-            // a position that is not there may hold anything: its value counts as zero (its weight is)
+            // a position that is not there may hold anything: any finite value will do (its weight is zero)
             u32x4 vp[2];
             if (!F16) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) vp[k >> 2][k & 3] = (f.ok >> k & 1) ? f.vp[k >> 2][k & 3] : 0u;
+                for (int k = 0; k < 8; ++k) vp[k >> 2][k & 3] = (f.ok >> k & 1) ? f.vp[k >> 2][k & 3] : kNoParameters;
             }
             f32x4 x[NB][2];
 #pragma unroll
@@ -283,23 +197,41 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const f16x8 k = __builtin_bit_cast(f16x8, F16 ? f.k[4 * kb + i] : centred(f.k[kb][i]));
+                    const f16x8 k = __builtin_bit_cast(f16x8, F16 ? f.k[4 * kb + i] : codes_of(f.k[kb][i]));
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
                         x[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(f16x8, qf[nb][i]), x[nb][kb], 0, 0, 0);
                 }
-            float ka[8], kz[8], vf[8], vz[8];
+            float ka[8], kz[8], vf[8], vr[8], vz[8];       // keys: slope and zero point; values: factor, its reciprocal, zero point over factor
             u32 power[4];
+            bool plain = true;
             if (!F16) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const f16x2 kp = as_f16x2(f.kp[k >> 2][k & 3]), vq = as_f16x2(vp[k >> 2][k & 3]);
-                    ka[k] = (float)kp[0] * (kLog2e * kScale);
-                    kz[k] = __builtin_fmaf(-8.f, (float)kp[0], (float)kp[1]);
-                    vz[k] = __builtin_fmaf(-8.f, (float)vq[0], (float)vq[1]);
-                    const u32 bits = power_bits(vp[k >> 2][k & 3]);
-                    vf[k] = (float)vq[0] * (float)as_f16x2(0x7800u - bits)[0];
-                    power[k >> 1] = k & 1 ? power[k >> 1] | bits << 16 : bits;
+                    const f16x2 kp = as_f16x2(f.kp[k >> 2][k & 3]);
+                    ka[k] = (float)kp[0] * (kLog2e * kScale * kCodeUnit);
+                    kz[k] = (float)kp[1];
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const u32 w0 = vp[k >> 1][2 * k & 3], w1 = vp[k >> 1][(2 * k & 3) + 1];
+                    power[k] = powers_of(w0, w1, plain);
+                }
+                plain = __builtin_amdgcn_ballot_w64(!plain) == 0;
+                if (plain) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) vf[k] = (float)as_f16x2(((u32)vp[k >> 2][k & 3] & 0x83FFu) | 0x3C00u)[0];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float scale = (float)as_f16x2(vp[k >> 2][k & 3])[0];
+                        vf[k] = factor_of(scale, power_of(scale));
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    vr[k] = __builtin_amdgcn_rcpf(vf[k]);
+                    vz[k] = (float)as_f16x2(vp[k >> 2][k & 3])[1] * vr[k];
                 }
             }
             f16x8 p[NB];
@@ -329,9 +261,9 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const float w = __builtin_amdgcn_exp2f(y[k] - m[nb]);
-                    d[nb] += w;
-                    if (!F16) pz[nb] = __builtin_fmaf(w, vz[k], pz[nb]);
                     p[nb][k] = (f16)(F16 ? w : w * vf[k]);
+                    d[nb] = F16 ? d[nb] + (float)p[nb][k] : __builtin_fmaf((float)p[nb][k], vr[k], d[nb]);
+                    if (!F16) pz[nb] = __builtin_fmaf((float)p[nb][k], vz[k], pz[nb]);
                 }
             }
             // the values: row m of block b is dimension 8 m + b
@@ -353,9 +285,9 @@ __global__ __launch_bounds__(256, 2) void chunk_rows_kernel(Chunk a) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const u32 w = __builtin_amdgcn_perm(f.v[2 * k + 1], f.v[2 * k], half ? 0x07060302u : 0x05040100u);
-                        const u32x4 codes = centred(w);
+                        const u32x4 scaled = plain ? scaled_codes(w, power[k]) : scaled_codes_slow(w, vp[k >> 1][2 * k & 3], vp[k >> 1][(2 * k & 3) + 1]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i][k] = __builtin_bit_cast(u32, as_f16x2(codes[i]) * as_f16x2(power[k]));
+                        for (int i = 0; i < 4; ++i) v[i][k] = scaled[i];
                     }
                 }
 #pragma unroll
@@ -452,19 +384,19 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const float* __restric
 
 // How a call is cut: column blocks per workgroup, tiles of rows per (sequence, key head), splits of the positions.
 struct ChunkPlan {
-    int nb, tiles, splits;
+    int nb, tiles, splits;            // nb 0: the kernel of 256 rows
 };
 ChunkPlan chunk_plan(int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     const int64_t rows = max_new_len * group, cus = qr_device().cus;
     ChunkPlan p;
-    p.nb = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const int64_t tiles = (rows + 16 * p.nb - 1) / (16 * p.nb);
+    p.nb = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 128 ? 4 : 0;
+    const int64_t per = p.nb ? 16 * p.nb : 256, tiles = (rows + per - 1) / per;
     p.tiles = (int)(tiles > 4096 ? 4096 : tiles);          // (a workgroup goes on to the next tile behind them)
     int64_t seen = max_seq_len > 0 ? max_seq_len : 0;
     if (window > 0 && seen > window + max_new_len + sinks + 64) seen = window + max_new_len + sinks + 64;
     const int64_t groups = batch * num_heads * p.tiles, steps = (seen + 31) / 32;
-    int64_t splits = (2 * cus + groups - 1) / groups;
+    int64_t splits = p.nb ? (2 * cus + groups - 1) / groups : cus / groups;
     if (splits > steps / 8) splits = steps / 8;            // (two steps per wave at least)
     if (splits > 32) splits = 32;
     p.splits = splits < 1 ? 1 : (int)splits;
@@ -509,6 +441,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     if (groups > 0x7fffffff) return QR_E_SHAPE;
     hipStream_t st = (hipStream_t)stream;
     const bool aligned = page_size % 16 == 0;
+    int lrc;
 #define QR_CHUNK(NB, F, AL) chunk_rows_kernel<NB, F, AL><<<dim3((unsigned)groups), dim3(256), 0, st>>>(a)
 #define QR_CHUNK_NB(F, AL)                                                              \
     do {                                                                                \
@@ -516,7 +449,9 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
         else if (plan.nb == 2) QR_CHUNK(2, F, AL);                                      \
         else QR_CHUNK(4, F, AL);                                                        \
     } while (0)
-    if (fp16) {
+    if (plan.nb == 0) {
+        lrc = qr_internal_chunk_tiles(fp16, a, groups, st);
+    } else if (fp16) {
         if (aligned) QR_CHUNK_NB(true, true);
         else QR_CHUNK_NB(true, false);
     } else {
@@ -525,7 +460,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     }
 #undef QR_CHUNK_NB
 #undef QR_CHUNK
-    const int lrc = qr_launch_status();
+    if (plan.nb) lrc = qr_launch_status();
     if (lrc != QR_OK || a.splits == 1) return lrc;
     chunk_merge_kernel<<<dim3((unsigned)((tokens * num_q_heads + 15) / 16)), dim3(256), 0, st>>>(a.part, a.starts, (int)batch_size, (int)tokens, num_q_heads,
                                                                                               a.splits, a.o, o_stride);

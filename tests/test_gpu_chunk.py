@@ -1,12 +1,14 @@
 """Attention of new tokens over the paged cache (batch_chunk_i4, batch_chunk_f16) against its definition in 64 bits.
 
-How far a result may be off is added up for every element.  With weights w_j (they add up to one), values x_j = scale_j (code - 8) on int4
-pages (z_j = zero_j - 8 scale_j is subtracted from them) and x_j = v_j on fp16 pages, half a step of fp16 being u = 2^-11:
-  u |o|                                the output's rounding (2^-25 where it is subnormal)
-  u sum w_j |x_j|                      every weight is rounded to fp16 once, as a factor of x_j
-  sum min(w_j, 2^-25) 8 |scale_j|      (or |v_j|) weights below fp16's normal range; sums are at least one in units of the largest weight
-  L sum w_j (|x_j| + |z_j|)            with L twice the largest error of a logit -- 140 steps of 2^-24 of its terms' absolute sum --, plus
-                                       that of exp2's argument and of sums over the positions, all in fp32."""
+How far a result may be off is added up for every element.  With weights w_j (they add up to one), values v_j, x_j = scale_j code (and
+zero_j, subtracted from it) on int4 pages, and half a step of fp16 being u = 2^-11:
+  u |o|                                   the output's rounding (2^-25 where it is subnormal)
+  u (sum w_j |v_j| + |o|)                 a weight is rounded to fp16 once and counts as rounded in all sums: w_j (1 + d_j), |d_j| <= u, changes
+                                          sum w v / sum w by sum w_j d_j (v_j - o), at most u sum w_j |v_j - o|
+  sum min(w_j, 2^-25) (|v_j| + |o|)       the same for weights below fp16's normal range; sums are at least one in units of the largest weight
+  L sum w_j (|x_j| + |zero_j|)            with L twice the largest error of a logit -- 140 steps of 2^-24 of its terms' absolute sum, and for queries
+                                          below 2^-10 a step of 2^-21 of a sixteenth of them --, plus that of exp2's argument and of sums over the
+                                          positions, all in fp32."""
 import math
 
 import numpy as np
@@ -71,18 +73,18 @@ def definition(specs, q, lens, news, layer, window=0, sinks=0, gone=()):
                 if s == b:
                     sees[:, p] = False
             for h in range(heads):
-                x, z, unit = [], [], []
+                x, z = [], []
                 for side in (0, 1):
                     rows = data[held, layer, side, h].reshape(-1, data.shape[-1])[:n]
                     if f16:
-                        x.append(rows.double()), z.append(torch.zeros(n, 1, dtype=torch.float64, device=DEV)), unit.append(rows.double().abs())
+                        x.append(rows.double()), z.append(torch.zeros(n, 1, dtype=torch.float64, device=DEV))
                     else:
                         pr = param[held, layer, side, h].reshape(-1, 2)[:n].double()
                         codes = torch.stack([rows & 15, rows >> 4], -1).reshape(n, 128).double()
-                        x.append(pr[:, :1] * (codes - 8)), z.append(pr[:, 1:] - 8 * pr[:, :1]), unit.append(8 * pr[:, :1].abs().repeat(1, 128))
+                        x.append(pr[:, :1] * codes), z.append(pr[:, 1:])
                 for s, p in gone:                           # (not to be read, whatever lies where its page number leads here)
                     if s == b:
-                        for v in (*x, *z, *unit):
+                        for v in (*x, *z):
                             v[p] = 0
                 qs = q[token:token + new, h * group:(h + 1) * group].reshape(-1, 128).double()
                 logits = (qs @ x[0].T - qs.sum(1, keepdim=True) * z[0].T) / math.sqrt(128)
@@ -93,9 +95,11 @@ def definition(specs, q, lens, news, layer, window=0, sinks=0, gone=()):
                 w = torch.where(sees, w, 0.0)
                 o = w @ (x[1] - z[1])
                 size = w @ (x[1].abs() + z[1].abs())
-                far = 2 * 140 * 2.0 ** -24 * torch.where(sees, terms, 0.0).amax(1, keepdim=True)
+                small = 2.0 ** -21 * x[0].abs().sum(1)[None] / math.sqrt(128)
+                far = 2 * torch.where(sees, 140 * 2.0 ** -24 * terms + small, 0.0).amax(1, keepdim=True)
                 far = far + 2.0 ** -22 * (1 + 1.5 * torch.where(sees, logits.abs(), 0.0).amax(1, keepdim=True)) + (n / 16 + 200) * 2.0 ** -24
-                t = 2.0 ** -11 * (o.abs() + w @ x[1].abs()) + w.clamp(max=2.0 ** -25) @ unit[1] + far * size + 2.0 ** -25
+                v, tiny = (x[1] - z[1]).abs(), w.clamp(max=2.0 ** -25)
+                t = 2.0 ** -11 * (2 * o.abs() + w @ v) + tiny @ v + tiny.sum(1, keepdim=True) * o.abs() + far * size + 2.0 ** -25
                 seen = sees.any(1, keepdim=True)
                 out[token:token + new, h * group:(h + 1) * group] = torch.where(seen, o, 0.0).reshape(new, group, 128)
                 tol[token:token + new, h * group:(h + 1) * group] = torch.where(seen, t, 0.0).reshape(new, group, 128)
@@ -328,3 +332,40 @@ def test_refusals():
         kv.batch_chunk_f16(o, q, **specs, layer_idx=1, seqlen_indptr=starts)
     empty = q[:0]
     kv.batch_chunk_i4(empty, empty, **specs, layer_idx=1, seqlen_indptr=starts * 0)          # no new tokens: nothing to do
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("page_size,lens,news,heads,group,window,sinks", [
+    (16, [600], [600], 2, 1, 0, 0), (16, [1500, 300, 2], [257, 300, 2], 1, 4, 0, 0), (64, [2000], [700], 2, 3, 0, 0), (5, [900], [400], 1, 2, 0, 0),
+    (7, [400, 90], [300, 0], 1, 1, 100, 4), (16, [3000], [513], 1, 5, 500, 70), (128, [1000, 1000], [40, 999], 1, 8, 64, 1), (2, [300], [290], 1, 1, 33, 0),
+    (1, [200], [200], 1, 2, 0, 0), (16, [70, 5], [200, 9], 2, 2, 0, 0),
+])
+def test_many_rows(page_size, lens, news, heads, group, window, sinks, f16):
+    """Tiles of 256 rows: several of them, rows and positions that fill none, sequences with more new tokens than they hold."""
+    specs, q, starts = make(page_size + heads, page_size, lens, news, heads, group, f16)
+    check(specs, q, starts, lens, news, window=window, sinks=sinks)
+
+
+def test_many_rows_large_logits_scales_and_missing_pages():
+    lens, news = [700], [400]
+    specs, q, starts = make(21, 16, lens, news, 1, 2, spread=12.0)
+    check(specs, q, starts, lens, news)
+    e = torch.randint(-20, 12, specs["kv_param"].shape[:-1], device=DEV)
+    specs["kv_param"][:, :, 1] *= torch.exp2(e.double()).half()[:, :, 1, ..., None]
+    specs["kv_param"][:, :, 1, :, ::5, 0] = 0
+    specs["kv_param"][:, :, 1, :, 1::5, 0] *= -1
+    check(specs, q, starts, lens, news)
+    specs["kv_indices"][3], specs["kv_indices"][20] = -1, 1 << 30
+    check(specs, q, starts, lens, news, gone=[(0, p) for p in [*range(48, 64), *range(320, 336)]])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_many_rows_with_the_transform_inside(f16):
+    lens, news = [500], [300]
+    specs, q, starts = make(22, 16, lens, news, 1, 2, f16)
+    qh = kv.matmul_had_cuda(q.contiguous(), torch.float16)
+    call = kv.batch_chunk_f16 if f16 else kv.batch_chunk_i4
+    apart, o = torch.empty_like(qh), torch.empty_like(qh)
+    call(apart, qh, **specs, layer_idx=1, seqlen_indptr=starts)
+    call(o, q, **specs, layer_idx=1, seqlen_indptr=starts, q_hadamard=True)
+    assert float((o - apart).double().norm() / apart.double().norm()) < 2.0 ** -10
