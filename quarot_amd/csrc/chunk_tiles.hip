@@ -20,19 +20,30 @@ struct Divisor {
 };
 __device__ __forceinline__ int divided(int n, Divisor d) { return (int)(__umulhi((u32)n << 2, d.inverse) >> d.shift); }
 
-// What a thread has fetched of a step: two of the eight 16-dimension pieces of a key, and four keys' values in four dimensions.
+// What a thread has fetched of a step: two of the sixteen pieces of a key and the parameters of that position, and four positions' values in four
+// dimensions.
 template <bool F16>
 struct Codes {
     u32x4 k4[F16 ? 2 : 1];
     u32x2 k2;
     u32x2 v2[F16 ? 4 : 1];
     unsigned short v1[F16 ? 1 : 4];
-    u32 kp, vp[4];
+    u32 kp, vp;                        // of the key's position
+    u32 scales[4];                     // of the four positions ({scale, zero})
     bool k_there;
-    u32 v_there;                       // bit i: key i of the four
+    u32 v_there;                       // bit i: position i of the four
 };
 
-template <bool F16>
+// weight times factor -> fp16, rounded once: two weights, two factors (a pair of fp16 numbers)
+__device__ __forceinline__ u32 scaled_pair(float w0, float w1, u32 factors) {
+    u32 r;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(w0), "v"(factors));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(r) : "v"(w1), "v"(factors));
+    return r;
+}
+
+// ALIGNED: pages of a multiple of 16 positions, so that a wave's eight keys and its sixteen positions of values lie in one page each
+template <bool F16, bool ALIGNED>
 __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pages) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const PagedKV& c = a.c;
@@ -132,37 +143,56 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
         };
         auto fetch = [&](Codes<F16>& f, int s) {
             const int at = steps.at(s) * kStep;
-            const int64_t ks = slot_at(at + key, f.k_there);
-            int64_t vs[4];
-            f.v_there = 0;
-            if ((c.page_size & 3) == 0) {
-                bool there;
-                vs[0] = slot_at(at + four, there) + kv_slots;
+            // (a position that is not there reads the first ones of page 0)
+            if (ALIGNED) {
+                bool k_page, v_page;
+                const int v_at = at + 32 * (wave >> 2) + 16 * (wave >> 1 & 1);              // (piece is the wave's number)
+                const int64_t kb = slot_at(at + 8 * wave, k_page), vb = slot_at(v_at, v_page) + kv_slots;
+                const uint32_t k_lane = lane >> 3, v_lane = 8 * jj + 4 * (wave & 1);
+                f.k_there = k_page && at + key < len;
+                f.v_there = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    vs[i] = vs[0] + i;
-                    f.v_there |= (there && at + four + i < len ? 1u : 0u) << i;
+                for (int i = 0; i < 4; ++i) f.v_there |= (v_page && v_at + (int)v_lane + i < len ? 1u : 0u) << i;
+                const uint8_t* const kd = c.data + kb * (F16 ? 256 : 64);
+                const uint8_t* const vd = c.data + vb * (F16 ? 256 : 64);
+                if (F16) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) f.k4[i] = *(const u32x4*)(kd + (k_lane * 256u + (uint32_t)e * 32u + 16u * i));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f.v2[i] = *(const u32x2*)(vd + ((v_lane + i) * 256u + (uint32_t)(2 * word + half) * 8u));
+                } else {
+                    f.k2 = *(const u32x2*)(kd + (k_lane * 64u + (uint32_t)e * 8u));
+                    const uint8_t* const kp = (const uint8_t*)(c.param + kb);
+                    f.kp = *(const u32*)(kp + k_lane * 4u);
+                    f.vp = *(const u32*)((const uint8_t*)(c.param + kb + kv_slots) + k_lane * 4u);
+                    const uint8_t* const vp = (const uint8_t*)(c.param + vb);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        f.v1[i] = *(const unsigned short*)(vd + ((v_lane + i) * 64u + (uint32_t)(2 * word + half) * 2u));
+                        f.scales[i] = *(const u32*)(vp + (v_lane + i) * 4u);
+                    }
                 }
             } else {
+                const int64_t ks = slot_at(at + key, f.k_there);
+                if (F16) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) f.k4[i] = ((const u32x4*)c.data)[ks * 16 + 2 * e + i];
+                } else {
+                    f.k2 = ((const u32x2*)c.data)[ks * 8 + e];
+                    f.kp = c.param[ks], f.vp = c.param[ks + kv_slots];
+                }
+                f.v_there = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     bool there;
-                    vs[i] = slot_at(at + four + i, there) + kv_slots;
+                    const int64_t vs = slot_at(at + four + i, there) + kv_slots;
                     f.v_there |= (there ? 1u : 0u) << i;
-                }
-            }
-            if (F16) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) f.k4[i] = ((const u32x4*)c.data)[ks * 16 + 2 * e + i];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f.v2[i] = ((const u32x2*)c.data)[vs[i] * 32 + 2 * word + half];
-            } else {
-                f.k2 = ((const u32x2*)c.data)[ks * 8 + e];
-                f.kp = c.param[ks];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    f.v1[i] = ((const unsigned short*)c.data)[vs[i] * 32 + 2 * word + half];
-                    f.vp[i] = c.param[vs[i]];
+                    if (F16) {
+                        f.v2[i] = ((const u32x2*)c.data)[vs * 32 + 2 * word + half];
+                    } else {
+                        f.v1[i] = ((const unsigned short*)c.data)[vs * 32 + 2 * word + half];
+                        f.scales[i] = c.param[vs];
+                    }
                 }
             }
         };
@@ -174,10 +204,18 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
                 krow[(2 * e + i) ^ (key & 15)] = F16 ? f.k4[i] : codes_of(f.k2[i]);
             }
             const int k_at = (key >> 5) * 32 + (key >> 4 & 1) * 16 + (key >> 2 & 1) * 8 + (key >> 3 & 1) * 4 + (key & 3);       // its place in the order of the second product
-            if (!F16 && e == 0) {
-                const f16x2 p = as_f16x2(f.kp);
-                ((float*)(buf + kSlope))[k_at] = (float)p[0] * (kLog2e * kScale * kCodeUnit);
-                ((float*)(buf + kOffset))[k_at] = (float)p[1] * -(kLog2e * kScale);
+            if (!F16) {
+                const f16x2 p = as_f16x2(f.kp), v = as_f16x2(f.k_there ? f.vp : kNoParameters);
+                const float factor = factor_of((float)v[0], power_of((float)v[0])), recip = __builtin_amdgcn_rcpf(factor), zero = (float)v[1] * recip;
+                const f16 recip_hi = (f16)recip, zero_hi = (f16)zero;
+                if (e == 0) {
+                    ((float*)(buf + kSlope))[k_at] = (float)p[0] * (kLog2e * kScale * kCodeUnit);
+                    ((float*)(buf + kOffset))[k_at] = (float)p[1] * -(kLog2e * kScale);
+                    ((f16*)(buf + kFactor))[k_at] = (f16)factor;
+                    f16* const extra_rows = (f16*)(buf + kValues + 128 * 128) + k_at;
+                    extra_rows[0] = recip_hi, extra_rows[64] = (f16)(recip - (float)recip_hi);
+                    extra_rows[128] = zero_hi, extra_rows[192] = (f16)(zero - (float)zero_hi);
+                }
             }
             {
                 const uint64_t there = __builtin_amdgcn_ballot_w64(f.k_there);
@@ -205,38 +243,25 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
             } else {
                 u32 vp[4], power[2];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) vp[i] = (f.v_there >> i & 1) ? f.vp[i] : kNoParameters;
+                for (int i = 0; i < 4; ++i) vp[i] = (f.v_there >> i & 1) ? f.scales[i] : kNoParameters;
                 bool plain = true;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) power[k] = powers_of(vp[2 * k], vp[2 * k + 1], plain);
-                plain = __builtin_amdgcn_ballot_w64(!plain) == 0;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const u32 w = (u32)f.v1[2 * k] | (u32)f.v1[2 * k + 1] << 16;
-                    const u32x4 scaled = plain ? scaled_codes(w, power[k]) : scaled_codes_slow(w, vp[2 * k], vp[2 * k + 1]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) out[i][k] = scaled[i];
-                }
-                if ((tid & 62) == 0) {                     // one thread for the four keys: their factors, reciprocals and zero points
-                    u32 one[5][2];
+                const u32 w[2] = {(u32)f.v1[0] | (u32)f.v1[1] << 16, (u32)f.v1[2] | (u32)f.v1[3] << 16};
+                if (__builtin_amdgcn_ballot_w64(!plain) == 0) {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        float f2[2], hi1[2], lo1[2], hi2[2], lo2[2];
+                        const u32x4 scaled = scaled_codes(w[k], power[k]);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const f16x2 p = as_f16x2(vp[2 * k + i]);
-                            f2[i] = factor_of((float)p[0], power_of((float)p[0]));
-                            const float recip = 1.f / f2[i], zero = (float)p[1] * recip;
-                            hi1[i] = (float)(f16)recip, lo1[i] = recip - hi1[i];
-                            hi2[i] = (float)(f16)zero, lo2[i] = zero - hi2[i];
-                        }
-                        one[0][k] = cvt_f16x2(f2[0], f2[1]);
-                        one[1][k] = cvt_f16x2(hi1[0], hi1[1]), one[2][k] = cvt_f16x2(lo1[0], lo1[1]);
-                        one[3][k] = cvt_f16x2(hi2[0], hi2[1]), one[4][k] = cvt_f16x2(lo2[0], lo2[1]);
+                        for (int i = 0; i < 4; ++i) out[i][k] = scaled[i];
                     }
-                    *(u32x2*)(buf + kFactor + piece * 16 + jj * 8) = u32x2{one[0][0], one[0][1]};
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) *(u32x2*)(buf + kValues + (128 + i) * 128 + piece * 16 + jj * 8) = u32x2{one[1 + i][0], one[1 + i][1]};
+                    for (int k = 0; k < 2; ++k) {
+                        const u32x4 scaled = scaled_codes_slow(w[k], vp[2 * k], vp[2 * k + 1]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) out[i][k] = scaled[i];
+                    }
                 }
             }
 #pragma unroll
@@ -310,13 +335,14 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
                     const int piece_at = 4 * kb + 2 * tt + h;
-                    f16x8 p;
-                    const f16x8 factor = F16 ? f16x8{} : *(const f16x8*)(buf + kFactor + piece_at * 16);
+                    u32x4 packed;
+                    const u32x4 factor = F16 ? u32x4{} : *(const u32x4*)(buf + kFactor + piece_at * 16);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float w = __builtin_amdgcn_exp2f(x[kb][8 * tt + j]);
-                        p[j] = (f16)(F16 ? w : w * (float)factor[j]);
+                    for (int j = 0; j < 4; ++j) {
+                        const float w0 = __builtin_amdgcn_exp2f(x[kb][8 * tt + 2 * j]), w1 = __builtin_amdgcn_exp2f(x[kb][8 * tt + 2 * j + 1]);
+                        packed[j] = F16 ? cvt_f16x2(w0, w1) : scaled_pair(w0, w1, factor[j]);
                     }
+                    const f16x8 p = __builtin_bit_cast(f16x8, packed);
 #pragma unroll
                     for (int db = 0; db < 4; ++db) {
                         const u32x4 v = ((const u32x4*)(buf + kValues + (32 * db + n) * 128))[piece_at ^ (n >> 1 & 7) ^ (db & 1)];
@@ -383,14 +409,14 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
 }  // namespace
 
 int qr_internal_chunk_tiles(bool fp16, const Chunk& a, int64_t groups, hipStream_t st) {
-    const void* kernel = fp16 ? (const void*)chunk_tiles_kernel<true> : (const void*)chunk_tiles_kernel<false>;
-    const hipError_t e = qr_allow_dynamic_lds(kernel, 2 * kBuffer);
+    using Kernel = void (*)(Chunk, Divisor);
+    const bool aligned = a.c.page_size % 16 == 0;
+    const Kernel kernel = fp16 ? (aligned ? chunk_tiles_kernel<true, true> : chunk_tiles_kernel<true, false>)
+                               : (aligned ? chunk_tiles_kernel<false, true> : chunk_tiles_kernel<false, false>);
+    const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, 2 * kBuffer);
     if (e != hipSuccess) return (int)e;
-    Divisor pages;
     const u32 log2 = a.c.page_size > 1 ? 64u - (u32)__builtin_clzll((unsigned long long)a.c.page_size - 1) : 0u;
-    pages.shift = log2;
-    pages.inverse = (u32)(((1ull << (30 + log2)) + (uint64_t)a.c.page_size - 1) / (uint64_t)a.c.page_size);
-    if (fp16) chunk_tiles_kernel<true><<<dim3((unsigned)groups), dim3(512), 2 * kBuffer, st>>>(a, pages);
-    else chunk_tiles_kernel<false><<<dim3((unsigned)groups), dim3(512), 2 * kBuffer, st>>>(a, pages);
+    const Divisor pages{(u32)(((1ull << (30 + log2)) + (uint64_t)a.c.page_size - 1) / (uint64_t)a.c.page_size), log2};
+    kernel<<<dim3((unsigned)groups), dim3(512), 2 * kBuffer, st>>>(a, pages);
     return qr_launch_status();
 }

@@ -446,17 +446,17 @@ struct Cache {
     int64_t pages, batch;
     int layers, heads, page_size;
 };
-bool cache_args(PyObject* const* a, int device, long long layer, Cache* c) {
+bool cache_args(PyObject* const* a, int device, long long layer, Cache* c, bool fp16_pages = false) {
     c->data = tensor(a[0]);
     c->param = tensor(a[1]);
     c->indptr = tensor(a[2]);
     c->indices = tensor(a[3]);
     c->last = tensor(a[4]);
-    if (!plain(c->data, kByte, device) || !plain(c->param, kHalf, device) || !plain(c->indptr, at::kInt, device) ||
+    if (!plain(c->data, fp16_pages ? kHalf : kByte, device) || !plain(c->param, kHalf, device) || !plain(c->indptr, at::kInt, device) ||
         !plain(c->indices, at::kInt, device) || !plain(c->last, at::kInt, device))
         return false;
     const auto d = c->data->sizes(), p = c->param->sizes();
-    if (d.size() != 6 || p.size() != 6 || d[2] != 2 || d[5] != 64 || p[5] != 2) return false;
+    if (d.size() != 6 || p.size() != 6 || d[2] != 2 || d[5] != (fp16_pages ? 128 : 64) || p[5] != 2) return false;
     for (int i = 0; i < 5; ++i)
         if (d[i] != p[i] || d[i] > 0x7fffffff) return false;
     c->pages = d[0];
@@ -573,6 +573,103 @@ PyObject* decode_step(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     QR_END
 }
 
+// fp16 [tokens, heads, 128] on the device, a token's heads contiguous, tokens at multiples of 8 elements: *stride elements apart
+bool token_rows(const at::Tensor* t, int device, int64_t* stride) {
+    if (!t || !t->is_cuda() || t->scalar_type() != kHalf || t->device().index() != device || t->dim() != 3 || t->size(2) != 128 || t->numel() == 0)
+        return false;
+    const int64_t heads = t->size(1), row = heads * 128;
+    *stride = t->size(0) > 1 ? t->stride(0) : row;
+    return t->stride(2) == 1 && (heads == 1 || t->stride(1) == 128) && *stride >= row && *stride % 8 == 0;
+}
+
+// chunk(fp16 pages, o, q, kv_data, kv_param, indptr, indices, last, layer, seqlen_indptr or None, max_new_len, max_seq_len, window, sinks,
+// q_hadamard, workspace or None) -> True
+PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    QR_ARGS(16)
+    const int device = device_of(tensor(a[3]));
+    long long layer, fresh_bound, bound, window, sinks;
+    bool fp16_pages, q_had;
+    Cache c;
+    if (!arg_bool(a[0], &fp16_pages) || !arg_int(a[8], &layer) || !arg_int(a[10], &fresh_bound) || !arg_int(a[11], &bound) || !arg_int(a[12], &window) ||
+        !arg_int(a[13], &sinks) || !arg_bool(a[14], &q_had) || !cache_args(a + 3, device, layer, &c, fp16_pages))
+        return none();
+    const at::Tensor *o = tensor(a[1]), *q = tensor(a[2]), *seq, *ws;
+    int64_t o_stride, q_stride;
+    if (!token_rows(o, device, &o_stride) || !token_rows(q, device, &q_stride) || o->sizes() != q->sizes() || !plain_or_none(a[9], at::kInt, device, &seq) ||
+        !plain_or_none(a[15], kByte, device, &ws))
+        return none();
+    const int64_t tokens = q->size(0), heads = q->size(1);
+    if (heads % c.heads || heads > 0x7fffffff || (seq ? (seq->dim() != 1 || seq->numel() != c.batch + 1) : tokens != c.batch) || fresh_bound < 0 ||
+        bound < 0 || window < 0 || sinks < 0)
+        return none();
+    if (!seq) fresh_bound = 1;
+    const size_t need = qr_batch_chunk_workspace_bytes(tokens, (int)heads, c.heads, c.batch, fresh_bound, bound, window, sinks);
+    const bool kept = need && ws && (size_t)ws->numel() >= need;
+    at::Tensor own;
+    const auto call = [&] {
+        if (need && !kept) own = fresh({(int64_t)need}, kByte, device);
+        return (fp16_pages ? qr_batch_chunk_f16 : qr_batch_chunk_i4)(
+            o->data_ptr(), o_stride, q->data_ptr(), q_stride, q_had ? 1 : 0, ptr(seq), tokens, (int)heads, c.data->data_ptr(), c.param->data_ptr(),
+            c.indptr->data_ptr(), c.indices->data_ptr(), c.last->data_ptr(), c.pages, c.layers, (int)layer, c.heads, c.page_size, 128, c.batch,
+            fresh_bound, bound, window, sinks, kept ? ws->data_ptr() : need ? own.data_ptr() : nullptr, need, stream(device));
+    };
+    if (!done(call)) return none();
+    Py_RETURN_TRUE;
+    QR_END
+}
+
+// build_page_tables(lengths, page_size, max_pages, block_table or None, new_lengths or None, tokens) -> the tables, in a dict
+PyObject* build_page_tables(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    QR_ARGS(6)
+    const at::Tensor *lengths = tensor(a[0]), *table = a[3] == Py_None ? nullptr : tensor(a[3]), *news;
+    const int device = device_of(lengths);
+    long long page, pages, tokens;
+    if (!plain(lengths, at::kInt, device) || lengths->dim() != 1 || lengths->numel() == 0 || !arg_int(a[1], &page) || !arg_int(a[2], &pages) ||
+        !arg_int(a[5], &tokens) || !plain_or_none(a[4], at::kInt, device, &news))
+        return none();
+    const int64_t batch = lengths->numel();
+    if (page <= 0 || page > 0x7fffffff || pages <= 0 || pages > 0x3fffffff || pages * batch > 0x3fffffff || tokens < 0 ||
+        (news ? (news->dim() != 1 || news->numel() != batch) : tokens != 0))
+        return none();
+    int64_t stride = 0;
+    if (a[3] != Py_None) {
+        if (!table || !table->is_cuda() || table->scalar_type() != at::kInt || table->device().index() != device || table->dim() != 2 ||
+            table->size(0) != batch || table->size(1) < pages || table->stride(1) != 1)
+            return none();
+        stride = batch > 1 ? table->stride(0) : table->size(1);
+        if (stride < pages) return none();
+    }
+    at::Tensor t[6];
+    const auto call = [&] {
+        t[0] = fresh({batch + 1}, at::kInt, device);
+        t[1] = fresh({batch * pages}, at::kInt, device);
+        t[2] = fresh({batch}, at::kInt, device);
+        if (news) {
+            t[3] = fresh({batch + 1}, at::kInt, device);
+            t[4] = fresh({tokens}, at::kLong, device);
+            t[5] = fresh({tokens}, at::kLong, device);
+        }
+        return qr_build_page_tables(lengths->data_ptr(), ptr(news), batch, (int)page, pages, ptr(table), stride, tokens, t[0].data_ptr(), t[1].data_ptr(),
+                                    t[2].data_ptr(), news ? t[3].data_ptr() : nullptr, news && tokens ? t[4].data_ptr() : nullptr,
+                                    news && tokens ? t[5].data_ptr() : nullptr, stream(device));
+    };
+    if (!done(call)) return none();
+    static const char* const names[6] = {"kv_indptr", "kv_indices", "last_page_offset", "seqlen_indptr", "positions", "slots"};
+    PyObject* d = PyDict_New();
+    if (!d) return nullptr;
+    for (int i = 0; i < (news ? 6 : 3); ++i) {
+        PyObject* v = wrap(std::move(t[i]));
+        const bool set = v && PyDict_SetItemString(d, names[i], v) == 0;
+        Py_XDECREF(v);
+        if (!set) {
+            Py_DECREF(d);
+            return nullptr;
+        }
+    }
+    return d;
+    QR_END
+}
+
 // outcome(code) -> whether the library's code means success: True, False for a refusal, RuntimeError for a HIP error
 PyObject* outcome(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     QR_ARGS(1)
@@ -595,6 +692,8 @@ PyMethodDef methods[] = {QR_METHOD(quantize_rows),
                          QR_METHOD(where),
                          QR_METHOD(quantize_append),
                          QR_METHOD(decode_step),
+                         QR_METHOD(chunk),
+                         QR_METHOD(build_page_tables),
                          QR_METHOD(outcome),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -291,6 +291,9 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
 
 def _chunk(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
            window, sinks, q_hadamard, workspace):
+    if _lib.host.chunk(f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
+                       window, sinks, q_hadamard, workspace):
+        return
     pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
     dev, batch = kv_data.device, last_page_offset.shape[0]
     for name, t in (("o", o), ("q", q)):
@@ -373,6 +376,11 @@ def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_
     [batch], all int32: the arguments of the cache's other functions.  With new_lengths int32 [batch], how many of the tokens are new
     (the last ones), and `tokens`, their number, also seqlen_indptr int32 [batch + 1], and for every new token int64 positions and
     slots (page * page_size + entry, -1 where it has no place)."""
+    if max_pages is None and isinstance(block_table, torch.Tensor) and block_table.dim() == 2:
+        max_pages = block_table.shape[1]
+    tables = _lib.host.build_page_tables(lengths, page_size, max_pages, block_table, new_lengths, tokens)
+    if tables is not None:
+        return tables
     fn = "build_page_tables"
     page_size, tokens = int(page_size), int(tokens)
     if not (lengths.is_cuda and lengths.is_contiguous() and lengths.dim() == 1 and lengths.dtype == torch.int32):
@@ -383,7 +391,6 @@ def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_
         if not (block_table.is_cuda and block_table.device == dev and block_table.dim() == 2 and block_table.dtype == torch.int32
                 and block_table.shape[0] == batch and (block_table.shape[1] <= 1 or block_table.stride(1) == 1)):
             raise RuntimeError(f"{fn}: block_table must be int32 [batch_size, max_pages] on {dev} with contiguous rows")
-        max_pages = block_table.shape[1] if max_pages is None else max_pages
         if not (int(max_pages) <= block_table.shape[1]):
             raise RuntimeError(f"{fn}: block_table has fewer than max_pages columns")
         stride = block_table.stride(0) if batch > 1 else block_table.shape[1]
