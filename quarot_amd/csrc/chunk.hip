@@ -17,23 +17,27 @@
 namespace {
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
-// A workgroup of four waves takes 16 NB rows of a (sequence, key head); its waves (and those of the other splits) take the steps of 32
+// A workgroup of NW waves takes 16 NB rows of a (sequence, key head); its waves (and those of the other splits) take the steps of 32
 // positions in turn, so a cached vector is read once per tile of rows.  A wave works on transposed tiles, positions x rows: the first product's
 // result has a row in every lane and positions in its registers, which is what the second product takes as its right operand, with no exchange
 // between lanes.  The contraction's order is free, so a position's codes are used as they lie: lane (n, g) of the first product takes bytes 16 g ..
-// of key n, the word s of them in step s; lane (m, g) of the second takes word m of the eight keys 4 g .. 4 g + 3 and 16 + 4 g .. of a step,
+// of key n, the word s of them in step s (fp16 pages: bytes 64 s + 16 g .., whole lines by every load); lane (m, g) of the second takes word m of the eight keys 4 g .. 4 g + 3 and 16 + 4 g .. of a step,
 // whose nibble b is row m of its block b of outputs.
 template <bool F16>
-struct Fetched {                       // the step that is on its way
+struct Fetched {                       // a step's keys, refilled behind the first product, and its values, refilled behind the second
     u32x4 k[F16 ? 8 : 2], kp[F16 ? 1 : 2], vp[F16 ? 1 : 2];
     u32x4 v4[F16 ? 8 : 1];
     u32 v[F16 ? 1 : 8];
+};
+struct There {
     u32 ok;                            // bit 4 kb + i: position 16 kb + 4 g + i is there
+    bool all;                          // all of them are, in every lane
 };
 
-template <int NB, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk a) {
-    __shared__ f32x4 st4[4 * 16 * 33];                     // per wave and row: maximum, sum, -, -, 128 outputs
+// ALIGNED: pages of a multiple of 16 positions, so that each half of a step lies in one page.
+template <int NB, int NW, bool F16, bool ALIGNED>
+__global__ __launch_bounds__(64 * NW, NB == 4 ? 1 : NB == 2 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) {
+    extern __shared__ __attribute__((aligned(16))) f32x4 st4[];            // per wave and row: maximum, sum, -, -, 128 outputs
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -52,15 +56,106 @@ __global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk 
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
     const int64_t kv_slots = (int64_t)c.num_heads * c.page_size;
-    constexpr int VEC = F16 ? 16 : 4;                      // 16-byte pieces of a vector
-    const u32x4* const data = (const u32x4*)c.data;
+    constexpr uint32_t VEC = F16 ? 256 : 64;               // bytes of a vector
 
     for (int tile = first_tile; tile * 16 * NB < rows; tile += a.tiles) {
         const int r0 = tile * 16 * NB, r1 = r0 + 16 * NB < rows ? r0 + 16 * NB : rows;
         const int lowest = len - fresh + r0 / a.group, highest = len - fresh + (r1 - 1) / a.group;
         const Steps steps = steps_of<5>(a, lowest, highest);
+        const int stride = NW * a.splits;
 
-        // the queries: lane (n, g) holds dimensions 32 g .. 32 g + 31 of row n of every block
+        // Loads are unconditional: a position that is not there reads the first entries of page 0 and is masked.  ALIGNED: the page numbers of a step are
+        // asked for a step ahead, so that its loads do not wait for them.
+        Fetched<F16> f;
+        int page_at[2] = {-1, -1};
+        int64_t slots[ALIGNED ? 2 : 8];                    // ALIGNED: of the step's halves; else of the lane's eight positions
+        auto ask_pages = [&](int s) {
+            if (ALIGNED && npages > 0) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const int it = divided(steps.at(s) * 32 + 16 * kb, pages);
+                    page_at[kb] = it < npages ? c.indices[p0 + it] : -1;
+                }
+            }
+        };
+        auto fetch_keys = [&](int s, int next) {
+            const int at = steps.at(s) * 32;
+            There t{0, true};
+            if (ALIGNED) {
+                uint32_t k_off = (uint32_t)n * VEC + (uint32_t)g * 16, p_off = (uint32_t)g * 16;
+                asm volatile("" : "+v"(k_off), "+v"(p_off));                       // (kept as 32-bit offsets behind wave-uniform addresses)
+                t.all = at + 32 <= len;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const int pos = at + 16 * kb, page = page_at[kb];
+                    const u32 entry = (u32)(pos - divided(pos, pages) * c.page_size);
+                    const bool there = page >= 0 && page < c.num_pages && entry < (u32)c.page_size;
+                    slots[kb] = there ? page * page_slots + head_slots + entry : head_slots;
+                    const uint8_t* const kd = c.data + slots[kb] * VEC;
+                    if (!there) t.all = false;
+                    else t.ok |= 15u << (4 * kb);
+#pragma unroll
+                    for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[F16 ? 4 * kb + i : kb] = __builtin_nontemporal_load((const u32x4*)(kd + k_off + 64 * i));
+                    if (!F16) {
+                        const uint8_t* const kp = (const uint8_t*)(c.param + slots[kb]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f.kp[kb][i] = *(const u32*)(kp + p_off + 4 * i);
+                    }
+                }
+                if (!t.all) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (at + 16 * (k >> 2) + 4 * g + (k & 3) >= len) t.ok &= ~(1u << k);
+                }
+                ask_pages(next);
+            } else {
+                const int pos = at + (lane & 31), it = divided(pos, pages);
+                const u32 entry = (u32)(pos - it * c.page_size);
+                const bool in = pos < len && it < npages && entry < (u32)c.page_size;
+                const int page = npages > 0 ? c.indices[p0 + (in ? it : 0)] : -1;
+                const bool mine_ok = in && page >= 0 && page < c.num_pages;
+                const int64_t mine = mine_ok ? page * page_slots + head_slots + entry : head_slots;
+                t.all = __builtin_amdgcn_ballot_w64(!mine_ok) == 0;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const uint8_t* const kd = c.data + __shfl(mine, 16 * kb + n, 64) * VEC + g * 16;
+#pragma unroll
+                    for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[F16 ? 4 * kb + i : kb] = *(const u32x4*)(kd + 64 * i);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        slots[(4 * kb + i) % (ALIGNED ? 2 : 8)] = __shfl(mine, 16 * kb + 4 * g + i, 64);
+                        t.ok |= (u32)__shfl((int)mine_ok, 16 * kb + 4 * g + i, 64) << (4 * kb + i);
+                        if (!F16) f.kp[kb][i] = c.param[slots[(4 * kb + i) % (ALIGNED ? 2 : 8)]];
+                    }
+                }
+            }
+            return t;
+        };
+        auto fetch_values = [&]() {                        // of the step whose keys were fetched last
+            uint32_t v_off = (uint32_t)g * 4 * VEC + (uint32_t)n * (VEC / 16), p_off = (uint32_t)g * 16;
+            asm volatile("" : "+v"(v_off), "+v"(p_off));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int64_t slot = (ALIGNED ? slots[k >> 2] : slots[k % (ALIGNED ? 2 : 8)]) + kv_slots;
+                const uint8_t* const vd = c.data + slot * VEC + (ALIGNED ? v_off + VEC * (k & 3) : (uint32_t)n * (VEC / 16));
+                if (F16) {
+                    f.v4[k] = __builtin_nontemporal_load((const u32x4*)vd);
+                } else {
+                    f.v[k] = *(const u32*)vd;
+                    f.vp[k >> 2][k & 3] = ALIGNED ? *(const u32*)((const uint8_t*)(c.param + slot) + p_off + 4 * (k & 3)) : c.param[slot];
+                }
+            }
+        };
+        int s = split * NW + wave;
+        There there{0, false};
+        ask_pages(s);
+        if (s < steps.all) {
+            there = fetch_keys(s, s + stride);
+            fetch_values();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
+        // the queries: lane (n, g) holds dimensions 32 g + 8 i .. + 7 (fp16 pages: 32 i + 8 g ..), i = 0 .. 3, of row n of every block
         u32x4 qf[NB][4];
         float qsum[NB];                                    // -log2(e) / sqrt(128) times the row's sum
         int place[NB];
@@ -70,13 +165,13 @@ __global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk 
             const bool in = r < rows;
             const int t = (in ? r : r0) / a.group, head = h * a.group + (in ? r : r0) - t * a.group;
             place[nb] = in ? len - fresh + t : -1;
-            const u32x4* src = (const u32x4*)(a.q + (int64_t)(start + t) * a.q_stride + (int64_t)head * 128) + 4 * g;
+            const u32x4* src = (const u32x4*)(a.q + (int64_t)(start + t) * a.q_stride + (int64_t)head * 128) + (F16 ? g : 4 * g);
             u32x4 w[4];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) w[s] = in ? src[s] : u32x4{0, 0, 0, 0};
-            if (a.q_had) {
-                // the Hadamard transform over the head dimension in 32 bits: index bits 0 .. 4 within the lane, 5 and 6 across the quarters;
-                // rounded to fp16 like the transform's own entry point
+            for (int i = 0; i < 4; ++i) w[i] = in ? src[F16 ? 4 * i : i] : u32x4{0, 0, 0, 0};
+            if (__builtin_expect(a.q_had, 0)) {
+                // the Hadamard transform over the head dimension in 32 bits: five of the index's bits within the lane, two across the quarters; rounded to
+                // fp16 like the transform's own entry point
                 float t32[32];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -109,7 +204,7 @@ __global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk 
             }
             qsum[nb] = quarters_sum(sum) * -(kLog2e * kScale);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) qf[nb][s] = F16 ? w[s] : query_for_codes(w[s]);
+            for (int i = 0; i < 4; ++i) qf[nb][i] = F16 ? w[i] : query_for_codes(w[i]);
         }
 
         float m[NB], d[NB], pz[NB];
@@ -121,74 +216,26 @@ __global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk 
             for (int k = 0; k < 8; ++k) acc[nb][k] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
 
-        // Loads are unconditional: a position that is not there reads the first entries of page 0 and is masked.
-        auto fetch = [&](Fetched<F16>& f, int s) {
-            const int at = steps.at(s) * 32;
-            f.ok = 0;
-            int64_t mine = 0;
-            bool mine_ok = false;
-            if (!ALIGNED) {
-                const int pos = at + (lane & 31), it = pos / c.page_size;
-                const bool in = pos < len && it < npages;
-                const int page = npages > 0 ? c.indices[p0 + (in ? it : 0)] : -1;
-                mine_ok = in && page >= 0 && page < c.num_pages;
-                mine = mine_ok ? page * page_slots + head_slots + (pos - it * c.page_size) : head_slots;
-            }
+        auto consume = [&](int step, int next) {
+            const int at = steps.at(step) * 32;
+            const There ok = there;
+            const bool whole = ok.all && at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks);
+            auto sees = [&](int nb, int k) {               // whether the lane's row sees its position k
+                const int pos = at + 16 * (k >> 2) + 4 * g + (k & 3);
+                return pos <= place[nb] && (a.window == 0 || pos > place[nb] - a.window || pos < a.sinks) && (ok.ok >> k & 1);
+            };
+            // Where some rows do not see a position its value must not reach them, whatever it is (zero times an infinity is none): int4 pages' scales and
+            // zero points that are not finite are replaced, and the rows that do see them become NaN, as their products would.
+            u32 odd = 0;
+            if (!F16 && !whole) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                if (ALIGNED) {
-                    const int pos = at + 16 * kb, it = pos / c.page_size;
-                    const bool in = it < npages;
-                    const int page = npages > 0 ? c.indices[p0 + (in ? it : 0)] : -1;
-                    const bool there = in && page >= 0 && page < c.num_pages;
-                    const int64_t slot = there ? page * page_slots + head_slots + (pos - it * c.page_size) : head_slots;
-                    const int64_t ks = slot + n, vs = slot + kv_slots + 4 * g;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) f.ok |= (there && pos + 4 * g + i < len ? 1u : 0u) << (4 * kb + i);
-                    if (F16) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) f.k[4 * kb + i] = data[ks * VEC + 4 * g + i];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) f.v4[4 * kb + i] = data[(vs + i) * VEC + n];
-                    } else {
-                        f.k[kb] = data[ks * VEC + g];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) f.v[4 * kb + i] = ((const u32*)c.data)[(vs + i) * 16 + n];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) f.kp[kb][i] = c.param[slot + 4 * g + i], f.vp[kb][i] = c.param[vs + i];
-                    }
-                } else {
-                    const int64_t ks = __shfl(mine, 16 * kb + n, 64);
-                    if (F16) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) f.k[4 * kb + i] = data[ks * VEC + 4 * g + i];
-                    } else {
-                        f.k[kb] = data[ks * VEC + g];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int64_t slot = __shfl(mine, 16 * kb + 4 * g + i, 64);
-                        f.ok |= (u32)__shfl((int)mine_ok, 16 * kb + 4 * g + i, 64) << (4 * kb + i);
-                        if (F16) {
-                            f.v4[4 * kb + i] = data[(slot + kv_slots) * VEC + n];
-                        } else {
-                            f.v[4 * kb + i] = ((const u32*)c.data)[(slot + kv_slots) * 16 + n];
-                            f.kp[kb][i] = c.param[slot], f.vp[kb][i] = c.param[slot + kv_slots];
-                        }
-                    }
+                for (int k = 0; k < 8; ++k) {
+                    const u32 w = f.vp[k >> 2][k & 3];
+                    const bool strange = (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u;
+                    odd |= (strange ? 1u : 0u) << k;
+                    f.vp[k >> 2][k & 3] = strange || !(ok.ok >> k & 1) ? kNoParameters : w;
                 }
-            }
-        };
-
-        auto consume = [&](Fetched<F16>& f, int s) {
-            const int at = steps.at(s) * 32;
-            const bool whole = at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks) &&
-                               __builtin_amdgcn_ballot_w64(f.ok != 0xFFu) == 0;
-            // a position that is not there may hold anything: any finite value will do (its weight is zero)
-            u32x4 vp[2];
-            if (!F16) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) vp[k >> 2][k & 3] = (f.ok >> k & 1) ? f.vp[k >> 2][k & 3] : kNoParameters;
+                odd &= ok.ok;
             }
             f32x4 x[NB][2];
 #pragma unroll
@@ -202,51 +249,56 @@ __global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk 
                     for (int nb = 0; nb < NB; ++nb)
                         x[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(f16x8, qf[nb][i]), x[nb][kb], 0, 0, 0);
                 }
-            float ka[8], kz[8], vf[8], vr[8], vz[8];       // keys: slope and zero point; values: factor, its reciprocal, zero point over factor
-            u32 power[4];
-            bool plain = true;
+            float ka[8], kz[8];                            // slope and zero point of the keys
             if (!F16) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     const f16x2 kp = as_f16x2(f.kp[k >> 2][k & 3]);
-                    ka[k] = (float)kp[0] * (kLog2e * kScale * kCodeUnit);
-                    kz[k] = (float)kp[1];
+                    ka[k] = __builtin_fmaf((float)kp[0], kLog2e * kScale * kCodeUnit, 0.f), kz[k] = (float)kp[1];
                 }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            there = fetch_keys(next, next + stride);
+            __builtin_amdgcn_sched_barrier(0);
+            float vr[8], vz[8];                            // 1 / f and zero point / f of the values
+            u32 factors[4], power[4];
+            bool plain = true;
+            if (!F16) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const u32 w0 = vp[k >> 1][2 * k & 3], w1 = vp[k >> 1][(2 * k & 3) + 1];
+                    const u32 w0 = f.vp[k >> 1][2 * k & 3], w1 = f.vp[k >> 1][(2 * k & 3) + 1];
                     power[k] = powers_of(w0, w1, plain);
+                    factors[k] = (__builtin_amdgcn_perm(w1, w0, 0x05040100u) & 0x83FF83FFu) | 0x3C003C00u;
                 }
                 plain = __builtin_amdgcn_ballot_w64(!plain) == 0;
-                if (plain) {
+                if (__builtin_expect(!plain, 0)) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) vf[k] = (float)as_f16x2(((u32)vp[k >> 2][k & 3] & 0x83FFu) | 0x3C00u)[0];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const float scale = (float)as_f16x2(vp[k >> 2][k & 3])[0];
-                        vf[k] = factor_of(scale, power_of(scale));
+                    for (int k = 0; k < 4; ++k) {
+                        const float s0 = (float)as_f16x2(f.vp[k >> 1][2 * k & 3])[0], s1 = (float)as_f16x2(f.vp[k >> 1][(2 * k & 3) + 1])[0];
+                        factors[k] = cvt_f16x2(factor_of(s0, power_of(s0)), factor_of(s1, power_of(s1)));
                     }
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    vr[k] = __builtin_amdgcn_rcpf(vf[k]);
-                    vz[k] = (float)as_f16x2(vp[k >> 2][k & 3])[1] * vr[k];
+                    vr[k] = __builtin_amdgcn_rcpf((float)as_f16x2(factors[k >> 1])[k & 1]);
+                    vz[k] = __builtin_fmaf((float)as_f16x2(f.vp[k >> 2][k & 3])[1], vr[k], 0.f);
                 }
             }
-            f16x8 p[NB];
+            u32x4 p[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 float y[8], top = -__builtin_inff();
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < 8; ++k) {
                     y[k] = F16 ? x[nb][k >> 2][k & 3] * (kLog2e * kScale) : __builtin_fmaf(x[nb][k >> 2][k & 3], ka[k], kz[k] * qsum[nb]);
+                }
                 if (!whole) {
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const int pos = at + 16 * (k >> 2) + 4 * g + (k & 3);
-                        const bool sees = pos <= place[nb] && (a.window == 0 || pos > place[nb] - a.window || pos < a.sinks) && (f.ok >> k & 1);
-                        y[k] = sees ? y[k] : -__builtin_inff();
+                    for (int k = 0; k < 8; ++k) y[k] = sees(nb, k) ? y[k] : -__builtin_inff();
+                    if (!F16 && __builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if ((odd >> k & 1) && sees(nb, k)) d[nb] = __builtin_nanf("");
                     }
                 }
 #pragma unroll
@@ -259,57 +311,104 @@ __global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk 
                     for (int k = 0; k < 8; ++k) acc[nb][k] *= keep;
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float w = __builtin_amdgcn_exp2f(y[k] - m[nb]);
-                    p[nb][k] = (f16)(F16 ? w : w * vf[k]);
-                    d[nb] = F16 ? d[nb] + (float)p[nb][k] : __builtin_fmaf((float)p[nb][k], vr[k], d[nb]);
-                    if (!F16) pz[nb] = __builtin_fmaf((float)p[nb][k], vz[k], pz[nb]);
+                for (int k = 0; k < 4; ++k) {
+                    const float w0 = __builtin_amdgcn_exp2f(y[2 * k] - m[nb]), w1 = __builtin_amdgcn_exp2f(y[2 * k + 1] - m[nb]);
+                    const u32 w = F16 ? cvt_f16x2(w0, w1) : scaled_pair(w0, w1, factors[k]);
+                    p[nb][k] = w;
+                    const f16x2 r = as_f16x2(w);
+                    d[nb] = F16 ? d[nb] + (float)r[0] : __builtin_fmaf((float)r[0], vr[2 * k], d[nb]);
+                    d[nb] = F16 ? d[nb] + (float)r[1] : __builtin_fmaf((float)r[1], vr[2 * k + 1], d[nb]);
+                    if (!F16) pz[nb] = __builtin_fmaf((float)r[1], vz[2 * k + 1], __builtin_fmaf((float)r[0], vz[2 * k], pz[nb]));
                 }
             }
             // the values: row m of block b is dimension 8 m + b
+            if (F16) {
+                auto product = [&](auto&& word, auto&& add) {      // word(key, word of its piece); add(block, operand)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {         // nibbles (words of a piece) 4 half .. 4 half + 3
-                u32x4 v[4];                                // [block][pair of keys]
-                if (F16) {
+                    for (int i = 0; i < 4; ++i) {
+                        u32x4 v[2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const bool ok0 = f.ok >> (2 * k) & 1, ok1 = f.ok >> (2 * k + 1) & 1;
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const u32 w0 = ok0 ? f.v4[2 * k][2 * half + i] : 0u, w1 = ok1 ? f.v4[2 * k + 1][2 * half + i] : 0u;
-                            v[2 * i][k] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
-                            v[2 * i + 1][k] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
+                        for (int k = 0; k < 4; ++k) {
+                            const u32 w0 = word(2 * k, i), w1 = word(2 * k + 1, i);
+                            v[0][k] = __builtin_amdgcn_perm(w1, w0, 0x05040100u);
+                            v[1][k] = __builtin_amdgcn_perm(w1, w0, 0x07060302u);
                         }
+                        add(2 * i, v[0]);
+                        add(2 * i + 1, v[1]);
                     }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const u32 w = __builtin_amdgcn_perm(f.v[2 * k + 1], f.v[2 * k], half ? 0x07060302u : 0x05040100u);
-                        const u32x4 scaled = plain ? scaled_codes(w, power[k]) : scaled_codes_slow(w, vp[k >> 1][2 * k & 3], vp[k >> 1][(2 * k & 3) + 1]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) v[i][k] = scaled[i];
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
+                };
+                auto add_all = [&](int block, u32x4 v) {
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
-                        acc[nb][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v[i]), p[nb], acc[nb][4 * half + i], 0, 0, 0);
+                        acc[nb][block] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v), __builtin_bit_cast(f16x8, p[nb]), acc[nb][block], 0, 0, 0);
+                };
+                // (opaque to the compiler, which would keep all masks of the loop below in registers)
+                auto strange = [](u32 w) {
+                    asm volatile("" : "+v"(w));
+                    return ((w & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((w & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
+                };
+                bool any = false;
+                if (!whole) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            f.v4[k][i] = (ok.ok >> k & 1) ? (u32)f.v4[k][i] : 0u;
+                            any = any || strange(f.v4[k][i]) != 0;
+                        }
+                }
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(any) == 0, 1)) {
+                    product([&](int k, int i) { return (u32)f.v4[k][i]; }, add_all);
+                } else {
+                    // infinities and NaN where not all rows see all positions: first all other values, then position by position the rest, for the rows that see it
+                    product([&](int k, int i) { return (u32)f.v4[k][i] & ~strange(f.v4[k][i]); }, add_all);
+#pragma unroll 1
+                    for (int j = 0; j < 32; ++j) {
+                        const int pos = at + j;
+                        product([&](int k, int i) { return 16 * (k >> 2) + 4 * g + (k & 3) == j ? (u32)f.v4[k][i] & strange(f.v4[k][i]) : 0u; },
+                                [&](int block, u32x4 v) {
+#pragma unroll
+                                    for (int nb = 0; nb < NB; ++nb) {
+                                        const bool seen = pos <= place[nb] && (a.window == 0 || pos > place[nb] - a.window || pos < a.sinks);
+                                        const f32x4 more = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v), __builtin_bit_cast(f16x8, p[nb]), f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                                        for (int i = 0; i < 4; ++i) acc[nb][block][i] += seen ? more[i] : 0.f;
+                                    }
+                                });
+                    }
+                }
+            } else {
+                auto product = [&](auto&& scaled) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {     // nibbles 4 half .. 4 half + 3
+                        u32x4 v[4];                        // [block][pair of keys]
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const u32x4 w = scaled(__builtin_amdgcn_perm(f.v[2 * k + 1], f.v[2 * k], half ? 0x07060302u : 0x05040100u), k);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[i][k] = w[i];
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+                                acc[nb][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v[i]), __builtin_bit_cast(f16x8, p[nb]), acc[nb][4 * half + i], 0, 0, 0);
+                    }
+                };
+                if (__builtin_expect(plain, 1)) product([&](u32 w, int k) { return scaled_codes(w, power[k]); });
+                else product([&](u32 w, int k) { return scaled_codes_slow(w, f.vp[k >> 1][2 * k & 3], f.vp[k >> 1][(2 * k & 3) + 1]); });
             }
         };
 
-        const int stride = 4 * a.splits;
-        int s = split * 4 + wave;
-        Fetched<F16> f;
-        if (s < steps.all) fetch(f, s);
         for (; s < steps.all; s += stride) {
-            Fetched<F16> now = f;
-            const int next = s + stride < steps.all ? s + stride : s;
-            fetch(f, next);
-            consume(now, s);
+            consume(s, s + stride < steps.all ? s + stride : s);       // (behind the last step the next one is the same again)
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_values();
+            __builtin_amdgcn_sched_barrier(0);
         }
 
-        // ---- merge: a wave's states are those of its rows; the four waves' through LDS, one block of 16 rows at a time
+        // ---- merge: a wave's states are those of its rows; the waves' through LDS, one block of 16 rows at a time
+        constexpr int LANES = 4 * NW, PER = 32 / LANES;    // threads of a row, and of its 32 pieces of four dimensions how many each takes
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const float dd = quarters_sum(d[nb]), zz = F16 ? 0.f : quarters_sum(pz[nb]);
@@ -322,35 +421,35 @@ __global__ __launch_bounds__(256, NB == 4 ? 1 : 2) void chunk_rows_kernel(Chunk 
                 mine[2 + 8 * g + 2 * i] = f32x4{acc[nb][4][i] - zz, acc[nb][5][i] - zz, acc[nb][6][i] - zz, acc[nb][7][i] - zz};
             }
             __syncthreads();
-            const int row = threadIdx.x >> 4, l = threadIdx.x & 15, r = r0 + 16 * nb + row;
+            const int row = threadIdx.x / LANES, l = threadIdx.x % LANES, r = r0 + 16 * nb + row;
             if (r < rows) {
                 float M = kEmpty, D = 0.f;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, st4[(w * 16 + row) * 33][0]);
-                f32x4 O[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                for (int w = 0; w < NW; ++w) M = __builtin_fmaxf(M, st4[(w * 16 + row) * 33][0]);
+                f32x4 O[PER];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
+                for (int i = 0; i < PER; ++i) O[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
                     const f32x4* src = st4 + (w * 16 + row) * 33;
                     const float keep = __builtin_amdgcn_exp2f(src[0][0] - M);
                     D = __builtin_fmaf(src[0][1], keep, D);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        O[0][i] = __builtin_fmaf(src[1 + 2 * l][i], keep, O[0][i]);
-                        O[1][i] = __builtin_fmaf(src[2 + 2 * l][i], keep, O[1][i]);
-                    }
+                    for (int i = 0; i < PER; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) O[i][j] = __builtin_fmaf(src[1 + PER * l + i][j], keep, O[i][j]);
                 }
                 const int t = r / a.group, head = h * a.group + r - t * a.group;
                 if (a.splits == 1) {
                     const float inv = D == 0.f ? 0.f : 1.f / D;                 // (a row that sees nothing is zero)
-                    u32x4 out;
+                    u32x2* const dst = (u32x2*)(a.o + (int64_t)(start + t) * a.o_stride + (int64_t)head * 128) + PER * l;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) out[i] = cvt_f16x2(O[i >> 1][2 * i & 2] * inv, O[i >> 1][(2 * i & 2) + 1] * inv);
-                    *((u32x4*)(a.o + (int64_t)(start + t) * a.o_stride + (int64_t)head * 128) + l) = out;
+                    for (int i = 0; i < PER; ++i) dst[i] = u32x2{cvt_f16x2(O[i][0] * inv, O[i][1] * inv), cvt_f16x2(O[i][2] * inv, O[i][3] * inv)};
                 } else {
                     float* dst = a.part + (((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.splits + split) * 132;
                     if (l == 0) dst[0] = M, dst[1] = D;
-                    *((f32x4*)dst + 1 + 2 * l) = O[0];
-                    *((f32x4*)dst + 2 + 2 * l) = O[1];
+#pragma unroll
+                    for (int i = 0; i < PER; ++i) *((f32x4*)dst + 1 + PER * l + i) = O[i];
                 }
             }
         }
@@ -382,9 +481,10 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const float* __restric
         u32x4{cvt_f16x2(a[0] * inv, a[1] * inv), cvt_f16x2(a[2] * inv, a[3] * inv), cvt_f16x2(b[0] * inv, b[1] * inv), cvt_f16x2(b[2] * inv, b[3] * inv)};
 }
 
-// How a call is cut: column blocks per workgroup, tiles of rows per (sequence, key head), splits of the positions.
+// How a call is cut: column blocks and waves of a workgroup (nb 0: the kernel of 256 rows), tiles of rows per (sequence, key head), splits of the
+// positions.
 struct ChunkPlan {
-    int nb, tiles, splits;            // nb 0: the kernel of 256 rows
+    int nb, nw, tiles, splits;
 };
 ChunkPlan chunk_plan(int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
@@ -396,11 +496,25 @@ ChunkPlan chunk_plan(int64_t tokens, int group, int num_heads, int64_t batch, in
     int64_t seen = max_seq_len > 0 ? max_seq_len : 0;
     if (window > 0 && seen > window + max_new_len + sinks + 64) seen = window + max_new_len + sinks + 64;
     const int64_t groups = batch * num_heads * p.tiles, steps = (seen + 31) / 32;
-    int64_t splits = p.nb ? (2 * cus + groups - 1) / groups : cus / groups;
-    if (splits > steps / 8) splits = steps / 8;            // (two steps per wave at least)
+    p.nw = p.nb == 4 || groups >= 2 * cus ? 4 : 8;
+    int64_t splits = p.nb ? ((p.nw == 8 ? 1 : 2) * cus + groups - 1) / groups : cus / groups;
+    if (splits > steps / (2 * p.nw)) splits = steps / (2 * p.nw);                // (two steps per wave at least)
     if (splits > 32) splits = 32;
     p.splits = splits < 1 ? 1 : (int)splits;
     return p;
+}
+
+template <bool F16, bool ALIGNED>
+int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st) {
+    using Kernel = void (*)(Chunk, Divisor);
+    const Kernel kernel = plan.nb == 4   ? chunk_rows_kernel<4, 4, F16, ALIGNED>
+                          : plan.nb == 2 ? (plan.nw == 8 ? chunk_rows_kernel<2, 8, F16, ALIGNED> : chunk_rows_kernel<2, 4, F16, ALIGNED>)
+                                         : (plan.nw == 8 ? chunk_rows_kernel<1, 8, F16, ALIGNED> : chunk_rows_kernel<1, 4, F16, ALIGNED>);
+    const size_t lds = (size_t)plan.nw * 16 * 33 * sizeof(f32x4);
+    const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, lds);
+    if (e != hipSuccess) return (int)e;
+    kernel<<<dim3((unsigned)groups), dim3(64 * plan.nw), lds, st>>>(a, pages);
+    return qr_launch_status();
 }
 
 size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? (size_t)tokens * q_heads * splits * 132 * sizeof(float) : 0; }
@@ -440,27 +554,11 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     const int64_t groups = batch_size * num_heads * plan.tiles * a.splits;
     if (groups > 0x7fffffff) return QR_E_SHAPE;
     hipStream_t st = (hipStream_t)stream;
+    const Divisor pages = divisor_of(page_size);
     const bool aligned = page_size % 16 == 0;
-    int lrc;
-#define QR_CHUNK(NB, F, AL) chunk_rows_kernel<NB, F, AL><<<dim3((unsigned)groups), dim3(256), 0, st>>>(a)
-#define QR_CHUNK_NB(F, AL)                                                              \
-    do {                                                                                \
-        if (plan.nb == 1) QR_CHUNK(1, F, AL);                                           \
-        else if (plan.nb == 2) QR_CHUNK(2, F, AL);                                      \
-        else QR_CHUNK(4, F, AL);                                                        \
-    } while (0)
-    if (plan.nb == 0) {
-        lrc = qr_internal_chunk_tiles(fp16, a, groups, st);
-    } else if (fp16) {
-        if (aligned) QR_CHUNK_NB(true, true);
-        else QR_CHUNK_NB(true, false);
-    } else {
-        if (aligned) QR_CHUNK_NB(false, true);
-        else QR_CHUNK_NB(false, false);
-    }
-#undef QR_CHUNK_NB
-#undef QR_CHUNK
-    if (plan.nb) lrc = qr_launch_status();
+    const int lrc = plan.nb == 0 ? qr_internal_chunk_tiles(fp16, a, pages, groups, st)
+                    : fp16       ? (aligned ? launch_rows<true, true>(plan, a, pages, groups, st) : launch_rows<true, false>(plan, a, pages, groups, st))
+                                 : (aligned ? launch_rows<false, true>(plan, a, pages, groups, st) : launch_rows<false, false>(plan, a, pages, groups, st));
     if (lrc != QR_OK || a.splits == 1) return lrc;
     chunk_merge_kernel<<<dim3((unsigned)((tokens * num_q_heads + 15) / 16)), dim3(256), 0, st>>>(a.part, a.starts, (int)batch_size, (int)tokens, num_q_heads,
                                                                                               a.splits, a.o, o_stride);

@@ -1,50 +1,67 @@
 // Attention of new tokens over the paged cache for many rows of a (sequence, key head): the mathematics of chunk.hip on tiles of 256 rows.
 //
-// Eight waves share the cached vectors of a step of 64 positions: each is unpacked once per workgroup, from registers into LDS, as the fp16
-// operand that the matrix instructions take.  A wave holds 32 rows, the positions in its registers (chunk.hip: no exchange between lanes from
-// the first product to the second), and of the second product's operand 132 rows: the 128 dimensions, and the reciprocal 1 / f_j and the zero
-// point zero_j / f_j of every position as pairs of fp16 numbers (22 bits of each).  Their sums are those of the weights as they were
-// rounded, sum p_j and sum p_j zero_j with p_j = fp16(weight_j f_j) / f_j, so a rounding changes a weight and nothing else.
+// Four waves, one per SIMD, of 64 rows each share the cached vectors of a step of 64 positions: each is unpacked once per workgroup, from
+// registers into LDS, as the fp16 operand that the matrix instructions take, and each operand read from LDS serves two of them (with 32 rows per wave
+// LDS was busy for longer than the matrix unit).  A wave holds the positions in its registers and the rows in its lanes (chunk.hip: no
+// exchange between lanes from the first product to the second).  Of the second product's operand there are 132 rows: the 128 dimensions, and
+// the reciprocal 1 / f_j and the zero point zero_j / f_j of every position as pairs of fp16 numbers (22 bits of each; the second ones times 2^11, so that small ones have them too).  Their sums are those of
+// the weights as they were rounded, sum p_j and sum p_j zero_j with p_j = fp16(weight_j f_j) / f_j.  The part of a logit that no code enters,
+// zero_j sum(q) and the row's running maximum, is a product as well, of bf16 pieces that hold 24 bits together (a lane's vector unit would take as
+// long for it as for the exponentials).
+//
+// A wave has its SIMD to itself, so the vector work is laid between the matrix instructions by hand, in slots of two (64 cycles): while the
+// first product of the next 32 positions runs, the weights of these 32; while their second product runs, the logits of the next, and
+// the unpacking of what the workgroup needs a step later.
 #include "qr_chunk.h"
 
 namespace {
 
 constexpr int kRows = 256, kStep = 64;
-// a step's place in LDS
-constexpr int kKeys = 0, kValues = 16384, kValueRows = 133, kSlope = kValues + kValueRows * 128, kOffset = kSlope + 256, kFactor = kOffset + 256,
-              kThere = kFactor + 128, kBuffer = (kThere + 8 + 255) / 256 * 256;
+// LDS: three steps' keys (the next step's are read while others still read this one's), two steps' values
+constexpr int kSlope = 16384, kLine = kSlope + 256, kThere = kLine + 2048, kKeys = (kThere + 8 + 511) / 512 * 512;
+constexpr int kFactor = 133 * 128, kOdd = kFactor + 128, kValues = (kOdd + 8 + 511) / 512 * 512;
+constexpr int kLds = 3 * kKeys + 2 * kValues;
 
-// n / d for n below 2^30: umulhi(4 n, inverse) >> shift
-struct Divisor {
-    u32 inverse, shift;
-};
-__device__ __forceinline__ int divided(int n, Divisor d) { return (int)(__umulhi((u32)n << 2, d.inverse) >> d.shift); }
-
-// What a thread has fetched of a step: two of the sixteen pieces of a key and the parameters of that position, and four positions' values in four
-// dimensions.
+// What a thread has fetched for a step: four of the sixteen pieces of a key and its parameters; four positions' values in eight dimensions, their
+// parameters and those of the position that has the key's number.  mask: which of the wave's sixteen positions are there.
 template <bool F16>
-struct Codes {
-    u32x4 k4[F16 ? 2 : 1];
-    u32x2 k2;
-    u32x2 v2[F16 ? 4 : 1];
-    unsigned short v1[F16 ? 1 : 4];
-    u32 kp, vp;                        // of the key's position
-    u32 scales[4];                     // of the four positions ({scale, zero})
-    bool k_there;
-    u32 v_there;                       // bit i: position i of the four
+struct KeyCodes {
+    u32x4 k[F16 ? 4 : 1];
+    u32 p, mask;
+};
+template <bool F16>
+struct ValueCodes {
+    u32x4 v4[F16 ? 4 : 1];
+    u32 v[F16 ? 1 : 4], scales[F16 ? 1 : 4], p, mask;
 };
 
-// weight times factor -> fp16, rounded once: two weights, two factors (a pair of fp16 numbers)
-__device__ __forceinline__ u32 scaled_pair(float w0, float w1, u32 factors) {
-    u32 r;
-    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(w0), "v"(factors));
-    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(r) : "v"(w1), "v"(factors));
-    return r;
+// Matrix instructions, spelled out: the first product's results and the logits' line are for the vector unit and have to lie where it reaches them, the
+// second product's accumulators in the half of the register file that only matrix instructions use.  (Left to itself the compiler puts all of
+// them into that half, and copies 64 values a unit back.)  It then inserts no wait states either.  A result is read by the vector unit two
+// matrix instructions after its last one at the earliest (32 cycles each; it is there after 11 of 4), or behind `settled`.
+__device__ __forceinline__ void mfma_first(f32x16& c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "a"(b)); }
+__device__ __forceinline__ void mfma_more(f32x16& c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "a"(b)); }
+__device__ __forceinline__ void mfma_line(f32x16& c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void mfma_second(f32x16& c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void mfma_overflow(f32x16& c, u32x4 a, u32x4 b) { asm volatile("s_nop 3\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
+__device__ __forceinline__ void settled() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+__device__ __forceinline__ f32x16 zeros() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    return z;
 }
+// the upper 16 bits of two floats: lo in the low half
+__device__ __forceinline__ u32 tops(float lo, float hi) { return __builtin_amdgcn_perm(as_u32(hi), as_u32(lo), 0x07060302u); }
+__device__ __forceinline__ float top(float v) { return as_f32(as_u32(v) & 0xFFFF0000u); }
+__device__ __forceinline__ bool strange(u32 w) { return (w & 0x7C00u) == 0x7C00u || (w & 0x7C000000u) == 0x7C000000u; }      // a half of it is not finite
 
-// ALIGNED: pages of a multiple of 16 positions, so that a wave's eight keys and its sixteen positions of values lie in one page each
+#define SLOT __builtin_amdgcn_sched_barrier(0)
+#define INLINE __attribute__((always_inline))        // (what a function that is not inlined captures lies in memory)
+
+// ALIGNED: pages of a multiple of 16 positions, so that the sixteen positions that a wave fetches lie in one page
 template <bool F16, bool ALIGNED>
-__global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pages) {
+__global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pages) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const PagedKV& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -52,48 +69,266 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
     int id = blockIdx.x;
     const int split = id % a.splits;
     id /= a.splits;
-    const int kvh_all = c.num_heads;
-    const int pair = id % (kvh_all * c.batch_size);        // (sequence, key head): neighbours are on different XCDs, a pair's tiles on one where 8 divides their number
-    const int tile = a.tiles - 1 - id / (kvh_all * c.batch_size);                  // the tiles with most positions first
-    const int b = pair / kvh_all, head = pair - b * kvh_all;
+    const int pairs = c.num_heads * c.batch_size;
+    const int pair = id % pairs;                           // (sequence, key head): neighbours are on different XCDs, a pair's tiles on one where 8 divides their number
+    const int tile = a.tiles - 1 - id / pairs;             // the tiles with most positions first
+    const int b = pair / c.num_heads, head = pair - b * c.num_heads;
     const Fresh tokens = fresh_of(a, b);
     const int rows = tokens.count * a.group;
+    if (tile * kRows >= rows) return;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;
     const int64_t kv_slots = (int64_t)c.num_heads * c.page_size;
+    constexpr uint32_t VEC = F16 ? 256 : 64;               // bytes of a vector
 
-    // rows of the operand that never change: fp16 pages have the weights' sum by a row of ones, and none are read beyond
-    for (int i = tid; i < 2 * 5 * 32; i += 512) {
-        const int at = i % 160, row = at >> 5;
-        *(u32*)(lds + (i / 160) * kBuffer + kValues + (128 + row) * 128 + (at & 31) * 4) = F16 && row == 0 ? 0x3C003C00u : 0u;
+    // what never changes: the values' operand beyond row 131 (fp16 pages: beyond 127, with a row of ones for the weights' sum), the second half of the logits'
+    // line, whose first factor is one
+    for (int i = tid; i < 2 * 5 * 32; i += 256) {
+        const int at = i % 160;
+        *(u32*)(lds + 3 * kKeys + (i / 160) * kValues + 128 * 128 + at * 4) = F16 && at < 32 ? 0x3C003C00u : 0u;
     }
+    for (int i = tid; i < 3 * 64; i += 256) *(u32x4*)(lds + (i >> 6) * kKeys + kLine + 1024 + (i & 63) * 16) = u32x4{0x00003F80u, 0, 0, 0};
+
+    // ---- a step's way into LDS.  Thread (key, e) takes pieces e, e + 4, e + 8, e + 12 of a key (int4: the words 4 e .. 4 e + 3); thread (four positions,
+    // word) their values in dimensions 8 word ...  The four positions are 16 wave + 8 jj + 4 hh ..: what lane half hh of the second product takes
+    // as its jj-th half.
+    const int key = tid >> 2, e = tid & 3;
+    const int jj = tid & 1, word = tid >> 1 & 15, hh = tid >> 5 & 1, piece = 2 * wave + hh;
+    const int first_of_four = 8 * jj + 4 * hh;             // of the wave's sixteen
+    const uint32_t k_at = (uint32_t)((key & ~15) + (key >> 2 & 1) * 8 + (key >> 3 & 1) * 4 + (key & 3));      // the key's place in the order of the second product
+    const uint32_t k_to = (uint32_t)key * 256 + (uint32_t)(((F16 ? e : 4 * e) ^ (key & 15)) << 4);           // piece p of a key at p ^ (key % 16)
+    const int v_row = 64 * (word & 1) + 8 * (word >> 2) + 4 * (word >> 1 & 1);              // row of dimension 8 word; 8 word + 4 is 32 rows on
+    const uint32_t v_to = (uint32_t)(v_row * 128 + jj * 8 + ((piece ^ (v_row >> 1 & 7) ^ (v_row >> 4 & 1)) << 4));
 
     for (int r_tile = tile * kRows; r_tile < rows; r_tile += a.tiles * kRows) {
         const int r_end = r_tile + kRows < rows ? r_tile + kRows : rows;
-        const Steps steps = steps_of<6>(a, len - tokens.count + r_tile / a.group, len - tokens.count + (r_end - 1) / a.group);
+        const int tile_lowest = len - tokens.count + r_tile / a.group, tile_highest = len - tokens.count + (r_end - 1) / a.group;
+        const Steps steps = steps_of<6>(a, tile_lowest, tile_highest);
         const int s_begin = (int)((int64_t)steps.all * split / a.splits), s_end = (int)((int64_t)steps.all * (split + 1) / a.splits);
-        // the wave's rows
-        const int r0 = r_tile + 32 * wave, r = r0 + n;
-        const bool in = r < rows;
-        const int t = (in ? r : r_tile) / a.group, q_head = head * a.group + (in ? r : r_tile) - t * a.group;
-        const int place = in ? len - tokens.count + t : -1;
-        const int r_last = r0 + 31 < rows ? r0 + 31 : rows - 1;
-        const int lowest = r0 < rows ? len - tokens.count + r0 / a.group : -1, highest = r0 < rows ? len - tokens.count + r_last / a.group : -1;
+        const int last = s_end - 1;
+        auto position = [&](int s) INLINE { return steps.at(s < last ? s : last) * kStep; };        // (behind the last step the last again)
 
-        // the queries: lane (n, h) holds dimensions 16 s + 8 h .. + 7 of row n
-        u32x4 qf[8];
-        float qsum;
-        {
-            const u32x4* src = (const u32x4*)(a.q + (int64_t)(tokens.start + t) * a.q_stride + (int64_t)q_head * 128) + h;
+        // ALIGNED: page numbers of the wave's sixteen positions in the next 64 steps, a lane each, -1: none; a step takes its own by a lane's number
+        int page64 = -1, page64_from = 0;
+        auto fetch_pages = [&](int s) INLINE {
+            const int it = divided(position(s + lane) + 16 * wave, pages);
+            const int page = npages > 0 ? c.indices[p0 + (it < npages ? it : 0)] : -1;
+            page64 = it < npages && page < c.num_pages ? page : -1;
+            page64_from = s;
+        };
+        // slot of the first of the wave's sixteen positions (of page 0 where they are not there) and which of them are
+        auto slot_of = [&](int s, u32& mask) INLINE {
+            const int at = position(s) + 16 * wave;
+            const int page = __builtin_amdgcn_readlane(page64, (s < last ? s : last) - page64_from & 63);
+            const u32 entry = (u32)(at - divided(at, pages) * c.page_size);
+            const bool there = page >= 0 && entry < (u32)c.page_size;
+            const int left = len - at;
+            mask = !there || left <= 0 ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u;
+            return there ? page * page_slots + head_slots + entry : head_slots;
+        };
+        auto slot_of_lane = [&](int pos, bool& there) INLINE {    // pages of any size: every lane for itself
+            const int it = divided(pos, pages);
+            const u32 entry = (u32)(pos - it * c.page_size);
+            const bool inside = pos < len && it < npages && entry < (u32)c.page_size;
+            const int page = npages > 0 ? c.indices[p0 + (inside ? it : 0)] : -1;
+            there = inside && page >= 0 && page < c.num_pages;
+            return there ? page * page_slots + head_slots + entry : head_slots;
+        };
+        auto mask_of = [&](bool there) INLINE {                   // of a bool that the four lanes of a key share
+            const uint64_t lanes = __builtin_amdgcn_ballot_w64(there);
+            u32 mask = 0;
 #pragma unroll
-            for (int s = 0; s < 8; ++s) qf[s] = in ? src[2 * s] : u32x4{0, 0, 0, 0};
-            if (a.q_had) {
+            for (int i = 0; i < 16; ++i) mask |= (u32)(lanes >> (4 * i) & 1) << i;
+            return mask;
+        };
+        auto fetch_keys = [&](KeyCodes<F16>& f, int s) INLINE {
+            if (ALIGNED) {
+                const int64_t base = slot_of(s, f.mask);
+                const uint8_t* const kd = c.data + base * VEC;
+                uint32_t off = (uint32_t)(lane >> 2) * VEC + (uint32_t)e * 16, p_off = (uint32_t)(lane >> 2) * 4;
+                asm volatile("" : "+v"(off), "+v"(p_off));                         // (32-bit offsets behind wave-uniform addresses)
+#pragma unroll
+                for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[i] = *(const u32x4*)(kd + off + 64 * i);
+                if (!F16) f.p = *(const u32*)((const uint8_t*)(c.param + base) + p_off);
+            } else {
+                bool there;
+                const int64_t base = slot_of_lane(position(s) + key, there);
+                f.mask = mask_of(there);
+                const uint8_t* const kd = c.data + base * VEC + e * 16;
+#pragma unroll
+                for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[i] = *(const u32x4*)(kd + 64 * i);
+                if (!F16) f.p = c.param[base];
+            }
+        };
+        auto fetch_values = [&](ValueCodes<F16>& f, int s) INLINE {
+            if (ALIGNED) {
+                const int64_t base = slot_of(s, f.mask) + kv_slots;
+                const uint8_t* const vd = c.data + base * VEC;
+                const uint8_t* const vp = (const uint8_t*)(c.param + base);
+                uint32_t off = (uint32_t)first_of_four * VEC + (uint32_t)word * (VEC / 16), p_off = (uint32_t)first_of_four * 4, own = (uint32_t)(lane >> 2) * 4;
+                asm volatile("" : "+v"(off), "+v"(p_off), "+v"(own));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (F16) f.v4[i] = *(const u32x4*)(vd + off + VEC * i);
+                    else f.v[i] = *(const u32*)(vd + off + VEC * i), f.scales[i] = *(const u32*)(vp + p_off + 4 * i);
+                }
+                if (!F16) f.p = *(const u32*)(vp + own);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bool there;
+                    const int64_t slot = slot_of_lane(position(s) + 16 * wave + first_of_four + i, there) + kv_slots;
+                    const uint8_t* const vd = c.data + slot * VEC + word * (VEC / 16);
+                    if (F16) f.v4[i] = *(const u32x4*)vd;
+                    else f.v[i] = *(const u32*)vd, f.scales[i] = c.param[slot];
+                }
+                bool there;
+                const int64_t own = slot_of_lane(position(s) + key, there) + kv_slots;
+                f.mask = mask_of(there);
+                if (!F16) f.p = c.param[own];
+            }
+        };
+        // pieces of the unpacking, small enough to stand between matrix instructions; kbuf, vbuf: offsets in LDS
+        auto place_key = [&](const KeyCodes<F16>& f, uint32_t kbuf, int i) INLINE {
+            *(u32x4*)(lds + ((k_to ^ (uint32_t)(F16 ? i << 6 : i << 4)) + kbuf)) = F16 ? f.k[F16 ? i : 0] : codes_of(f.k[0][i]);
+        };
+        auto place_key_parameters = [&](const KeyCodes<F16>& f, uint32_t kbuf) INLINE {
+            if (!F16) {
+                const f16x2 p = as_f16x2(f.p);
+                const float zero = (float)p[1], zero_hi = top(zero), zero_lo = zero - zero_hi;
+                const u32 hi2 = tops(zero_hi, zero_hi), lo2 = tops(zero_lo, zero_lo);
+                if (e == 0) {
+                    *(float*)(lds + (kbuf + kSlope + k_at * 4)) = (float)p[0] * (kLog2e * kScale * kCodeUnit);
+                    *(u32x4*)(lds + (kbuf + kLine + (uint32_t)key * 16)) = u32x4{hi2, tops(zero_hi, zero_lo), lo2, 0x3F803F80u};
+                }
+            }
+            if (lane == 0) *(unsigned short*)(lds + (kbuf + kThere + 2 * wave)) = (unsigned short)f.mask;
+        };
+        auto store_values = [&](uint32_t vbuf, int half, const u32 (&out)[4][2]) INLINE {             // rows v_row + 32 half + i
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(u32x2*)(lds + ((v_to ^ (uint32_t)((i >> 1) << 4)) + vbuf + half * 4096 + i * 128)) = u32x2{out[i][0], out[i][1]};
+        };
+        auto place_value = [&](const ValueCodes<F16>& f, uint32_t vbuf, int half, const u32* power) INLINE {         // dimensions 8 word + 4 half ..
+            u32 out[4][2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (F16) {
+                    const u32x4 x = f.v4[F16 ? 2 * k : 0], y = f.v4[F16 ? 2 * k + 1 : 0];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        out[2 * i][k] = __builtin_amdgcn_perm(y[2 * half + i], x[2 * half + i], 0x05040100u);
+                        out[2 * i + 1][k] = __builtin_amdgcn_perm(y[2 * half + i], x[2 * half + i], 0x07060302u);
+                    }
+                } else {
+                    const u32x4 w = scaled_codes(__builtin_amdgcn_perm(f.v[F16 ? 0 : 2 * k + 1], f.v[F16 ? 0 : 2 * k], half ? 0x07060302u : 0x05040100u), power[k]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) out[i][k] = w[i];
+                }
+            }
+            store_values(vbuf, half, out);
+        };
+        auto place_value_parameters = [&](u32 p, u32 odd, uint32_t vbuf) INLINE {                     // p: of the position with the key's number
+            if (!F16) {
+                const f16x2 v = as_f16x2(p);
+                const float factor = factor_of((float)v[0], power_of((float)v[0])), recip = __builtin_amdgcn_rcpf(factor), zero = (float)v[1] * recip;
+                const f16 recip_hi = (f16)recip, zero_hi = (f16)zero;
+                if (e == 0) {
+                    *(f16*)(lds + (vbuf + kFactor + k_at * 2)) = (f16)factor;
+                    uint8_t* const extra_rows = lds + (vbuf + 128 * 128 + k_at * 2);
+                    *(f16*)extra_rows = recip_hi, *(f16*)(extra_rows + 128) = (f16)((recip - (float)recip_hi) * 2048.f);
+                    *(f16*)(extra_rows + 256) = zero_hi, *(f16*)(extra_rows + 384) = (f16)((zero - (float)zero_hi) * 2048.f);
+                }
+            }
+            if (lane == 0) *(unsigned short*)(lds + (vbuf + kOdd + 2 * wave)) = (unsigned short)odd;
+        };
+        // 2^e of the four positions' scales in pairs; whether the short way is right for all of the wave's positions (fp16 pages: only where all of the tile's
+        // rows see them)
+        auto regular = [&](const ValueCodes<F16>& f, u32* power, bool all_see) INLINE {
+            if (F16) return f.mask == 0xFFFFu && all_see;
+            bool plain = !strange(f.p);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) power[k] = powers_of(f.scales[F16 ? 0 : 2 * k], f.scales[F16 ? 0 : 2 * k + 1], plain);
+            return f.mask == 0xFFFFu && __builtin_amdgcn_ballot_w64(!plain) == 0;
+        };
+        // any values: positions that are not there count as zero, those whose parameters are not finite (fp16 pages: their entries that are not) as well, and are
+        // marked
+        auto place_values_any = [&](const ValueCodes<F16>& f, uint32_t vbuf) INLINE {
+            auto there = [&](int i) { return (f.mask >> (first_of_four + i) & 1) != 0; };
+            if (F16) {
+                ValueCodes<F16> g = f;
+                u32 odd = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    bool any = false;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const u32 w = there(i) ? (u32)f.v4[F16 ? i : 0][j] : 0u;
+                        any = any || strange(w);
+                        g.v4[F16 ? i : 0][j] = ((w & 0x7C00u) == 0x7C00u ? 0u : w & 0xFFFFu) | ((w & 0x7C000000u) == 0x7C000000u ? 0u : w & 0xFFFF0000u);
+                    }
+                    const uint64_t lanes = __builtin_amdgcn_ballot_w64(any);
+                    odd |= ((lanes & 0x55555555u) ? 1u << i : 0) | ((lanes & 0xAAAAAAAAu) ? 1u << (8 + i) : 0);
+                    odd |= ((lanes >> 32 & 0x55555555u) ? 1u << (4 + i) : 0) | ((lanes >> 32 & 0xAAAAAAAAu) ? 1u << (12 + i) : 0);
+                }
+                place_value_parameters(0, odd, vbuf);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) place_value(g, vbuf, half, nullptr);
+            } else {
+                u32 p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = !there(i) || strange(f.scales[F16 ? 0 : i]) ? kNoParameters : f.scales[F16 ? 0 : i];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    u32 out[4][2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const u32x4 w = scaled_codes_slow(__builtin_amdgcn_perm(f.v[F16 ? 0 : 2 * k + 1], f.v[F16 ? 0 : 2 * k], half ? 0x07060302u : 0x05040100u), p[2 * k], p[2 * k + 1]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) out[i][k] = w[i];
+                    }
+                    store_values(vbuf, half, out);
+                }
+                const bool mine = (f.mask >> (lane >> 2) & 1) != 0, odd = mine && strange(f.p);
+                place_value_parameters(mine && !odd ? f.p : kNoParameters, mask_of(odd), vbuf);
+            }
+        };
+
+        // the wave's rows: block cb has rows r0 + 32 cb + n
+        const int r0 = r_tile + 64 * wave;
+        const int r_last = r0 + 63 < rows ? r0 + 63 : rows - 1;
+        const int lowest = r0 < rows ? len - tokens.count + r0 / a.group : -1, highest = r0 < rows ? len - tokens.count + r_last / a.group : -1;
+        auto row_of = [&](int cb) { return r0 + 32 * cb + n; };
+        auto token_of = [&](int cb) { return (row_of(cb) < rows ? row_of(cb) : r_tile) / a.group; };
+        auto head_of = [&](int cb, int token) { return head * a.group + (row_of(cb) < rows ? row_of(cb) : r_tile) - token * a.group; };
+        int place[2];
+
+        __syncthreads();                                   // (what never changes; the last tile's buffers)
+        KeyCodes<F16> fk;
+        ValueCodes<F16> fv;
+        if (s_begin < s_end) {
+            if (ALIGNED) fetch_pages(s_begin);
+            fetch_keys(fk, s_begin);
+            fetch_values(fv, s_begin);
+        }
+
+        // the queries: lane (n, h) holds dimensions 16 s + 8 h .. + 7 of its rows
+        u32x4 qf[2][8], line[2];                           // line: the logits' line, {-zero-point slope in three pieces, twice; the maximum's}
+        float slope[2];
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) {
+            const bool in = row_of(cb) < rows;
+            const int token = token_of(cb);
+            place[cb] = in ? len - tokens.count + token : -1;
+            const u32x4* src = (const u32x4*)(a.q + (int64_t)(tokens.start + token) * a.q_stride + (int64_t)head_of(cb, token) * 128) + h;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) qf[cb][s] = in ? src[2 * s] : u32x4{0, 0, 0, 0};
+            if (__builtin_expect(a.q_had, 0)) {
                 float v[64];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const f16x2 p = as_f16x2(qf[i >> 2][i & 3]);
+                    const f16x2 p = as_f16x2(qf[cb][i >> 2][i & 3]);
                     v[2 * i] = (float)p[0], v[2 * i + 1] = (float)p[1];
                 }
 #pragma unroll
@@ -106,281 +341,311 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
                         }
 #pragma unroll
                 for (int i = 0; i < 64; ++i) {
-                    const u32x2 e = both_halves<32>(as_u32(v[i]));
-                    v[i] = h ? as_f32(e.x) - as_f32(e.y) : as_f32(e.x) + as_f32(e.y);
+                    const u32x2 w = both_halves<32>(as_u32(v[i]));
+                    v[i] = h ? as_f32(w.x) - as_f32(w.y) : as_f32(w.x) + as_f32(w.y);
                 }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) qf[i >> 2][i & 3] = narrow_f16x2(v[2 * i] * kScale, v[2 * i + 1] * kScale);
+                for (int i = 0; i < 32; ++i) qf[cb][i >> 2][i & 3] = narrow_f16x2(v[2 * i] * kScale, v[2 * i + 1] * kScale);
             }
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                const f16x2 p = as_f16x2(qf[i >> 2][i & 3]);
+                const f16x2 p = as_f16x2(qf[cb][i >> 2][i & 3]);
                 sum += (float)p[0] + (float)p[1];
             }
-            const u32x2 e = both_halves<32>(as_u32(sum));
-            qsum = as_f32(e.x) + as_f32(e.y);
+            const u32x2 w = both_halves<32>(as_u32(sum));
+            slope[cb] = (as_f32(w.x) + as_f32(w.y)) * -(kLog2e * kScale);
             if (!F16) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) qf[s] = query_for_codes(qf[s]);
+                for (int s = 0; s < 8; ++s) qf[cb][s] = query_for_codes(qf[cb][s]);
             }
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) asm volatile("" : "+a"(qf[0][i]), "+a"(qf[1][i]));       // (where they stay)
+        float most[2] = {0.f, 0.f}, m[2] = {0.f, 0.f}, limit[2] = {-3e38f, -3e38f}, poison[2] = {0.f, 0.f};         // limit: until a row has seen a position, any logit moves its maximum
+        auto draw_line = [&](int cb) INLINE {                     // lane half 0: slope pieces 1 2 3, 1 2 3, maximum pieces 1 2; half 1: piece 3
+            const float s1 = top(slope[cb]), s2 = top(slope[cb] - s1), s3 = slope[cb] - s1 - s2;
+            const float m1 = top(-m[cb]), m2 = top(-m[cb] - m1), m3 = -m[cb] - m1 - m2;
+            const u32x4 lower = {tops(s1, s2), tops(s3, s1), tops(s2, s3), tops(m1, m2)}, upper = {tops(m3, 0.f), 0, 0, 0};
+            line[cb] = h ? upper : lower;
+        };
+        draw_line(0), draw_line(1);
 
-        // ---- a step's way into LDS.  Thread (key, e) takes pieces 2 e, 2 e + 1 of a key; thread (four keys, word, half) four keys' values in dimensions
-        // 8 word + 4 half ..  The four keys are 32 kb + 16 tt + 8 jj + 4 hh ..: what lane half hh of the second product takes in step tt as its
-        // jj-th half.
-        const int key = tid >> 3, e = tid & 7;
-        const int jj = tid & 1, half = tid >> 1 & 1, word = tid >> 2 & 15, piece = tid >> 6;           // piece: 4 kb + 2 tt + hh
-        const int four = 32 * (piece >> 2) + 16 * (piece >> 1 & 1) + 8 * jj + 4 * (piece & 1);
-        const int v_row = 32 * (2 * (word & 1) + half) + 8 * (word >> 2) + 4 * (word >> 1 & 1);
-        auto slot_at = [&](int pos, bool& there) {
-            const int it = divided(pos, pages);
-            const u32 entry = (u32)(pos - it * c.page_size);
-            const bool inside = pos < len && it < npages && entry < (u32)c.page_size;
-            const int page = npages > 0 ? c.indices[p0 + (inside ? it : 0)] : -1;
-            there = inside && page >= 0 && page < c.num_pages;
-            return there ? page * page_slots + head_slots + entry : head_slots;
-        };
-        auto fetch = [&](Codes<F16>& f, int s) {
-            const int at = steps.at(s) * kStep;
-            // (a position that is not there reads the first ones of page 0)
-            if (ALIGNED) {
-                bool k_page, v_page;
-                const int v_at = at + 32 * (wave >> 2) + 16 * (wave >> 1 & 1);              // (piece is the wave's number)
-                const int64_t kb = slot_at(at + 8 * wave, k_page), vb = slot_at(v_at, v_page) + kv_slots;
-                const uint32_t k_lane = lane >> 3, v_lane = 8 * jj + 4 * (wave & 1);
-                f.k_there = k_page && at + key < len;
-                f.v_there = 0;
+        f32x16 acc[2][4], extra[2], x[2], y[2];            // y: the logits of the unit at work, then x those of the next
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f.v_there |= (v_page && v_at + (int)v_lane + i < len ? 1u : 0u) << i;
-                const uint8_t* const kd = c.data + kb * (F16 ? 256 : 64);
-                const uint8_t* const vd = c.data + vb * (F16 ? 256 : 64);
-                if (F16) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) f.k4[i] = *(const u32x4*)(kd + (k_lane * 256u + (uint32_t)e * 32u + 16u * i));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) f.v2[i] = *(const u32x2*)(vd + ((v_lane + i) * 256u + (uint32_t)(2 * word + half) * 8u));
-                } else {
-                    f.k2 = *(const u32x2*)(kd + (k_lane * 64u + (uint32_t)e * 8u));
-                    const uint8_t* const kp = (const uint8_t*)(c.param + kb);
-                    f.kp = *(const u32*)(kp + k_lane * 4u);
-                    f.vp = *(const u32*)((const uint8_t*)(c.param + kb + kv_slots) + k_lane * 4u);
-                    const uint8_t* const vp = (const uint8_t*)(c.param + vb);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        f.v1[i] = *(const unsigned short*)(vd + ((v_lane + i) * 64u + (uint32_t)(2 * word + half) * 2u));
-                        f.scales[i] = *(const u32*)(vp + (v_lane + i) * 4u);
-                    }
-                }
-            } else {
-                const int64_t ks = slot_at(at + key, f.k_there);
-                if (F16) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) f.k4[i] = ((const u32x4*)c.data)[ks * 16 + 2 * e + i];
-                } else {
-                    f.k2 = ((const u32x2*)c.data)[ks * 8 + e];
-                    f.kp = c.param[ks], f.vp = c.param[ks + kv_slots];
-                }
-                f.v_there = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    bool there;
-                    const int64_t vs = slot_at(at + four + i, there) + kv_slots;
-                    f.v_there |= (there ? 1u : 0u) << i;
-                    if (F16) {
-                        f.v2[i] = ((const u32x2*)c.data)[vs * 32 + 2 * word + half];
-                    } else {
-                        f.v1[i] = ((const unsigned short*)c.data)[vs * 32 + 2 * word + half];
-                        f.scales[i] = c.param[vs];
-                    }
-                }
-            }
-        };
-        auto place_codes = [&](const Codes<F16>& f, uint8_t* buf) {
-            // the key: piece p of 16 at p ^ (key % 16)
-            u32x4* const krow = (u32x4*)(buf + kKeys + key * 256);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                krow[(2 * e + i) ^ (key & 15)] = F16 ? f.k4[i] : codes_of(f.k2[i]);
-            }
-            const int k_at = (key >> 5) * 32 + (key >> 4 & 1) * 16 + (key >> 2 & 1) * 8 + (key >> 3 & 1) * 4 + (key & 3);       // its place in the order of the second product
-            if (!F16) {
-                const f16x2 p = as_f16x2(f.kp), v = as_f16x2(f.k_there ? f.vp : kNoParameters);
-                const float factor = factor_of((float)v[0], power_of((float)v[0])), recip = __builtin_amdgcn_rcpf(factor), zero = (float)v[1] * recip;
-                const f16 recip_hi = (f16)recip, zero_hi = (f16)zero;
-                if (e == 0) {
-                    ((float*)(buf + kSlope))[k_at] = (float)p[0] * (kLog2e * kScale * kCodeUnit);
-                    ((float*)(buf + kOffset))[k_at] = (float)p[1] * -(kLog2e * kScale);
-                    ((f16*)(buf + kFactor))[k_at] = (f16)factor;
-                    f16* const extra_rows = (f16*)(buf + kValues + 128 * 128) + k_at;
-                    extra_rows[0] = recip_hi, extra_rows[64] = (f16)(recip - (float)recip_hi);
-                    extra_rows[128] = zero_hi, extra_rows[192] = (f16)(zero - (float)zero_hi);
-                }
-            }
-            {
-                const uint64_t there = __builtin_amdgcn_ballot_w64(f.k_there);
-                if (lane == 0) {
-                    uint32_t bits = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) bits |= (uint32_t)(there >> (8 * i) & 1) << i;
-                    buf[kThere + wave] = (uint8_t)bits;
-                }
-            }
-            // the values: row v_row + i holds dimension 8 word + 4 half + i
-            uint8_t* const vrow = buf + kValues + v_row * 128 + jj * 8;
-            u32 out[4][2];
-            if (F16) {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    u32x2 x = f.v2[2 * k], y = f.v2[2 * k + 1];
-                    if (!(f.v_there >> (2 * k) & 1)) x = u32x2{0, 0};
-                    if (!(f.v_there >> (2 * k + 1) & 1)) y = u32x2{0, 0};
-                    out[0][k] = __builtin_amdgcn_perm(y.x, x.x, 0x05040100u);
-                    out[1][k] = __builtin_amdgcn_perm(y.x, x.x, 0x07060302u);
-                    out[2][k] = __builtin_amdgcn_perm(y.y, x.y, 0x05040100u);
-                    out[3][k] = __builtin_amdgcn_perm(y.y, x.y, 0x07060302u);
-                }
-            } else {
-                u32 vp[4], power[2];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vp[i] = (f.v_there >> i & 1) ? f.scales[i] : kNoParameters;
-                bool plain = true;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) power[k] = powers_of(vp[2 * k], vp[2 * k + 1], plain);
-                const u32 w[2] = {(u32)f.v1[0] | (u32)f.v1[1] << 16, (u32)f.v1[2] | (u32)f.v1[3] << 16};
-                if (__builtin_amdgcn_ballot_w64(!plain) == 0) {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const u32x4 scaled = scaled_codes(w[k], power[k]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) out[i][k] = scaled[i];
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const u32x4 scaled = scaled_codes_slow(w[k], vp[2 * k], vp[2 * k + 1]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) out[i][k] = scaled[i];
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = v_row + i;
-                *(u32x2*)(vrow + i * 128 + ((piece ^ (row >> 1 & 7) ^ (row >> 5 & 1)) << 4)) = u32x2{out[i][0], out[i][1]};
-            }
+        for (int cb = 0; cb < 2; ++cb) acc[cb][0] = acc[cb][1] = acc[cb][2] = acc[cb][3] = extra[cb] = zeros();
+        u32x4 p[2][2];                                     // weights: [rows][half unit]
+
+        const uint32_t k_from = n * 256 + ((uint32_t)(h ^ (n & 15)) << 4), v_from = n * 128 + ((uint32_t)(h ^ (n >> 1 & 7) ^ (n >> 4)) << 4);
+        const uint32_t e_from = (128 + (n < 4 ? n : 4)) * 128 + h * 16, l_from = kLine + h * 1024 + n * 16, s_from = kSlope + h * 32;
+        auto key_piece = [&](uint32_t kbuf, int kb, int i) INLINE { return *(const u32x4*)(lds + ((k_from + kbuf ^ (uint32_t)(i << 5)) + kb * 8192)); };
+        auto value_piece = [&](uint32_t vbuf, int chunk, int db) INLINE {
+            return db < 4 ? *(const u32x4*)(lds + ((v_from + vbuf ^ (uint32_t)(chunk << 5)) + db * 4096)) : *(const u32x4*)(lds + (e_from + vbuf + chunk * 32));
         };
 
-        f32x16 acc[4], extra;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[0][i] = acc[1][i] = acc[2][i] = acc[3][i] = extra[i] = 0.f;
-        float m = 0.f, limit = -3e38f;                     // (until the row has seen a position, any logit moves its maximum)
-
-        auto consume = [&](const uint8_t* buf, int s) {
-            const int at = steps.at(s) * kStep;
-            if (at > highest) return;                      // (nothing in it for this wave's rows)
-            const uint64_t there = *(const uint64_t*)(buf + kThere);
-            const bool whole = at + kStep - 1 <= lowest && (a.window == 0 || at > highest - a.window || at + kStep - 1 < a.sinks) && ~there == 0;
-            f32x16 x[2];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[0][i] = x[1][i] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const u32x4 k = ((const u32x4*)(buf + kKeys + (32 * kb + n) * 256))[(2 * i + h) ^ (n & 15)];
-                    x[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, qf[i]), x[kb], 0, 0, 0);
-                }
-            // logits less the running maximum, base 2; register 8 tt + j of half h is place 32 kb + 16 tt + 8 h + j of the second product's order
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const f32x4* slope = (const f32x4*)(buf + kSlope) + 8 * kb + 4 * tt + 2 * h;
-                    const f32x4* offset = (const f32x4*)(buf + kOffset) + 8 * kb + 4 * tt + 2 * h;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        if (F16) x[kb][8 * tt + j] = __builtin_fmaf(x[kb][8 * tt + j], kLog2e * kScale, -m);
-                        else x[kb][8 * tt + j] = __builtin_fmaf(x[kb][8 * tt + j], slope[j >> 2][j & 3], __builtin_fmaf(offset[j >> 2][j & 3], qsum, -m));
-                    }
-                }
+        auto sees = [&](int cb, int pos) INLINE { return pos <= place[cb] && (a.window == 0 || pos > place[cb] - a.window || pos < a.sinks); };
+        // what rows do not see of the next unit's logits; whether a maximum has to be raised
+        u32 there = 0;                                     // of the next unit
+        auto settle = [&](int at) INLINE {
+            const u32 all = __builtin_amdgcn_readfirstlane(there);
+            const bool whole = at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks) && ~all == 0;
             if (!whole) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int cb = 0; cb < 2; ++cb) {
+                    most[cb] = -__builtin_inff();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int k = 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3), pos = at + k;
-                        const bool sees = pos <= place && (a.window == 0 || pos > place - a.window || pos < a.sinks) && (there >> k & 1);
-                        x[kb][i] = sees ? x[kb][i] : -__builtin_inff();
+                        const int k = 8 * (i >> 2) + 4 * h + (i & 3);
+                        y[cb][i] = sees(cb, at + k) && (all >> k & 1) ? y[cb][i] : -__builtin_inff();
+                        most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
                     }
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, __builtin_fmaxf(x[0][i], x[1][i]));
-            if (__builtin_amdgcn_ballot_w64(top > limit)) {
-                const u32x2 both = both_halves<32>(as_u32(top));
-                top = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
-                const bool moves = top > (limit < 0.f ? limit : 0.f);
-                const float by = moves ? top : 0.f, keep = __builtin_amdgcn_exp2f(-by);
-                limit = moves ? kGrow : limit;
-                m += by;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[0][i] -= by, x[1][i] -= by;
-                    acc[0][i] *= keep, acc[1][i] *= keep, acc[2][i] *= keep, acc[3][i] *= keep, extra[i] *= keep;
                 }
             }
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const int piece_at = 4 * kb + 2 * tt + h;
-                    u32x4 packed;
-                    const u32x4 factor = F16 ? u32x4{} : *(const u32x4*)(buf + kFactor + piece_at * 16);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float w0 = __builtin_amdgcn_exp2f(x[kb][8 * tt + 2 * j]), w1 = __builtin_amdgcn_exp2f(x[kb][8 * tt + 2 * j + 1]);
-                        packed[j] = F16 ? cvt_f16x2(w0, w1) : scaled_pair(w0, w1, factor[j]);
+            return __builtin_amdgcn_ballot_w64(most[0] > limit[0] || most[1] > limit[1]) != 0;
+        };
+        // Marked positions of the unit at work.  Int4 pages: rows that see one become NaN.  Fp16 pages: its entries that are not finite are added for the rows that
+        // see it, by a product of bf16 powers of two that overflows to an infinity (a NaN: to one of each sign).
+        u32 odd = 0;
+        auto mark = [&](int at) INLINE {
+            const u32 bits = __builtin_amdgcn_readfirstlane(odd);
+            if (__builtin_expect(bits != 0, 0)) {
+#pragma unroll 1
+                for (int k = 0; k < 32; ++k) {
+                    if (!(bits >> k & 1)) continue;
+                    if (!F16) {
+                        poison[0] = sees(0, at + k) ? __builtin_nanf("") : poison[0];
+                        poison[1] = sees(1, at + k) ? __builtin_nanf("") : poison[1];
+                        continue;
                     }
-                    const f16x8 p = __builtin_bit_cast(f16x8, packed);
+                    bool there;
+                    const unsigned short* const v = (const unsigned short*)(c.data + (slot_of_lane(at + k, there) + kv_slots) * VEC) + 32 * (n >> 3) + 16 * (n >> 2 & 1) + (n & 3);
+                    const u32x4 seen[2] = {{h == 0 && sees(0, at + k) ? 0x7F00u : 0u, 0, 0, 0}, {h == 0 && sees(1, at + k) ? 0x7F00u : 0u, 0, 0, 0}};
 #pragma unroll
                     for (int db = 0; db < 4; ++db) {
-                        const u32x4 v = ((const u32x4*)(buf + kValues + (32 * db + n) * 128))[piece_at ^ (n >> 1 & 7) ^ (db & 1)];
-                        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), p, acc[db], 0, 0, 0);
+                        const u32 bf = v[4 * db], sign = bf & 0x8000u;
+                        const bool nan = (bf & 0x7FFFu) > 0x7C00u, inf = (bf & 0x7FFFu) == 0x7C00u;
+                        const u32x4 up = {h == 0 && (nan || (inf && !sign)) ? 0x7F00u : 0u, 0, 0, 0}, down = {h == 0 && (nan || (inf && sign)) ? 0xFF00u : 0u, 0, 0, 0};
+#pragma unroll
+                        for (int cb = 0; cb < 2; ++cb) {
+                            mfma_overflow(acc[cb][db], up, seen[cb]);
+                            mfma_overflow(acc[cb][db], down, seen[cb]);
+                        }
                     }
-                    const u32x4 v = ((const u32x4*)(buf + kValues + (128 + (n < 4 ? n : 4)) * 128))[piece_at];
-                    extra = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), p, extra, 0, 0, 0);
                 }
+            }
+        };
+        auto raise = [&]() INLINE {
+#pragma unroll
+            for (int cb = 0; cb < 2; ++cb) {
+                const u32x2 both = both_halves<32>(as_u32(most[cb]));
+                const float now = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
+                const bool moves = now > (limit[cb] < 0.f ? limit[cb] : 0.f);
+                const float by = moves ? now : 0.f, keep = __builtin_amdgcn_exp2f(-by);
+                limit[cb] = moves ? kGrow : limit[cb];
+                m[cb] += by;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[cb][i] -= by;
+#pragma unroll
+                for (int k = 0; k < 5; ++k) {
+                    f32x16& block = k < 4 ? acc[cb][k & 3] : extra[cb];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) block[i] *= keep;
+                }
+                draw_line(cb);
+            }
+        };
+        // two weights of half unit tt: registers 8 tt + 2 j, + 1
+        auto weights = [&](const f32x16& v, u32x4 factors, int tt, int j) INLINE {
+            const float w0 = __builtin_amdgcn_exp2f(v[8 * tt + 2 * j]), w1 = __builtin_amdgcn_exp2f(v[8 * tt + 2 * j + 1]);
+            return F16 ? cvt_f16x2(w0, w1) : scaled_pair(w0, w1, factors[j]);
+        };
+        // First product of unit kb of the keys at kbuf into x; between it the weights of the unit at work, unit `unit` of the values at vbuf.  Operands come from
+        // LDS three slots ahead.
+        u32x4 kp[3], vp[3], ln, factors[2];
+        f32x4 slopes[4];
+        auto ask_keys = [&](uint32_t kbuf, int kb) INLINE {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) kp[i] = key_piece(kbuf, kb, i);
+        };
+        auto ask_factors = [&](uint32_t vbuf, int unit) INLINE {
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) factors[tt] = F16 ? u32x4{} : *(const u32x4*)(lds + (vbuf + kFactor + h * 16) + (4 * unit + 2 * tt) * 16);
+        };
+        auto ask_line = [&](uint32_t kbuf, int kb) INLINE {
+            if (F16) return;
+            ln = *(const u32x4*)(lds + (l_from + kbuf) + kb * 512);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) slopes[i] = *(const f32x4*)(lds + (s_from + kbuf) + kb * 128 + (i >> 1) * 64 + (i & 1) * 16);
+        };
+        auto first_product = [&](uint32_t kbuf, int kb, uint32_t vbuf, int unit, bool with_weights, auto&& other) INLINE {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int cb = 0; cb < 2; ++cb) {
+                    if (i == 0) mfma_first(x[cb], kp[i % 3], qf[cb][i]);
+                    else mfma_more(x[cb], kp[i % 3], qf[cb][i]);
+                    if (with_weights) p[cb][i >> 2][i & 3] = weights(y[cb], factors[i >> 2], i >> 2, i & 3);
+                    if (cb == 0) other(i);
+                    if (cb == 1 && i < 5) kp[i % 3] = key_piece(kbuf, kb, i + 3);
+                    if (cb == 1 && i == 5) ask_line(kbuf, kb);
+                    if (cb == 0 && i > 4) vp[i - 5] = value_piece(vbuf, 2 * unit, i - 5);
+                    SLOT;
+                }
+            }
+        };
+        // Second product of the unit at work; between it the logits of the next one, unit next_kb of the keys at kbuf, from its first product and their line,
+        // and their maxima.
+        auto second_product = [&](uint32_t vbuf, int unit, uint32_t kbuf, int next_kb, auto&& other) INLINE {
+            f32x16 t[2];
+            if (!F16) {
+                mfma_line(t[0], ln, line[0]);
+                mfma_line(t[1], ln, line[1]);
+                SLOT;
+            }
+            there = *(const u32*)(lds + (kbuf + kThere) + 4 * next_kb);
+            odd = *(const u32*)(lds + (vbuf + kOdd) + 4 * unit);
+#pragma unroll
+            for (int i = 0; i < 10; ++i) {
+                const int tt = i / 5, db = i % 5;
+#pragma unroll
+                for (int cb = 0; cb < 2; ++cb) {
+                    mfma_second(db < 4 ? acc[cb][db & 3] : extra[cb], vp[i % 3], p[cb][tt]);
+                    if (i > 1) {
+                        const int reg = 2 * (i - 2);
+                        float y0 = F16 ? __builtin_fmaf(x[cb][reg], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][reg], slopes[reg >> 2][reg & 3], t[cb][reg]);
+                        float y1 = F16 ? __builtin_fmaf(x[cb][reg + 1], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][reg + 1], slopes[reg >> 2][(reg & 3) + 1], t[cb][reg + 1]);
+                        most[cb] = i == 2 ? __builtin_fmaxf(y0, y1) : __builtin_fmaxf(__builtin_fmaxf(most[cb], y0), y1);
+                        asm volatile("" : "+v"(y0), "+v"(y1), "+v"(most[cb]));         // (here, not where they are used)
+                        y[cb][reg] = y0, y[cb][reg + 1] = y1;
+                    }
+                    if (cb == 1 && i < 7) vp[i % 3] = value_piece(vbuf, 2 * unit + (i + 3) / 5, (i + 3) % 5);
+                    if (cb == 1) other(i);
+                    SLOT;
+                }
+            }
         };
 
-        __syncthreads();                                   // (the rows above; the last tile's buffers)
-        Codes<F16> f;
+        // offsets in LDS: this step's keys, the next one's and those of the step behind it; this step's values and the next one's
+        uint32_t k0 = 0, k1 = kKeys, k2 = 2 * kKeys, v0 = 3 * kKeys, v1 = 3 * kKeys + kValues;
+        bool grow = false;
+        int s = s_begin;
         if (s_begin < s_end) {
-            fetch(f, s_begin);
-            place_codes(f, lds);
-            fetch(f, s_begin + 1 < s_end ? s_begin + 1 : s_begin);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) place_key(fk, k0, i);
+            place_key_parameters(fk, k0);
+            place_values_any(fv, v0);
+            fetch_keys(fk, s_begin + 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) place_key(fk, k1, i);
+            place_key_parameters(fk, k1);
+            fetch_keys(fk, s_begin + 2);
         }
         __syncthreads();
-        for (int s = s_begin; s < s_end; ++s) {
-            uint8_t* const buf = lds + (s - s_begin & 1) * kBuffer;
-            uint8_t* const other = lds + (s - s_begin + 1 & 1) * kBuffer;
-            if (s + 1 < s_end) {
-                place_codes(f, other);
-                fetch(f, s + 2 < s_end ? s + 2 : s + 1);
+        if (s_begin < s_end) {
+            ask_keys(k0, 0);
+            first_product(k0, 0, v0, 0, false, [](int) {});
+            f32x16 t[2];
+            if (!F16) {
+                mfma_line(t[0], ln, line[0]);
+                mfma_line(t[1], ln, line[1]);
             }
-            consume(buf, s);
+            there = *(const u32*)(lds + k0 + kThere);
+            settled();
+#pragma unroll
+            for (int cb = 0; cb < 2; ++cb) {
+                most[cb] = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float slope_i = F16 ? 0.f : *(const float*)(lds + s_from + k0 + (i >> 3) * 64 + (i & 7) * 4);
+                    y[cb][i] = F16 ? __builtin_fmaf(x[cb][i], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][i], slope_i, t[cb][i]);
+                    most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
+                }
+            }
+            grow = settle(position(s_begin));
+            ask_keys(k0, 1);
+            ask_factors(v0, 0);
+        }
+        // Units of 32 positions, two to a step.  (A wave whose rows see none of them goes through them all the same: it would wait for the others.)
+        auto first_unit = [&]() INLINE {
+            first_product(k0, 1, v0, 0, true, [&](int i) {
+                if (i == 2) fetch_values(fv, s + 1);
+            });
+            second_product(v0, 0, k0, 1, [&](int i) {
+                if (i >= 2 && i < 6) place_key(fk, k2, i - 2);
+                if (i == 7) place_key_parameters(fk, k2);
+                if (i == 8) ask_factors(v0, 1);
+                if (i == 9) ask_keys(k1, 0);
+            });
+            mark(position(s));
+            grow = settle(position(s) + 32);
+        };
+        auto second_unit = [&]() INLINE {
+            u32 power[2];
+            bool usual = false;
+            first_product(k1, 0, v0, 1, true, [&](int i) {
+                if (i == 2) fetch_keys(fk, s + 3);
+            });
+            const int at_next = position(s + 1);
+            usual = regular(fv, power, at_next + 63 <= tile_lowest && (a.window == 0 || at_next > tile_highest - a.window || at_next + 63 < a.sinks));
+            second_product(v0, 1, k1, 0, [&](int i) {
+                if (i == 3 || i == 5) place_value(fv, v1, i == 5, power);
+                if (i == 7) place_value_parameters(fv.p, 0, v1);
+                if (i == 9) ask_keys(k1, 1);
+            });
+            if (__builtin_expect(!usual, 0)) place_values_any(fv, v1);
+            mark(position(s) + 32);
+            ++s;
+            if (ALIGNED && __builtin_expect(s + 3 - page64_from >= 64, 0)) fetch_pages(s);
             __syncthreads();
+            const uint32_t k = k0, v = v0;
+            k0 = k1, k1 = k2, k2 = k, v0 = v1, v1 = v;
+            ask_factors(v0, 0);
+            grow = s < s_end && settle(position(s));
+        };
+        // Raising maxima changes accumulators, which only matrix instructions touch otherwise: that is done outside the inner loop, or they would be moved between
+        // the halves of the register file in every turn.  It is rare behind a row's first positions.
+        bool middle = false;
+        for (;;) {
+            if (__builtin_expect(grow, 1)) {
+                settled();
+                raise();
+            }
+            grow = false;
+            if (middle) {
+                second_unit();
+                middle = false;
+                if (grow) continue;
+            }
+            while (s < s_end) {
+                first_unit();
+                if (__builtin_expect(grow, 0)) {
+                    middle = true;
+                    break;
+                }
+                second_unit();
+                if (__builtin_expect(grow, 0)) break;
+            }
+            if (!grow) break;
         }
 
+        settled();
         // rows 0 .. 3 of the extra block, in the registers of the lower half: sums of weights (as pairs) and of weights times zero points
-        float sum = F16 ? extra[0] : extra[0] + extra[1], zero = F16 ? 0.f : extra[2] + extra[3];
-        sum = as_f32(both_halves<32>(as_u32(sum)).x);
-        if (!F16) zero = as_f32(both_halves<32>(as_u32(zero)).x);
-        if (in) {
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) {
+            float sum = F16 ? extra[cb][0] : __builtin_fmaf(extra[cb][1], 1.f / 2048.f, extra[cb][0]);
+            float zero = F16 ? 0.f : __builtin_fmaf(extra[cb][3], 1.f / 2048.f, extra[cb][2]);
+            sum = as_f32(both_halves<32>(as_u32(sum)).x);
+            if (!F16) {
+                zero = as_f32(both_halves<32>(as_u32(zero)).x);
+                const u32x2 both = both_halves<32>(as_u32(poison[cb]));
+                sum += as_f32(both.x) + as_f32(both.y);
+            }
+            if (row_of(cb) >= rows) continue;
+            const int token = token_of(cb), q_head = head_of(cb, token);
             // lane (n, h): dimensions 32 i + 16 h + 4 db + j of row n in register 4 i + j of block db
             if (a.splits == 1) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                u32x4* const dst = (u32x4*)(a.o + (int64_t)(tokens.start + t) * a.o_stride + (int64_t)q_head * 128) + 2 * h;
+                u32x4* const dst = (u32x4*)(a.o + (int64_t)(tokens.start + token) * a.o_stride + (int64_t)q_head * 128) + 2 * h;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -389,18 +654,19 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int db = 2 * k + (j >> 1), reg = 4 * i + 2 * (j & 1);
-                            w[j] = cvt_f16x2((acc[db][reg] - zero) * inv, (acc[db][reg + 1] - zero) * inv);
+                            w[j] = cvt_f16x2((acc[cb][db][reg] - zero) * inv, (acc[cb][db][reg + 1] - zero) * inv);
                         }
                         dst[4 * i + k] = w;
                     }
             } else {
-                float* const dst = a.part + (((int64_t)(tokens.start + t) * (c.num_heads * a.group) + q_head) * a.splits + split) * 132;
-                if (h == 0) dst[0] = limit < 0.f ? kEmpty : m, dst[1] = sum;
+                float* const dst = a.part + (((int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head) * a.splits + split) * 132;
+                if (h == 0) dst[0] = limit[cb] < 0.f ? kEmpty : m[cb], dst[1] = sum;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int db = 0; db < 4; ++db)
-                        *(f32x4*)(dst + 4 + 32 * i + 16 * h + 4 * db) = f32x4{acc[db][4 * i] - zero, acc[db][4 * i + 1] - zero, acc[db][4 * i + 2] - zero, acc[db][4 * i + 3] - zero};
+                        *(f32x4*)(dst + 4 + 32 * i + 16 * h + 4 * db) =
+                            f32x4{acc[cb][db][4 * i] - zero, acc[cb][db][4 * i + 1] - zero, acc[cb][db][4 * i + 2] - zero, acc[cb][db][4 * i + 3] - zero};
             }
         }
     }
@@ -408,15 +674,13 @@ __global__ __launch_bounds__(512, 2) void chunk_tiles_kernel(Chunk a, Divisor pa
 
 }  // namespace
 
-int qr_internal_chunk_tiles(bool fp16, const Chunk& a, int64_t groups, hipStream_t st) {
+int qr_internal_chunk_tiles(bool fp16, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st) {
     using Kernel = void (*)(Chunk, Divisor);
     const bool aligned = a.c.page_size % 16 == 0;
     const Kernel kernel = fp16 ? (aligned ? chunk_tiles_kernel<true, true> : chunk_tiles_kernel<true, false>)
                                : (aligned ? chunk_tiles_kernel<false, true> : chunk_tiles_kernel<false, false>);
-    const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, 2 * kBuffer);
+    const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, kLds);
     if (e != hipSuccess) return (int)e;
-    const u32 log2 = a.c.page_size > 1 ? 64u - (u32)__builtin_clzll((unsigned long long)a.c.page_size - 1) : 0u;
-    const Divisor pages{(u32)(((1ull << (30 + log2)) + (uint64_t)a.c.page_size - 1) / (uint64_t)a.c.page_size), log2};
-    kernel<<<dim3((unsigned)groups), dim3(512), 2 * kBuffer, st>>>(a, pages);
+    kernel<<<dim3((unsigned)groups), dim3(256), kLds, st>>>(a, pages);
     return qr_launch_status();
 }

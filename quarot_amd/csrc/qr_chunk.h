@@ -45,6 +45,16 @@ __device__ __forceinline__ float quarters_max(float v) {
     return __builtin_fmaxf(as_f32(b.x), as_f32(b.y));
 }
 
+// n / d for n below 2^30: umulhi(4 n, inverse) >> shift
+struct Divisor {
+    u32 inverse, shift;
+};
+__device__ __forceinline__ int divided(int n, Divisor d) { return (int)(__umulhi((u32)n << 2, d.inverse) >> d.shift); }
+static inline Divisor divisor_of(int64_t d) {
+    const u32 log2 = d > 1 ? 64u - (u32)__builtin_clzll((unsigned long long)d - 1) : 0u;       // the least s for which 2^s reaches d
+    return Divisor{(u32)(((1ull << (30 + log2)) + (uint64_t)d - 1) / (uint64_t)d), log2};
+}
+
 // ---- int4 operands
 // The codes of a word as fp16 operands: pairs (0, 4), (1, 5), (2, 6), (3, 7).  A code in the lowest (next) four bits of a half is the subnormal number
 // code 2^-24 (code 2^-20), which the matrix instructions take exactly: no conversion.  The query's dimensions come in that order, those that meet an
@@ -72,6 +82,13 @@ __device__ __forceinline__ u32 powers_of(u32 w0, u32 w1, bool& plain) {
     const u32 p = __builtin_amdgcn_perm(w1, w0, 0x05040100u) & 0x7C007C00u;
     plain = plain && (p & 0xFFFFu) - 0x0400u <= 0x4C00u && (p >> 16) - 0x0400u <= 0x4C00u;
     return p;
+}
+// weight times factor -> fp16, rounded once: two weights, two factors (a pair of fp16 numbers)
+__device__ __forceinline__ u32 scaled_pair(float w0, float w1, u32 factors) {
+    u32 r;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0 op_sel_hi:[0,1,0]" : "=v"(r) : "v"(w0), "v"(factors));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(r) : "v"(w1), "v"(factors));
+    return r;
 }
 // w: four codes of one vector in the low half, of another in the high half -> code 2^e of both, code by code: (1024 + code) 2^e - 1024 2^e is exact
 __device__ __forceinline__ u32x4 scaled_codes(u32 w, u32 power) {
@@ -129,4 +146,4 @@ __device__ __forceinline__ Steps steps_of(const Chunk& a, int lowest, int highes
 }
 
 // chunk_tiles.hip
-int qr_internal_chunk_tiles(bool fp16, const Chunk& a, int64_t groups, hipStream_t st);
+int qr_internal_chunk_tiles(bool fp16, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st);

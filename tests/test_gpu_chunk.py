@@ -156,15 +156,22 @@ def test_one_token_per_sequence(page_size, lens, heads, group, window, sinks, f1
     check(specs, q, starts, lens, news, window=window, sinks=sinks)
 
 
+def scale_values(specs, seed):
+    """Values' parameters times powers of two from 2^-20 to 2^11."""
+    e = torch.randint(-20, 12, specs["kv_param"].shape[:-1], generator=torch.Generator().manual_seed(seed)).to(DEV)
+    specs["kv_param"][:, :, 1] *= torch.exp2(e.double()).half()[:, :, 1, ..., None]
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("news", [[40, 90], [10, 20]])
 @pytest.mark.parametrize("f16", [False, True])
-def test_large_logits_and_scales(f16):
-    """Softmaxes that a few positions decide, running maxima that grow by hundreds, and scales from 2^-20 to 2^12."""
-    lens, news = [600, 90], [40, 90]
-    specs, q, starts = make(5, 16, lens, news, 2, 2, f16, spread=12.0)
+def test_large_logits_and_scales(f16, news, seed):
+    """Softmaxes that a few positions decide, running maxima that grow by hundreds, and scales from 2^-24 to 2^10."""
+    lens = [600, 90]
+    specs, q, starts = make(5 + seed, 16, lens, news, 2, 2, f16, spread=12.0)
     check(specs, q, starts, lens, news)
     if not f16:
-        e = torch.randint(-20, 12, specs["kv_param"].shape[:-1], device=DEV)
-        specs["kv_param"][:, :, 1] *= torch.exp2(e.double()).half()[:, :, 1, ..., None]
+        scale_values(specs, seed)
         check(specs, q, starts, lens, news)
 
 
@@ -350,8 +357,7 @@ def test_many_rows_large_logits_scales_and_missing_pages():
     lens, news = [700], [400]
     specs, q, starts = make(21, 16, lens, news, 1, 2, spread=12.0)
     check(specs, q, starts, lens, news)
-    e = torch.randint(-20, 12, specs["kv_param"].shape[:-1], device=DEV)
-    specs["kv_param"][:, :, 1] *= torch.exp2(e.double()).half()[:, :, 1, ..., None]
+    scale_values(specs, 21)
     specs["kv_param"][:, :, 1, :, ::5, 0] = 0
     specs["kv_param"][:, :, 1, :, 1::5, 0] *= -1
     check(specs, q, starts, lens, news)
@@ -369,3 +375,39 @@ def test_many_rows_with_the_transform_inside(f16):
     call(apart, qh, **specs, layer_idx=1, seqlen_indptr=starts)
     call(o, q, **specs, layer_idx=1, seqlen_indptr=starts, q_hadamard=True)
     assert float((o - apart).double().norm() / apart.double().norm()) < 2.0 ** -10
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("lens,news,heads,group,window,sinks", [([70], [40], 2, 1, 0, 0), ([90, 33], [30, 33], 1, 4, 20, 3), ([300], [1], 2, 3, 100, 2),
+                                                                ([600], [400], 1, 2, 0, 0), ([900], [500], 1, 1, 70, 5)])
+def test_infinities_and_nans_reach_only_rows_that_see_them(lens, news, heads, group, window, sinks, f16):
+    """A key or a value that is no number, or infinite, at a position that some rows do not see (later, outside the window): those rows' results are as if
+    it were any other, bit for bit; a row that sees one of them is not finite in the dimensions concerned."""
+    specs, q, starts = make(30 + sum(lens), 16, lens, news, heads, group, f16)
+    call = kv.batch_chunk_f16 if f16 else kv.batch_chunk_i4
+    page = lambda b, pos: int(specs["kv_indices"][int(specs["kv_indptr"][b]) + pos // 16])
+    at = [(0, lens[0] - 2, 1), (0, lens[0] - 5, 0), (0, 1, 1), (0, lens[0] - news[0], 1), (len(lens) - 1, lens[-1] - 1, 1), (0, lens[0] // 2, 1)]
+    clean = torch.empty(q.shape, dtype=torch.float16, device=DEV)
+    call(clean, q, **specs, layer_idx=1, seqlen_indptr=starts, window=window, sinks=sinks)
+    for k, (b, pos, side) in enumerate(at):
+        bad = {**specs, "kv_data": specs["kv_data"].clone(), "kv_param": specs["kv_param"].clone()}
+        value = (float("inf"), float("nan"), -float("inf"))[k % 3]
+        if f16:
+            bad["kv_data"][page(b, pos), 1, side, :, pos % 16, 5::40] = value
+        else:
+            bad["kv_param"][page(b, pos), 1, side, :, pos % 16, k % 2] = value
+        o = torch.full_like(clean, 9.0)
+        call(o, q, **bad, layer_idx=1, seqlen_indptr=starts, window=window, sinks=sinks)
+        first = sum(news[:b])
+        for t in range(q.shape[0]):
+            place = lens[b] - news[b] + t - first
+            sees = first <= t < first + news[b] and pos <= place and (not window or place - pos < window or pos < sinks)
+            if not sees:
+                assert torch.equal(o[t], clean[t]), (k, t)
+            elif side == 1 and f16:
+                assert not bool(torch.isfinite(o[t, :, 5::40]).any()), (k, t)
+                rest = torch.ones(128, dtype=torch.bool)
+                rest[5::40] = False
+                assert torch.equal(o[t][:, rest], clean[t][:, rest]), (k, t)
+            elif side == 1:
+                assert not bool(torch.isfinite(o[t]).any()), (k, t)
