@@ -304,7 +304,7 @@ __global__ __launch_bounds__(64 * NW, NB == 4 ? 1 : NB == 2 ? 2 : 3) void chunk_
 #pragma unroll
                 for (int k = 0; k < 8; ++k) top = __builtin_fmaxf(top, y[k]);
                 if (__builtin_amdgcn_ballot_w64(top > m[nb] + kGrow)) {
-                    const float now = __builtin_fmaxf(m[nb], quarters_max(top)), keep = __builtin_amdgcn_exp2f(m[nb] - now);
+                    const float high = quarters_max(top), now = high > m[nb] + kGrow ? high : m[nb], keep = __builtin_amdgcn_exp2f(m[nb] - now);      // (of the row alone)
                     m[nb] = now;
                     d[nb] *= keep, pz[nb] *= keep;
 #pragma unroll

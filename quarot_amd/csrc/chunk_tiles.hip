@@ -18,8 +18,13 @@ namespace {
 
 constexpr int kRows = 256, kStep = 64;
 // LDS: three steps' keys (the next step's are read while others still read this one's), two steps' values
-constexpr int kSlope = 16384, kLine = kSlope + 256, kThere = kLine + 2048, kKeys = (kThere + 8 + 511) / 512 * 512;
-constexpr int kFactor = 133 * 128, kOdd = kFactor + 128, kValues = (kOdd + 8 + 511) / 512 * 512;
+// A key's row is padded by 16 bytes, a dimension's too, and 16 more behind every 16th and 15 times that behind every 64th: so that neither the reads (16 lanes
+// of 16 bytes, rows that follow one another) nor the writes (32 lanes of 8 bytes, rows 4, 8 and 64 apart) meet in a bank, and every piece's place is one
+// address per lane and a constant.
+constexpr int kKeyRow = 272, kDimRow = 144;
+__host__ __device__ constexpr int dim_row(int r) { return r * kDimRow + ((r >> 4) + 14 * (r >> 6)) * 16; }
+constexpr int kSlope = 64 * kKeyRow, kLine = kSlope + 256, kThere = kLine + 2048, kKeys = (kThere + 8 + 511) / 512 * 512;
+constexpr int kOdd = dim_row(133), kValues = (kOdd + 8 + 511) / 512 * 512;
 constexpr int kLds = 3 * kKeys + 2 * kValues;
 
 // What a thread has fetched for a step: four of the sixteen pieces of a key and its parameters; four positions' values in eight dimensions, their
@@ -27,7 +32,7 @@ constexpr int kLds = 3 * kKeys + 2 * kValues;
 template <bool F16>
 struct KeyCodes {
     u32x4 k[F16 ? 4 : 1];
-    u32 p, mask;
+    u32 p, pv, mask;                   // pv: the value's parameters
 };
 template <bool F16>
 struct ValueCodes {
@@ -44,6 +49,11 @@ __device__ __forceinline__ void mfma_more(f32x16& c, u32x4 a, u32x4 b) { asm vol
 __device__ __forceinline__ void mfma_line(f32x16& c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void mfma_second(f32x16& c, u32x4 a, u32x4 b) { asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
 __device__ __forceinline__ void mfma_overflow(f32x16& c, u32x4 a, u32x4 b) { asm volatile("s_nop 3\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b)); }
+// a register of that half times v: where it lies (the compiler would move whole accumulators to the vector unit's half and back in every turn)
+__device__ __forceinline__ void scale_accumulator(float& c, float v) {
+    float t;
+    asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1" : "+a"(c), "=&v"(t) : "v"(v));
+}
 __device__ __forceinline__ void settled() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 __device__ __forceinline__ f32x16 zeros() {
     f32x16 z;
@@ -87,7 +97,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     // line, whose first factor is one
     for (int i = tid; i < 2 * 5 * 32; i += 256) {
         const int at = i % 160;
-        *(u32*)(lds + 3 * kKeys + (i / 160) * kValues + 128 * 128 + at * 4) = F16 && at < 32 ? 0x3C003C00u : 0u;
+        *(u32*)(lds + 3 * kKeys + (i / 160) * kValues + dim_row(128) + (at >> 5) * kDimRow + (at & 31) * 4) = F16 && at < 32 ? 0x3C003C00u : 0u;
     }
     for (int i = tid; i < 3 * 64; i += 256) *(u32x4*)(lds + (i >> 6) * kKeys + kLine + 1024 + (i & 63) * 16) = u32x4{0x00003F80u, 0, 0, 0};
 
@@ -98,9 +108,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     const int jj = tid & 1, word = tid >> 1 & 15, hh = tid >> 5 & 1, piece = 2 * wave + hh;
     const int first_of_four = 8 * jj + 4 * hh;             // of the wave's sixteen
     const uint32_t k_at = (uint32_t)((key & ~15) + (key >> 2 & 1) * 8 + (key >> 3 & 1) * 4 + (key & 3));      // the key's place in the order of the second product
-    const uint32_t k_to = (uint32_t)key * 256 + (uint32_t)(((F16 ? e : 4 * e) ^ (key & 15)) << 4);           // piece p of a key at p ^ (key % 16)
+    const uint32_t k_to = (uint32_t)(key * kKeyRow + e * 64);                 // piece 4 e + i of a key's row (fp16 pages: it holds dimensions 8 (e + 4 i) ..)
     const int v_row = 64 * (word & 1) + 8 * (word >> 2) + 4 * (word >> 1 & 1);              // row of dimension 8 word; 8 word + 4 is 32 rows on
-    const uint32_t v_to = (uint32_t)(v_row * 128 + jj * 8 + ((piece ^ (v_row >> 1 & 7) ^ (v_row >> 4 & 1)) << 4));
+    const uint32_t v_to = (uint32_t)(dim_row(v_row) + jj * 8 + piece * 16);
 
     for (int r_tile = tile * kRows; r_tile < rows; r_tile += a.tiles * kRows) {
         const int r_end = r_tile + kRows < rows ? r_tile + kRows : rows;
@@ -119,14 +129,17 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             page64_from = s;
         };
         // slot of the first of the wave's sixteen positions (of page 0 where they are not there) and which of them are
-        auto slot_of = [&](int s, u32& mask) INLINE {
+        struct Sixteen {
+            int64_t slot;
+            u32 mask;
+        };
+        auto sixteen_of = [&](int s) INLINE {
             const int at = position(s) + 16 * wave;
             const int page = __builtin_amdgcn_readlane(page64, (s < last ? s : last) - page64_from & 63);
             const u32 entry = (u32)(at - divided(at, pages) * c.page_size);
             const bool there = page >= 0 && entry < (u32)c.page_size;
             const int left = len - at;
-            mask = !there || left <= 0 ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u;
-            return there ? page * page_slots + head_slots + entry : head_slots;
+            return Sixteen{there ? page * page_slots + head_slots + entry : head_slots, !there || left <= 0 ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u};
         };
         auto slot_of_lane = [&](int pos, bool& there) INLINE {    // pages of any size: every lane for itself
             const int it = divided(pos, pages);
@@ -143,15 +156,19 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             for (int i = 0; i < 16; ++i) mask |= (u32)(lanes >> (4 * i) & 1) << i;
             return mask;
         };
-        auto fetch_keys = [&](KeyCodes<F16>& f, int s) INLINE {
+        auto fetch_keys = [&](KeyCodes<F16>& f, int s, Sixteen all) INLINE {
             if (ALIGNED) {
-                const int64_t base = slot_of(s, f.mask);
+                const int64_t base = all.slot;
+                f.mask = all.mask;
                 const uint8_t* const kd = c.data + base * VEC;
                 uint32_t off = (uint32_t)(lane >> 2) * VEC + (uint32_t)e * 16, p_off = (uint32_t)(lane >> 2) * 4;
                 asm volatile("" : "+v"(off), "+v"(p_off));                         // (32-bit offsets behind wave-uniform addresses)
 #pragma unroll
                 for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[i] = *(const u32x4*)(kd + off + 64 * i);
-                if (!F16) f.p = *(const u32*)((const uint8_t*)(c.param + base) + p_off);
+                if (!F16) {
+                    f.p = *(const u32*)((const uint8_t*)(c.param + base) + p_off);
+                    f.pv = *(const u32*)((const uint8_t*)(c.param + base + kv_slots) + p_off);
+                }
             } else {
                 bool there;
                 const int64_t base = slot_of_lane(position(s) + key, there);
@@ -159,12 +176,13 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 const uint8_t* const kd = c.data + base * VEC + e * 16;
 #pragma unroll
                 for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[i] = *(const u32x4*)(kd + 64 * i);
-                if (!F16) f.p = c.param[base];
+                if (!F16) f.p = c.param[base], f.pv = c.param[base + kv_slots];
             }
         };
-        auto fetch_values = [&](ValueCodes<F16>& f, int s) INLINE {
+        auto fetch_values = [&](ValueCodes<F16>& f, int s, Sixteen all) INLINE {
             if (ALIGNED) {
-                const int64_t base = slot_of(s, f.mask) + kv_slots;
+                const int64_t base = all.slot + kv_slots;
+                f.mask = all.mask;
                 const uint8_t* const vd = c.data + base * VEC;
                 const uint8_t* const vp = (const uint8_t*)(c.param + base);
                 uint32_t off = (uint32_t)first_of_four * VEC + (uint32_t)word * (VEC / 16), p_off = (uint32_t)first_of_four * 4, own = (uint32_t)(lane >> 2) * 4;
@@ -192,23 +210,39 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         };
         // pieces of the unpacking, small enough to stand between matrix instructions; kbuf, vbuf: offsets in LDS
         auto place_key = [&](const KeyCodes<F16>& f, uint32_t kbuf, int i) INLINE {
-            *(u32x4*)(lds + ((k_to ^ (uint32_t)(F16 ? i << 6 : i << 4)) + kbuf)) = F16 ? f.k[F16 ? i : 0] : codes_of(f.k[0][i]);
+            *(u32x4*)(lds + (k_to + kbuf) + 16 * i) = F16 ? f.k[F16 ? i : 0] : codes_of(f.k[0][i]);
         };
-        auto place_key_parameters = [&](const KeyCodes<F16>& f, uint32_t kbuf) INLINE {
-            if (!F16) {
-                const f16x2 p = as_f16x2(f.p);
-                const float zero = (float)p[1], zero_hi = top(zero), zero_lo = zero - zero_hi;
-                const u32 hi2 = tops(zero_hi, zero_hi), lo2 = tops(zero_lo, zero_lo);
-                if (e == 0) {
-                    *(float*)(lds + (kbuf + kSlope + k_at * 4)) = (float)p[0] * (kLog2e * kScale * kCodeUnit);
-                    *(u32x4*)(lds + (kbuf + kLine + (uint32_t)key * 16)) = u32x4{hi2, tops(zero_hi, zero_lo), lo2, 0x3F803F80u};
+        struct KeyLine {                                   // a key's slope and what the logits' line has of it: zero point, log2 of its value's factor
+            float slope;
+            u32x4 lower;
+            u32x2 upper;
+        };
+        auto key_line = [&](const KeyCodes<F16>& f) INLINE {
+            KeyLine l;
+            if (F16) return l;
+            const f16x2 p = as_f16x2(f.p);
+            const float zero = (float)p[1], zero_hi = top(zero), zero_lo = zero - zero_hi;
+            const u32 hi2 = tops(zero_hi, zero_hi), lo2 = tops(zero_lo, zero_lo);
+            const float scale = __builtin_fabsf((float)as_f16x2(f.pv)[0]), log = __builtin_amdgcn_logf(factor_of(scale, power_of(scale)));
+            const float l1 = top(log), l2 = top(log - l1), l3 = log - l1 - l2;
+            l.slope = (float)p[0] * (kLog2e * kScale * kCodeUnit);
+            l.lower = u32x4{hi2, tops(zero_hi, zero_lo), lo2, 0x3F803F80u};
+            l.upper = u32x2{tops(1.f, l1), tops(l2, l3)};
+            return l;
+        };
+        auto place_key_line = [&](const KeyCodes<F16>& f, const KeyLine& l, uint32_t kbuf) INLINE {
+            if (e == 0) {
+                if (!F16) {
+                    *(float*)(lds + (kbuf + kSlope + k_at * 4)) = l.slope;
+                    *(u32x4*)(lds + (kbuf + kLine + (uint32_t)key * 16)) = l.lower;
+                    *(u32x2*)(lds + (kbuf + kLine + 1024 + (uint32_t)key * 16)) = l.upper;
                 }
+                if (lane == 0) *(unsigned short*)(lds + (kbuf + kThere + 2 * wave)) = (unsigned short)f.mask;
             }
-            if (lane == 0) *(unsigned short*)(lds + (kbuf + kThere + 2 * wave)) = (unsigned short)f.mask;
         };
         auto store_values = [&](uint32_t vbuf, int half, const u32 (&out)[4][2]) INLINE {             // rows v_row + 32 half + i
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *(u32x2*)(lds + ((v_to ^ (uint32_t)((i >> 1) << 4)) + vbuf + half * 4096 + i * 128)) = u32x2{out[i][0], out[i][1]};
+            for (int i = 0; i < 4; ++i) *(u32x2*)(lds + (v_to + vbuf) + dim_row(32 * half + i)) = u32x2{out[i][0], out[i][1]};
         };
         auto place_value = [&](const ValueCodes<F16>& f, uint32_t vbuf, int half, const u32* power) INLINE {         // dimensions 8 word + 4 half ..
             u32 out[4][2];
@@ -229,25 +263,27 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             }
             store_values(vbuf, half, out);
         };
+        auto place_value_half = [&](const ValueCodes<F16>& f, uint32_t vbuf, int half, int cb, const u32* power) INLINE {
+            if (cb == 1) place_value(f, vbuf, half, power);
+        };
         auto place_value_parameters = [&](u32 p, u32 odd, uint32_t vbuf) INLINE {                     // p: of the position with the key's number
             if (!F16) {
                 const f16x2 v = as_f16x2(p);
-                const float factor = factor_of((float)v[0], power_of((float)v[0])), recip = __builtin_amdgcn_rcpf(factor), zero = (float)v[1] * recip;
-                const f16 recip_hi = (f16)recip, zero_hi = (f16)zero;
+                const float scale = __builtin_fabsf((float)v[0]), recip = __builtin_amdgcn_rcpf(factor_of(scale, power_of(scale))), zero = (float)v[1] * recip;
+                const f16 recip_hi = (f16)recip, zero_hi = (f16)zero, recip_lo = (f16)((recip - (float)recip_hi) * 2048.f), zero_lo = (f16)((zero - (float)zero_hi) * 2048.f);
                 if (e == 0) {
-                    *(f16*)(lds + (vbuf + kFactor + k_at * 2)) = (f16)factor;
-                    uint8_t* const extra_rows = lds + (vbuf + 128 * 128 + k_at * 2);
-                    *(f16*)extra_rows = recip_hi, *(f16*)(extra_rows + 128) = (f16)((recip - (float)recip_hi) * 2048.f);
-                    *(f16*)(extra_rows + 256) = zero_hi, *(f16*)(extra_rows + 384) = (f16)((zero - (float)zero_hi) * 2048.f);
+                    uint8_t* const extra_rows = lds + (vbuf + dim_row(128) + k_at * 2);
+                    *(f16*)extra_rows = recip_hi, *(f16*)(extra_rows + kDimRow) = recip_lo;
+                    *(f16*)(extra_rows + 2 * kDimRow) = zero_hi, *(f16*)(extra_rows + 3 * kDimRow) = zero_lo;
                 }
             }
             if (lane == 0) *(unsigned short*)(lds + (vbuf + kOdd + 2 * wave)) = (unsigned short)odd;
         };
-        // 2^e of the four positions' scales in pairs; whether the short way is right for all of the wave's positions (fp16 pages: only where all of the tile's
+        // 2^e of the four positions' scales in pairs (a negative scale's sign is its power's: not plain); whether the short way is right for all of the wave's positions (fp16 pages: only where all of the tile's
         // rows see them)
         auto regular = [&](const ValueCodes<F16>& f, u32* power, bool all_see) INLINE {
             if (F16) return f.mask == 0xFFFFu && all_see;
-            bool plain = !strange(f.p);
+            bool plain = !strange(f.p) && !(f.p & 0x8000u);
 #pragma unroll
             for (int k = 0; k < 2; ++k) power[k] = powers_of(f.scales[F16 ? 0 : 2 * k], f.scales[F16 ? 0 : 2 * k + 1], plain);
             return f.mask == 0xFFFFu && __builtin_amdgcn_ballot_w64(!plain) == 0;
@@ -286,7 +322,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                     for (int k = 0; k < 2; ++k) {
                         const u32x4 w = scaled_codes_slow(__builtin_amdgcn_perm(f.v[F16 ? 0 : 2 * k + 1], f.v[F16 ? 0 : 2 * k], half ? 0x07060302u : 0x05040100u), p[2 * k], p[2 * k + 1]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) out[i][k] = w[i];
+                        for (int i = 0; i < 4; ++i) out[i][k] = w[i] ^ (p[2 * k] & 0x8000u) ^ (p[2 * k + 1] & 0x8000u) << 16;
                     }
                     store_values(vbuf, half, out);
                 }
@@ -307,13 +343,14 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         __syncthreads();                                   // (what never changes; the last tile's buffers)
         KeyCodes<F16> fk;
         ValueCodes<F16> fv;
+        Sixteen all0{}, all1{}, all2{};                    // of this step, the next one and the one behind it
         if (s_begin < s_end) {
-            if (ALIGNED) fetch_pages(s_begin);
-            fetch_keys(fk, s_begin);
-            fetch_values(fv, s_begin);
+            if (ALIGNED) fetch_pages(s_begin), all0 = sixteen_of(s_begin), all1 = sixteen_of(s_begin + 1), all2 = sixteen_of(s_begin + 2);
+            fetch_keys(fk, s_begin, all0);
+            fetch_values(fv, s_begin, all0);
         }
 
-        // the queries: lane (n, h) holds dimensions 16 s + 8 h .. + 7 of its rows
+        // the queries: lane (n, h) holds piece 2 s + h of its rows, dimensions 16 s + 8 h .. + 7 (fp16 pages: in the order of k_to)
         u32x4 qf[2][8], line[2];                           // line: the logits' line, {-zero-point slope in three pieces, twice; the maximum's}
         float slope[2];
 #pragma unroll
@@ -321,9 +358,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             const bool in = row_of(cb) < rows;
             const int token = token_of(cb);
             place[cb] = in ? len - tokens.count + token : -1;
-            const u32x4* src = (const u32x4*)(a.q + (int64_t)(tokens.start + token) * a.q_stride + (int64_t)head_of(cb, token) * 128) + h;
+            const u32x4* src = (const u32x4*)(a.q + (int64_t)(tokens.start + token) * a.q_stride + (int64_t)head_of(cb, token) * 128) + (F16 ? 4 * h : h);
 #pragma unroll
-            for (int s = 0; s < 8; ++s) qf[cb][s] = in ? src[2 * s] : u32x4{0, 0, 0, 0};
+            for (int s = 0; s < 8; ++s) qf[cb][s] = in ? src[F16 ? (s >> 1) + 8 * (s & 1) : 2 * s] : u32x4{0, 0, 0, 0};
             if (__builtin_expect(a.q_had, 0)) {
                 float v[64];
 #pragma unroll
@@ -363,10 +400,10 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 #pragma unroll
         for (int i = 0; i < 8; ++i) asm volatile("" : "+a"(qf[0][i]), "+a"(qf[1][i]));       // (where they stay)
         float most[2] = {0.f, 0.f}, m[2] = {0.f, 0.f}, limit[2] = {-3e38f, -3e38f}, poison[2] = {0.f, 0.f};         // limit: until a row has seen a position, any logit moves its maximum
-        auto draw_line = [&](int cb) INLINE {                     // lane half 0: slope pieces 1 2 3, 1 2 3, maximum pieces 1 2; half 1: piece 3
+        auto draw_line = [&](int cb) INLINE {                     // lane half 0: slope pieces 1 2 3, 1 2 3, maximum pieces 1 2; half 1: piece 3, and ones
             const float s1 = top(slope[cb]), s2 = top(slope[cb] - s1), s3 = slope[cb] - s1 - s2;
             const float m1 = top(-m[cb]), m2 = top(-m[cb] - m1), m3 = -m[cb] - m1 - m2;
-            const u32x4 lower = {tops(s1, s2), tops(s3, s1), tops(s2, s3), tops(m1, m2)}, upper = {tops(m3, 0.f), 0, 0, 0};
+            const u32x4 lower = {tops(s1, s2), tops(s3, s1), tops(s2, s3), tops(m1, m2)}, upper = {tops(m3, 1.f), 0x3F803F80u, 0, 0};
             line[cb] = h ? upper : lower;
         };
         draw_line(0), draw_line(1);
@@ -376,39 +413,36 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         for (int cb = 0; cb < 2; ++cb) acc[cb][0] = acc[cb][1] = acc[cb][2] = acc[cb][3] = extra[cb] = zeros();
         u32x4 p[2][2];                                     // weights: [rows][half unit]
 
-        const uint32_t k_from = n * 256 + ((uint32_t)(h ^ (n & 15)) << 4), v_from = n * 128 + ((uint32_t)(h ^ (n >> 1 & 7) ^ (n >> 4)) << 4);
-        const uint32_t e_from = (128 + (n < 4 ? n : 4)) * 128 + h * 16, l_from = kLine + h * 1024 + n * 16, s_from = kSlope + h * 32;
-        auto key_piece = [&](uint32_t kbuf, int kb, int i) INLINE { return *(const u32x4*)(lds + ((k_from + kbuf ^ (uint32_t)(i << 5)) + kb * 8192)); };
+        const uint32_t k_from = n * kKeyRow + h * 16, v_from = dim_row(n) + h * 16;
+        const uint32_t e_from = dim_row(128) + (n < 4 ? n : 4) * kDimRow + h * 16, l_from = kLine + h * 1024 + n * 16, s_from = kSlope + h * 32;
+        auto key_piece = [&](uint32_t kbuf, int kb, int i) INLINE { return *(const u32x4*)(lds + (k_from + kbuf) + kb * 32 * kKeyRow + i * 32); };
         auto value_piece = [&](uint32_t vbuf, int chunk, int db) INLINE {
-            return db < 4 ? *(const u32x4*)(lds + ((v_from + vbuf ^ (uint32_t)(chunk << 5)) + db * 4096)) : *(const u32x4*)(lds + (e_from + vbuf + chunk * 32));
+            return db < 4 ? *(const u32x4*)(lds + (v_from + vbuf) + dim_row(32 * db) + chunk * 32) : *(const u32x4*)(lds + (e_from + vbuf) + chunk * 32);
         };
 
         auto sees = [&](int cb, int pos) INLINE { return pos <= place[cb] && (a.window == 0 || pos > place[cb] - a.window || pos < a.sinks); };
-        // what rows do not see of the next unit's logits; whether a maximum has to be raised
-        u32 there = 0;                                     // of the next unit
-        auto settle = [&](int at) INLINE {
+        // Of the next unit: whether its positions are all there and all seen (`at`: its first); else the logits that are not seen are taken out
+        u32 there = 0;
+        auto all_seen = [&](int at) INLINE { return at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks); };
+        auto hide = [&](int at) INLINE {
             const u32 all = __builtin_amdgcn_readfirstlane(there);
-            const bool whole = at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks) && ~all == 0;
-            if (!whole) {
 #pragma unroll
-                for (int cb = 0; cb < 2; ++cb) {
-                    most[cb] = -__builtin_inff();
+            for (int cb = 0; cb < 2; ++cb) {
+                most[cb] = -__builtin_inff();
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int k = 8 * (i >> 2) + 4 * h + (i & 3);
-                        y[cb][i] = sees(cb, at + k) && (all >> k & 1) ? y[cb][i] : -__builtin_inff();
-                        most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    const int k = 8 * (i >> 2) + 4 * h + (i & 3);
+                    y[cb][i] = sees(cb, at + k) && (all >> k & 1) ? y[cb][i] : -__builtin_inff();
+                    most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
                 }
             }
-            return __builtin_amdgcn_ballot_w64(most[0] > limit[0] || most[1] > limit[1]) != 0;
         };
         // Marked positions of the unit at work.  Int4 pages: rows that see one become NaN.  Fp16 pages: its entries that are not finite are added for the rows that
         // see it, by a product of bf16 powers of two that overflows to an infinity (a NaN: to one of each sign).
         u32 odd = 0;
         auto mark = [&](int at) INLINE {
             const u32 bits = __builtin_amdgcn_readfirstlane(odd);
-            if (__builtin_expect(bits != 0, 0)) {
+            if (bits != 0) {
 #pragma unroll 1
                 for (int k = 0; k < 32; ++k) {
                     if (!(bits >> k & 1)) continue;
@@ -439,7 +473,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             for (int cb = 0; cb < 2; ++cb) {
                 const u32x2 both = both_halves<32>(as_u32(most[cb]));
                 const float now = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
-                const bool moves = now > (limit[cb] < 0.f ? limit[cb] : 0.f);
+                const bool moves = now > limit[cb];        // (of the row alone: what other rows see changes nothing)
                 const float by = moves ? now : 0.f, keep = __builtin_amdgcn_exp2f(-by);
                 limit[cb] = moves ? kGrow : limit[cb];
                 m[cb] += by;
@@ -449,27 +483,31 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 for (int k = 0; k < 5; ++k) {
                     f32x16& block = k < 4 ? acc[cb][k & 3] : extra[cb];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) block[i] *= keep;
+                    for (int i = 0; i < 16; ++i) {
+                        float v = block[i];
+                        scale_accumulator(v, keep);
+                        block[i] = v;
+                    }
                 }
                 draw_line(cb);
             }
         };
-        // two weights of half unit tt: registers 8 tt + 2 j, + 1
-        auto weights = [&](const f32x16& v, u32x4 factors, int tt, int j) INLINE {
-            const float w0 = __builtin_amdgcn_exp2f(v[8 * tt + 2 * j]), w1 = __builtin_amdgcn_exp2f(v[8 * tt + 2 * j + 1]);
-            return F16 ? cvt_f16x2(w0, w1) : scaled_pair(w0, w1, factors[j]);
+        // two weights (times the values' factors, which are in the logits) of half unit tt: registers 8 tt + 2 j, + 1
+        auto weights = [&](const f32x16& v, int tt, int j) INLINE {
+            return cvt_f16x2(__builtin_amdgcn_exp2f(v[8 * tt + 2 * j]), __builtin_amdgcn_exp2f(v[8 * tt + 2 * j + 1]));
         };
-        // First product of unit kb of the keys at kbuf into x; between it the weights of the unit at work, unit `unit` of the values at vbuf.  Operands come from
-        // LDS three slots ahead.
-        u32x4 kp[3], vp[3], ln, factors[2];
+        auto weigh = [&]() INLINE {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i >> 3][i >> 2 & 1][i & 3] = weights(y[i >> 3], i >> 2 & 1, i & 3);
+        };
+        // First product of unit kb of the keys at kbuf into x; between it the weights of the unit at work, unit `unit` of the values at vbuf, and whether one of
+        // its maxima has to be raised (which makes the weights anew).  Operands come from LDS three slots ahead.
+        u32x4 kp[3], vp[3], ln;
         f32x4 slopes[4];
+        bool grow = false;
         auto ask_keys = [&](uint32_t kbuf, int kb) INLINE {
 #pragma unroll
             for (int i = 0; i < 3; ++i) kp[i] = key_piece(kbuf, kb, i);
-        };
-        auto ask_factors = [&](uint32_t vbuf, int unit) INLINE {
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt) factors[tt] = F16 ? u32x4{} : *(const u32x4*)(lds + (vbuf + kFactor + h * 16) + (4 * unit + 2 * tt) * 16);
         };
         auto ask_line = [&](uint32_t kbuf, int kb) INLINE {
             if (F16) return;
@@ -484,7 +522,10 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 for (int cb = 0; cb < 2; ++cb) {
                     if (i == 0) mfma_first(x[cb], kp[i % 3], qf[cb][i]);
                     else mfma_more(x[cb], kp[i % 3], qf[cb][i]);
-                    if (with_weights) p[cb][i >> 2][i & 3] = weights(y[cb], factors[i >> 2], i >> 2, i & 3);
+                    if (with_weights) {
+                        p[cb][i >> 2][i & 3] = weights(y[cb], i >> 2, i & 3);
+                        if (cb == 0 && i == 1) grow = __builtin_amdgcn_ballot_w64(most[0] > limit[0] || most[1] > limit[1]) != 0;
+                    }
                     if (cb == 0) other(i);
                     if (cb == 1 && i < 5) kp[i % 3] = key_piece(kbuf, kb, i + 3);
                     if (cb == 1 && i == 5) ask_line(kbuf, kb);
@@ -519,7 +560,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                         y[cb][reg] = y0, y[cb][reg + 1] = y1;
                     }
                     if (cb == 1 && i < 7) vp[i % 3] = value_piece(vbuf, 2 * unit + (i + 3) / 5, (i + 3) % 5);
-                    if (cb == 1) other(i);
+                    other(i, cb);
                     SLOT;
                 }
             }
@@ -527,18 +568,17 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 
         // offsets in LDS: this step's keys, the next one's and those of the step behind it; this step's values and the next one's
         uint32_t k0 = 0, k1 = kKeys, k2 = 2 * kKeys, v0 = 3 * kKeys, v1 = 3 * kKeys + kValues;
-        bool grow = false;
         int s = s_begin;
         if (s_begin < s_end) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) place_key(fk, k0, i);
-            place_key_parameters(fk, k0);
+            place_key_line(fk, key_line(fk), k0);
             place_values_any(fv, v0);
-            fetch_keys(fk, s_begin + 1);
+            fetch_keys(fk, s_begin + 1, all1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) place_key(fk, k1, i);
-            place_key_parameters(fk, k1);
-            fetch_keys(fk, s_begin + 2);
+            place_key_line(fk, key_line(fk), k1);
+            fetch_keys(fk, s_begin + 2, all2);
         }
         __syncthreads();
         if (s_begin < s_end) {
@@ -552,80 +592,69 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             there = *(const u32*)(lds + k0 + kThere);
             settled();
 #pragma unroll
-            for (int cb = 0; cb < 2; ++cb) {
-                most[cb] = -__builtin_inff();
+            for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float slope_i = F16 ? 0.f : *(const float*)(lds + s_from + k0 + (i >> 3) * 64 + (i & 7) * 4);
-                    y[cb][i] = F16 ? __builtin_fmaf(x[cb][i], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][i], slope_i, t[cb][i]);
-                    most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
-                }
-            }
-            grow = settle(position(s_begin));
+                for (int i = 0; i < 16; ++i)
+                    y[cb][i] = F16 ? __builtin_fmaf(x[cb][i], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][i], slopes[i >> 2][i & 3], t[cb][i]);
+            hide(position(s_begin));
             ask_keys(k0, 1);
-            ask_factors(v0, 0);
         }
         // Units of 32 positions, two to a step.  (A wave whose rows see none of them goes through them all the same: it would wait for the others.)
-        auto first_unit = [&]() INLINE {
+        auto first_of_0 = [&]() INLINE {                   // weights of unit 0, first product of unit 1
             first_product(k0, 1, v0, 0, true, [&](int i) {
-                if (i == 2) fetch_values(fv, s + 1);
+                if (i == 2) fetch_values(fv, s + 1, all1);
             });
-            second_product(v0, 0, k0, 1, [&](int i) {
-                if (i >= 2 && i < 6) place_key(fk, k2, i - 2);
-                if (i == 7) place_key_parameters(fk, k2);
-                if (i == 8) ask_factors(v0, 1);
-                if (i == 9) ask_keys(k1, 0);
-            });
-            mark(position(s));
-            grow = settle(position(s) + 32);
         };
-        auto second_unit = [&]() INLINE {
+        auto second_of_0 = [&]() INLINE {
+            bool usual = false;
+            KeyLine l;
+            const int at = position(s);
+            second_product(v0, 0, k0, 1, [&](int i, int cb) {
+                if (i < 2) place_key(fk, k2, 2 * i + cb);
+                if (i == 4 && cb == 0) l = key_line(fk);
+                if (i == 6 && cb == 0) place_key_line(fk, l, k2);
+                if (i == 8 && cb == 0) usual = all_seen(at + 32) && (~__builtin_amdgcn_readfirstlane(there) | __builtin_amdgcn_readfirstlane(odd)) == 0;
+                if (i == 9 && cb == 1) ask_keys(k1, 0);
+            });
+            if (__builtin_expect(!usual, 0)) mark(at), hide(at + 32);
+        };
+        auto first_of_1 = [&]() INLINE {
+            if (ALIGNED) all0 = all1, all1 = all2, all2 = sixteen_of(s + 3);
+            first_product(k1, 0, v0, 1, true, [&](int i) {
+                if (i == 2) fetch_keys(fk, s + 3, all2);
+            });
+        };
+        auto second_of_1 = [&]() INLINE {
             u32 power[2];
             bool usual = false;
-            first_product(k1, 0, v0, 1, true, [&](int i) {
-                if (i == 2) fetch_keys(fk, s + 3);
+            const int at = position(s), next = position(s + 1);
+            const bool regular_values = regular(fv, power, next + 63 <= tile_lowest && (a.window == 0 || next > tile_highest - a.window || next + 63 < a.sinks));
+            second_product(v0, 1, k1, 0, [&](int i, int cb) {
+                if (i == 0 || i == 3) place_value_half(fv, v1, i == 3, cb, power);
+                if (i == 6 && cb == 0) place_value_parameters(fv.p, 0, v1);
+                if (i == 8 && cb == 0) usual = all_seen(next) && (~__builtin_amdgcn_readfirstlane(there) | __builtin_amdgcn_readfirstlane(odd)) == 0;
+                if (i == 9 && cb == 1) ask_keys(k1, 1);
             });
-            const int at_next = position(s + 1);
-            usual = regular(fv, power, at_next + 63 <= tile_lowest && (a.window == 0 || at_next > tile_highest - a.window || at_next + 63 < a.sinks));
-            second_product(v0, 1, k1, 0, [&](int i) {
-                if (i == 3 || i == 5) place_value(fv, v1, i == 5, power);
-                if (i == 7) place_value_parameters(fv.p, 0, v1);
-                if (i == 9) ask_keys(k1, 1);
-            });
-            if (__builtin_expect(!usual, 0)) place_values_any(fv, v1);
-            mark(position(s) + 32);
+            if (__builtin_expect(!regular_values, 0)) place_values_any(fv, v1);
+            if (__builtin_expect(!usual, 0)) mark(at + 32), hide(next);
             ++s;
             if (ALIGNED && __builtin_expect(s + 3 - page64_from >= 64, 0)) fetch_pages(s);
             __syncthreads();
             const uint32_t k = k0, v = v0;
             k0 = k1, k1 = k2, k2 = k, v0 = v1, v1 = v;
-            ask_factors(v0, 0);
-            grow = s < s_end && settle(position(s));
         };
-        // Raising maxima changes accumulators, which only matrix instructions touch otherwise: that is done outside the inner loop, or they would be moved between
-        // the halves of the register file in every turn.  It is rare behind a row's first positions.
-        bool middle = false;
-        for (;;) {
-            if (__builtin_expect(grow, 1)) {
-                settled();
-                raise();
-            }
-            grow = false;
-            if (middle) {
-                second_unit();
-                middle = false;
-                if (grow) continue;
-            }
-            while (s < s_end) {
-                first_unit();
-                if (__builtin_expect(grow, 0)) {
-                    middle = true;
-                    break;
-                }
-                second_unit();
-                if (__builtin_expect(grow, 0)) break;
-            }
-            if (!grow) break;
+        auto raised = [&]() INLINE {
+            settled();
+            raise();
+            weigh();
+        };
+        while (s < s_end) {
+            first_of_0();
+            if (__builtin_expect(grow, 0)) raised();
+            second_of_0();
+            first_of_1();
+            if (__builtin_expect(grow, 0)) raised();
+            second_of_1();
         }
 
         settled();
