@@ -18,13 +18,13 @@ namespace {
 
 constexpr int kRows = 256, kStep = 64;
 // LDS: three steps' keys (the next step's are read while others still read this one's), two steps' values
-// A key's row is padded by 16 bytes, a dimension's too, and 16 more behind every 16th and 15 times that behind every 64th: so that neither the reads (16 lanes
-// of 16 bytes, rows that follow one another) nor the writes (32 lanes of 8 bytes, rows 4, 8 and 64 apart) meet in a bank, and every piece's place is one
-// address per lane and a constant.
+// A key's row is padded by 16 bytes, a dimension's too, and 16 more behind every 32nd: so that neither the reads (16 lanes of 16 bytes, rows that follow one
+// another) nor the writes (32 lanes of 8 bytes, rows 4, 8, 32 and 64 apart) meet in a bank, and every piece's place is one address per lane and a constant.
 constexpr int kKeyRow = 272, kDimRow = 144;
-__host__ __device__ constexpr int dim_row(int r) { return r * kDimRow + ((r >> 4) + 14 * (r >> 6)) * 16; }
+__host__ __device__ constexpr int dim_row(int r) { return r * kDimRow + (r >> 5) * 16; }
 constexpr int kSlope = 64 * kKeyRow, kLine = kSlope + 256, kThere = kLine + 2048, kKeys = (kThere + 8 + 511) / 512 * 512;
 constexpr int kOdd = dim_row(133), kValues = (kOdd + 8 + 511) / 512 * 512;
+constexpr float kHigh = 15.f;                              // a maximum is raised when a logit (base 2, with the value's factor) is this far above it: 2^15 is an fp16 number
 constexpr int kLds = 3 * kKeys + 2 * kValues;
 
 // What a thread has fetched for a step: four of the sixteen pieces of a key and its parameters; four positions' values in eight dimensions, their
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     const int first_of_four = 8 * jj + 4 * hh;             // of the wave's sixteen
     const uint32_t k_at = (uint32_t)((key & ~15) + (key >> 2 & 1) * 8 + (key >> 3 & 1) * 4 + (key & 3));      // the key's place in the order of the second product
     const uint32_t k_to = (uint32_t)(key * kKeyRow + e * 64);                 // piece 4 e + i of a key's row (fp16 pages: it holds dimensions 8 (e + 4 i) ..)
-    const int v_row = 64 * (word & 1) + 8 * (word >> 2) + 4 * (word >> 1 & 1);              // row of dimension 8 word; 8 word + 4 is 32 rows on
+    const int v_row = 4 * (word & 1) + 8 * (word >> 1 & 1) + 32 * (word >> 2);              // row of dimension 8 word; 8 word + 4 is 16 rows on
     const uint32_t v_to = (uint32_t)(dim_row(v_row) + jj * 8 + piece * 16);
 
     for (int r_tile = tile * kRows; r_tile < rows; r_tile += a.tiles * kRows) {
@@ -240,9 +240,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 if (lane == 0) *(unsigned short*)(lds + (kbuf + kThere + 2 * wave)) = (unsigned short)f.mask;
             }
         };
-        auto store_values = [&](uint32_t vbuf, int half, const u32 (&out)[4][2]) INLINE {             // rows v_row + 32 half + i
+        auto store_values = [&](uint32_t vbuf, int half, const u32 (&out)[4][2]) INLINE {             // rows v_row + 16 half + i
 #pragma unroll
-            for (int i = 0; i < 4; ++i) *(u32x2*)(lds + (v_to + vbuf) + dim_row(32 * half + i)) = u32x2{out[i][0], out[i][1]};
+            for (int i = 0; i < 4; ++i) *(u32x2*)(lds + (v_to + vbuf) + (16 * half + i) * kDimRow) = u32x2{out[i][0], out[i][1]};
         };
         auto place_value = [&](const ValueCodes<F16>& f, uint32_t vbuf, int half, const u32* power) INLINE {         // dimensions 8 word + 4 half ..
             u32 out[4][2];
@@ -452,11 +452,11 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                         continue;
                     }
                     bool there;
-                    const unsigned short* const v = (const unsigned short*)(c.data + (slot_of_lane(at + k, there) + kv_slots) * VEC) + 32 * (n >> 3) + 16 * (n >> 2 & 1) + (n & 3);
+                    const unsigned short* const v = (const unsigned short*)(c.data + (slot_of_lane(at + k, there) + kv_slots) * VEC) + 8 * (n >> 2 & 3) + 4 * (n >> 4) + (n & 3);
                     const u32x4 seen[2] = {{h == 0 && sees(0, at + k) ? 0x7F00u : 0u, 0, 0, 0}, {h == 0 && sees(1, at + k) ? 0x7F00u : 0u, 0, 0, 0}};
 #pragma unroll
                     for (int db = 0; db < 4; ++db) {
-                        const u32 bf = v[4 * db], sign = bf & 0x8000u;
+                        const u32 bf = v[32 * db], sign = bf & 0x8000u;
                         const bool nan = (bf & 0x7FFFu) > 0x7C00u, inf = (bf & 0x7FFFu) == 0x7C00u;
                         const u32x4 up = {h == 0 && (nan || (inf && !sign)) ? 0x7F00u : 0u, 0, 0, 0}, down = {h == 0 && (nan || (inf && sign)) ? 0xFF00u : 0u, 0, 0, 0};
 #pragma unroll
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 const float now = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
                 const bool moves = now > limit[cb];        // (of the row alone: what other rows see changes nothing)
                 const float by = moves ? now : 0.f, keep = __builtin_amdgcn_exp2f(-by);
-                limit[cb] = moves ? kGrow : limit[cb];
+                limit[cb] = moves ? kHigh : limit[cb];
                 m[cb] += by;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) y[cb][i] -= by;
@@ -537,10 +537,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         // Second product of the unit at work; between it the logits of the next one, unit next_kb of the keys at kbuf, from its first product and their line,
         // and their maxima.
         auto second_product = [&](uint32_t vbuf, int unit, uint32_t kbuf, int next_kb, auto&& other) INLINE {
-            f32x16 t[2];
             if (!F16) {
-                mfma_line(t[0], ln, line[0]);
-                mfma_line(t[1], ln, line[1]);
+                mfma_line(y[0], ln, line[0]);
+                mfma_line(y[1], ln, line[1]);
                 SLOT;
             }
             there = *(const u32*)(lds + (kbuf + kThere) + 4 * next_kb);
@@ -553,8 +552,8 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                     mfma_second(db < 4 ? acc[cb][db & 3] : extra[cb], vp[i % 3], p[cb][tt]);
                     if (i > 1) {
                         const int reg = 2 * (i - 2);
-                        float y0 = F16 ? __builtin_fmaf(x[cb][reg], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][reg], slopes[reg >> 2][reg & 3], t[cb][reg]);
-                        float y1 = F16 ? __builtin_fmaf(x[cb][reg + 1], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][reg + 1], slopes[reg >> 2][(reg & 3) + 1], t[cb][reg + 1]);
+                        float y0 = F16 ? __builtin_fmaf(x[cb][reg], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][reg], slopes[reg >> 2][reg & 3], y[cb][reg]);
+                        float y1 = F16 ? __builtin_fmaf(x[cb][reg + 1], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][reg + 1], slopes[reg >> 2][(reg & 3) + 1], y[cb][reg + 1]);
                         most[cb] = i == 2 ? __builtin_fmaxf(y0, y1) : __builtin_fmaxf(__builtin_fmaxf(most[cb], y0), y1);
                         asm volatile("" : "+v"(y0), "+v"(y1), "+v"(most[cb]));         // (here, not where they are used)
                         y[cb][reg] = y0, y[cb][reg + 1] = y1;
@@ -671,30 +670,30 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             }
             if (row_of(cb) >= rows) continue;
             const int token = token_of(cb), q_head = head_of(cb, token);
-            // lane (n, h): dimensions 32 i + 16 h + 4 db + j of row n in register 4 i + j of block db
+            // lane (n, h): dimensions 32 db + 16 i + 8 h + 4 k + j of row n in register 4 (i + 2 k) + j of block db
             if (a.splits == 1) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                u32x4* const dst = (u32x4*)(a.o + (int64_t)(tokens.start + token) * a.o_stride + (int64_t)q_head * 128) + 2 * h;
+                u32x4* const dst = (u32x4*)(a.o + (int64_t)(tokens.start + token) * a.o_stride + (int64_t)q_head * 128) + h;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int db = 0; db < 4; ++db)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
+                    for (int i = 0; i < 2; ++i) {
                         u32x4 w;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int db = 2 * k + (j >> 1), reg = 4 * i + 2 * (j & 1);
+                            const int reg = 4 * (i + 2 * (j >> 1)) + 2 * (j & 1);
                             w[j] = cvt_f16x2((acc[cb][db][reg] - zero) * inv, (acc[cb][db][reg + 1] - zero) * inv);
                         }
-                        dst[4 * i + k] = w;
+                        dst[4 * db + 2 * i] = w;
                     }
             } else {
                 float* const dst = a.part + (((int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head) * a.splits + split) * 132;
                 if (h == 0) dst[0] = limit[cb] < 0.f ? kEmpty : m[cb], dst[1] = sum;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int db = 0; db < 4; ++db)
 #pragma unroll
-                    for (int db = 0; db < 4; ++db)
-                        *(f32x4*)(dst + 4 + 32 * i + 16 * h + 4 * db) =
+                    for (int i = 0; i < 4; ++i)
+                        *(f32x4*)(dst + 4 + 32 * db + 16 * (i & 1) + 8 * h + 4 * (i >> 1)) =
                             f32x4{acc[cb][db][4 * i] - zero, acc[cb][db][4 * i + 1] - zero, acc[cb][db][4 * i + 2] - zero, acc[cb][db][4 * i + 3] - zero};
             }
         }
