@@ -533,7 +533,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     if (!o || !q) return QR_E_NULL;
     if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || q_stride % 8 || o_stride % 8) return QR_E_ALIGN;
     const int64_t width = (int64_t)num_q_heads * 128;
-    if (q_stride < width || o_stride < width || tokens * num_q_heads > 0x7fffffff || num_q_heads / num_heads > 1024) return QR_E_SHAPE;
+    if (q_stride < width || o_stride < width || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024) return QR_E_SHAPE;
     const ChunkPlan plan = chunk_plan(tokens, num_q_heads / num_heads, num_heads, batch_size, seqlen_indptr_or_null ? max_new_len : 1, max_seq_len, window, sinks);
     Chunk a;
     a.c = qr_internal_paged_kv((void*)kv_data, (void*)kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,
@@ -544,12 +544,14 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     a.q_stride = q_stride, a.o_stride = o_stride;
     a.tokens = (int)tokens;
     a.group = num_q_heads / num_heads;
+    a.per_group = divisor_of(a.group);
     a.tiles = plan.tiles;
     a.window = (int)(window > 0x3fffffff ? 0 : window);    // (longer than any sequence)
     a.sinks = (int)(sinks > 0x3fffffff ? 0x3fffffff : sinks);
     a.q_had = q_had_mode;
     a.splits = plan.splits;
     if (a.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < chunk_part_bytes(tokens, num_q_heads, a.splits))) a.splits = 1;
+    a.per_split = divisor_of(a.splits);
     a.part = (float*)workspace;
     const int64_t groups = batch_size * num_heads * plan.tiles * a.splits;
     if (groups > 0x7fffffff) return QR_E_SHAPE;

@@ -95,11 +95,11 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 
     // what never changes: the values' operand beyond row 131 (fp16 pages: beyond 127, with a row of ones for the weights' sum), the second half of the logits'
     // line, whose first factor is one
-    for (int i = tid; i < 2 * 5 * 32; i += 256) {
-        const int at = i % 160;
-        *(u32*)(lds + 3 * kKeys + (i / 160) * kValues + dim_row(128) + (at >> 5) * kDimRow + (at & 31) * 4) = F16 && at < 32 ? 0x3C003C00u : 0u;
+    if (tid < 2 * 40) {
+        const int at = tid % 40;
+        *(u32x4*)(lds + 3 * kKeys + (tid < 40 ? 0 : kValues) + dim_row(128) + (at >> 3) * kDimRow + (at & 7) * 16) = F16 && at < 8 ? u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u} : u32x4{0, 0, 0, 0};
     }
-    for (int i = tid; i < 3 * 64; i += 256) *(u32x4*)(lds + (i >> 6) * kKeys + kLine + 1024 + (i & 63) * 16) = u32x4{0x00003F80u, 0, 0, 0};
+    if (tid < 3 * 64) *(u32x4*)(lds + (tid >> 6) * kKeys + kLine + 1024 + (tid & 63) * 16) = u32x4{0x00003F80u, 0, 0, 0};
 
     // ---- a step's way into LDS.  Thread (key, e) takes pieces e, e + 4, e + 8, e + 12 of a key (int4: the words 4 e .. 4 e + 3); thread (four positions,
     // word) their values in dimensions 8 word ...  The four positions are 16 wave + 8 jj + 4 hh ..: what lane half hh of the second product takes
@@ -114,32 +114,23 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 
     for (int r_tile = tile * kRows; r_tile < rows; r_tile += a.tiles * kRows) {
         const int r_end = r_tile + kRows < rows ? r_tile + kRows : rows;
-        const int tile_lowest = len - tokens.count + r_tile / a.group, tile_highest = len - tokens.count + (r_end - 1) / a.group;
+        const int tile_lowest = len - tokens.count + divided(r_tile, a.per_group), tile_highest = len - tokens.count + divided(r_end - 1, a.per_group);
         const Steps steps = steps_of<6>(a, tile_lowest, tile_highest);
-        const int s_begin = (int)((int64_t)steps.all * split / a.splits), s_end = (int)((int64_t)steps.all * (split + 1) / a.splits);
+        const int s_begin = divided(steps.all * split, a.per_split), s_end = divided(steps.all * (split + 1), a.per_split);      // (below 2^24 steps, 2^5 splits)
         const int last = s_end - 1;
         auto position = [&](int s) INLINE { return steps.at(s < last ? s : last) * kStep; };        // (behind the last step the last again)
 
         // ALIGNED: page numbers of the wave's sixteen positions in the next 64 steps, a lane each, -1: none; a step takes its own by a lane's number
         int page64 = -1, page64_from = 0;
+        auto ask_pages = [&](int s, int& it) INLINE {
+            it = divided(position(s + lane) + 16 * wave, pages);
+            return npages > 0 ? c.indices[p0 + (it < npages ? it : 0)] : -1;
+        };
         auto fetch_pages = [&](int s) INLINE {
-            const int it = divided(position(s + lane) + 16 * wave, pages);
-            const int page = npages > 0 ? c.indices[p0 + (it < npages ? it : 0)] : -1;
+            int it;
+            const int page = ask_pages(s, it);
             page64 = it < npages && page < c.num_pages ? page : -1;
             page64_from = s;
-        };
-        // slot of the first of the wave's sixteen positions (of page 0 where they are not there) and which of them are
-        struct Sixteen {
-            int64_t slot;
-            u32 mask;
-        };
-        auto sixteen_of = [&](int s) INLINE {
-            const int at = position(s) + 16 * wave;
-            const int page = __builtin_amdgcn_readlane(page64, (s < last ? s : last) - page64_from & 63);
-            const u32 entry = (u32)(at - divided(at, pages) * c.page_size);
-            const bool there = page >= 0 && entry < (u32)c.page_size;
-            const int left = len - at;
-            return Sixteen{there ? page * page_slots + head_slots + entry : head_slots, !there || left <= 0 ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u};
         };
         auto slot_of_lane = [&](int pos, bool& there) INLINE {    // pages of any size: every lane for itself
             const int it = divided(pos, pages);
@@ -149,6 +140,25 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             there = inside && page >= 0 && page < c.num_pages;
             return there ? page * page_slots + head_slots + entry : head_slots;
         };
+        // slot of the first of the wave's sixteen positions (of page 0 where they are not there; pages of any size: of the lane's own, the first sixteen lanes') and
+        // which of them are there
+        struct Sixteen {
+            int64_t slot;
+            u32 mask;
+        };
+        auto sixteen_of = [&](int s) INLINE {
+            const int at = position(s) + 16 * wave;
+            if (!ALIGNED) {
+                bool there;
+                const int64_t slot = slot_of_lane(at + (lane & 15), there);
+                return Sixteen{slot, (u32)__builtin_amdgcn_ballot_w64(there) & 0xFFFFu};
+            }
+            const int page = __builtin_amdgcn_readlane(page64, (s < last ? s : last) - page64_from & 63);
+            const u32 entry = (u32)(at - divided(at, pages) * c.page_size);
+            const bool there = page >= 0 && entry < (u32)c.page_size;
+            const int left = len - at;
+            return Sixteen{there ? page * page_slots + head_slots + entry : head_slots, !there || left <= 0 ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u};
+        };
         auto mask_of = [&](bool there) INLINE {                   // of a bool that the four lanes of a key share
             const uint64_t lanes = __builtin_amdgcn_ballot_w64(there);
             u32 mask = 0;
@@ -156,7 +166,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             for (int i = 0; i < 16; ++i) mask |= (u32)(lanes >> (4 * i) & 1) << i;
             return mask;
         };
-        auto fetch_keys = [&](KeyCodes<F16>& f, int s, Sixteen all) INLINE {
+        auto fetch_keys = [&](KeyCodes<F16>& f, const Sixteen& all) INLINE {
             if (ALIGNED) {
                 const int64_t base = all.slot;
                 f.mask = all.mask;
@@ -170,16 +180,15 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                     f.pv = *(const u32*)((const uint8_t*)(c.param + base + kv_slots) + p_off);
                 }
             } else {
-                bool there;
-                const int64_t base = slot_of_lane(position(s) + key, there);
-                f.mask = mask_of(there);
+                const int64_t base = __shfl(all.slot, lane >> 2, 64);
+                f.mask = all.mask;
                 const uint8_t* const kd = c.data + base * VEC + e * 16;
 #pragma unroll
                 for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[i] = *(const u32x4*)(kd + 64 * i);
                 if (!F16) f.p = c.param[base], f.pv = c.param[base + kv_slots];
             }
         };
-        auto fetch_values = [&](ValueCodes<F16>& f, int s, Sixteen all) INLINE {
+        auto fetch_values = [&](ValueCodes<F16>& f, const Sixteen& all) INLINE {
             if (ALIGNED) {
                 const int64_t base = all.slot + kv_slots;
                 f.mask = all.mask;
@@ -196,16 +205,13 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    bool there;
-                    const int64_t slot = slot_of_lane(position(s) + 16 * wave + first_of_four + i, there) + kv_slots;
+                    const int64_t slot = __shfl(all.slot, first_of_four + i, 64) + kv_slots;
                     const uint8_t* const vd = c.data + slot * VEC + word * (VEC / 16);
                     if (F16) f.v4[i] = *(const u32x4*)vd;
                     else f.v[i] = *(const u32*)vd, f.scales[i] = c.param[slot];
                 }
-                bool there;
-                const int64_t own = slot_of_lane(position(s) + key, there) + kv_slots;
-                f.mask = mask_of(there);
-                if (!F16) f.p = c.param[own];
+                f.mask = all.mask;
+                if (!F16) f.p = c.param[__shfl(all.slot, lane >> 2, 64) + kv_slots];
             }
         };
         // pieces of the unpacking, small enough to stand between matrix instructions; kbuf, vbuf: offsets in LDS
@@ -334,23 +340,15 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         // the wave's rows: block cb has rows r0 + 32 cb + n
         const int r0 = r_tile + 64 * wave;
         const int r_last = r0 + 63 < rows ? r0 + 63 : rows - 1;
-        const int lowest = r0 < rows ? len - tokens.count + r0 / a.group : -1, highest = r0 < rows ? len - tokens.count + r_last / a.group : -1;
+        const int lowest = r0 < rows ? len - tokens.count + divided(r0, a.per_group) : -1, highest = r0 < rows ? len - tokens.count + divided(r_last, a.per_group) : -1;
         auto row_of = [&](int cb) { return r0 + 32 * cb + n; };
-        auto token_of = [&](int cb) { return (row_of(cb) < rows ? row_of(cb) : r_tile) / a.group; };
+        auto token_of = [&](int cb) { return divided(row_of(cb) < rows ? row_of(cb) : r_tile, a.per_group); };
         auto head_of = [&](int cb, int token) { return head * a.group + (row_of(cb) < rows ? row_of(cb) : r_tile) - token * a.group; };
         int place[2];
 
-        __syncthreads();                                   // (what never changes; the last tile's buffers)
-        KeyCodes<F16> fk;
-        ValueCodes<F16> fv;
-        Sixteen all0{}, all1{}, all2{};                    // of this step, the next one and the one behind it
-        if (s_begin < s_end) {
-            if (ALIGNED) fetch_pages(s_begin), all0 = sixteen_of(s_begin), all1 = sixteen_of(s_begin + 1), all2 = sixteen_of(s_begin + 2);
-            fetch_keys(fk, s_begin, all0);
-            fetch_values(fv, s_begin, all0);
-        }
-
         // the queries: lane (n, h) holds piece 2 s + h of its rows, dimensions 16 s + 8 h .. + 7 (fp16 pages: in the order of k_to)
+        int first_it = 0, first_page = -1;                 // (asked for ahead of the queries, taken behind them)
+        if (ALIGNED && s_begin < s_end) first_page = ask_pages(s_begin, first_it);
         u32x4 qf[2][8], line[2];                           // line: the logits' line, {-zero-point slope in three pieces, twice; the maximum's}
         float slope[2];
 #pragma unroll
@@ -360,7 +358,22 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             place[cb] = in ? len - tokens.count + token : -1;
             const u32x4* src = (const u32x4*)(a.q + (int64_t)(tokens.start + token) * a.q_stride + (int64_t)head_of(cb, token) * 128) + (F16 ? 4 * h : h);
 #pragma unroll
-            for (int s = 0; s < 8; ++s) qf[cb][s] = in ? src[F16 ? (s >> 1) + 8 * (s & 1) : 2 * s] : u32x4{0, 0, 0, 0};
+            for (int s = 0; s < 8; ++s) qf[cb][s] = src[F16 ? (s >> 1) + 8 * (s & 1) : 2 * s];       // (rows that are not there: another one's, whose results go nowhere)
+        }
+        KeyCodes<F16> fk, fk1;
+        ValueCodes<F16> fv;
+        Sixteen all0{}, all1{}, all2{};                    // of this step, the next one and the one behind it
+        if (s_begin < s_end) {
+            page64 = first_it < npages && first_page < c.num_pages ? first_page : -1, page64_from = s_begin;
+            all0 = sixteen_of(s_begin), all1 = sixteen_of(s_begin + 1), all2 = sixteen_of(s_begin + 2);
+            fetch_keys(fk, all0);
+            fetch_values(fv, all0);
+            fetch_keys(fk1, all1);
+        }
+        __syncthreads();                                   // (what never changes; the last tile's buffers)
+
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) {
             if (__builtin_expect(a.q_had, 0)) {
                 float v[64];
 #pragma unroll
@@ -420,7 +433,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             return db < 4 ? *(const u32x4*)(lds + (v_from + vbuf) + dim_row(32 * db) + chunk * 32) : *(const u32x4*)(lds + (e_from + vbuf) + chunk * 32);
         };
 
-        auto sees = [&](int cb, int pos) INLINE { return pos <= place[cb] && (a.window == 0 || pos > place[cb] - a.window || pos < a.sinks); };
+        // row of block cb: sees positions up to its place, from behind `before` on, and the sinks
+        auto before = [&](int cb) INLINE { return a.window ? place[cb] - a.window : -1; };
+        auto sees = [&](int cb, int pos) INLINE { return (pos <= place[cb]) & ((pos > before(cb)) | (pos < a.sinks)); };
         // Of the next unit: whether its positions are all there and all seen (`at`: its first); else the logits that are not seen are taken out
         u32 there = 0;
         auto all_seen = [&](int at) INLINE { return at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks); };
@@ -428,13 +443,19 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             const u32 all = __builtin_amdgcn_readfirstlane(there);
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb) {
+                const int from = at + 4 * h, high = place[cb] - from, low = before(cb) - from, sinks = a.sinks - from;
                 most[cb] = -__builtin_inff();
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int k = 8 * (i >> 2) + 4 * h + (i & 3);
-                    y[cb][i] = sees(cb, at + k) && (all >> k & 1) ? y[cb][i] : -__builtin_inff();
-                    most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
+                    const int k = 8 * (i >> 2) + (i & 3);
+                    y[cb][i] = (k <= high) & ((k > low) | (k < sinks)) ? y[cb][i] : -__builtin_inff();
                 }
+                if (~all) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[cb][i] = all >> (8 * (i >> 2) + 4 * h + (i & 3)) & 1 ? y[cb][i] : -__builtin_inff();
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
             }
         };
         // Marked positions of the unit at work.  Int4 pages: rows that see one become NaN.  Fp16 pages: its entries that are not finite are added for the rows that
@@ -466,6 +487,19 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                         }
                     }
                 }
+            }
+        };
+        auto begin = [&]() INLINE {                         // the first maxima
+#pragma unroll
+            for (int cb = 0; cb < 2; ++cb) {
+                const u32x2 both = both_halves<32>(as_u32(most[cb]));
+                const float now = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
+                const bool any = now > limit[cb];
+                m[cb] = any ? now : 0.f, most[cb] -= m[cb];
+                limit[cb] = any ? kHigh : limit[cb];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[cb][i] -= m[cb];
+                draw_line(cb);
             }
         };
         auto raise = [&]() INLINE {
@@ -523,7 +557,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                     if (i == 0) mfma_first(x[cb], kp[i % 3], qf[cb][i]);
                     else mfma_more(x[cb], kp[i % 3], qf[cb][i]);
                     if (with_weights) {
-                        p[cb][i >> 2][i & 3] = weights(y[cb], i >> 2, i & 3);
+                        u32 w = weights(y[cb], i >> 2, i & 3);
+                        asm volatile("" : "+v"(w));        // (here, not behind the question whether they are made anew)
+                        p[cb][i >> 2][i & 3] = w;
                         if (cb == 0 && i == 1) grow = __builtin_amdgcn_ballot_w64(most[0] > limit[0] || most[1] > limit[1]) != 0;
                     }
                     if (cb == 0) other(i);
@@ -573,11 +609,10 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             for (int i = 0; i < 4; ++i) place_key(fk, k0, i);
             place_key_line(fk, key_line(fk), k0);
             place_values_any(fv, v0);
-            fetch_keys(fk, s_begin + 1, all1);
+            fetch_keys(fk, all2);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) place_key(fk, k1, i);
-            place_key_line(fk, key_line(fk), k1);
-            fetch_keys(fk, s_begin + 2, all2);
+            for (int i = 0; i < 4; ++i) place_key(fk1, k1, i);
+            place_key_line(fk1, key_line(fk1), k1);
         }
         __syncthreads();
         if (s_begin < s_end) {
@@ -596,12 +631,13 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 for (int i = 0; i < 16; ++i)
                     y[cb][i] = F16 ? __builtin_fmaf(x[cb][i], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][i], slopes[i >> 2][i & 3], t[cb][i]);
             hide(position(s_begin));
+            begin();
             ask_keys(k0, 1);
         }
         // Units of 32 positions, two to a step.  (A wave whose rows see none of them goes through them all the same: it would wait for the others.)
         auto first_of_0 = [&]() INLINE {                   // weights of unit 0, first product of unit 1
             first_product(k0, 1, v0, 0, true, [&](int i) {
-                if (i == 2) fetch_values(fv, s + 1, all1);
+                if (i == 2) fetch_values(fv, all1);
             });
         };
         auto second_of_0 = [&]() INLINE {
@@ -618,9 +654,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             if (__builtin_expect(!usual, 0)) mark(at), hide(at + 32);
         };
         auto first_of_1 = [&]() INLINE {
-            if (ALIGNED) all0 = all1, all1 = all2, all2 = sixteen_of(s + 3);
+            all0 = all1, all1 = all2, all2 = sixteen_of(s + 3);
             first_product(k1, 0, v0, 1, true, [&](int i) {
-                if (i == 2) fetch_keys(fk, s + 3, all2);
+                if (i == 2) fetch_keys(fk, all2);
             });
         };
         auto second_of_1 = [&]() INLINE {
@@ -672,7 +708,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             const int token = token_of(cb), q_head = head_of(cb, token);
             // lane (n, h): dimensions 32 db + 16 i + 8 h + 4 k + j of row n in register 4 (i + 2 k) + j of block db
             if (a.splits == 1) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const float inv = sum == 0.f ? 0.f : 1.f / sum, less = -zero * inv;
                 u32x4* const dst = (u32x4*)(a.o + (int64_t)(tokens.start + token) * a.o_stride + (int64_t)q_head * 128) + h;
 #pragma unroll
                 for (int db = 0; db < 4; ++db)
@@ -682,7 +718,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const int reg = 4 * (i + 2 * (j >> 1)) + 2 * (j & 1);
-                            w[j] = cvt_f16x2((acc[cb][db][reg] - zero) * inv, (acc[cb][db][reg + 1] - zero) * inv);
+                            w[j] = cvt_f16x2(__builtin_fmaf(acc[cb][db][reg], inv, less), __builtin_fmaf(acc[cb][db][reg + 1], inv, less));
                         }
                         dst[4 * db + 2 * i] = w;
                     }

@@ -2,6 +2,16 @@
 #pragma once
 #include "qr_paged.h"
 
+// n / d for n below 2^30: umulhi(4 n, inverse) >> shift
+struct Divisor {
+    u32 inverse, shift;
+};
+__device__ __forceinline__ int divided(int n, Divisor d) { return (int)(__umulhi((u32)n << 2, d.inverse) >> d.shift); }
+static inline Divisor divisor_of(int64_t d) {
+    const u32 log2 = d > 1 ? 64u - (u32)__builtin_clzll((unsigned long long)d - 1) : 0u;       // the least s for which 2^s reaches d
+    return Divisor{(u32)(((1ull << (30 + log2)) + (uint64_t)d - 1) / (uint64_t)d), log2};
+}
+
 // What a launch works on.  Rows of a (sequence, key head): row r is new token r / group, query head kv_head * group + r % group.
 struct Chunk {
     PagedKV c;
@@ -12,6 +22,7 @@ struct Chunk {
     int64_t q_stride, o_stride;       // halves from a token to the next
     int tokens, group, tiles, splits, window, sinks;      // window 0: none
     int q_had;
+    Divisor per_group, per_split;     // of `group`, `splits`
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -43,16 +54,6 @@ __device__ __forceinline__ float quarters_max(float v) {
     v = __builtin_fmaxf(as_f32(a.x), as_f32(a.y));
     const u32x2 b = both_halves<32>(as_u32(v));
     return __builtin_fmaxf(as_f32(b.x), as_f32(b.y));
-}
-
-// n / d for n below 2^30: umulhi(4 n, inverse) >> shift
-struct Divisor {
-    u32 inverse, shift;
-};
-__device__ __forceinline__ int divided(int n, Divisor d) { return (int)(__umulhi((u32)n << 2, d.inverse) >> d.shift); }
-static inline Divisor divisor_of(int64_t d) {
-    const u32 log2 = d > 1 ? 64u - (u32)__builtin_clzll((unsigned long long)d - 1) : 0u;       // the least s for which 2^s reaches d
-    return Divisor{(u32)(((1ull << (30 + log2)) + (uint64_t)d - 1) / (uint64_t)d), log2};
 }
 
 // ---- int4 operands
