@@ -448,7 +448,7 @@ int qr_batch_decode_f16(void* o, const void* q, const void* kv_data, const void*
  *   0; they size the launch and may be wrong at the cost of time only.  With a workspace of qr_batch_chunk_workspace_bytes
  *   bytes (16-byte aligned, contents arbitrary) few rows are split along the positions, and a second launch merges.
  */
-size_t qr_batch_chunk_workspace_bytes(int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
+size_t qr_batch_chunk_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                       int64_t max_seq_len, int64_t window, int64_t sinks);
 int qr_batch_chunk_i4(void* o, int64_t o_stride, const void* q, int64_t q_stride, int q_had_mode,
                       const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,

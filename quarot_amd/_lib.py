@@ -59,7 +59,7 @@ SIGNATURES = {
     "qr_kv_append_f16": (_int, (_ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int,
                                 _i64, _ptr)),
     "qr_batch_decode_f16": (_int, (_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int, _i64, _ptr)),
-    "qr_batch_chunk_workspace_bytes": (_c.c_size_t, (_i64, _int, _int, _i64, _i64, _i64, _i64, _i64)),
+    "qr_batch_chunk_workspace_bytes": (_c.c_size_t, (_int, _i64, _int, _int, _i64, _i64, _i64, _i64, _i64)),
     "qr_batch_chunk_i4": (_int, _CHUNK),
     "qr_batch_chunk_f16": (_int, _CHUNK),
     "qr_build_page_tables": (_int, (_ptr, _ptr, _i64, _int, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr)),

@@ -36,7 +36,7 @@ struct There {
 
 // ALIGNED: pages of a multiple of 16 positions, so that each half of a step lies in one page.
 template <int NB, int NW, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(64 * NW, NB == 4 ? 1 : NB == 2 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) {
+__global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) {
     extern __shared__ __attribute__((aligned(16))) f32x4 st4[];            // per wave and row: maximum, sum, -, -, 128 outputs
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -483,33 +483,64 @@ __global__ __launch_bounds__(256) void chunk_merge_kernel(const float* __restric
 
 // How a call is cut: column blocks and waves of a workgroup (nb 0: the kernel of 256 rows), tiles of rows per (sequence, key head), splits of the
 // positions.
+//
+// 16 rows and fewer read the cache once, whoever does it: as many workgroups as fill the chip.  More rows are a choice between tiles of 32, each of which reads and
+// unpacks the cache for itself, and tiles of 256, whose workgroups have a compute unit to themselves and a long way to their first product.  Microseconds, from
+// the two kernels' own times: a wave's step of 32 positions by 32 rows 3.0 with two waves per SIMD (fp16 pages, which reach the caches' bandwidth, 7.2), 6.5 around
+// them; a step of 64 positions by 256 rows 2.9, 14 around them; partial states are written and read at about 4 TB/s, by one more launch.  The cut of the least sum
+// is taken.  Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 160 rows 66 and 60 us, 8 x 96 167 and 266, 8 x 256 386 and 208, 8 x 512
+// 777 and 410; 500 cached: 256 rows 20 and 39, 8 x 256 99 and 57; fp16 pages: 40 rows 48 and 50, 96 rows 97 and 53.  Splits of tiles of 256: 512 rows after 4001
+// 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave per SIMD, were slower than 32 everywhere, by up to 3 times.)
 struct ChunkPlan {
     int nb, nw, tiles, splits;
 };
-ChunkPlan chunk_plan(int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
+ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
+    const bool even = max_new_len > 0 && max_new_len <= tokens && max_new_len * batch == tokens;
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     const int64_t rows = max_new_len * group, cus = qr_device().cus;
-    ChunkPlan p;
-    p.nb = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 128 ? 4 : 0;
-    const int64_t per = p.nb ? 16 * p.nb : 256, tiles = (rows + per - 1) / per;
-    p.tiles = (int)(tiles > 4096 ? 4096 : tiles);          // (a workgroup goes on to the next tile behind them)
     int64_t seen = max_seq_len > 0 ? max_seq_len : 0;
     if (window > 0 && seen > window + max_new_len + sinks + 64) seen = window + max_new_len + sinks + 64;
-    const int64_t groups = batch * num_heads * p.tiles, steps = (seen + 31) / 32;
-    p.nw = p.nb == 4 || groups >= 2 * cus ? 4 : 8;
-    int64_t splits = p.nb ? ((p.nw == 8 ? 1 : 2) * cus + groups - 1) / groups : cus / groups;
-    if (splits > steps / (2 * p.nw)) splits = steps / (2 * p.nw);                // (two steps per wave at least)
-    if (splits > 32) splits = 32;
-    p.splits = splits < 1 ? 1 : (int)splits;
+    ChunkPlan p{1, 4, 1, 1};
+    if (rows <= 16) {
+        const int64_t groups = batch * num_heads, steps = (seen + 31) / 32;
+        p.nw = groups >= 2 * cus ? 4 : 8;
+        int64_t splits = ((p.nw == 8 ? 1 : 2) * cus + groups - 1) / groups;
+        if (splits > steps / (2 * p.nw)) splits = steps / (2 * p.nw);            // (two steps per wave at least)
+        p.splits = splits < 1 ? 1 : splits > 32 ? 32 : (int)splits;
+        return p;
+    }
+    float least = -1.f;
+    auto consider = [&](int nb, int nw, int64_t per, int64_t at_once, int64_t step, float each, float around) {
+        const int64_t tiles = (rows + per - 1) / per;
+        int64_t groups = batch * tiles;
+        if (!even) {                                       // (a ragged batch's tiles are guessed)
+            int64_t some = tokens * group / per + batch / 2;
+            if (some < batch) some = batch;
+            if (some < groups) groups = some;
+        }
+        groups *= num_heads;
+        const int64_t late = max_new_len - per / group;    // (what the first tile does not see of the last one's positions, at most)
+        const float steps = (float)(seen - (late > 0 ? (late < seen ? late : seen) / 2 : 0)) / (float)step;
+        for (int s = 1; s <= 32; ++s) {
+            if (s > 1 && steps < (float)(3 * s)) break;
+            const float turns = (float)((int64_t)(steps / (float)s) + 1);
+            const float time = (float)((groups * s + at_once - 1) / at_once) * (turns * each + around) +
+                               (s > 1 ? 6.f + (float)(tokens * group * num_heads) * (float)s * (1056.f / 4e6f) : 0.f);
+            if (least < 0.f || time < least) least = time, p = ChunkPlan{nb, nw, (int)(tiles > 4096 ? 4096 : tiles), s};       // (a workgroup goes on to the next tile behind them)
+        }
+    };
+    const float small = fp16 ? 7.2f : 3.f;
+    consider(2, 8, 32, cus, 32 * 8, small, 6.5f);
+    consider(2, 4, 32, 2 * cus, 32 * 4, small, 6.5f);
+    consider(0, 4, 256, cus, 64, 2.9f, 14.f);
     return p;
 }
 
 template <bool F16, bool ALIGNED>
 int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st) {
     using Kernel = void (*)(Chunk, Divisor);
-    const Kernel kernel = plan.nb == 4   ? chunk_rows_kernel<4, 4, F16, ALIGNED>
-                          : plan.nb == 2 ? (plan.nw == 8 ? chunk_rows_kernel<2, 8, F16, ALIGNED> : chunk_rows_kernel<2, 4, F16, ALIGNED>)
-                                         : (plan.nw == 8 ? chunk_rows_kernel<1, 8, F16, ALIGNED> : chunk_rows_kernel<1, 4, F16, ALIGNED>);
+    const Kernel kernel = plan.nb == 2 ? (plan.nw == 8 ? chunk_rows_kernel<2, 8, F16, ALIGNED> : chunk_rows_kernel<2, 4, F16, ALIGNED>)
+                                       : (plan.nw == 8 ? chunk_rows_kernel<1, 8, F16, ALIGNED> : chunk_rows_kernel<1, 4, F16, ALIGNED>);
     const size_t lds = (size_t)plan.nw * 16 * 33 * sizeof(f32x4);
     const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, lds);
     if (e != hipSuccess) return (int)e;
@@ -534,7 +565,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || q_stride % 8 || o_stride % 8) return QR_E_ALIGN;
     const int64_t width = (int64_t)num_q_heads * 128;
     if (q_stride < width || o_stride < width || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024) return QR_E_SHAPE;
-    const ChunkPlan plan = chunk_plan(tokens, num_q_heads / num_heads, num_heads, batch_size, seqlen_indptr_or_null ? max_new_len : 1, max_seq_len, window, sinks);
+    const ChunkPlan plan = chunk_plan(fp16, tokens, num_q_heads / num_heads, num_heads, batch_size, seqlen_indptr_or_null ? max_new_len : 1, max_seq_len, window, sinks);
     Chunk a;
     a.c = qr_internal_paged_kv((void*)kv_data, (void*)kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,
                                page_size, batch_size);
@@ -569,10 +600,10 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
 
 }  // namespace
 
-extern "C" size_t qr_batch_chunk_workspace_bytes(int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
+extern "C" size_t qr_batch_chunk_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                                  int64_t max_seq_len, int64_t window, int64_t sinks) {
     if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0) return 0;
-    const int splits = chunk_plan(tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, max_seq_len, window, sinks).splits;
+    const int splits = chunk_plan(fp16_pages != 0, tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, max_seq_len, window, sinks).splits;
     return chunk_part_bytes(tokens, num_q_heads, splits);
 }
 

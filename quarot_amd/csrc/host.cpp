@@ -603,7 +603,7 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         bound < 0 || window < 0 || sinks < 0)
         return none();
     if (!seq) fresh_bound = 1;
-    const size_t need = qr_batch_chunk_workspace_bytes(tokens, (int)heads, c.heads, c.batch, fresh_bound, bound, window, sinks);
+    const size_t need = qr_batch_chunk_workspace_bytes(fp16_pages ? 1 : 0, tokens, (int)heads, c.heads, c.batch, fresh_bound, bound, window, sinks);
     const bool kept = need && ws && (size_t)ws->numel() >= need;
     at::Tensor own;
     const auto call = [&] {

@@ -324,7 +324,7 @@ def _chunk(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
     if window < 0 or sinks < 0 or max_new_len < 0 or max_seq_len < 0:
         raise RuntimeError(f"{fn}: window, sinks and the lengths must not be negative")
     with _lib.on_device(dev):
-        ws_bytes = _lib.lib().qr_batch_chunk_workspace_bytes(tokens, q_heads, heads, batch, 1 if seqlen_indptr is None else max_new_len,
+        ws_bytes = _lib.lib().qr_batch_chunk_workspace_bytes(1 if f16 else 0, tokens, q_heads, heads, batch, 1 if seqlen_indptr is None else max_new_len,
                                                              max_seq_len, window, sinks)
         ws = None
         if ws_bytes:
