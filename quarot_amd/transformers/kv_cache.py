@@ -431,7 +431,8 @@ def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_
 
 class _AttentionStub(object):
     """What MultiLayerPagedKVCache4Bit.update hands back for a decode step (kv_cache.py:104-129): called
-    with the query states it runs attention over the cache."""
+    with the query states it runs attention over the cache.  Several new tokens, a window, or more query heads than
+    the cache has go to batch_chunk_i4 / batch_chunk_f16."""
 
     def __init__(self, cache_page_size, device, n_layers, disable_quant, hadamard_dtype):
         self.cache_page_size = cache_page_size
@@ -439,9 +440,14 @@ class _AttentionStub(object):
         self.disable_quant = disable_quant
         self.hadamard_dtype = hadamard_dtype
 
-    def forward(self, q, num_kv_heads, attention_kwargs, layer_idx, max_seq_len=0, cache=None, token=None):
-        _, q_len, _, _ = q.shape
-        assert q_len == 1
+    def forward(self, q, num_kv_heads, attention_kwargs, layer_idx, max_seq_len=0, cache=None, token=None, added=1, window=0, sinks=0):
+        _, q_len, num_qo_heads, _ = q.shape
+        assert q_len == added
+        if added > 1 or window or num_qo_heads != num_kv_heads:
+            held = cache._pending.get(layer_idx) if cache is not None else None
+            if held is not None and held[0] is token:
+                cache._flush(layer_idx)
+            return self._attend_chunk(q, attention_kwargs, layer_idx, max_seq_len, window, sinks)
         o = workspace = held = None
         if cache is not None:
             # the step's new token, if the cache still holds it back for this call (see MultiLayerPagedKVCache4Bit.update; otherwise it
@@ -463,6 +469,19 @@ class _AttentionStub(object):
         if held is not None:
             cache._pending.pop(layer_idx, None)
         return o
+
+    def _attend_chunk(self, q, attention_kwargs, layer_idx, max_seq_len, window, sinks):
+        batch_size, q_len, num_qo_heads, head_dim = q.shape
+        q = q.reshape(batch_size * q_len, num_qo_heads, head_dim)
+        fused = self.hadamard_dtype == torch.float16 and q.dtype == torch.float16
+        if self.hadamard_dtype is not None and not fused:
+            q = matmul_had_cuda(q.contiguous(), dtype=self.hadamard_dtype)
+        attn_output = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        starts = torch.arange(batch_size + 1, device=q.device, dtype=torch.int32) * q_len if q_len > 1 else None
+        attend = batch_chunk_f16 if self.disable_quant else batch_chunk_i4
+        attend(attn_output, q, **attention_kwargs, layer_idx=layer_idx, seqlen_indptr=starts, max_new_len=q_len, max_seq_len=max_seq_len,
+               window=window, sinks=sinks, q_hadamard=fused)
+        return attn_output.view(batch_size, q_len, num_qo_heads, head_dim)
 
     def _attend(self, q, attention_kwargs, layer_idx, max_seq_len, workspace, held):
         append = None
@@ -492,15 +511,20 @@ _MAX_WORKSPACES = 8      # streams whose decode workspace a cache keeps
 class MultiLayerPagedKVCache4Bit:
     """Paged int4 KV cache of all layers with the interface of kv_cache.py:132-289: `update` quantises
     and stores the new keys and values (the first call per layer takes the whole prompt and returns the
-    fp16 states for the prefill's own attention; later calls take one token per sequence and return a
-    callable that runs decode attention over the cache).  Keys pass through the Hadamard transform over
-    the head dimension before quantisation, queries before attention (hadamard_dtype, None to skip).
+    fp16 states for the prefill's own attention; later calls take one token per sequence, or as many more of each -- a
+    further turn, drafted tokens -- and return a callable that runs attention over the cache, causal among the new tokens).
+    Keys pass through the Hadamard transform over the head dimension before quantisation, queries before attention
+    (hadamard_dtype, None to skip).  The callable takes any multiple of num_heads as query heads.  window > 0: it lets a token see the
+    last `window` positions, its own among them, and the first `sinks`.
     The reference derives the class from transformers' Cache for the methods that base supplied in the
     version it pins (get_usable_length); they are defined here instead, so the class does not depend on the
     installed transformers version."""
 
     def __init__(self, batch_size, page_size, max_seq_len, device, n_layers, num_heads, head_dim, disable_quant=False,
-                 hadamard_dtype=torch.float16):
+                 hadamard_dtype=torch.float16, window=0, sinks=0):
+        if window < 0 or sinks < 0:
+            raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
+        self.window, self.sinks = int(window), int(sinks)
         self.page_size = page_size
         self.batch_size = batch_size
         max_page_cnt = self.page_cnt_from_length(max_seq_len)
@@ -638,7 +662,14 @@ class MultiLayerPagedKVCache4Bit:
                                       v=value_states.reshape(-1, num_heads, head_dim).contiguous(), seqlen_indptr=seqlens,
                                       layer_idx=layer_idx, hadamard=fused_had)
             return key_states, value_states
-        assert added_length == 1
+        attend = functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
+                                   max_seq_len=self.length)
+        if added_length > 1 or self.window:
+            starts = torch.arange(b_sz + 1, device=self.device, dtype=torch.int32) * added_length if added_length > 1 else None
+            quantize_append_kv_i4(**specs, k=k_in.reshape(-1, num_heads, head_dim).contiguous(),
+                                  v=value_states.reshape(-1, num_heads, head_dim).contiguous(), seqlen_indptr=starts, layer_idx=layer_idx,
+                                  hadamard=fused_had)
+            return functools.partial(attend, added=added_length, window=self.window, sinks=self.sinks)
         k1, v1 = k_in.contiguous(), value_states.contiguous()
         if k1.dtype == torch.float16 and v1.dtype == torch.float16 and head_dim == 128:
             # held for the attention call, which quantises and stores the token itself
@@ -648,8 +679,7 @@ class MultiLayerPagedKVCache4Bit:
             quantize_append_kv_i4(**specs, k=k1.view(b_sz, num_heads, head_dim), v=v1.view(b_sz, num_heads, head_dim),
                                   seqlen_indptr=None, layer_idx=layer_idx, hadamard=fused_had)
             token = None
-        return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
-                                 max_seq_len=self.length, cache=self, token=token)
+        return functools.partial(attend, cache=self, token=token)
 
     def _update_f16(self, key_states, value_states, layer_idx, attention_mask, first, specs):
         """update() with fp16 pages (kv_cache.py:187-251 with disable_quant): the transformed keys and the values are
@@ -672,9 +702,13 @@ class MultiLayerPagedKVCache4Bit:
                 seqlens = torch.arange(self.batch_size + 1, device=self.device, dtype=torch.int32) * added_length
             init_kv_f16(**specs, k=k, v=v, k_param=param, v_param=param, seqlen_indptr=seqlens, layer_idx=layer_idx)
             return key_states, value_states
-        assert added_length == 1
-        append_kv_f16(**specs, k=k, v=v, k_param=param, v_param=param, layer_idx=layer_idx)
-        return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx)
+        if added_length > 1:
+            starts = torch.arange(self.batch_size + 1, device=self.device, dtype=torch.int32) * added_length
+            init_kv_f16(**specs, k=k, v=v, k_param=param, v_param=param, seqlen_indptr=starts, layer_idx=layer_idx)
+        else:
+            append_kv_f16(**specs, k=k, v=v, k_param=param, v_param=param, layer_idx=layer_idx)
+        return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
+                                 max_seq_len=self.length, added=added_length, window=self.window, sinks=self.sinks)
 
     def get_cache_specs_for_flash_infer(self, attention_mask):
         """Page tables of the current state (kv_cache.py:253-275): page i of sequence b is page number
