@@ -44,10 +44,9 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
     int id = blockIdx.x;
     const int split = id % a.splits;
     id /= a.splits;
-    const int first_tile = id % a.tiles;
-    id /= a.tiles;
-    const int h = id % c.num_heads, b = id / c.num_heads;
-
+    const int h = id % c.num_heads;
+    int b, first_tile;
+    if (!item_of<16 * NB>(a, id / c.num_heads, b, first_tile)) return;
     const Fresh mine_tokens = fresh_of(a, b);
     const int start = mine_tokens.start, fresh = mine_tokens.count;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;

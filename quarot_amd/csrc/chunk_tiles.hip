@@ -79,13 +79,11 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     int id = blockIdx.x;
     const int split = id % a.splits;
     id /= a.splits;
-    const int pairs = c.num_heads * c.batch_size;
-    const int pair = id % pairs;                           // (sequence, key head): neighbours are on different XCDs, a pair's tiles on one where 8 divides their number
-    const int tile = a.tiles - 1 - id / pairs;             // the tiles with most positions first
-    const int b = pair / c.num_heads, head = pair - b * c.num_heads;
+    const int head = id % c.num_heads;                     // neighbours are on different XCDs, a head's tiles on one where 8 divides the heads
+    int b, tile;
+    if (!item_of<kRows>(a, id / c.num_heads, b, tile)) return;
     const Fresh tokens = fresh_of(a, b);
     const int rows = tokens.count * a.group;
-    if (tile * kRows >= rows) return;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;

@@ -124,6 +124,45 @@ __device__ __forceinline__ Fresh fresh_of(const Chunk& a, int b) {
     return Fresh{start, end > start ? end - start : 0};
 }
 
+__device__ __forceinline__ int lanes_sum(int v) {          // over the wave
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);       // row_shr 1, 2, 4, 8: a row's last lane has its sum
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);       // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return __builtin_amdgcn_readlane(v, 63);
+}
+// Work item `number` of a head: a sequence and one of its tiles of PER rows, last tiles (most positions) first; false: there is none.  Items without rows come
+// last: between others they leave whole shader engines idle, since workgroups are handed out to them in turn (8 sequences of 2048, 1792 .. 256 tokens, 64 on 8
+// heads: 552 us with them, 383 without).  Of more than 64 sequences the tiles are not counted.
+template <int PER>
+__device__ __forceinline__ bool item_of(const Chunk& a, int number, int& b, int& tile) {
+    const int batch = a.c.batch_size;
+    if (a.tiles == 1 || batch > 64) {
+        tile = a.tiles == 1 ? 0 : a.tiles - 1 - number / batch;
+        b = a.tiles == 1 ? number : number % batch;
+        return tile * PER < fresh_of(a, b).count * a.group;
+    }
+    const int lane = threadIdx.x & 63;
+    const int held = (fresh_of(a, lane < batch ? lane : 0).count * a.group + PER - 1) / PER;
+    const int mine = lane >= batch ? 0 : held < a.tiles ? held : a.tiles;
+    auto above = [&](int t) { return lanes_sum(mine > t ? mine - t : 0); };      // tiles t and higher of all sequences
+    if (above(0) <= number) return false;
+    int low = 0, high = a.tiles;                           // above(low) > number >= above(high)
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (above(mid) > number) low = mid;
+        else high = mid;
+    }
+    tile = low;
+    const int rank = number - above(low + 1);
+    const uint64_t who = __builtin_amdgcn_ballot_w64(mine > low);
+    const int before = __builtin_amdgcn_mbcnt_hi((u32)(who >> 32), __builtin_amdgcn_mbcnt_lo((u32)who, 0));
+    b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(mine > low && before == rank));
+    return true;
+}
+
 // The positions that the rows of a tile see, in steps of 1 << LOG: steps [0, near) hold the sinks, then [far, far + rest).
 struct Steps {
     int near, far, all;
