@@ -606,7 +606,14 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 #pragma unroll
             for (int i = 0; i < 4; ++i) place_key(fk, k0, i);
             place_key_line(fk, key_line(fk), k0);
-            place_values_any(fv, v0);
+            u32 power[2];
+            if (!F16 && regular(fv, power, true)) {
+                place_value(fv, v0, 0, power);
+                place_value(fv, v0, 1, power);
+                place_value_parameters(fv.p, 0, v0);
+            } else {
+                place_values_any(fv, v0);
+            }
             fetch_keys(fk, all2);
 #pragma unroll
             for (int i = 0; i < 4; ++i) place_key(fk1, k1, i);
@@ -628,7 +635,16 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     y[cb][i] = F16 ? __builtin_fmaf(x[cb][i], kLog2e * kScale, -m[cb]) : __builtin_fmaf(x[cb][i], slopes[i >> 2][i & 3], t[cb][i]);
-            hide(position(s_begin));
+            if (!F16 && all_seen(position(s_begin)) && ~__builtin_amdgcn_readfirstlane(there) == 0) {
+#pragma unroll
+                for (int cb = 0; cb < 2; ++cb) {
+                    most[cb] = y[cb][0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) most[cb] = __builtin_fmaxf(most[cb], y[cb][i]);
+                }
+            } else {
+                hide(position(s_begin));
+            }
             begin();
             ask_keys(k0, 1);
         }
