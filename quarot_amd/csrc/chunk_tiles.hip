@@ -548,6 +548,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             for (int i = 0; i < 4; ++i) slopes[i] = *(const f32x4*)(lds + (s_from + kbuf) + kb * 128 + (i >> 1) * 64 + (i & 1) * 16);
         };
         auto first_product = [&](uint32_t kbuf, int kb, uint32_t vbuf, int unit, bool with_weights, auto&& other) INLINE {
+            float ahead[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
 #pragma unroll
@@ -555,9 +556,16 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                     if (i == 0) mfma_first(x[cb], kp[i % 3], qf[cb][i]);
                     else mfma_more(x[cb], kp[i % 3], qf[cb][i]);
                     if (with_weights) {
-                        u32 w = weights(y[cb], i >> 2, i & 3);
-                        asm volatile("" : "+v"(w));        // (here, not behind the question whether they are made anew)
-                        p[cb][i >> 2][i & 3] = w;
+                        // (a pair's exponentials in one slot, their conversion in the next; here, not behind the question whether they are made anew)
+                        float w0 = __builtin_amdgcn_exp2f(y[cb][2 * i]), w1 = __builtin_amdgcn_exp2f(y[cb][2 * i + 1]);
+                        if (i + cb > 0) {
+                            const int j = cb ? i : i - 1;
+                            u32 w = cvt_f16x2(ahead[0], ahead[1]);
+                            asm volatile("" : "+v"(w));
+                            p[cb ^ 1][j >> 2][j & 3] = w;
+                        }
+                        asm volatile("" : "+v"(w0), "+v"(w1));
+                        ahead[0] = w0, ahead[1] = w1;
                         if (cb == 0 && i == 1) grow = __builtin_amdgcn_ballot_w64(most[0] > limit[0] || most[1] > limit[1]) != 0;
                     }
                     if (cb == 0) other(i);
@@ -567,6 +575,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                     SLOT;
                 }
             }
+            if (with_weights) p[1][1][3] = cvt_f16x2(ahead[0], ahead[1]);
         };
         // Second product of the unit at work; between it the logits of the next one, unit next_kb of the keys at kbuf, from its first product and their line,
         // and their maxima.
