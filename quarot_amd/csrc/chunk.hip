@@ -407,7 +407,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
         }
 
         // ---- merge: a wave's states are those of its rows; the waves' through LDS, one block of 16 rows at a time
-        constexpr int LANES = 4 * NW, PER = 32 / LANES;    // threads of a row, and of its 32 pieces of four dimensions how many each takes
+        constexpr int LANES = NW < 8 ? 4 * NW : 32, PER = 32 / LANES;        // threads of a row, and of its 32 pieces of four dimensions how many each takes
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const float dd = quarters_sum(d[nb]), zz = F16 ? 0.f : quarters_sum(pz[nb]);
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
             }
             __syncthreads();
             const int row = threadIdx.x / LANES, l = threadIdx.x % LANES, r = r0 + 16 * nb + row;
-            if (r < rows) {
+            if (row < 16 && r < rows) {
                 float M = kEmpty, D = 0.f;
 #pragma unroll
                 for (int w = 0; w < NW; ++w) M = __builtin_fmaxf(M, st4[(w * 16 + row) * 33][0]);
@@ -500,7 +500,10 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
 // How a call is cut: column blocks and waves of a workgroup (nb 0: the kernel of 256 rows), tiles of rows per (sequence, key head), splits of the
 // positions.
 //
-// 16 rows and fewer read the cache once, whoever does it: as many workgroups as fill the chip.  More rows are a choice between tiles of 32, each of which reads and
+// 16 rows and fewer read the cache once, whoever does it.  Int4 pages: twelve waves to a compute unit, in one workgroup where there are sequences and heads enough,
+// or little to read (one token, 64 on 8 heads: 64 x 2000 36 us, 8 waves 40; 32 x 500 10.4 and 12.3), else in three, split (4 x 4000, 32 heads: 23.6 us; 8 waves,
+// split in two 28), or one with the most splits there are (30000, 64 on 8 heads: 22.5; in three 26.8).  Fp16 pages want fewer: 8, or 2 x 4 (64 x 1000, 32 heads: 138 us;
+// 12 waves 178).  More rows are a choice between tiles of 32, each of which reads and
 // unpacks the cache for itself, and tiles of 256, whose workgroups have a compute unit to themselves and a long way to their first product.  Microseconds, from
 // the two kernels' own times: a wave's step of 32 positions by 32 rows 3.0 with two waves per SIMD (fp16 pages, which reach the caches' bandwidth, 7.2), 6.5 around
 // them; a step of 64 positions by 256 rows 2.9, 14 around them; partial states are written and read at about 4 TB/s, by one more launch.  The cut of the least sum
@@ -519,9 +522,20 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
     ChunkPlan p{1, 4, 1, 1};
     if (rows <= 16) {
         const int64_t groups = batch * num_heads, steps = (seen + 31) / 32;
-        p.nw = groups >= 2 * cus ? 4 : 8;
-        int64_t splits = ((p.nw == 8 ? 1 : 2) * cus + groups - 1) / groups;
-        if (splits > steps / (2 * p.nw)) splits = steps / (2 * p.nw);            // (two steps per wave at least)
+        int64_t splits = 1;
+        if (fp16) {
+            p.nw = groups >= 2 * cus ? 4 : 8;
+            splits = ((p.nw == 8 ? 1 : 2) * cus + groups - 1) / groups;
+            if (splits > steps / (2 * p.nw)) splits = steps / (2 * p.nw);        // (two steps per wave at least)
+        } else if (groups >= cus || steps <= 24) {
+            p.nw = steps <= 8 ? 4 : 12;
+        } else if (32 * groups >= 3 * cus) {
+            splits = (3 * cus + groups - 1) / groups;
+            if (splits > steps / 4) splits = steps / 4;
+        } else {
+            p.nw = 12;
+            splits = steps / 12 < cus / groups ? steps / 12 : cus / groups;
+        }
         p.splits = splits < 1 ? 1 : splits > 32 ? 32 : (int)splits;
         return p;
     }
@@ -556,7 +570,7 @@ template <bool F16, bool ALIGNED>
 int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st) {
     using Kernel = void (*)(Chunk, Divisor);
     const Kernel kernel = plan.nb == 2 ? (plan.nw == 8 ? chunk_rows_kernel<2, 8, F16, ALIGNED> : chunk_rows_kernel<2, 4, F16, ALIGNED>)
-                                       : (plan.nw == 8 ? chunk_rows_kernel<1, 8, F16, ALIGNED> : chunk_rows_kernel<1, 4, F16, ALIGNED>);
+                                       : (plan.nw == 4 ? chunk_rows_kernel<1, 4, F16, ALIGNED> : chunk_rows_kernel<1, F16 ? 8 : 12, F16, ALIGNED>);
     const size_t lds = (size_t)plan.nw * 16 * 33 * sizeof(f32x4);
     const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, lds);
     if (e != hipSuccess) return (int)e;
