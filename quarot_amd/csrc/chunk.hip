@@ -507,8 +507,8 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
 // unpacks the cache for itself, and tiles of 256, whose workgroups have a compute unit to themselves and a long way to their first product.  Microseconds, from
 // the two kernels' own times: a wave's step of 32 positions by 32 rows 3.0 with two waves per SIMD (fp16 pages, which reach the caches' bandwidth, 7.2), 6.5 around
 // them; a step of 64 positions by 256 rows 2.9, 14 around them; partial states are written and read at about 4 TB/s, by one more launch.  The cut of the least sum
-// is taken.  Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 160 rows 66 and 60 us, 8 x 96 167 and 266, 8 x 256 386 and 208, 8 x 512
-// 777 and 410; 500 cached: 256 rows 20 and 39, 8 x 256 99 and 57; fp16 pages: 40 rows 48 and 50, 96 rows 97 and 53.  Splits of tiles of 256: 512 rows after 4001
+// is taken.  Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 192 rows 54 and 54 us, 8 x 96 170 and 190, 8 x 192 300 and 207, 8 x 256
+// 387 and 211; 500 cached: 256 rows 19 and 39, 8 x 256 97 and 58; fp16 pages: 40 rows 41 and 42, 96 rows 61 and 45.  Splits of tiles of 256: 512 rows after 4001
 // 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave per SIMD, were slower than 32 everywhere, by up to 3 times.)
 struct ChunkPlan {
     int nb, nw, tiles, splits;

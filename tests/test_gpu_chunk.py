@@ -411,3 +411,14 @@ def test_infinities_and_nans_reach_only_rows_that_see_them(lens, news, heads, gr
                 assert torch.equal(o[t][:, rest], clean[t][:, rest]), (k, t)
             elif side == 1:
                 assert not bool(torch.isfinite(o[t]).any()), (k, t)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("batch,most,group", [(64, 40, 4), (65, 40, 4), (70, 70, 8), (130, 3, 8)])
+def test_many_sequences(batch, most, group, f16):
+    """Ragged batches whose work items are counted (64 sequences) and are not (more), sequences without new tokens among them."""
+    news = [(7 * b) % (most + 1) for b in range(batch)]
+    lens = [n + (13 * b) % 90 for b, n in enumerate(news)]
+    specs, q, starts = make(batch, 16, lens, news, 2, group, f16)
+    check(specs, q, starts, lens, news)
+    check(specs, q, starts, lens, news, window=30, sinks=3)
