@@ -662,14 +662,13 @@ class MultiLayerPagedKVCache4Bit:
                                       v=value_states.reshape(-1, num_heads, head_dim).contiguous(), seqlen_indptr=seqlens,
                                       layer_idx=layer_idx, hadamard=fused_had)
             return key_states, value_states
-        attend = functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
-                                   max_seq_len=self.length)
         if added_length > 1 or self.window:
             starts = torch.arange(b_sz + 1, device=self.device, dtype=torch.int32) * added_length if added_length > 1 else None
             quantize_append_kv_i4(**specs, k=k_in.reshape(-1, num_heads, head_dim).contiguous(),
                                   v=value_states.reshape(-1, num_heads, head_dim).contiguous(), seqlen_indptr=starts, layer_idx=layer_idx,
                                   hadamard=fused_had)
-            return functools.partial(attend, added=added_length, window=self.window, sinks=self.sinks)
+            return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
+                                     max_seq_len=self.length, added=added_length, window=self.window, sinks=self.sinks)
         k1, v1 = k_in.contiguous(), value_states.contiguous()
         if k1.dtype == torch.float16 and v1.dtype == torch.float16 and head_dim == 128:
             # held for the attention call, which quantises and stores the token itself
@@ -679,7 +678,8 @@ class MultiLayerPagedKVCache4Bit:
             quantize_append_kv_i4(**specs, k=k1.view(b_sz, num_heads, head_dim), v=v1.view(b_sz, num_heads, head_dim),
                                   seqlen_indptr=None, layer_idx=layer_idx, hadamard=fused_had)
             token = None
-        return functools.partial(attend, cache=self, token=token)
+        return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
+                                 max_seq_len=self.length, cache=self, token=token)
 
     def _update_f16(self, key_states, value_states, layer_idx, attention_mask, first, specs):
         """update() with fp16 pages (kv_cache.py:187-251 with disable_quant): the transformed keys and the values are
