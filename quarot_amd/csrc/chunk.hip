@@ -36,7 +36,7 @@ struct There {
 
 // ALIGNED: pages of a multiple of 16 positions, so that each half of a step lies in one page.
 template <int NB, int NW, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) {
+__global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) {
     extern __shared__ __attribute__((aligned(16))) f32x4 st4[];            // per wave and row: maximum, sum, -, -, 128 outputs
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -63,21 +63,18 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
         const Steps steps = steps_of<5>(a, lowest, highest);
         const int stride = NW * a.splits;
 
-        // Loads are unconditional: a position that is not there reads the first entries of page 0 and is masked.  ALIGNED: the page numbers of a step are
-        // asked for a step ahead, so that its loads do not wait for them.
+        // Loads are unconditional: a position that is not there reads the first entries of page 0 and is masked.  ALIGNED: the page numbers of the wave's next 32
+        // steps are held by its lanes, two a step (-1: none), and taken by number: a load of its own per step would be waited for, and with it all that is under way.
         Fetched<F16> f;
-        int page_at[2] = {-1, -1};
+        int held_pages = -1, turn = 0;                     // turn: which of the 32 the step is that is fetched next
         int64_t slots[ALIGNED ? 2 : 8];                    // ALIGNED: of the step's halves; else of the lane's eight positions
-        auto ask_pages = [&](int s) {
-            if (ALIGNED && npages > 0) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const int it = divided(steps.at(s) * 32 + 16 * kb, pages);
-                    page_at[kb] = it < npages ? c.indices[p0 + it] : -1;
-                }
-            }
+        auto fetch_pages = [&](int s) {
+            const int later = s + (lane >> 1) * stride, it = divided(steps.at(later < steps.all ? later : steps.all - 1) * 32 + 16 * (lane & 1), pages);
+            const int page = npages > 0 ? c.indices[p0 + (it < npages ? it : 0)] : -1;
+            held_pages = it < npages && page < c.num_pages ? page : -1;
+            turn = 0;
         };
-        auto fetch_keys = [&](int s, int next) {
+        auto fetch_keys = [&](int s) {
             const int at = steps.at(s) * 32;
             There t{0, true};
             if (ALIGNED) {
@@ -86,15 +83,15 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
                 t.all = at + 32 <= len;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
-                    const int pos = at + 16 * kb, page = page_at[kb];
+                    const int pos = at + 16 * kb, page = __builtin_amdgcn_readlane(held_pages, 2 * turn + kb);
                     const u32 entry = (u32)(pos - divided(pos, pages) * c.page_size);
-                    const bool there = page >= 0 && page < c.num_pages && entry < (u32)c.page_size;
+                    const bool there = page >= 0 && entry < (u32)c.page_size;
                     slots[kb] = there ? page * page_slots + head_slots + entry : head_slots;
                     const uint8_t* const kd = c.data + slots[kb] * VEC;
                     if (!there) t.all = false;
                     else t.ok |= 15u << (4 * kb);
 #pragma unroll
-                    for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[F16 ? 4 * kb + i : kb] = __builtin_nontemporal_load((const u32x4*)(kd + k_off + 64 * i));
+                    for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[F16 ? 4 * kb + i : kb] = *(const u32x4*)(kd + k_off + 64 * i);
                     if (!F16) {
                         const uint8_t* const kp = (const uint8_t*)(c.param + slots[kb]);
 #pragma unroll
@@ -106,7 +103,6 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
                     for (int k = 0; k < 8; ++k)
                         if (at + 16 * (k >> 2) + 4 * g + (k & 3) >= len) t.ok &= ~(1u << k);
                 }
-                ask_pages(next);
             } else {
                 const int pos = at + (lane & 31), it = divided(pos, pages);
                 const u32 entry = (u32)(pos - it * c.page_size);
@@ -138,7 +134,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
                 const int64_t slot = (ALIGNED ? slots[k >> 2] : slots[k % (ALIGNED ? 2 : 8)]) + kv_slots;
                 const uint8_t* const vd = c.data + slot * VEC + (ALIGNED ? v_off + VEC * (k & 3) : (uint32_t)n * (VEC / 16));
                 if (F16) {
-                    f.v4[k] = __builtin_nontemporal_load((const u32x4*)vd);
+                    f.v4[k] = *(const u32x4*)vd;
                 } else {
                     f.v[k] = *(const u32*)vd;
                     f.vp[k >> 2][k & 3] = ALIGNED ? *(const u32*)((const uint8_t*)(c.param + slot) + p_off + 4 * (k & 3)) : c.param[slot];
@@ -147,9 +143,9 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
         };
         int s = split * NW + wave;
         There there{0, false};
-        ask_pages(s);
         if (s < steps.all) {
-            there = fetch_keys(s, s + stride);
+            if (ALIGNED) fetch_pages(s);
+            there = fetch_keys(s);
             fetch_values();
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -257,7 +253,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            there = fetch_keys(next, next + stride);
+            there = fetch_keys(next);
             __builtin_amdgcn_sched_barrier(0);
             float vr[8], vz[8];                            // 1 / f and zero point / f of the values
             u32 factors[4], power[4];
@@ -400,7 +396,9 @@ __global__ __launch_bounds__(64 * NW, NB == 2 ? 2 : 3) void chunk_rows_kernel(Ch
         };
 
         for (; s < steps.all; s += stride) {
-            consume(s, s + stride < steps.all ? s + stride : s);       // (behind the last step the next one is the same again)
+            const int next = s + stride < steps.all ? s + stride : s;  // (behind the last step the next one is the same again)
+            if (ALIGNED && next != s && ++turn == 32) fetch_pages(next);
+            consume(s, next);
             __builtin_amdgcn_sched_barrier(0);
             fetch_values();
             __builtin_amdgcn_sched_barrier(0);
