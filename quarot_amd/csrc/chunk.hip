@@ -152,7 +152,8 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
 
         // the queries: lane (n, g) holds dimensions 32 g + 8 i .. + 7 (fp16 pages: 32 i + 8 g ..), i = 0 .. 3, of row n of every block
         u32x4 qf[NB][4];
-        float qsum[NB];                                    // -log2(e) / sqrt(128) times the row's sum
+        float qsum[NB];                                    // minus the row's sum, in units of the products'
+        constexpr float kUnit = kLog2e * kScale * (F16 ? 1.f : kCodeUnit);         // of a logit, base 2
         int place[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -197,11 +198,12 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                 const f16x2 p = as_f16x2(w[i >> 2][i & 3]);
                 sum += (float)p[0] + (float)p[1];
             }
-            qsum[nb] = quarters_sum(sum) * -(kLog2e * kScale);
+            qsum[nb] = quarters_sum(sum) * (-1.f / kCodeUnit);
 #pragma unroll
             for (int i = 0; i < 4; ++i) qf[nb][i] = F16 ? w[i] : query_for_codes(w[i]);
         }
 
+        const CodeMasks masks = code_masks();
         float m[NB], d[NB], pz[NB];
         f32x4 acc[NB][8];
 #pragma unroll
@@ -244,14 +246,9 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                     for (int nb = 0; nb < NB; ++nb)
                         x[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(f16x8, qf[nb][i]), x[nb][kb], 0, 0, 0);
                 }
-            float ka[8], kz[8];                            // slope and zero point of the keys
-            if (!F16) {
+            u32 keys[8];                                   // {scale, zero} of the keys
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const f16x2 kp = as_f16x2(f.kp[k >> 2][k & 3]);
-                    ka[k] = __builtin_fmaf((float)kp[0], kLog2e * kScale * kCodeUnit, 0.f), kz[k] = (float)kp[1];
-                }
-            }
+            for (int k = 0; k < 8; ++k) keys[k] = F16 ? 0u : f.kp[F16 ? 0 : k >> 2][k & 3];
             __builtin_amdgcn_sched_barrier(0);
             there = fetch_keys(next);
             __builtin_amdgcn_sched_barrier(0);
@@ -285,7 +282,8 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                 float y[8], top = -__builtin_inff();
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    y[k] = F16 ? x[nb][k >> 2][k & 3] * (kLog2e * kScale) : __builtin_fmaf(x[nb][k >> 2][k & 3], ka[k], kz[k] * qsum[nb]);
+                    const f16x2 kp = as_f16x2(keys[k]);
+                    y[k] = F16 ? x[nb][k >> 2][k & 3] : __builtin_fmaf(x[nb][k >> 2][k & 3], (float)kp[0], (float)kp[1] * qsum[nb]);
                 }
                 if (!whole) {
 #pragma unroll
@@ -298,6 +296,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) top = __builtin_fmaxf(top, y[k]);
+                top *= kUnit;
                 if (__builtin_amdgcn_ballot_w64(top > m[nb] + kGrow)) {
                     const float high = quarters_max(top), now = high > m[nb] + kGrow ? high : m[nb], keep = __builtin_amdgcn_exp2f(m[nb] - now);      // (of the row alone)
                     m[nb] = now;
@@ -307,7 +306,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float w0 = __builtin_amdgcn_exp2f(y[2 * k] - m[nb]), w1 = __builtin_amdgcn_exp2f(y[2 * k + 1] - m[nb]);
+                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * k], kUnit, -m[nb])), w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[2 * k + 1], kUnit, -m[nb]));
                     const u32 w = F16 ? cvt_f16x2(w0, w1) : scaled_pair(w0, w1, factors[k]);
                     p[nb][k] = w;
                     const f16x2 r = as_f16x2(w);
@@ -390,7 +389,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                                 acc[nb][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v[i]), __builtin_bit_cast(f16x8, p[nb]), acc[nb][4 * half + i], 0, 0, 0);
                     }
                 };
-                if (__builtin_expect(plain, 1)) product([&](u32 w, int k) { return scaled_codes(w, power[k]); });
+                if (__builtin_expect(plain, 1)) product([&](u32 w, int k) { return scaled_codes(w, power[k], masks); });
                 else product([&](u32 w, int k) { return scaled_codes_slow(w, f.vp[k >> 1][2 * k & 3], f.vp[k >> 1][(2 * k & 3) + 1]); });
             }
         };

@@ -92,7 +92,28 @@ __device__ __forceinline__ u32 scaled_pair(float w0, float w1, u32 factors) {
     return r;
 }
 // w: four codes of one vector in the low half, of another in the high half -> code 2^e of both, code by code: (1024 + code) 2^e - 1024 2^e is exact
-__device__ __forceinline__ u32x4 scaled_codes(u32 w, u32 power) {
+struct CodeMasks {                     // in registers: a literal for the mask and one for the exponent are more than one instruction takes
+    u32 low, high;
+};
+__device__ __forceinline__ CodeMasks code_masks() {
+    CodeMasks m{0x000F000Fu, 0x00F000F0u};
+    asm("" : "+v"(m.low), "+v"(m.high));
+    return m;
+}
+__device__ __forceinline__ u32 and_or(u32 w, u32 mask, u32 bits) {
+    u32 r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "v"(mask), "s"(bits));
+    return r;
+}
+__device__ __forceinline__ u32x4 scaled_codes(u32 w, u32 power, CodeMasks m) {
+    const u32 w8 = w >> 8;
+    const f16x2 p = as_f16x2(power), lo = p * f16x2{(f16)-1024.f, (f16)-1024.f}, hi = p * f16x2{(f16)-64.f, (f16)-64.f};
+    return u32x4{__builtin_bit_cast(u32, __builtin_elementwise_fma(as_f16x2(and_or(w, m.low, 0x64006400u)), p, lo)),
+                 __builtin_bit_cast(u32, __builtin_elementwise_fma(as_f16x2(and_or(w, m.high, 0x54005400u)), p, hi)),
+                 __builtin_bit_cast(u32, __builtin_elementwise_fma(as_f16x2(and_or(w8, m.low, 0x64006400u)), p, lo)),
+                 __builtin_bit_cast(u32, __builtin_elementwise_fma(as_f16x2(and_or(w8, m.high, 0x54005400u)), p, hi))};
+}
+__device__ __forceinline__ u32x4 scaled_codes(u32 w, u32 power) {              // (two registers less)
     const u32 w8 = w >> 8;
     const f16x2 p = as_f16x2(power), lo = p * f16x2{(f16)-1024.f, (f16)-1024.f}, hi = p * f16x2{(f16)-64.f, (f16)-64.f};
     return u32x4{__builtin_bit_cast(u32, __builtin_elementwise_fma(as_f16x2((w & 0x000F000Fu) | 0x64006400u), p, lo)),
