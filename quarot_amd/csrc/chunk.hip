@@ -497,16 +497,18 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
 // How a call is cut: column blocks and waves of a workgroup (nb 0: the kernel of 256 rows), tiles of rows per (sequence, key head), splits of the
 // positions.
 //
-// 16 rows and fewer read the cache once, whoever does it.  Int4 pages: twelve waves to a compute unit, in one workgroup where there are sequences and heads enough,
-// or little to read (one token, 64 on 8 heads: 64 x 2000 36 us, 8 waves 40; 32 x 500 10.4 and 12.3), else in three, split (4 x 4000, 32 heads: 23.6 us; 8 waves,
-// split in two 28), or one with the most splits there are (30000, 64 on 8 heads: 22.5; in three 26.8).  Fp16 pages want fewer: 8, or 2 x 4 (64 x 1000, 32 heads: 138 us;
-// 12 waves 178).  More rows are a choice between tiles of 32, each of which reads and
-// unpacks the cache for itself, and tiles of 256, whose workgroups have a compute unit to themselves and a long way to their first product.  Microseconds, from
-// the two kernels' own times: a wave's step of 32 positions by 32 rows 3.0 with two waves per SIMD (fp16 pages, which reach the caches' bandwidth, 7.2), 6.5 around
-// them; a step of 64 positions by 256 rows 2.9, 14 around them; partial states are written and read at about 4 TB/s, by one more launch.  The cut of the least sum
-// is taken.  Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 192 rows 54 and 54 us, 8 x 96 170 and 190, 8 x 192 300 and 207, 8 x 256
-// 387 and 211; 500 cached: 256 rows 19 and 39, 8 x 256 97 and 58; fp16 pages: 40 rows 41 and 42, 96 rows 61 and 45.  Splits of tiles of 256: 512 rows after 4001
-// 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave per SIMD, were slower than 32 everywhere, by up to 3 times.)
+// 16 rows and fewer read the cache once, whoever does it.  Int4 pages: twelve waves to a compute unit, in one workgroup where there are sequences
+// and heads enough, or little to read (one token, 64 on 8 heads: 64 x 2000 36 us, 8 waves 40; 32 x 500 10.4 and 12.3), else in three, split
+// (4 x 4000, 32 heads: 23.6 us; 8 waves, split in two 28), or one with the most splits there are (30000, 64 on 8 heads: 22.5; in three 26.8).  Fp16
+// pages have registers for two workgroups of four waves (64 x 1000, 32 heads: 104 us; one of eight 124; 2000: 12.8 in 8 splits, 15 of 8 waves).
+//
+// More rows are a choice between tiles of 32, each of which reads and unpacks the cache for itself, and tiles of 256, whose workgroups have a
+// compute unit to themselves and a long way to their first product.  Microseconds, from the two kernels' own times: a wave's step of 32
+// positions by 32 rows 2.4 with two waves per SIMD (fp16 pages, which reach the caches' bandwidth, 5.5), 6.5 around them; a step of 64
+// positions by 256 rows 2.9, 14 around them; partial states 0.17 a thousand, and 6 for one more launch.  The cut of the least sum is taken.  Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 192 rows 47 and 54 us, 8 x 96 138 and 181, 8 x 128 156 and
+// 187, 8 x 192 231 and 199, 8 x 256 299 and 205; 500 cached: 256 rows 18 and 39, 8 x 256 78 and 57; fp16 pages: 8 x 64 179 and 187, 8 x 96 369
+// and 195.  Splits of tiles of 256: 512 rows after 4001 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave per SIMD,
+// were slower than 32 everywhere, by up to 3 times.)
 struct ChunkPlan {
     int nb, nw, tiles, splits;
 };
@@ -521,9 +523,8 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
         const int64_t groups = batch * num_heads, steps = (seen + 31) / 32;
         int64_t splits = 1;
         if (fp16) {
-            p.nw = groups >= 2 * cus ? 4 : 8;
-            splits = ((p.nw == 8 ? 1 : 2) * cus + groups - 1) / groups;
-            if (splits > steps / (2 * p.nw)) splits = steps / (2 * p.nw);        // (two steps per wave at least)
+            if (groups < cus) splits = (2 * cus + groups - 1) / groups;
+            if (splits > steps / 8) splits = steps / 8;                          // (two steps per wave at least)
         } else if (groups >= cus || steps <= 24) {
             p.nw = steps <= 8 ? 4 : 12;
         } else if (32 * groups >= 3 * cus) {
@@ -552,11 +553,11 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
             if (s > 1 && steps < (float)(3 * s)) break;
             const float turns = (float)((int64_t)(steps / (float)s) + 1);
             const float time = (float)((groups * s + at_once - 1) / at_once) * (turns * each + around) +
-                               (s > 1 ? 6.f + (float)(tokens * group * num_heads) * (float)s * (1056.f / 4e6f) : 0.f);
+                               (s > 1 ? 6.f + (float)(tokens * group * num_heads) * (float)s * (660.f / 4e6f) : 0.f);
             if (least < 0.f || time < least) least = time, p = ChunkPlan{nb, nw, (int)(tiles > 4096 ? 4096 : tiles), s};       // (a workgroup goes on to the next tile behind them)
         }
     };
-    const float small = fp16 ? 7.2f : 3.f;
+    const float small = fp16 ? 5.5f : 2.4f;
     consider(2, 8, 32, cus, 32 * 8, small, 6.5f);
     consider(2, 4, 32, 2 * cus, 32 * 4, small, 6.5f);
     consider(0, 4, 256, cus, 64, 2.9f, 14.f);
@@ -567,7 +568,7 @@ template <bool F16, bool ALIGNED>
 int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st) {
     using Kernel = void (*)(Chunk, Divisor);
     const Kernel kernel = plan.nb == 2 ? (plan.nw == 8 ? chunk_rows_kernel<2, 8, F16, ALIGNED> : chunk_rows_kernel<2, 4, F16, ALIGNED>)
-                                       : (plan.nw == 4 ? chunk_rows_kernel<1, 4, F16, ALIGNED> : chunk_rows_kernel<1, F16 ? 8 : 12, F16, ALIGNED>);
+                                       : (F16 || plan.nw == 4 ? chunk_rows_kernel<1, 4, F16, ALIGNED> : chunk_rows_kernel<1, F16 ? 4 : 12, F16, ALIGNED>);
     const size_t lds = (size_t)plan.nw * 16 * 33 * sizeof(f32x4);
     const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, lds);
     if (e != hipSuccess) return (int)e;
