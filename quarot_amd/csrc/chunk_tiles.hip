@@ -13,8 +13,8 @@
 //
 // A wave has its SIMD to itself, so the vector work is laid between the matrix instructions by hand, in slots: while the first product of the
 // next 32 positions runs, the weights of these 32; while their second product runs, the logits of the next, and the unpacking of what the
-// workgroup needs a step later.  2048 tokens after 30720, 64 on 8 heads: 2.4 ms, 880 TFLOP/s, 1046 with the products for the sums and the lines;
-// a step takes 5200 cycles, 2432 of them matrix instructions, at the 2.0 - 2.2 GHz that its power allows (a large library product: 1140).
+// workgroup needs a step later.  2048 tokens after 30720, 64 on 8 heads: 2.3 ms, 930 TFLOP/s, 1100 with the products for the sums and the lines;
+// a step takes some 5000 cycles, 2432 of them matrix instructions, at the 2.0 - 2.2 GHz that its power allows (a large library product: 1140).
 #include "qr_chunk.h"
 
 namespace {
@@ -441,16 +441,26 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         // Of the next unit: whether its positions are all there and all seen (`at`: its first); else the logits that are not seen are taken out
         u32 there = 0;
         auto all_seen = [&](int at) INLINE { return at + 31 <= lowest && (a.window == 0 || at > highest - a.window || at + 31 < a.sinks); };
+        // (most units that are not all seen lie on one edge only: of the diagonal, or of the window)
         auto hide = [&](int at) INLINE {
             const u32 all = __builtin_amdgcn_readfirstlane(there);
+            const bool all_begun = a.window == 0 || at > highest - a.window, all_ended = at + 31 <= lowest && at >= a.sinks;
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb) {
                 const int from = at + 4 * h, high = place[cb] - from, low = before(cb) - from, sinks = a.sinks - from;
                 most[cb] = -__builtin_inff();
+                if (all_begun) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int k = 8 * (i >> 2) + (i & 3);
-                    y[cb][i] = (k <= high) & ((k > low) | (k < sinks)) ? y[cb][i] : -__builtin_inff();
+                    for (int i = 0; i < 16; ++i) y[cb][i] = 8 * (i >> 2) + (i & 3) <= high ? y[cb][i] : -__builtin_inff();
+                } else if (all_ended) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[cb][i] = 8 * (i >> 2) + (i & 3) > low ? y[cb][i] : -__builtin_inff();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int k = 8 * (i >> 2) + (i & 3);
+                        y[cb][i] = (k <= high) & ((k > low) | (k < sinks)) ? y[cb][i] : -__builtin_inff();
+                    }
                 }
                 if (~all) {
 #pragma unroll
