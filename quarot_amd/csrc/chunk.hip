@@ -21,8 +21,9 @@ namespace {
 // positions in turn, so a cached vector is read once per tile of rows.  A wave works on transposed tiles, positions x rows: the first product's
 // result has a row in every lane and positions in its registers, which is what the second product takes as its right operand, with no exchange
 // between lanes.  The contraction's order is free, so a position's codes are used as they lie: lane (n, g) of the first product takes bytes 16 g ..
-// of key n, the word s of them in step s (fp16 pages: bytes 64 s + 16 g .., whole lines by every load); lane (m, g) of the second takes word m of the eight keys 4 g .. 4 g + 3 and 16 + 4 g .. of a step,
-// whose nibble b is row m of its block b of outputs.
+// of key n, the word s of them in step s (fp16 pages: bytes 64 s + 16 g ..); lane (m, g) of the second takes word m of the eight keys
+// 4 g .. 4 g + 3 and 16 + 4 g .. of a step, whose nibble b is row m of its block b of outputs.  A wave has the next step's keys and values under
+// way (32 sequences of 4001 in a window, 64 on 8 heads: 20 us, 3.6 TB/s, bound by the vector unit; fp16 pages, 16 x 2500: 69 us, 4.85 TB/s).
 template <bool F16>
 struct Fetched {                       // a step's keys, refilled behind the first product, and its values, refilled behind the second
     u32x4 k[F16 ? 8 : 2], kp[F16 ? 1 : 2], vp[F16 ? 1 : 2];
@@ -505,10 +506,11 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
 // More rows are a choice between tiles of 32, each of which reads and unpacks the cache for itself, and tiles of 256, whose workgroups have a
 // compute unit to themselves and a long way to their first product.  Microseconds, from the two kernels' own times: a wave's step of 32
 // positions by 32 rows 2.4 with two waves per SIMD (fp16 pages, which reach the caches' bandwidth, 5.5), 6.5 around them; a step of 64
-// positions by 256 rows 2.9, 14 around them; partial states 0.17 a thousand, and 6 for one more launch.  The cut of the least sum is taken.  Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 192 rows 47 and 54 us, 8 x 96 138 and 181, 8 x 128 156 and
-// 187, 8 x 192 231 and 199, 8 x 256 299 and 205; 500 cached: 256 rows 18 and 39, 8 x 256 78 and 57; fp16 pages: 8 x 64 179 and 187, 8 x 96 369
-// and 195.  Splits of tiles of 256: 512 rows after 4001 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave per SIMD,
-// were slower than 32 everywhere, by up to 3 times.)
+// positions by 256 rows 2.9, 14 around them; partial states 0.17 a thousand, and 6 for one more launch.  The cut of the least sum is taken.
+// Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 192 rows 47 and 54 us, 8 x 96 138 and 181, 8 x 128 156 and 187,
+// 8 x 192 231 and 199, 8 x 256 299 and 205; 500 cached: 256 rows 18 and 39, 8 x 256 78 and 57; fp16 pages: 8 x 64 179 and 187, 8 x 96 369
+// and 195.  Splits of tiles of 256: 512 rows after 4001 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave
+// per SIMD, were slower than 32 everywhere, by up to 3 times.)
 struct ChunkPlan {
     int nb, nw, tiles, splits;
 };
@@ -517,7 +519,7 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     const int64_t rows = max_new_len * group, cus = qr_device().cus;
     int64_t seen = max_seq_len > 0 ? max_seq_len : 0;
-    if (window > 0 && seen > window + max_new_len + sinks + 64) seen = window + max_new_len + sinks + 64;
+    if (window > 0 && window < seen && sinks < seen && seen > window + max_new_len + sinks + 64) seen = window + max_new_len + sinks + 64;
     ChunkPlan p{1, 4, 1, 1};
     if (rows <= 16) {
         const int64_t groups = batch * num_heads, steps = (seen + 31) / 32;
@@ -592,7 +594,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     if (!o || !q) return QR_E_NULL;
     if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || q_stride % 8 || o_stride % 8) return QR_E_ALIGN;
     const int64_t width = (int64_t)num_q_heads * 128;
-    if (q_stride < width || o_stride < width || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024) return QR_E_SHAPE;
+    if (q_stride < width || o_stride < width || tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024) return QR_E_SHAPE;
     const ChunkPlan plan = chunk_plan(fp16, tokens, num_q_heads / num_heads, num_heads, batch_size, seqlen_indptr_or_null ? max_new_len : 1, max_seq_len, window, sinks);
     Chunk a;
     a.c = qr_internal_paged_kv((void*)kv_data, (void*)kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,

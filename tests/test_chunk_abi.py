@@ -72,3 +72,12 @@ def test_table_argument_errors(lib, code, change):
 
 def test_tables_of_nothing(lib):
     assert lib.qr_build_page_tables(*_table_args(batch=0)) == 0
+
+
+def test_chunk_workspace_of_absurd_lengths(lib):
+    """Nothing overflows: lengths, windows and sinks of 63 bits only size the launch."""
+    huge = (1 << 63) - 1
+    usual = lib.qr_batch_chunk_workspace_bytes(0, 5, 32, 32, 1, 5, 4096, 0, 0)
+    for window, sinks in ((huge, 0), (5, huge), (huge, huge)):
+        assert lib.qr_batch_chunk_workspace_bytes(0, 5, 32, 32, 1, 5, 4096, window, sinks) == usual
+    assert lib.qr_batch_chunk_workspace_bytes(0, 5, 32, 32, 1, 5, huge >> 1, 0, 0) >= usual
