@@ -42,12 +42,9 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    int id = blockIdx.x;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int h = id % c.num_heads;
+    const int id = divided(blockIdx.x, a.per_split), split = blockIdx.x - id * a.splits, item = divided(id, a.per_head), h = id - item * c.num_heads;
     int b, first_tile;
-    if (!item_of<16 * NB>(a, id / c.num_heads, b, first_tile)) return;
+    if (!item_of<16 * NB>(a, item, b, first_tile)) return;
     const Fresh mine_tokens = fresh_of(a, b);
     const int start = mine_tokens.start, fresh = mine_tokens.count;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
@@ -60,7 +57,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
 
     for (int tile = first_tile; tile * 16 * NB < rows; tile += a.tiles) {
         const int r0 = tile * 16 * NB, r1 = r0 + 16 * NB < rows ? r0 + 16 * NB : rows;
-        const int lowest = len - fresh + r0 / a.group, highest = len - fresh + (r1 - 1) / a.group;
+        const int lowest = len - fresh + divided(r0, a.per_group), highest = len - fresh + divided(r1 - 1, a.per_group);
         const Steps steps = steps_of<5>(a, lowest, highest);
         const int stride = NW * a.splits;
 
@@ -160,7 +157,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
         for (int nb = 0; nb < NB; ++nb) {
             const int r = r0 + 16 * nb + n;
             const bool in = r < rows;
-            const int t = (in ? r : r0) / a.group, head = h * a.group + (in ? r : r0) - t * a.group;
+            const int t = divided(in ? r : r0, a.per_group), head = h * a.group + (in ? r : r0) - t * a.group;
             place[nb] = in ? len - fresh + t : -1;
             const u32x4* src = (const u32x4*)(a.q + (int64_t)(start + t) * a.q_stride + (int64_t)head * 128) + (F16 ? g : 4 * g);
             u32x4 w[4];
@@ -436,7 +433,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
 #pragma unroll
                         for (int j = 0; j < 4; ++j) O[i][j] = __builtin_fmaf(src[1 + PER * l + i][j], keep, O[i][j]);
                 }
-                const int t = r / a.group, head = h * a.group + r - t * a.group;
+                const int t = divided(r, a.per_group), head = h * a.group + r - t * a.group;
                 if (a.splits == 1) {
                     const float inv = D == 0.f ? 0.f : 1.f / D;                 // (a row that sees nothing is zero)
                     u32x2* const dst = (u32x2*)(a.o + (int64_t)(start + t) * a.o_stride + (int64_t)head * 128) + PER * l;
@@ -456,10 +453,10 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
 // The partial states of every row -> its output: sixteen lanes per row, eight dimensions each.  The states' maxima and sums are read by a lane each (at most 32),
 // so that all loads are on their way at once: with few rows this launch is their latency (64 rows of 32 states: 5.6 us; with the states read one after the other 20.3).
 __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict__ part, const int32_t* __restrict__ starts, int batch, int tokens,
-                                                          int heads, int splits, f16* __restrict__ o, int64_t o_stride) {
+                                                          int heads, Divisor per_head, int splits, f16* __restrict__ o, int64_t o_stride) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 4);
     const int l = threadIdx.x & 15;
-    const int64_t token = row / heads;
+    const int64_t token = divided((int)row, per_head);     // (rows are fewer than 2^30)
     const int head = (int)(row - token * heads);
     // (rows that belong to no sequence have no states and are left as they are)
     if (token >= tokens || (starts && (token < starts[0] || token >= starts[batch]))) return;
@@ -606,6 +603,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     a.tokens = (int)tokens;
     a.group = num_q_heads / num_heads;
     a.per_group = divisor_of(a.group);
+    a.per_head = divisor_of(num_heads);
     a.tiles = plan.tiles;
     a.window = (int)(window > 0x3fffffff ? 0 : window);    // (longer than any sequence)
     a.sinks = (int)(sinks > 0x3fffffff ? 0x3fffffff : sinks);
@@ -615,7 +613,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     a.per_split = divisor_of(a.splits);
     a.part = (float*)workspace;
     const int64_t groups = batch_size * num_heads * plan.tiles * a.splits;
-    if (groups > 0x7fffffff) return QR_E_SHAPE;
+    if (groups > 0x3fffffff) return QR_E_SHAPE;
     hipStream_t st = (hipStream_t)stream;
     const Divisor pages = divisor_of(page_size);
     const bool aligned = page_size % 16 == 0;
@@ -623,7 +621,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
                     : fp16       ? (aligned ? launch_rows<true, true>(plan, a, pages, groups, st) : launch_rows<true, false>(plan, a, pages, groups, st))
                                  : (aligned ? launch_rows<false, true>(plan, a, pages, groups, st) : launch_rows<false, false>(plan, a, pages, groups, st));
     if (lrc != QR_OK || a.splits == 1) return lrc;
-    chunk_merge_kernel<<<dim3((unsigned)((tokens * num_q_heads + 3) / 4)), dim3(64), 0, st>>>(a.part, a.starts, (int)batch_size, (int)tokens, num_q_heads,
+    chunk_merge_kernel<<<dim3((unsigned)((tokens * num_q_heads + 3) / 4)), dim3(64), 0, st>>>(a.part, a.starts, (int)batch_size, (int)tokens, num_q_heads, divisor_of(num_q_heads),
                                                                                               a.splits, a.o, o_stride);
     return qr_launch_status();
 }

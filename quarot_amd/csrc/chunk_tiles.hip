@@ -79,12 +79,10 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     const PagedKV& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
-    int id = blockIdx.x;
-    const int split = id % a.splits;
-    id /= a.splits;
-    const int head = id % c.num_heads;                     // neighbours are on different XCDs, a head's tiles on one where 8 divides the heads
+    const int id = divided(blockIdx.x, a.per_split), split = blockIdx.x - id * a.splits, item = divided(id, a.per_head);
+    const int head = id - item * c.num_heads;              // neighbours are on different XCDs, a head's tiles on one where 8 divides the heads
     int b, tile;
-    if (!item_of<kRows>(a, id / c.num_heads, b, tile)) return;
+    if (!item_of<kRows>(a, item, b, tile)) return;
     const Fresh tokens = fresh_of(a, b);
     const int rows = tokens.count * a.group;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;

@@ -22,7 +22,7 @@ struct Chunk {
     int64_t q_stride, o_stride;       // halves from a token to the next
     int tokens, group, tiles, splits, window, sinks;      // window 0: none
     int q_had;
-    Divisor per_group, per_split;     // of `group`, `splits`
+    Divisor per_group, per_split, per_head;     // of `group`, `splits`, the key heads
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
