@@ -618,6 +618,15 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     QR_END
 }
 
+// A vector that lies in part of another tensor's memory and keeps all of it (the six tables of a call: 5.7 us, with an allocation each 9.0)
+at::Tensor part_of(const at::Tensor& whole, int64_t byte, int64_t count, at::ScalarType dtype) {
+    const auto meta = c10::scalarTypeToTypeMeta(dtype);
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), meta);
+    t.unsafeGetTensorImpl()->set_storage_offset(byte / (int64_t)meta.itemsize());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({count});
+    return t;
+}
+
 // build_page_tables(lengths, page_size, max_pages, block_table or None, new_lengths or None, tokens) -> the tables, in a dict
 PyObject* build_page_tables(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     QR_ARGS(6)
@@ -641,14 +650,12 @@ PyObject* build_page_tables(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     }
     at::Tensor t[6];
     const auto call = [&] {
-        t[0] = fresh({batch + 1}, at::kInt, device);
-        t[1] = fresh({batch * pages}, at::kInt, device);
-        t[2] = fresh({batch}, at::kInt, device);
-        if (news) {
-            t[3] = fresh({batch + 1}, at::kInt, device);
-            t[4] = fresh({tokens}, at::kLong, device);
-            t[5] = fresh({tokens}, at::kLong, device);
-        }
+        const int64_t counts[6] = {batch + 1, batch * pages, batch, batch + 1, tokens, tokens};
+        const int n = news ? 6 : 3;
+        int64_t at[7] = {0};
+        for (int i = 0; i < n; ++i) at[i + 1] = at[i] + (counts[i] * (i < 4 ? 4 : 8) + 63) / 64 * 64;
+        const at::Tensor whole = fresh({at[n]}, kByte, device);
+        for (int i = 0; i < n; ++i) t[i] = part_of(whole, at[i], counts[i], i < 4 ? at::kInt : at::kLong);
         return qr_build_page_tables(lengths->data_ptr(), ptr(news), batch, (int)page, pages, ptr(table), stride, tokens, t[0].data_ptr(), t[1].data_ptr(),
                                     t[2].data_ptr(), news ? t[3].data_ptr() : nullptr, news && tokens ? t[4].data_ptr() : nullptr,
                                     news && tokens ? t[5].data_ptr() : nullptr, stream(device));

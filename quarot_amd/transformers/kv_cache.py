@@ -375,7 +375,7 @@ def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_
     Returns a dict with kv_indptr [batch + 1], kv_indices [batch * max_pages] (-1 behind the last list) and last_page_offset
     [batch], all int32: the arguments of the cache's other functions.  With new_lengths int32 [batch], how many of the tokens are new
     (the last ones), and `tokens`, their number, also seqlen_indptr int32 [batch + 1], and for every new token int64 positions and
-    slots (page * page_size + entry, -1 where it has no place)."""
+    slots (page * page_size + entry, -1 where it has no place).  The tensors may lie in one allocation."""
     if max_pages is None and isinstance(block_table, torch.Tensor) and block_table.dim() == 2:
         max_pages = block_table.shape[1]
     tables = _lib.host.build_page_tables(lengths, page_size, max_pages, block_table, new_lengths, tokens)
