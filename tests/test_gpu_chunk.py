@@ -9,6 +9,7 @@ zero_j, subtracted from it) on int4 pages, and half a step of fp16 being u = 2^-
   L sum w_j (|x_j| + |zero_j|)            with L twice the largest error of a logit -- 140 steps of 2^-24 of its terms' absolute sum, and for queries
                                           below 2^-10 a step of 2^-21 of a sixteenth of them --, plus that of exp2's argument and of sums over the
                                           positions, all in fp32."""
+import gc
 import math
 
 import numpy as np
@@ -19,6 +20,15 @@ from quarot_amd.transformers import kv_cache as kv
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_goes_back():
+    """What the module's tests allocated goes back to the device behind them (others fill the memory up to a limit)."""
+    yield
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
 
 
 def make(seed, page_size, lens, news, heads, group, f16=False, layers=2, spare=3, fused=0, spread=1.0):

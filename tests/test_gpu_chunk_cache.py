@@ -1,5 +1,7 @@
 """The multi-layer cache with more than one new token, with a window, and with grouped query heads: its pages are those of the entry points, its attention is
 batch_chunk_i4's and batch_chunk_f16's, against the definition in 64 bits (test_gpu_chunk.py, with its tolerances)."""
+import gc
+
 import pytest
 import torch
 
@@ -8,6 +10,15 @@ from quarot_amd.transformers import kv_cache as kv
 from tests.test_gpu_chunk import DEV, check, definition, make
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_goes_back():
+    """What the module's tests allocated goes back to the device behind them (others fill the memory up to a limit)."""
+    yield
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
 
 
 def rows(seed, *shape):

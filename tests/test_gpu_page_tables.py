@@ -1,4 +1,6 @@
 """build_page_tables: whole numbers, equal to a loop over the sequences on the CPU."""
+import gc
+
 import pytest
 import torch
 
@@ -6,6 +8,15 @@ from quarot_amd.transformers import kv_cache as kv
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def memory_goes_back():
+    """What the module's tests allocated goes back to the device behind them (others fill the memory up to a limit)."""
+    yield
+    gc.collect()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
 
 
 def by_hand(lengths, page_size, max_pages, table, new, tokens):
