@@ -518,7 +518,8 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 const u32x2 both = both_halves<32>(as_u32(most[cb]));
                 const float now = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
                 const bool moves = now > limit[cb];        // (of the row alone: what other rows see changes nothing)
-                const float by = moves ? now : 0.f, keep = __builtin_amdgcn_exp2f(-by);
+                // (nothing seen so far: the sums are zero, and a first maximum far below zero would make them zero times an infinity)
+                const float by = moves ? now : 0.f, keep = limit[cb] < 0.f ? 0.f : __builtin_amdgcn_exp2f(-by);
                 limit[cb] = moves ? kHigh : limit[cb];
                 m[cb] += by;
 #pragma unroll
