@@ -27,7 +27,12 @@ constexpr int kKeyRow = 272, kDimRow = 144;
 __host__ __device__ constexpr int dim_row(int r) { return r * kDimRow + (r >> 5) * 16; }
 constexpr int kSlope = 64 * kKeyRow, kLine = kSlope + 256, kThere = kLine + 2048, kKeys = (kThere + 8 + 511) / 512 * 512;
 constexpr int kOdd = dim_row(133), kValues = (kOdd + 8 + 511) / 512 * 512;
-constexpr float kHigh = 15.f;                              // a maximum is raised when a logit (base 2, with the value's factor) is this far above it: 2^15 is an fp16 number
+// A row's largest weight times its value's factor lies between 2^kBase and 2^kHigh, an fp16 number: a first maximum is put at kBase, and so is one that a logit
+// (base 2, with the factor) exceeds kHigh by.  Factors are below two (up to 16 only for scales from 2^13 on), so the largest weight is one at least, and the
+// smallest ones are rounded in steps of 2^-24 of it; with maxima put at zero it could be a half, and the steps as much more of it (scales of 2^-24 .. 2^10, logits of
+// hundreds: errors of 1.56 times what rounded weights explain).  Higher maxima leave less room until they are raised: kBase 4 and kHigh 15 took 428 us for 8 x up
+// to 2048 tokens on 64 and 8 heads, these 361, 0 and 15 363.
+constexpr float kHigh = 15.9f, kBase = 1.f;
 constexpr int kLds = 3 * kKeys + 2 * kValues;
 
 // What a thread has fetched for a step: four of the sixteen pieces of a key and its parameters; four positions' values in eight dimensions, their
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 const u32x2 both = both_halves<32>(as_u32(most[cb]));
                 const float now = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
                 const bool any = now > limit[cb];
-                m[cb] = any ? now : 0.f, most[cb] -= m[cb];
+                m[cb] = any ? now - kBase : 0.f, most[cb] -= m[cb];
                 limit[cb] = any ? kHigh : limit[cb];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) y[cb][i] -= m[cb];
@@ -519,7 +524,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                 const float now = __builtin_fmaxf(as_f32(both.x), as_f32(both.y));
                 const bool moves = now > limit[cb];        // (of the row alone: what other rows see changes nothing)
                 // (nothing seen so far: the sums are zero, and a first maximum far below zero would make them zero times an infinity)
-                const float by = moves ? now : 0.f, keep = limit[cb] < 0.f ? 0.f : __builtin_amdgcn_exp2f(-by);
+                const float by = moves ? now - kBase : 0.f, keep = limit[cb] < 0.f ? 0.f : __builtin_amdgcn_exp2f(-by);
                 limit[cb] = moves ? kHigh : limit[cb];
                 m[cb] += by;
 #pragma unroll

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from quarot_amd import _lib
-from tests.test_gpu_chunk import check, make
+from tests.test_gpu_chunk import check, make, scale_values
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +55,18 @@ def test_splits_whose_first_positions_are_hidden_with_logits_far_below_zero(wind
     missing = [p for p in range(4513) if gone and p // 128 % 2 == 0]
     specs["kv_indices"][sorted({p // 16 for p in missing})] = -1
     check(specs, q, starts, lens, news, layer=0, window=window, sinks=sinks, gone=[(0, p) for p in missing], hints=(True,))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_large_logits_scales_and_missing_pages(f16):
+    lens, news = [700], [256]
+    specs, q, starts = make(21, 16, lens, news, 28, 8, f16, spread=12.0)
+    check(specs, q, starts, lens, news)
+    check(specs, q, starts, lens, news, window=90, sinks=2)
+    if not f16:
+        scale_values(specs, 21)
+        specs["kv_param"][:, :, 1, :, ::5, 0] = 0
+        specs["kv_param"][:, :, 1, :, 1::5, 0] *= -1
+        check(specs, q, starts, lens, news)
+    specs["kv_indices"][0], specs["kv_indices"][3], specs["kv_indices"][20] = 1 << 20, -1, 1 << 30
+    check(specs, q, starts, lens, news, gone=[(0, p) for p in [*range(16), *range(48, 64), *range(320, 336)]])
