@@ -446,8 +446,9 @@ int qr_batch_decode_f16(void* o, const void* q, const void* kv_data, const void*
  *   (QR_E_SHAPE otherwise).  q_had_mode 1: q through H_128 / sqrt(128) first, rounded to
  *   fp16, as matmul_had_cuda gives it.
  *   max_new_len, max_seq_len: the largest number of new tokens and of positions of a sequence if the caller knows them, else
- *   0; they size the launch and may be wrong at the cost of time only.  With a workspace of qr_batch_chunk_workspace_bytes
- *   bytes (16-byte aligned, contents arbitrary) few rows are split along the positions, and a second launch merges.
+ *   0; they size the launch and may be wrong at the cost of time only (a max_new_len below tokens / batch_size counts as that).
+ *   With a workspace of qr_batch_chunk_workspace_bytes bytes (at most 1 GiB; the same arguments, max_new_len 1 where
+ *   seqlen_indptr is NULL; 16-byte aligned, contents arbitrary) few rows are split along the positions, and a second launch merges.
  */
 size_t qr_batch_chunk_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                       int64_t max_seq_len, int64_t window, int64_t sinks);

@@ -508,14 +508,21 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
 // 8 x 192 231 and 199, 8 x 256 299 and 205; 500 cached: 256 rows 18 and 39, 8 x 256 78 and 57; fp16 pages: 8 x 64 179 and 187, 8 x 96 369
 // and 195.  Splits of tiles of 256: 512 rows after 4001 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave
 // per SIMD, were slower than 32 everywhere, by up to 3 times.)
+//
+// Partial states fill at most kMostParts bytes: a call of that many rows (16384 tokens of 64 heads in two splits) has 16 turns of tiles of 256 and more, and a split
+// gains no more than a part of the last one.
 struct ChunkPlan {
     int nb, nw, tiles, splits;
 };
+constexpr size_t kMostParts = (size_t)1 << 30;
+size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? (size_t)tokens * q_heads * splits * 132 * sizeof(float) : 0; }
 ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
-    const bool even = max_new_len > 0 && max_new_len <= tokens && max_new_len * batch == tokens;
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
+    if (max_new_len < (tokens + batch - 1) / batch) max_new_len = (tokens + batch - 1) / batch;        // (some sequence has as many)
+    const bool even = max_new_len * batch == tokens;
     const int64_t rows = max_new_len * group, cus = qr_device().cus;
-    int64_t seen = max_seq_len > 0 ? max_seq_len : 0;
+    int64_t seen = max_seq_len < 0 ? 0 : max_seq_len < 0x3fffffff ? max_seq_len : 0x3fffffff;              // (no sequence is as long)
+    window = window < 0x3fffffff ? window : 0x3fffffff, sinks = sinks < 0x3fffffff ? sinks : 0x3fffffff;
     if (window > 0 && window < seen && sinks < seen && seen > window + max_new_len + sinks + 64) seen = window + max_new_len + sinks + 64;
     ChunkPlan p{1, 4, 1, 1};
     if (rows <= 16) {
@@ -549,7 +556,7 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
         const int64_t late = max_new_len - per / group;    // (what the first tile does not see of the last one's positions, at most)
         const float steps = (float)(seen - (late > 0 ? (late < seen ? late : seen) / 2 : 0)) / (float)step;
         for (int s = 1; s <= 32; ++s) {
-            if (s > 1 && steps < (float)(3 * s)) break;
+            if (s > 1 && (steps < (float)(3 * s) || chunk_part_bytes(tokens, (int64_t)group * num_heads, s) > kMostParts)) break;
             const float turns = (float)((int64_t)(steps / (float)s) + 1);
             const float time = (float)((groups * s + at_once - 1) / at_once) * (turns * each + around) +
                                (s > 1 ? 6.f + (float)(tokens * group * num_heads) * (float)s * (660.f / 4e6f) : 0.f);
@@ -574,8 +581,6 @@ int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t gr
     kernel<<<dim3((unsigned)groups), dim3(64 * plan.nw), lds, st>>>(a, pages);
     return qr_launch_status();
 }
-
-size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? (size_t)tokens * q_heads * splits * 132 * sizeof(float) : 0; }
 
 int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_stride, int q_had_mode, const void* seqlen_indptr_or_null, int64_t tokens,
                 int num_q_heads, const void* kv_data, const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
@@ -630,7 +635,8 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
 
 extern "C" size_t qr_batch_chunk_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                                  int64_t max_seq_len, int64_t window, int64_t sinks) {
-    if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0) return 0;
+    if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0 || batch_size > 0x7fffffff) return 0;
+    if (tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024) return 0;        // (the call itself refuses them)
     const int splits = chunk_plan(fp16_pages != 0, tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, max_seq_len, window, sinks).splits;
     return chunk_part_bytes(tokens, num_q_heads, splits);
 }
