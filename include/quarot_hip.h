@@ -442,8 +442,8 @@ int qr_batch_decode_f16(void* o, const void* q, const void* kv_data, const void*
  * qr_batch_chunk_i4: int4 pages, k_j[i] = code * scale_j - zero_j (codes enter the products as they are, weights are rounded to
  *   fp16 once, everything else is in 32 bits).  qr_batch_chunk_f16: fp16 pages, kv_param is not read.
  *   q, o fp16, a token's num_q_heads * 128 halves contiguous, q_stride / o_stride halves from one token to the next (multiples
- *   of 8; 16-byte aligned); num_q_heads a multiple of num_heads, at most 1024 times, and tokens * num_q_heads below 2^30
- *   (QR_E_SHAPE otherwise).  q_had_mode 1: q through H_128 / sqrt(128) first, rounded to
+ *   of 8; 16-byte aligned); num_q_heads a multiple of num_heads, at most 1024 times, num_heads at most 65536,
+ *   and tokens * num_q_heads below 2^30 (QR_E_SHAPE otherwise); any batch_size.  q_had_mode 1: q through H_128 / sqrt(128) first, rounded to
  *   fp16, as matmul_had_cuda gives it.
  *   max_new_len, max_seq_len: the largest number of new tokens and of positions of a sequence if the caller knows them, else
  *   0; they size the launch and may be wrong at the cost of time only (a max_new_len below tokens / batch_size counts as that).

@@ -515,6 +515,7 @@ struct ChunkPlan {
     int nb, nw, tiles, splits;
 };
 constexpr size_t kMostParts = (size_t)1 << 30;
+constexpr int kMostHeads = 65536;                          // (with most splits a sequence's heads are a launch)
 size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? (size_t)tokens * q_heads * splits * 132 * sizeof(float) : 0; }
 ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
@@ -596,7 +597,8 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     if (!o || !q) return QR_E_NULL;
     if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || q_stride % 8 || o_stride % 8) return QR_E_ALIGN;
     const int64_t width = (int64_t)num_q_heads * 128;
-    if (q_stride < width || o_stride < width || tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024) return QR_E_SHAPE;
+    if (q_stride < width || o_stride < width || tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > kMostHeads)
+        return QR_E_SHAPE;
     const ChunkPlan plan = chunk_plan(fp16, tokens, num_q_heads / num_heads, num_heads, batch_size, seqlen_indptr_or_null ? max_new_len : 1, max_seq_len, window, sinks);
     Chunk a;
     a.c = qr_internal_paged_kv((void*)kv_data, (void*)kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,
@@ -617,14 +619,25 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
     if (a.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < chunk_part_bytes(tokens, num_q_heads, a.splits))) a.splits = 1;
     a.per_split = divisor_of(a.splits);
     a.part = (float*)workspace;
-    const int64_t groups = batch_size * num_heads * plan.tiles * a.splits;
-    if (groups > 0x3fffffff) return QR_E_SHAPE;
+    // A launch has fewer than 2^32 threads: fewer tiles at a time where hints are missing (a workgroup goes on to the next one behind them), then fewer sequences
+    const int64_t most = 0xffffffffll / (plan.nb == 0 ? 256 : 64 * plan.nw), wide = (int64_t)num_heads * a.splits;
+    if (batch_size * wide * plan.tiles > most) a.tiles = (int)(batch_size * wide < most ? most / (batch_size * wide) : 1);
+    const int64_t at_once = batch_size * wide <= most ? batch_size : most / wide;
     hipStream_t st = (hipStream_t)stream;
     const Divisor pages = divisor_of(page_size);
     const bool aligned = page_size % 16 == 0;
-    const int lrc = plan.nb == 0 ? qr_internal_chunk_tiles(fp16, a, pages, groups, st)
-                    : fp16       ? (aligned ? launch_rows<true, true>(plan, a, pages, groups, st) : launch_rows<true, false>(plan, a, pages, groups, st))
-                                 : (aligned ? launch_rows<false, true>(plan, a, pages, groups, st) : launch_rows<false, false>(plan, a, pages, groups, st));
+    int lrc = QR_OK;
+    for (int64_t first = 0; first < batch_size && lrc == QR_OK; first += at_once) {
+        Chunk some = a;
+        some.c.batch_size = (int)(batch_size - first < at_once ? batch_size - first : at_once);
+        some.c.indptr += first, some.c.last_page_offset += first;
+        if (a.starts) some.starts += first;
+        else some.q += first * q_stride, some.o += first * o_stride, some.part += a.splits > 1 ? first * num_q_heads * a.splits * 132 : 0;
+        const int64_t groups = some.c.batch_size * wide * a.tiles;
+        lrc = plan.nb == 0 ? qr_internal_chunk_tiles(fp16, some, pages, groups, st)
+              : fp16       ? (aligned ? launch_rows<true, true>(plan, some, pages, groups, st) : launch_rows<true, false>(plan, some, pages, groups, st))
+                           : (aligned ? launch_rows<false, true>(plan, some, pages, groups, st) : launch_rows<false, false>(plan, some, pages, groups, st));
+    }
     if (lrc != QR_OK || a.splits == 1) return lrc;
     chunk_merge_kernel<<<dim3((unsigned)((tokens * num_q_heads + 3) / 4)), dim3(64), 0, st>>>(a.part, a.starts, (int)batch_size, (int)tokens, num_q_heads, divisor_of(num_q_heads),
                                                                                               a.splits, a.o, o_stride);
@@ -636,7 +649,7 @@ int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_s
 extern "C" size_t qr_batch_chunk_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                                  int64_t max_seq_len, int64_t window, int64_t sinks) {
     if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0 || batch_size > 0x7fffffff) return 0;
-    if (tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024) return 0;        // (the call itself refuses them)
+    if (tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > kMostHeads) return 0;        // (the call itself refuses them)
     const int splits = chunk_plan(fp16_pages != 0, tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, max_seq_len, window, sinks).splits;
     return chunk_part_bytes(tokens, num_q_heads, splits);
 }

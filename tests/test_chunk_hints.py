@@ -1,4 +1,6 @@
 """Attention of new tokens over the paged cache: what wrong or missing hints may cost, without a GPU (the workspace function plans as the call does)."""
+import ctypes
+
 import pytest
 
 from quarot_amd import _lib
@@ -47,3 +49,11 @@ def test_lengths_windows_and_sinks_of_63_bits_count_as_longer_than_any_sequence(
         long = size(0, tokens, 32, 32, 1, tokens, 1 << 30, 0, 0)
         for window, sinks in ((0, 0), (huge, 0), (huge, huge), (huge - 70, 3), (1, huge)):
             assert size(0, tokens, 32, 32, 1, tokens, huge, window, sinks) == long
+
+
+@pytest.mark.parametrize("entry", ["qr_batch_chunk_i4", "qr_batch_chunk_f16"])
+def test_key_heads_that_no_launch_holds_are_refused(size, entry):
+    at = ctypes.c_void_p(4096)                             # never dereferenced
+    heads = 65537
+    assert getattr(_lib.lib(), entry)(at, heads * 128, at, heads * 128, 0, None, 1, heads, at, at, at, at, at, 1, 1, 0, heads, 16, 128, 1, 0, 0, 0, 0, None, 0, None) == -2
+    assert size(0, 1, heads, heads, 1, 1, 4096, 0, 0) == 0
