@@ -599,7 +599,7 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         !plain_or_none(a[15], kByte, device, &ws))
         return none();
     const int64_t tokens = q->size(0), heads = q->size(1);
-    if (heads % c.heads || heads > 0x7fffffff || (seq ? (seq->dim() != 1 || seq->numel() != c.batch + 1) : tokens != c.batch) || fresh_bound < 0 ||
+    if (c.heads == 0 || heads % c.heads || heads > 0x7fffffff || (seq ? (seq->dim() != 1 || seq->numel() != c.batch + 1) : tokens != c.batch) || fresh_bound < 0 ||
         bound < 0 || window < 0 || sinks < 0)
         return none();
     if (!seq) fresh_bound = 1;

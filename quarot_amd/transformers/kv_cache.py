@@ -306,7 +306,7 @@ def _chunk(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
     if not (o.shape == q.shape):
         raise RuntimeError(f"{fn}: o.size() != q.size()")
     tokens, q_heads = q.shape[0], q.shape[1]
-    if not (q_heads > 0 and q_heads % heads == 0):
+    if not (q_heads > 0 and heads > 0 and q_heads % heads == 0):
         raise RuntimeError(f"{fn}: q's heads must be a multiple of the cache's {heads}")
     if not (kv_indptr.shape[0] == batch + 1):
         raise RuntimeError(f"{fn}: CHECK_EQ(kv_indptr.size(0), batch_size + 1) failed")
