@@ -475,7 +475,7 @@ int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_strid
  *   new_lengths_or_null int32 [batch_size]: how many of the tokens are new, the last ones.  Then seqlen_indptr int32 [batch_size + 1]
  *   gets their bounds, and positions, slots int64 [tokens] every new token's position and its place page * page_size + entry
  *   (-1: none, because the sequence is shorter than its new tokens, or the block table has a negative page there); both are -1
- *   behind the last new token, and new tokens beyond `tokens` are left out.
+ *   behind the last new token, and new tokens beyond `tokens` (below 2^30) are left out.
  */
 int qr_build_page_tables(const void* lengths, const void* new_lengths_or_null, int64_t batch_size, int page_size,
                          int64_t max_pages, const void* block_table_or_null, int64_t table_stride, int64_t tokens,

@@ -637,7 +637,7 @@ PyObject* build_page_tables(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         !arg_int(a[5], &tokens) || !plain_or_none(a[4], at::kInt, device, &news))
         return none();
     const int64_t batch = lengths->numel();
-    if (page <= 0 || page > 0x7fffffff || pages <= 0 || pages > 0x3fffffff || pages * batch > 0x3fffffff || tokens < 0 || tokens > 1ll << 40 ||
+    if (page <= 0 || page > 0x7fffffff || pages <= 0 || pages > 0x3fffffff || pages * batch > 0x3fffffff || tokens < 0 || tokens > 0x3fffffff ||
         (news ? (news->dim() != 1 || news->numel() != batch) : tokens != 0))
         return none();
     int64_t stride = 0;

@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void build_page_tables_kernel(Tables t) {
 extern "C" int qr_build_page_tables(const void* lengths, const void* new_lengths_or_null, int64_t batch_size, int page_size, int64_t max_pages,
                                     const void* block_table_or_null, int64_t table_stride, int64_t tokens, void* kv_indptr, void* kv_indices,
                                     void* last_page_offset, void* seqlen_indptr, void* positions, void* slots, void* stream) {
-    if (batch_size < 0 || page_size <= 0 || max_pages <= 0 || tokens < 0) return QR_E_SHAPE;
+    if (batch_size < 0 || page_size <= 0 || max_pages <= 0 || tokens < 0 || tokens > 0x3fffffff) return QR_E_SHAPE;        // (counted in 32 bits)
     if (batch_size == 0) return QR_OK;
     if (batch_size > 0x3fffffff || max_pages > 0x3fffffff || max_pages * batch_size > 0x3fffffff || max_pages * page_size > 0x7fffffff) return QR_E_SHAPE;
     if (block_table_or_null && table_stride < max_pages) return QR_E_SHAPE;

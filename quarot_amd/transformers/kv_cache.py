@@ -374,7 +374,7 @@ def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_
     (default: the block table's width) bounds the pages of a sequence; a longer length counts as max_pages * page_size.
     Returns a dict with kv_indptr [batch + 1], kv_indices [batch * max_pages] (-1 behind the last list) and last_page_offset
     [batch], all int32: the arguments of the cache's other functions.  With new_lengths int32 [batch], how many of the tokens are new
-    (the last ones), and `tokens`, their number, also seqlen_indptr int32 [batch + 1], and for every new token int64 positions and
+    (the last ones), and `tokens`, their number (below 2^30), also seqlen_indptr int32 [batch + 1], and for every new token int64 positions and
     slots (page * page_size + entry, -1 where it has no place).  The tensors may lie in one allocation."""
     if max_pages is None and isinstance(block_table, torch.Tensor) and block_table.dim() == 2:
         max_pages = block_table.shape[1]
@@ -401,6 +401,8 @@ def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_
     max_pages = int(max_pages)
     if not (page_size > 0 and max_pages > 0 and tokens >= 0):
         raise RuntimeError(f"{fn}: page_size and max_pages must be positive, tokens not negative")
+    if tokens >= 1 << 30:
+        raise RuntimeError(f"{fn}: tokens must be below 2^30")
     if new_lengths is None:
         if tokens:
             raise RuntimeError(f"{fn}: tokens without new_lengths")

@@ -23,3 +23,10 @@ def test_caches_without_heads_entries_pages_or_layers(axis, match, f16, route):
     empty = {**specs, **{name: specs[name].narrow(axis, 0, 0).contiguous() for name in ("kv_data", "kv_param")}}
     with pytest.raises(RuntimeError, match=match):
         (kv.batch_chunk_f16 if f16 else kv.batch_chunk_i4)(torch.empty_like(q), q, **empty, layer_idx=0, seqlen_indptr=starts)
+
+
+def test_new_tokens_that_32_bits_do_not_count(route):
+    n = torch.tensor([3, 4], dtype=torch.int32, device=DEV)
+    for tokens in (1 << 30, 1 << 31, 1 << 45):
+        with pytest.raises(RuntimeError, match="below 2.30"):
+            kv.build_page_tables(n, 16, 2, new_lengths=n, tokens=tokens)
