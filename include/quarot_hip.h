@@ -473,7 +473,7 @@ int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_strid
  *   kv_indptr int32 [batch_size + 1], kv_indices int32 [batch_size * max_pages] (the lists one behind the other, -1 behind the
  *   last one), last_page_offset int32 [batch_size] (0: no pages).
  *   new_lengths_or_null int32 [batch_size]: how many of the tokens are new, the last ones.  Then seqlen_indptr int32 [batch_size + 1]
- *   gets their bounds, and positions, slots int64 [tokens] every new token's position and its place page * page_size + entry
+ *   gets their bounds (at most 2^31 - 1), and positions, slots int64 [tokens] every new token's position and its place page * page_size + entry
  *   (-1: none, because the sequence is shorter than its new tokens, or the block table has a negative page there); both are -1
  *   behind the last new token, and new tokens beyond `tokens` (below 2^30) are left out.
  */

@@ -57,14 +57,15 @@ __global__ __launch_bounds__(256) void build_page_tables_kernel(Tables t) {
     tokens_all = token_sums[0][1] + token_sums[1][1] + token_sums[2][1] + token_sums[3][1];
 
     const int n = held(t, b), pages = pages_of(t, n);
+    auto bound = [](int64_t tokens) { return (int)(tokens > 0x7fffffff ? 0x7fffffff : tokens); };        // (behind all tokens that there are)
     auto page_at = [&](int i) { return t.block_table ? t.block_table[b * t.table_stride + i] : i * t.batch + b; };
     if (threadIdx.x == 0) {
         t.indptr[b] = before;
         t.last[b] = n > 0 ? n - (pages - 1) * t.page_size : 0;
-        if (t.starts) t.starts[b] = (int)tokens_before;
+        if (t.starts) t.starts[b] = bound(tokens_before);
         if (b == 0) {
             t.indptr[t.batch] = all;
-            if (t.starts) t.starts[t.batch] = (int)tokens_all;
+            if (t.starts) t.starts[t.batch] = bound(tokens_all);
         }
     }
     for (int i = threadIdx.x; i < pages; i += 256) t.indices[(int64_t)before + i] = page_at(i);
