@@ -517,7 +517,8 @@ class MultiLayerPagedKVCache4Bit:
     further turn, drafted tokens -- and return a callable that runs attention over the cache, causal among the new tokens).
     Keys pass through the Hadamard transform over the head dimension before quantisation, queries before attention
     (hadamard_dtype, None to skip).  The callable takes any multiple of num_heads as query heads.  window > 0: it lets a token see the
-    last `window` positions, its own among them, and the first `sinks`.
+    last `window` positions, its own among them, and the first `sinks`.  After a padded prompt (cache_kwargs["attention_mask"], as the
+    reference takes it) turns of several tokens, or with a window, need the mask of all tokens so far, none of the new ones left out.
     The reference derives the class from transformers' Cache for the methods that base supplied in the
     version it pins (get_usable_length); they are defined here instead, so the class does not depend on the
     installed transformers version."""
@@ -543,6 +544,7 @@ class MultiLayerPagedKVCache4Bit:
         self._captured_specs = None     # (length, page tables, _where()) of the capture under way
         self.max_seq_len = max_seq_len
         self._needs_init = [True] * n_layers
+        self._padded = False            # the prompt's mask left tokens out
         self.length = 0
         self.device = device
         self.hadamard_dtype = hadamard_dtype
@@ -623,17 +625,30 @@ class MultiLayerPagedKVCache4Bit:
     def seen_tokens(self):
         return self.length
 
+    def _check_turn(self, attention_mask, added_length, length):
+        """A turn behind the prompt appends and attends with the last `added_length` tokens of every sequence: the mask has to cover all tokens so far
+        and keep the new ones, and a prompt with padding needs it again, for the sequences' own lengths."""
+        if attention_mask is None:
+            if self._padded:
+                raise ValueError("the prompt was padded: later turns need its attention_mask, with the tokens since")
+        elif tuple(attention_mask.shape) != (self.batch_size, length):
+            raise ValueError(f"attention_mask must be [{self.batch_size}, {length}], all tokens so far, got {list(attention_mask.shape)}")
+        elif not attention_mask[:, length - added_length:].all():
+            raise NotImplementedError("Current implementation does not support padding among the new tokens of a later turn")
+
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
         b_sz, added_length, num_heads, head_dim = key_states.shape
         assert b_sz == self.batch_size
+        attention_mask = cache_kwargs.get("attention_mask") if cache_kwargs else None
+        first = self._needs_init[layer_idx]
+        if not first and (added_length > 1 or self.window):
+            self._check_turn(attention_mask, added_length, self.length + (added_length if layer_idx == 0 else 0))
         if self._pending:
             self._flush()
         if layer_idx == 0:
             new_length = self.length + added_length
             self._ensure_page_cnt_per_batch(self.page_cnt_from_length(new_length))
             self.length = new_length
-        attention_mask = cache_kwargs.get("attention_mask") if cache_kwargs else None
-        first = self._needs_init[layer_idx]
         made = self._specs
         if made is not None and made[0] == self.length and attention_mask is None and type(_lib.host.where(self._pages)) is int:
             specs = made[1]                      # (what the call below finds for a later layer, outside a capture)
@@ -652,6 +667,7 @@ class MultiLayerPagedKVCache4Bit:
                 vq, vs, vz = asym_quantize_and_pack_i4(value_states)
                 keep = torch.nonzero(attention_mask.flatten(), as_tuple=False).flatten()
                 rows = self.batch_size * added_length
+                self._padded = keep.numel() != rows
                 pick = lambda t, w: t.reshape(rows, num_heads, w).index_select(0, keep).contiguous()
                 seqlens = torch.nn.functional.pad(torch.cumsum(attention_mask.sum(dim=-1, dtype=torch.int32), dim=0,
                                                                dtype=torch.int32), (1, 0))
@@ -697,6 +713,7 @@ class MultiLayerPagedKVCache4Bit:
             self._needs_init[layer_idx] = False
             if attention_mask is not None:
                 keep = torch.nonzero(attention_mask.flatten(), as_tuple=False).flatten()
+                self._padded = keep.numel() != rows
                 k, v, param = k.index_select(0, keep), v.index_select(0, keep), param.index_select(0, keep)
                 seqlens = torch.nn.functional.pad(torch.cumsum(attention_mask.sum(dim=-1, dtype=torch.int32), dim=0,
                                                                dtype=torch.int32), (1, 0))
