@@ -641,6 +641,7 @@ class MultiLayerPagedKVCache4Bit:
         assert b_sz == self.batch_size
         attention_mask = cache_kwargs.get("attention_mask") if cache_kwargs else None
         first = self._needs_init[layer_idx]
+        assert first or added_length >= 1
         if not first and (added_length > 1 or self.window):
             self._check_turn(attention_mask, added_length, self.length + (added_length if layer_idx == 0 else 0))
         if self._pending:

@@ -39,3 +39,12 @@ def test_masks_of_later_turns(added, window, layer, disable_quant):
     with pytest.raises(ValueError, match="padded"):
         turn(cache, added, None, layer)
     assert cache.length == (20 if layer == 0 else 20 + added)
+
+
+@pytest.mark.parametrize("disable_quant", [False, True])
+@pytest.mark.parametrize("window", [0, 10])
+def test_a_turn_without_tokens(window, disable_quant):
+    cache = cache_of(20, disable_quant=disable_quant, window=window)
+    with pytest.raises(AssertionError):
+        turn(cache, 0, None)
+    assert not cache._pending and cache.length == 20
