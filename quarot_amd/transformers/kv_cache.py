@@ -646,6 +646,7 @@ class MultiLayerPagedKVCache4Bit:
             self._check_turn(attention_mask, added_length, self.length + (added_length if layer_idx == 0 else 0))
         if self._pending:
             self._flush()
+        length = self.length
         if layer_idx == 0:
             new_length = self.length + added_length
             self._ensure_page_cnt_per_batch(self.page_cnt_from_length(new_length))
@@ -654,7 +655,11 @@ class MultiLayerPagedKVCache4Bit:
         if made is not None and made[0] == self.length and attention_mask is None and type(_lib.host.where(self._pages)) is int:
             specs = made[1]                      # (what the call below finds for a later layer, outside a capture)
         else:
-            specs = self.get_cache_specs_for_flash_infer(attention_mask)
+            try:
+                specs = self.get_cache_specs_for_flash_infer(attention_mask)
+            except NotImplementedError:          # a mask of unequal page counts: nothing has been stored
+                self.length = length
+                raise
         if self.disable_quant:
             return self._update_f16(key_states, value_states, layer_idx, attention_mask, first, specs)
         k_in, fused_had = key_states, self.hadamard_dtype is not None

@@ -48,3 +48,15 @@ def test_a_turn_without_tokens(window, disable_quant):
     with pytest.raises(AssertionError):
         turn(cache, 0, None)
     assert not cache._pending and cache.length == 20
+
+
+@pytest.mark.parametrize("disable_quant", [False, True])
+@pytest.mark.parametrize("added", [1, 3])
+def test_a_refused_turn_leaves_the_length(added, disable_quant):
+    """Page counts that differ are refused (kv_cache.py:253-275); the cache holds what it held."""
+    cache = cache_of(20, disable_quant=disable_quant)
+    mask = torch.ones(BATCH, 20 + added, dtype=torch.int64)
+    mask[0, :10] = 0
+    with pytest.raises(NotImplementedError, match="different number of pages"):
+        turn(cache, added, mask)
+    assert cache.length == 20
