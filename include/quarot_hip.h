@@ -437,8 +437,9 @@ int qr_batch_decode_f16(void* o, const void* q, const void* kv_data, const void*
  * values are in the pages already (qr_kv_append_i4, qr_kv_quant_append_f16_i4, qr_kv_append_f16 with the same bounds):
  *   o[t, h, :] = sum_j softmax_j( q[t, h, :] . k[j, h / G] / sqrt(128) ) v[j, h / G],   G = num_q_heads / num_heads,
  *   over the positions j <= P, P the token's own; with window > 0 only those with P - j < window or j < sinks.
- *   Sequences of fewer than 2^29 positions.  A row that sees no position is zero (a sequence without pages, more new tokens than the sequence holds); rows of q and
- *   o behind the last sequence are neither read nor written.  Positions on page numbers outside [0, num_pages) are skipped.
+ *   Sequences of fewer than 2^29 positions.  A row that sees no position is zero (a sequence without pages, more new tokens than the sequence
+ *   holds); rows of q and o behind the last sequence are neither read nor written, and new tokens behind the last row are left out (as
+ *   qr_build_page_tables leaves them out).  Positions on page numbers outside [0, num_pages) are skipped.
  * qr_batch_chunk_i4: int4 pages, k_j[i] = code * scale_j - zero_j (codes enter the products as they are, weights are rounded to
  *   fp16 once, everything else is in 32 bits).  qr_batch_chunk_f16: fp16 pages, kv_param is not read.
  *   q, o fp16, a token's num_q_heads * 128 halves contiguous, q_stride / o_stride halves from one token to the next (multiples

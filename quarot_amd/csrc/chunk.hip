@@ -46,10 +46,10 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
     int b, first_tile;
     if (!item_of<16 * NB>(a, item, b, first_tile)) return;
     const Fresh mine_tokens = fresh_of(a, b);
-    const int start = mine_tokens.start, fresh = mine_tokens.count;
+    const int start = mine_tokens.start;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
-    const int rows = fresh * a.group;
+    const int rows = mine_tokens.count * a.group, first_place = len - mine_tokens.all;        // (the first new token's position)
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
     const int64_t kv_slots = (int64_t)c.num_heads * c.page_size;
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
 
     for (int tile = first_tile; tile * 16 * NB < rows; tile += a.tiles) {
         const int r0 = tile * 16 * NB, r1 = r0 + 16 * NB < rows ? r0 + 16 * NB : rows;
-        const int lowest = len - fresh + divided(r0, a.per_group), highest = len - fresh + divided(r1 - 1, a.per_group);
+        const int lowest = first_place + divided(r0, a.per_group), highest = first_place + divided(r1 - 1, a.per_group);
         const Steps steps = steps_of<5>(a, lowest, highest);
         const int stride = NW * a.splits;
 
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
             const int r = r0 + 16 * nb + n;
             const bool in = r < rows;
             const int t = divided(in ? r : r0, a.per_group), head = h * a.group + (in ? r : r0) - t * a.group;
-            place[nb] = in ? len - fresh + t : -1;
+            place[nb] = in ? first_place + t : -1;
             const u32x4* src = (const u32x4*)(a.q + (int64_t)(start + t) * a.q_stride + (int64_t)head * 128) + (F16 ? g : 4 * g);
             u32x4 w[4];
 #pragma unroll

@@ -92,6 +92,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     const int rows = tokens.count * a.group;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
+    const int first_place = len - tokens.all;              // the first new token's position
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;
     const int64_t kv_slots = (int64_t)c.num_heads * c.page_size;
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 
     for (int r_tile = tile * kRows; r_tile < rows; r_tile += a.tiles * kRows) {
         const int r_end = r_tile + kRows < rows ? r_tile + kRows : rows;
-        const int tile_lowest = len - tokens.count + divided(r_tile, a.per_group), tile_highest = len - tokens.count + divided(r_end - 1, a.per_group);
+        const int tile_lowest = first_place + divided(r_tile, a.per_group), tile_highest = first_place + divided(r_end - 1, a.per_group);
         const Steps steps = steps_of<6>(a, tile_lowest, tile_highest);
         const int s_begin = divided(steps.all * split, a.per_split), s_end = divided(steps.all * (split + 1), a.per_split);      // (below 2^24 steps, 2^5 splits)
         const int last = s_end - 1;
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         const int r0 = r_tile + 64 * wave;
         const int r_last = r0 + 63 < rows ? r0 + 63 : rows - 1;
         // (a wave without rows hides nothing: its results go nowhere, and the others wait for it)
-        const int lowest = r0 < rows ? len - tokens.count + divided(r0, a.per_group) : 0x7fffffff, highest = r0 < rows ? len - tokens.count + divided(r_last, a.per_group) : -1;
+        const int lowest = r0 < rows ? first_place + divided(r0, a.per_group) : 0x7fffffff, highest = r0 < rows ? first_place + divided(r_last, a.per_group) : -1;
         auto row_of = [&](int cb) { return r0 + 32 * cb + n; };
         auto token_of = [&](int cb) { return divided(row_of(cb) < rows ? row_of(cb) : r_tile, a.per_group); };
         auto head_of = [&](int cb, int token) { return head * a.group + (row_of(cb) < rows ? row_of(cb) : r_tile) - token * a.group; };
@@ -360,7 +361,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         for (int cb = 0; cb < 2; ++cb) {
             const bool in = row_of(cb) < rows;
             const int token = token_of(cb);
-            place[cb] = in ? len - tokens.count + token : -1;
+            place[cb] = in ? first_place + token : -1;
             const u32x4* src = (const u32x4*)(a.q + (int64_t)(tokens.start + token) * a.q_stride + (int64_t)head_of(cb, token) * 128) + (F16 ? 4 * h : h);
 #pragma unroll
             for (int s = 0; s < 8; ++s) qf[cb][s] = src[F16 ? (s >> 1) + 8 * (s & 1) : 2 * s];       // (rows that are not there: another one's, whose results go nowhere)

@@ -133,16 +133,18 @@ __device__ __forceinline__ u32x4 scaled_codes_slow(u32 w, u32 w0, u32 w1) {
     return out;
 }
 
-// the new tokens of sequence b: the first one's row in q and o, and how many (kept inside q and o, whatever the bounds say)
+// the new tokens of sequence b: the first one's row in q and o, how many rows there are of them (kept inside q and o, whatever the bounds say), and how many
+// tokens from that row on the bounds say: those that q has no rows for are the sequence's last ones
 struct Fresh {
-    int start, count;
+    int start, count, all;
 };
 __device__ __forceinline__ Fresh fresh_of(const Chunk& a, int b) {
-    if (!a.starts) return Fresh{b, 1};
-    int start = a.starts[b], end = a.starts[b + 1];
+    if (!a.starts) return Fresh{b, 1, 1};
+    int start = a.starts[b];
+    const int end = a.starts[b + 1];
     start = start < 0 ? 0 : start;
-    end = end > a.tokens ? a.tokens : end;
-    return Fresh{start, end > start ? end - start : 0};
+    const int stop = end > a.tokens ? a.tokens : end;
+    return Fresh{start, stop > start ? stop - start : 0, end > start ? end - start : 0};
 }
 
 __device__ __forceinline__ int lanes_sum(int v) {          // over the wave
