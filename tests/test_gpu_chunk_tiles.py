@@ -178,3 +178,20 @@ def test_a_call_twice_gives_the_same_bits(f16):
         for o in (first, second):
             (kv.batch_chunk_f16 if f16 else kv.batch_chunk_i4)(o, q, **specs, layer_idx=0, seqlen_indptr=starts, max_new_len=news[0], max_seq_len=lens[0])
         assert torch.equal(first, second)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_pages_beyond_32_bit_offsets(f16):
+    """A pool of more than 2^32 bytes, its last pages in use: the same bits as from a small one."""
+    lens, news = [600, 90], [250, 6]
+    specs, q, starts = make(5, 16, lens, news, 28, 8, f16, layers=2, spare=0)
+    per, data = specs["kv_data"].shape[0], specs["kv_data"]
+    total = (5 << 30) // (data[0].numel() * data.element_size())
+    pool = {name: torch.empty((total, *specs[name].shape[1:]), dtype=specs[name].dtype, device=DEV) for name in ("kv_data", "kv_param")}
+    for name, t in pool.items():
+        t[total - per:] = specs[name]
+    assert pool["kv_data"].numel() * data.element_size() > 1 << 32
+    outs = [torch.empty_like(q) for _ in range(2)]
+    for o, used in zip(outs, (specs, {**specs, **pool, "kv_indices": specs["kv_indices"] + (total - per)})):
+        (kv.batch_chunk_f16 if f16 else kv.batch_chunk_i4)(o, q, **used, layer_idx=1, seqlen_indptr=starts)
+    assert torch.equal(*outs)
