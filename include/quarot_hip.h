@@ -441,7 +441,8 @@ int qr_batch_decode_f16(void* o, const void* q, const void* kv_data, const void*
  *   holds); rows of q and o behind the last sequence are neither read nor written, and new tokens behind the last row are left out (as
  *   qr_build_page_tables leaves them out).  Positions on page numbers outside [0, num_pages) are skipped.
  * qr_batch_chunk_i4: int4 pages, k_j[i] = code * scale_j - zero_j (codes enter the products as they are, weights are rounded to
- *   fp16 once, everything else is in 32 bits).  qr_batch_chunk_f16: fp16 pages, kv_param is not read.
+ *   fp16 once, every second entry of q that is below 2^-10 to a multiple of 2^-20, everything else is in 32 bits).
+ *   qr_batch_chunk_f16: fp16 pages (weights rounded likewise, q as it is), kv_param is not read.
  *   q, o fp16, a token's num_q_heads * 128 halves contiguous, q_stride / o_stride halves from one token to the next (multiples
  *   of 8; 16-byte aligned); num_q_heads a multiple of num_heads, at most 1024 times, num_heads at most 65536,
  *   and tokens * num_q_heads below 2^30 (QR_E_SHAPE otherwise); any batch_size.  q_had_mode 1: q through H_128 / sqrt(128) first, rounded to

@@ -23,7 +23,7 @@ namespace {
 // between lanes.  The contraction's order is free, so a position's codes are used as they lie: lane (n, g) of the first product takes bytes 16 g ..
 // of key n, the word s of them in step s (fp16 pages: bytes 64 s + 16 g ..); lane (m, g) of the second takes word m of the eight keys
 // 4 g .. 4 g + 3 and 16 + 4 g .. of a step, whose nibble b is row m of its block b of outputs.  A wave has the next step's keys and values under
-// way (32 sequences of 4001 in a window, 64 on 8 heads: 20 us, 3.6 TB/s, bound by the vector unit; fp16 pages, 16 x 2500: 69 us, 4.85 TB/s).
+// way (32 sequences of 4001 in a window, 64 on 8 heads: 20 us, 3.6 TB/s, bound by the vector unit; fp16 pages, 16 x 2500 in a window: 69 us, 4.85 TB/s).
 template <bool F16>
 struct Fetched {                       // a step's keys, refilled behind the first product, and its values, refilled behind the second
     u32x4 k[F16 ? 8 : 2], kp[F16 ? 1 : 2], vp[F16 ? 1 : 2];
@@ -495,18 +495,20 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
 // How a call is cut: column blocks and waves of a workgroup (nb 0: the kernel of 256 rows), tiles of rows per (sequence, key head), splits of the
 // positions.
 //
-// 16 rows and fewer read the cache once, whoever does it.  Int4 pages: twelve waves to a compute unit, in one workgroup where there are sequences
-// and heads enough, or little to read (one token, 64 on 8 heads: 64 x 2000 36 us, 8 waves 40; 32 x 500 10.4 and 12.3), else in three, split
-// (4 x 4000, 32 heads: 23.6 us; 8 waves, split in two 28), or one with the most splits there are (30000, 64 on 8 heads: 22.5; in three 26.8).  Fp16
-// pages have registers for two workgroups of four waves (64 x 1000, 32 heads: 104 us; one of eight 124; 2000: 12.8 in 8 splits, 15 of 8 waves).
+// (Microseconds of sequences of one length, median of calls back to back.)  16 rows and fewer read the cache once, whoever does it.  Int4 pages: twelve waves to a
+// compute unit, in one workgroup where there are sequences and heads enough, or little to read (one token, 64 on 8 heads: 32 x 4096 33, 8 waves 35, 4 waves 41;
+// 32 x 500 11.0, 10.9 and 10.8; where two such workgroups follow one another on a compute unit 4 waves are ahead, 64 x 2000 39.5, 38.5 and 32.5, which the rule
+// does not go by), else in three, split (4 x 4000, 32 heads: 22.5; 8 waves, split in two 22.5; 12 waves 29), or one with the most splits there are (30000, 64 on 8
+// heads: 21.4; 4 waves 21.0, in 24 splits 22.1).  Fp16 pages have registers for two workgroups of four waves (64 x 1000, 32 heads: 189 us, 5.5 TB/s; one of eight
+// 203; 2000: 14.5 in 7 splits, 16.0 of 8 waves in 4).
 //
 // More rows are a choice between tiles of 32, each of which reads and unpacks the cache for itself, and tiles of 256, whose workgroups have a
 // compute unit to themselves and a long way to their first product.  Microseconds, from the two kernels' own times: a wave's step of 32
 // positions by 32 rows 2.4 with two waves per SIMD (fp16 pages, which reach the caches' bandwidth, 5.5), 6.5 around them; a step of 64
 // positions by 256 rows 2.9, 14 around them; partial states 0.17 a thousand, and 6 for one more launch.  The cut of the least sum is taken.
-// Measured, tiles of 32 and of 256 (4000 tokens cached, 32 heads, int4): 192 rows 47 and 54 us, 8 x 96 138 and 181, 8 x 128 156 and 187,
-// 8 x 192 231 and 199, 8 x 256 299 and 205; 500 cached: 256 rows 18 and 39, 8 x 256 78 and 57; fp16 pages: 8 x 64 179 and 187, 8 x 96 369
-// and 195.  Splits of tiles of 256: 512 rows after 4001 127, 98, 86, 111 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave
+// Measured, tiles of 32 and of 256, each at its best (4000 tokens cached, 32 heads, int4): 192 rows 46 and 50 us, 8 x 96 119 and 162, 8 x 128 151 and 171,
+// 8 x 192 222 and 179, 8 x 256 293 and 186; 500 cached: 256 rows 17 and 32, 8 x 256 74 and 52; fp16 pages: 8 x 64 162 and 175, 8 x 96 326
+// and 181.  Splits of tiles of 256: 512 rows after 4001 119, 89, 77, 103 with 2, 3, 4, 6.  (64 rows per wave of the small kernel, at one wave
 // per SIMD, were slower than 32 everywhere, by up to 3 times.)
 //
 // Partial states fill at most kMostParts bytes: a call of that many rows (16384 tokens of 64 heads in two splits) has 16 turns of tiles of 256 and more, and a split

@@ -13,16 +13,17 @@
 //
 // A wave has its SIMD to itself, so the vector work is laid between the matrix instructions by hand, in slots: while the first product of the
 // next 32 positions runs, the weights of these 32; while their second product runs, the logits of the next, and the unpacking of what the
-// workgroup needs a step later.  2048 tokens after 30720, 64 on 8 heads: 2.3 ms, 930 TFLOP/s, 1100 with the products for the sums and the lines;
-// a step takes some 5000 cycles, 2432 of them matrix instructions, at the 2.0 - 2.2 GHz that its power allows (a large library product: 1140).
+// workgroup needs a step later.  2048 tokens after 30720, 64 on 8 heads: 2.31 to 2.50 ms on different cards, 850 to 920 TFLOP/s, 1000 to 1090 with the products for
+// the sums and the lines; a step takes some 5000 cycles, 2432 of them matrix instructions, at the 2.0 - 2.2 GHz that its power allows (a large library product: 1140).
 #include "qr_chunk.h"
 
 namespace {
 
 constexpr int kRows = 256, kStep = 64;
 // LDS: three steps' keys (the next step's are read while others still read this one's), two steps' values
-// A key's row is padded by 16 bytes, a dimension's too, and 16 more behind every 32nd: so that neither the reads (16 lanes of 16 bytes, rows that follow one
-// another) nor the writes (32 lanes of 8 bytes, rows 4, 8, 32 and 64 apart) meet in a bank, and every piece's place is one address per lane and a constant.
+// A key's row is padded by 16 bytes, a dimension's too, and 16 more behind every 32nd, so that the reads (16 lanes of 16 bytes, rows that follow one another) and the
+// writes (32 lanes of 8 bytes, rows 4, 8, 32 and 64 apart) spread over the banks, and every piece's place is one address per lane and a constant.  Of 2048 tokens after
+// 30720 conflicts are 18 % of the cycles that LDS works (SQ_LDS_BANK_CONFLICT 6.5e7 of SQ_LDS_IDX_ACTIVE 3.5e8).
 constexpr int kKeyRow = 272, kDimRow = 144;
 __host__ __device__ constexpr int dim_row(int r) { return r * kDimRow + (r >> 5) * 16; }
 constexpr int kSlope = 64 * kKeyRow, kLine = kSlope + 256, kThere = kLine + 2048, kKeys = (kThere + 8 + 511) / 512 * 512;

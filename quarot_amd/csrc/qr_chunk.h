@@ -59,7 +59,7 @@ __device__ __forceinline__ float quarters_max(float v) {
 // ---- int4 operands
 // The codes of a word as fp16 operands: pairs (0, 4), (1, 5), (2, 6), (3, 7).  A code in the lowest (next) four bits of a half is the subnormal number
 // code 2^-24 (code 2^-20), which the matrix instructions take exactly: no conversion.  The query's dimensions come in that order, those that meet an
-// upper nibble a sixteenth (exact from 2^-10 on), and logits take 2^24.
+// upper nibble a sixteenth (exact from 2^-10 on, below in units of 2^-20), and logits take 2^24.
 constexpr float kCodeUnit = 16777216.f;
 constexpr u32 kNoParameters = 0x00003C00u;                 // scale 1, zero 0
 __device__ __forceinline__ u32x4 codes_of(u32 w) {
@@ -158,7 +158,7 @@ __device__ __forceinline__ int lanes_sum(int v) {          // over the wave
 }
 // Work item `number` of a head: a sequence and one of its tiles of PER rows, last tiles (most positions) first; false: there is none.  Items without rows come
 // last: between others they leave whole shader engines idle, since workgroups are handed out to them in turn (8 sequences of 2048, 1792 .. 256 tokens, 64 on 8
-// heads: 552 us with them, 383 without).  Of more than 64 sequences the tiles are not counted.
+// heads: 528 us with them, 369 without).  Of more than 64 sequences the tiles are not counted.
 template <int PER>
 __device__ __forceinline__ bool item_of(const Chunk& a, int number, int& b, int& tile) {
     const int batch = a.c.batch_size;
