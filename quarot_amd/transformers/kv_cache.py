@@ -351,10 +351,11 @@ def batch_chunk_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
 
     q_heads may be a multiple of the cache's heads: query heads h G .. h G + G - 1 share key head h.  window > 0: a token sees the last
     `window` positions, its own among them, and the first `sinks` of the sequence.  A row that sees nothing is zero; rows of `o`
-    outside seqlen_indptr's bounds are left as they are, and new tokens that the bounds count behind q's last row are left out.  q and o may be slices of wider rows (a fused projection), each token's heads
-    contiguous.  max_new_len, max_seq_len (optional): the largest counts of new tokens and of positions; they size the launch, and the
-    latter lets few rows be split along the positions.  q_hadamard: the kernel applies matmul_had_cuda(q, torch.float16) first.
-    workspace: as batch_decode_i4's, with arbitrary contents.  Writes into `o` and returns None."""
+    outside seqlen_indptr's bounds are left as they are, and new tokens that the bounds count behind q's last row are left out.  q and o
+    may be slices of wider rows (a fused projection), each token's heads contiguous.  max_new_len, max_seq_len (optional): the largest
+    counts of new tokens and of positions; they size the launch, may be wrong at the cost of time only, and the latter lets few rows be
+    split along the positions.  q_hadamard: the kernel applies matmul_had_cuda(q, torch.float16) first.  workspace: as
+    batch_decode_i4's, with arbitrary contents (at most 1 GiB is asked for).  Writes into `o` and returns None."""
     _chunk("batch_chunk_i4", False, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
            max_seq_len, window, sinks, q_hadamard, workspace)
 
