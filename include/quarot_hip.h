@@ -468,6 +468,80 @@ int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_strid
                        void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Attention of new tokens of sequences that begin with the same text, whose pages are held once (no counterpart in the reference):
+ *   the first prefixes of positions lie on page lists of their own, prefix_indptr int32 [prefixes + 1], prefix_indices,
+ *   prefix_last_page_offset int32 [prefixes], in the same pool of pages; prefix p is that of the sequences prefix_sequences[p] ..
+ *   prefix_sequences[p + 1] - 1 (int32 [prefixes + 1], not descending; NULL, with one prefix: of all sequences).  The page tables of the
+ *   sequences hold what follows.  Every new token sees all of its sequence's prefix and, as qr_batch_chunk_i4, its own positions up to its own.
+ *   A sequence of no prefix (before the first bound, behind the last) sees its own positions only.
+ * Everything else as qr_batch_chunk_i4 / qr_batch_chunk_f16, except:
+ *   lse_or_null fp32 [tokens, num_q_heads]: the natural logarithm of every row's sum of exponentials of its logits (over 1 / sqrt(128) included),
+ *   -inf for a row that sees nothing; of the weights as they were rounded, so within 2^-11 of the exact one.  Rows that are left stay as they are.
+ *   prefixes == 0: the sequences' own positions only (qr_batch_chunk with lse); window > 0 only then (QR_E_SHAPE).
+ *   max_prefix_len: the largest number of a prefix's positions if the caller knows it, else 0.
+ *   With prefixes a workspace of qr_batch_shared_workspace_bytes bytes is required (QR_E_WORKSPACE): a row's partial states, two at least, 528
+ *   bytes each.
+ */
+size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
+                                       int64_t max_seq_len, int64_t window, int64_t sinks, int64_t prefixes, int64_t max_prefix_len);
+int qr_batch_shared_i4(void* o, int64_t o_stride, void* lse_or_null, const void* q, int64_t q_stride, int q_had_mode,
+                       const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,
+                       const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                       int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim,
+                       int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
+                       const void* prefix_indptr, const void* prefix_indices, const void* prefix_last_page_offset,
+                       const void* prefix_sequences_or_null, int64_t prefixes, int64_t max_prefix_len, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int qr_batch_shared_f16(void* o, int64_t o_stride, void* lse_or_null, const void* q, int64_t q_stride, int q_had_mode,
+                        const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,
+                        const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                        int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim,
+                        int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
+                        const void* prefix_indptr, const void* prefix_indices, const void* prefix_last_page_offset,
+                        const void* prefix_sequences_or_null, int64_t prefixes, int64_t max_prefix_len, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
+ * Eviction from the paged cache by accumulated attention weight (no counterpart in the reference).
+ *
+ * qr_accumulate_weights_i4 / _f16: weights[b, h, j] += sum over the new tokens t of sequence b and the query heads g of key head h of
+ *   exp( q[t, g, :] . k[j, h] / sqrt(128) - lse[t, g] ), over the positions j that t sees: what the attention of qr_batch_chunk_* or
+ *   qr_batch_shared_* with that lse gives to position j.  weights fp32 [batch_size, num_heads, capacity]; positions from `capacity` on are left
+ *   out.  q, q_stride, q_had_mode, seqlen_indptr_or_null, tokens, the cache, max_new_len, max_seq_len, window and sinks as qr_batch_chunk_i4;
+ *   lse fp32 [tokens, num_q_heads] (a row whose lse is -inf gives nothing).  Everything in 32 bits, int4 codes as they are; no atomics: the
+ *   same inputs give the same bits.  A NaN or infinity of a key reaches that position alone, one of a query the positions that it sees.
+ *   Positions on page numbers outside [0, num_pages) get nothing.
+ * qr_heavy_positions: of every sequence b and key head h that holds more than `keep` of lengths[b] positions the first `sinks`, the last
+ *   `recent` (sinks + recent <= keep) and between them those of the largest weights, of equal ones the lowest positions (NaN counts below all
+ *   numbers): kept int32 [batch_size, num_heads, keep], ascending; of shorter sequences all of them, then -1.  lengths int32 (below 0: 0,
+ *   above `capacity`: capacity), new_lengths int32 [batch_size] = min(length, keep).  batch_size * num_heads below 2^22, capacity and keep below 2^30.
+ * qr_keep_positions_i4 / _f16: entry i of kept int32 [batch_size, num_heads, keep] (ascending where it is not negative) goes to position i of its
+ *   sequence, in place, for one layer: keys, values, their parameters, and weights if they are given, whose other entries up to the sequence's
+ *   length (as the page tables have it, before) become zero.  Entries that are no position of the sequence, or lie on a page number outside
+ *   [0, num_pages), are skipped.  Sequences of one prefix's pages must not be among those that move.
+ */
+int qr_accumulate_weights_i4(void* weights, int64_t capacity, const void* q, int64_t q_stride, int q_had_mode, const void* lse,
+                             const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,
+                             const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                             int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim,
+                             int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
+                             void* stream);
+int qr_accumulate_weights_f16(void* weights, int64_t capacity, const void* q, int64_t q_stride, int q_had_mode, const void* lse,
+                              const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,
+                              const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                              int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim,
+                              int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
+                              void* stream);
+int qr_heavy_positions(const void* weights, int64_t capacity, const void* lengths, int64_t batch_size, int num_heads, int64_t keep,
+                       int64_t sinks, int64_t recent, void* kept, void* new_lengths, void* stream);
+int qr_keep_positions_i4(const void* kept, int64_t keep, void* kv_data, void* kv_param, const void* kv_indptr, const void* kv_indices,
+                         const void* last_page_offset, int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size,
+                         int head_dim, int64_t batch_size, void* weights_or_null, int64_t capacity, void* stream);
+int qr_keep_positions_f16(const void* kept, int64_t keep, void* kv_data, void* kv_param, const void* kv_indptr, const void* kv_indices,
+                          const void* last_page_offset, int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size,
+                          int head_dim, int64_t batch_size, void* weights_or_null, int64_t capacity, void* stream);
+
+/*
  * Page tables of sequences of unequal lengths, from lengths on the device (qr_page_tables is for one common length):
  *   lengths int32 [batch_size], the tokens every sequence holds (negative: none; more than max_pages * page_size: that many);
  *   block_table_or_null int32 [batch_size, >= max_pages], rows table_stride apart: the pages of every sequence (NULL: page i of

@@ -17,6 +17,11 @@ _i64, _int, _f32, _ptr = _c.c_int64, _c.c_int, _c.c_float, _c.c_void_p
 _CHUNK = (_ptr, _i64, _ptr, _i64, _int, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int, _i64, _i64, _i64, _i64,
           _i64, _ptr, _c.c_size_t, _ptr)
 
+_SHARED = (_ptr, _i64, _ptr, *_CHUNK[2:24], _ptr, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _c.c_size_t, _ptr)
+_WEIGHTS = (_ptr, _i64, _ptr, _i64, _int, _ptr, _ptr, _i64, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int, _i64, _i64, _i64, _i64,
+            _i64, _ptr)
+_KEEP = (_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _int, _int, _int, _int, _int, _i64, _ptr, _i64, _ptr)
+
 # name -> (restype, argtypes); mirrors include/quarot_hip.h one to one
 SIGNATURES = {
     "qr_version": (_int, ()),
@@ -62,6 +67,14 @@ SIGNATURES = {
     "qr_batch_chunk_workspace_bytes": (_c.c_size_t, (_int, _i64, _int, _int, _i64, _i64, _i64, _i64, _i64)),
     "qr_batch_chunk_i4": (_int, _CHUNK),
     "qr_batch_chunk_f16": (_int, _CHUNK),
+    "qr_batch_shared_workspace_bytes": (_c.c_size_t, (_int, _i64, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64)),
+    "qr_batch_shared_i4": (_int, _SHARED),
+    "qr_batch_shared_f16": (_int, _SHARED),
+    "qr_accumulate_weights_i4": (_int, _WEIGHTS),
+    "qr_accumulate_weights_f16": (_int, _WEIGHTS),
+    "qr_heavy_positions": (_int, (_ptr, _i64, _ptr, _i64, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr)),
+    "qr_keep_positions_i4": (_int, _KEEP),
+    "qr_keep_positions_f16": (_int, _KEEP),
     "qr_build_page_tables": (_int, (_ptr, _ptr, _i64, _int, _i64, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr)),
     "qr_calib_mfma_i8": (_int, (_int, _int, _int, _ptr, _ptr)),
     "qr_calib_copy": (_int, (_ptr, _ptr, _i64, _ptr)),

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
 
     for (int tile = first_tile; tile * 16 * NB < rows; tile += a.tiles) {
         const int r0 = tile * 16 * NB, r1 = r0 + 16 * NB < rows ? r0 + 16 * NB : rows;
-        const int lowest = first_place + divided(r0, a.per_group), highest = first_place + divided(r1 - 1, a.per_group);
+        const int lowest = first_place + divided(r0, a.per_place), highest = first_place + divided(r1 - 1, a.per_place);
         const Steps steps = steps_of<5>(a, lowest, highest);
         const int stride = NW * a.splits;
 
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
             const int r = r0 + 16 * nb + n;
             const bool in = r < rows;
             const int t = divided(in ? r : r0, a.per_group), head = h * a.group + (in ? r : r0) - t * a.group;
-            place[nb] = in ? first_place + t : -1;
+            place[nb] = in ? first_place + divided(r, a.per_place) : -1;
             const u32x4* src = (const u32x4*)(a.q + (int64_t)(start + t) * a.q_stride + (int64_t)head * 128) + (F16 ? g : 4 * g);
             u32x4 w[4];
 #pragma unroll
@@ -434,13 +434,14 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                         for (int j = 0; j < 4; ++j) O[i][j] = __builtin_fmaf(src[1 + PER * l + i][j], keep, O[i][j]);
                 }
                 const int t = divided(r, a.per_group), head = h * a.group + r - t * a.group;
-                if (a.splits == 1) {
+                if (a.parts == 1) {
                     const float inv = D == 0.f ? 0.f : 1.f / D;                 // (a row that sees nothing is zero)
+                    if (a.lse && l == 0) a.lse[(int64_t)(start + t) * (c.num_heads * a.group) + head] = lse_of(M, D);
                     u32x2* const dst = (u32x2*)(a.o + (int64_t)(start + t) * a.o_stride + (int64_t)head * 128) + PER * l;
 #pragma unroll
                     for (int i = 0; i < PER; ++i) dst[i] = u32x2{cvt_f16x2(O[i][0] * inv, O[i][1] * inv), cvt_f16x2(O[i][2] * inv, O[i][3] * inv)};
                 } else {
-                    float* dst = a.part + (((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.splits + split) * 132;
+                    float* dst = a.part + (((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.parts + a.part_at + split) * 132;
                     if (l == 0) dst[0] = M, dst[1] = D;
 #pragma unroll
                     for (int i = 0; i < PER; ++i) *((f32x4*)dst + 1 + PER * l + i) = O[i];
@@ -492,6 +493,62 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
         u32x4{cvt_f16x2(a[0] * inv, a[1] * inv), cvt_f16x2(a[2] * inv, a[3] * inv), cvt_f16x2(b[0] * inv, b[1] * inv), cvt_f16x2(b[2] * inv, b[3] * inv)};
 }
 
+// The same where a row's states are of two launches, `own` of its sequence's positions and then those of the prefix that its sequence shares (a row of a sequence
+// outside members[0] .. members[prefixes] has none of these), and where the logarithms of the sums are asked for: sixteen lanes per row, eight dimensions each.
+struct Joined {
+    const float* part;
+    const int32_t *starts, *members;
+    f16* o;
+    float* lse;                        // may be nullptr
+    int64_t o_stride;
+    int batch, tokens, heads, prefixes, own, parts;
+    Divisor per_head;
+};
+__global__ __launch_bounds__(64) void chunk_join_kernel(Joined a) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 4);
+    const int l = threadIdx.x & 15;
+    const int64_t token = divided((int)row, a.per_head);
+    const int head = (int)(row - token * a.heads);
+    if (token >= a.tokens || (a.starts && (token < a.starts[0] || token >= a.starts[a.batch]))) return;
+    int from_token = 0, to_token = 0x7fffffff;             // tokens of sequences that have a prefix
+    if (a.members) {
+        auto bound = [&](int i) {
+            const int s = a.members[i], in = s < 0 ? 0 : s > a.batch ? a.batch : s;
+            return a.starts ? a.starts[in] : in;
+        };
+        from_token = bound(0), to_token = bound(a.prefixes);
+    }
+    const int states = token >= from_token && token < to_token ? a.parts : a.own;
+    const f32x4* src = (const f32x4*)(a.part + row * a.parts * 132);
+    float M = kEmpty;
+    for (int s = l; s < states; s += 16) M = __builtin_fmaxf(M, src[s * 33][0]);
+#pragma unroll
+    for (int bit = 1; bit < 16; bit *= 2) M = __builtin_fmaxf(M, __shfl_xor(M, bit, 16));
+    float D = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+    for (int from = 0; from < states; from += 4) {
+        f32x4 head4[4], x4[4], y4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4* const at = src + (from + i < states ? from + i : states - 1) * 33;
+            head4[i] = at[0], x4[i] = at[1 + 2 * l], y4[i] = at[2 + 2 * l];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (from + i < states) {
+                const float k = __builtin_amdgcn_exp2f(head4[i][0] - M);
+                D = __builtin_fmaf(head4[i][1], k, D);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(x4[i][j], k, x[j]), y[j] = __builtin_fmaf(y4[i][j], k, y[j]);
+            }
+        }
+    }
+    const float inv = D == 0.f ? 0.f : 1.f / D;
+    if (a.lse && l == 0) a.lse[row] = lse_of(M, D);
+    *((u32x4*)(a.o + token * a.o_stride + (int64_t)head * 128) + l) =
+        u32x4{cvt_f16x2(x[0] * inv, x[1] * inv), cvt_f16x2(x[2] * inv, x[3] * inv), cvt_f16x2(y[0] * inv, y[1] * inv), cvt_f16x2(y[2] * inv, y[3] * inv)};
+}
+
 // How a call is cut: column blocks and waves of a workgroup (nb 0: the kernel of 256 rows), tiles of rows per (sequence, key head), splits of the
 // positions.
 //
@@ -519,7 +576,8 @@ struct ChunkPlan {
 constexpr size_t kMostParts = (size_t)1 << 30;
 constexpr int kMostHeads = 65536;                          // (with most splits a sequence's heads are a launch)
 size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? (size_t)tokens * q_heads * splits * 132 * sizeof(float) : 0; }
-ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
+ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
+                     bool causal = true) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     if (max_new_len < (tokens + batch - 1) / batch) max_new_len = (tokens + batch - 1) / batch;        // (some sequence has as many)
     const bool even = max_new_len * batch == tokens;
@@ -556,7 +614,7 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
             if (some < groups) groups = some;
         }
         groups *= num_heads;
-        const int64_t late = max_new_len - per / group;    // (what the first tile does not see of the last one's positions, at most)
+        const int64_t late = causal ? max_new_len - per / group : 0;    // (what the first tile does not see of the last one's positions, at most)
         const float steps = (float)(seen - (late > 0 ? (late < seen ? late : seen) / 2 : 0)) / (float)step;
         for (int s = 1; s <= 32; ++s) {
             if (s > 1 && (steps < (float)(3 * s) || chunk_part_bytes(tokens, (int64_t)group * num_heads, s) > kMostParts)) break;
@@ -585,64 +643,163 @@ int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t gr
     return qr_launch_status();
 }
 
-int batch_chunk(bool fp16, void* o, int64_t o_stride, const void* q, int64_t q_stride, int q_had_mode, const void* seqlen_indptr_or_null, int64_t tokens,
-                int num_q_heads, const void* kv_data, const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
-                int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim, int64_t batch_size, int64_t max_new_len,
-                int64_t max_seq_len, int64_t window, int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
-    const int rc = qr_internal_check_paged_cache(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,
-                                                 page_size, head_dim, batch_size);
-    if (rc != QR_OK) return rc;
-    if (q_had_mode != 0 && q_had_mode != 1) return QR_E_DTYPE;
-    if (tokens < 0 || num_q_heads <= 0 || num_q_heads % num_heads || window < 0 || sinks < 0 || max_new_len < 0 || max_seq_len < 0) return QR_E_SHAPE;
-    if (tokens == 0 || batch_size == 0) return QR_OK;
-    if (!seqlen_indptr_or_null && tokens != batch_size) return QR_E_SHAPE;       // one new token per sequence
-    if (!o || !q) return QR_E_NULL;
-    if (((uintptr_t)q & 15) || ((uintptr_t)o & 15) || q_stride % 8 || o_stride % 8) return QR_E_ALIGN;
-    const int64_t width = (int64_t)num_q_heads * 128;
-    if (q_stride < width || o_stride < width || tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > kMostHeads)
-        return QR_E_SHAPE;
-    const ChunkPlan plan = chunk_plan(fp16, tokens, num_q_heads / num_heads, num_heads, batch_size, seqlen_indptr_or_null ? max_new_len : 1, max_seq_len, window, sinks);
-    Chunk a;
-    a.c = qr_internal_paged_kv((void*)kv_data, (void*)kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,
-                               page_size, batch_size);
-    a.q = (const f16*)q;
-    a.o = (f16*)o;
-    a.starts = (const int32_t*)seqlen_indptr_or_null;
-    a.q_stride = q_stride, a.o_stride = o_stride;
-    a.tokens = (int)tokens;
-    a.group = num_q_heads / num_heads;
-    a.per_group = divisor_of(a.group);
-    a.per_head = divisor_of(num_heads);
+// The launches of one set of page tables: a's sequences (or prefixes) as the plan cuts them.  A launch has fewer than 2^32 threads: fewer tiles at a time where hints
+// are missing (a workgroup goes on to the next one behind them), then fewer sequences.
+int launch_chunk(bool fp16, const ChunkPlan& plan, Chunk a, hipStream_t st) {
+    const int64_t batch_size = a.c.batch_size, num_q_heads = (int64_t)a.c.num_heads * a.group;
     a.tiles = plan.tiles;
-    a.window = (int)(window > 0x3fffffff ? 0 : window);    // (longer than any sequence)
-    a.sinks = (int)(sinks > 0x3fffffff ? 0x3fffffff : sinks);
-    a.q_had = q_had_mode;
-    a.splits = plan.splits;
-    if (a.splits > 1 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < chunk_part_bytes(tokens, num_q_heads, a.splits))) a.splits = 1;
-    a.per_split = divisor_of(a.splits);
-    a.part = (float*)workspace;
-    // A launch has fewer than 2^32 threads: fewer tiles at a time where hints are missing (a workgroup goes on to the next one behind them), then fewer sequences
-    const int64_t most = 0xffffffffll / (plan.nb == 0 ? 256 : 64 * plan.nw), wide = (int64_t)num_heads * a.splits;
+    a.splits = plan.splits, a.per_split = divisor_of(plan.splits);
+    const int64_t most = 0xffffffffll / (plan.nb == 0 ? 256 : 64 * plan.nw), wide = (int64_t)a.c.num_heads * a.splits;
     if (batch_size * wide * plan.tiles > most) a.tiles = (int)(batch_size * wide < most ? most / (batch_size * wide) : 1);
     const int64_t at_once = batch_size * wide <= most ? batch_size : most / wide;
-    hipStream_t st = (hipStream_t)stream;
-    const Divisor pages = divisor_of(page_size);
-    const bool aligned = page_size % 16 == 0;
-    int lrc = QR_OK;
-    for (int64_t first = 0; first < batch_size && lrc == QR_OK; first += at_once) {
+    const Divisor pages = divisor_of(a.c.page_size);
+    const bool aligned = a.c.page_size % 16 == 0;
+    int rc = QR_OK;
+    for (int64_t first = 0; first < batch_size && rc == QR_OK; first += at_once) {
         Chunk some = a;
         some.c.batch_size = (int)(batch_size - first < at_once ? batch_size - first : at_once);
         some.c.indptr += first, some.c.last_page_offset += first;
-        if (a.starts) some.starts += first;
-        else some.q += first * q_stride, some.o += first * o_stride, some.part += a.splits > 1 ? first * num_q_heads * a.splits * 132 : 0;
+        if (a.prefix) some.members += a.members ? first : 0;
+        else if (a.starts) some.starts += first;
+        else {
+            some.q += first * a.q_stride, some.o += first * a.o_stride;
+            some.part += a.parts > 1 ? first * num_q_heads * a.parts * 132 : 0;
+            some.lse += a.lse ? first * num_q_heads : 0;
+        }
         const int64_t groups = some.c.batch_size * wide * a.tiles;
-        lrc = plan.nb == 0 ? qr_internal_chunk_tiles(fp16, some, pages, groups, st)
-              : fp16       ? (aligned ? launch_rows<true, true>(plan, some, pages, groups, st) : launch_rows<true, false>(plan, some, pages, groups, st))
-                           : (aligned ? launch_rows<false, true>(plan, some, pages, groups, st) : launch_rows<false, false>(plan, some, pages, groups, st));
+        rc = plan.nb == 0 ? qr_internal_chunk_tiles(fp16, some, pages, groups, st)
+             : fp16       ? (aligned ? launch_rows<true, true>(plan, some, pages, groups, st) : launch_rows<true, false>(plan, some, pages, groups, st))
+                          : (aligned ? launch_rows<false, true>(plan, some, pages, groups, st) : launch_rows<false, false>(plan, some, pages, groups, st));
     }
-    if (lrc != QR_OK || a.splits == 1) return lrc;
-    chunk_merge_kernel<<<dim3((unsigned)((tokens * num_q_heads + 3) / 4)), dim3(64), 0, st>>>(a.part, a.starts, (int)batch_size, (int)tokens, num_q_heads, divisor_of(num_q_heads),
-                                                                                              a.splits, a.o, o_stride);
+    return rc;
+}
+
+struct ChunkCall {
+    void* o;
+    int64_t o_stride;
+    const void* q;
+    int64_t q_stride;
+    int q_had_mode;
+    const void* starts;
+    int64_t tokens;
+    int num_q_heads;
+    const void *kv_data, *kv_param, *kv_indptr, *kv_indices, *last_page_offset;
+    int64_t num_pages;
+    int num_layers, layer_idx, num_heads, page_size, head_dim;
+    int64_t batch_size, max_new_len, max_seq_len, window, sinks;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+};
+int check_chunk(const ChunkCall& t) {
+    const int rc = qr_internal_check_paged_cache(t.kv_data, t.kv_param, t.kv_indptr, t.kv_indices, t.last_page_offset, t.num_pages, t.num_layers, t.layer_idx, t.num_heads,
+                                                 t.page_size, t.head_dim, t.batch_size);
+    if (rc != QR_OK) return rc;
+    if (t.q_had_mode != 0 && t.q_had_mode != 1) return QR_E_DTYPE;
+    if (t.tokens < 0 || t.num_q_heads <= 0 || t.num_q_heads % t.num_heads || t.window < 0 || t.sinks < 0 || t.max_new_len < 0 || t.max_seq_len < 0) return QR_E_SHAPE;
+    if (t.tokens == 0 || t.batch_size == 0) return QR_OK;
+    if (!t.starts && t.tokens != t.batch_size) return QR_E_SHAPE;                // one new token per sequence
+    if (!t.o || !t.q) return QR_E_NULL;
+    if (((uintptr_t)t.q & 15) || ((uintptr_t)t.o & 15) || t.q_stride % 8 || t.o_stride % 8) return QR_E_ALIGN;
+    const int64_t width = (int64_t)t.num_q_heads * 128;
+    if (t.q_stride < width || t.o_stride < width || t.tokens > 0x3fffffff || t.tokens * t.num_q_heads > 0x3fffffff || t.num_q_heads / t.num_heads > 1024 || t.num_heads > kMostHeads)
+        return QR_E_SHAPE;
+    return QR_OK;
+}
+Chunk chunk_of(const ChunkCall& t) {
+    Chunk a;
+    a.c = qr_internal_paged_kv((void*)t.kv_data, (void*)t.kv_param, t.kv_indptr, t.kv_indices, t.last_page_offset, t.num_pages, t.num_layers, t.layer_idx, t.num_heads,
+                               t.page_size, t.batch_size);
+    a.q = (const f16*)t.q;
+    a.o = (f16*)t.o;
+    a.starts = (const int32_t*)t.starts;
+    a.q_stride = t.q_stride, a.o_stride = t.o_stride;
+    a.tokens = (int)t.tokens;
+    a.group = t.num_q_heads / t.num_heads;
+    a.per_group = a.per_place = divisor_of(a.group);
+    a.per_head = divisor_of(t.num_heads);
+    a.window = (int)(t.window > 0x3fffffff ? 0 : t.window);              // (longer than any sequence)
+    a.sinks = (int)(t.sinks > 0x3fffffff ? 0x3fffffff : t.sinks);
+    a.q_had = t.q_had_mode;
+    a.members = nullptr;
+    a.prefix = 0, a.sequences = (int)t.batch_size;
+    a.part = (float*)t.workspace;
+    a.part_at = 0;
+    a.lse = nullptr;
+    return a;
+}
+ChunkPlan plan_of(bool fp16, const ChunkCall& t) {
+    return chunk_plan(fp16, t.tokens, t.num_q_heads / t.num_heads, t.num_heads, t.batch_size, t.starts ? t.max_new_len : 1, t.max_seq_len, t.window, t.sinks);
+}
+
+int batch_chunk(bool fp16, const ChunkCall& t) {
+    const int rc = check_chunk(t);
+    if (rc != QR_OK || t.tokens == 0 || t.batch_size == 0) return rc;
+    ChunkPlan plan = plan_of(fp16, t);
+    if (plan.splits > 1 && (!t.workspace || ((uintptr_t)t.workspace & 15) || t.workspace_bytes < chunk_part_bytes(t.tokens, t.num_q_heads, plan.splits))) plan.splits = 1;
+    Chunk a = chunk_of(t);
+    a.parts = plan.splits;
+    hipStream_t st = (hipStream_t)t.stream;
+    const int lrc = launch_chunk(fp16, plan, a, st);
+    if (lrc != QR_OK || plan.splits == 1) return lrc;
+    chunk_merge_kernel<<<dim3((unsigned)((t.tokens * t.num_q_heads + 3) / 4)), dim3(64), 0, st>>>(a.part, a.starts, (int)t.batch_size, (int)t.tokens, t.num_q_heads,
+                                                                                                  divisor_of(t.num_q_heads), plan.splits, a.o, t.o_stride);
+    return qr_launch_status();
+}
+
+// ---- prefixes that several sequences share ---------------------------------------------------------------------------------------------------
+// A prefix is a page list that is attended to by the rows of all its sequences' tokens, as if they were one sequence's that see all of it: its vectors are read (and
+// unpacked) once per tile of those rows instead of once per sequence.  States of both launches are joined by a third.
+struct Prefixes {
+    const void *indptr, *indices, *last_page_offset, *members;
+    int64_t count, max_len;
+};
+struct SharedPlan {
+    ChunkPlan own, prefix;
+    int parts;                         // states per row; 1: none are written
+};
+SharedPlan shared_plan(bool fp16, const ChunkCall& t, int64_t prefixes, int64_t max_prefix_len, bool one_prefix) {
+    SharedPlan p{plan_of(fp16, t), ChunkPlan{0, 0, 0, 0}, 0};
+    if (prefixes > 0)
+        p.prefix = chunk_plan(fp16, t.tokens, t.num_q_heads / t.num_heads, t.num_heads, prefixes, one_prefix ? t.tokens : 0, max_prefix_len, 0, 0, false);
+    p.parts = p.own.splits + p.prefix.splits;
+    return p;
+}
+
+int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
+    int rc = check_chunk(t);
+    if (rc != QR_OK) return rc;
+    if (p.count < 0 || p.count > 0x7fffffff || p.max_len < 0 || (p.count > 0 && t.window > 0) || (p.count > 1 && !p.members)) return QR_E_SHAPE;
+    if (p.count > 0 && t.batch_size > 0 && (!p.indptr || !p.indices || !p.last_page_offset)) return QR_E_NULL;
+    if (t.tokens == 0 || t.batch_size == 0) return rc;
+    if ((uintptr_t)lse & 3) return QR_E_ALIGN;
+    SharedPlan plan = shared_plan(fp16, t, p.count, p.max_len, p.count == 1);
+    if (plan.parts > 1 && (!t.workspace || ((uintptr_t)t.workspace & 15) || t.workspace_bytes < chunk_part_bytes(t.tokens, t.num_q_heads, plan.parts))) {
+        if (p.count > 0) return QR_E_WORKSPACE;                // (its states are joined through memory)
+        plan.own.splits = plan.parts = 1;
+    }
+    Chunk a = chunk_of(t);
+    a.parts = plan.parts;
+    a.lse = lse;
+    hipStream_t st = (hipStream_t)t.stream;
+    rc = launch_chunk(fp16, plan.own, a, st);
+    if (rc != QR_OK || plan.parts == 1) return rc;
+    if (p.count > 0) {
+        Chunk b = a;
+        b.c.indptr = (const int32_t*)p.indptr, b.c.indices = (const int32_t*)p.indices, b.c.last_page_offset = (const int32_t*)p.last_page_offset;
+        b.c.batch_size = (int)p.count;
+        b.members = (const int32_t*)p.members;
+        b.prefix = 1, b.per_place = kNoPlace;
+        b.part_at = plan.own.splits;
+        rc = launch_chunk(fp16, plan.prefix, b, st);
+        if (rc != QR_OK) return rc;
+    }
+    Joined j;
+    j.part = a.part, j.starts = a.starts, j.members = (const int32_t*)p.members;
+    j.o = a.o, j.lse = lse, j.o_stride = t.o_stride;
+    j.batch = (int)t.batch_size, j.tokens = (int)t.tokens, j.heads = t.num_q_heads, j.prefixes = (int)p.count, j.own = plan.own.splits, j.parts = plan.parts;
+    j.per_head = divisor_of(t.num_q_heads);
+    chunk_join_kernel<<<dim3((unsigned)((t.tokens * t.num_q_heads + 3) / 4)), dim3(64), 0, st>>>(j);
     return qr_launch_status();
 }
 
@@ -662,9 +819,37 @@ extern "C" size_t qr_batch_chunk_workspace_bytes(int fp16_pages, int64_t tokens,
                         const void* kv_indices, const void* last_page_offset, int64_t num_pages, int num_layers, int layer_idx, int num_heads,     \
                         int page_size, int head_dim, int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,  \
                         void* workspace, size_t workspace_bytes, void* stream) {                                                                  \
-        return batch_chunk(FP16, o, o_stride, q, q_stride, q_had_mode, seqlen_indptr_or_null, tokens, num_q_heads, kv_data, kv_param, kv_indptr,    \
-                           kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size, head_dim, batch_size,           \
-                           max_new_len, max_seq_len, window, sinks, workspace, workspace_bytes, stream);                                          \
+        return batch_chunk(FP16, ChunkCall{o, o_stride, q, q_stride, q_had_mode, seqlen_indptr_or_null, tokens, num_q_heads, kv_data, kv_param,     \
+                                           kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size,       \
+                                           head_dim, batch_size, max_new_len, max_seq_len, window, sinks, workspace, workspace_bytes, stream});    \
     }
 QR_CHUNK_ENTRY(qr_batch_chunk_i4, false)
 QR_CHUNK_ENTRY(qr_batch_chunk_f16, true)
+
+extern "C" size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
+                                                  int64_t max_seq_len, int64_t window, int64_t sinks, int64_t prefixes, int64_t max_prefix_len) {
+    if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0 || batch_size > 0x7fffffff || prefixes < 0 || prefixes > 0x7fffffff) return 0;
+    if (tokens > 0x3fffffff || tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > kMostHeads) return 0;        // (the call itself refuses them)
+    ChunkCall t{};
+    t.starts = &t;                     // (the caller gives max_new_len 1 where there are no bounds)
+    t.tokens = tokens, t.num_q_heads = num_q_heads, t.num_heads = num_heads, t.batch_size = batch_size;
+    t.max_new_len = max_new_len, t.max_seq_len = max_seq_len, t.window = window, t.sinks = sinks;
+    return chunk_part_bytes(tokens, num_q_heads, shared_plan(fp16_pages != 0, t, prefixes, max_prefix_len, prefixes == 1).parts);
+}
+
+#define QR_SHARED_ENTRY(NAME, FP16)                                                                                                                   \
+    extern "C" int NAME(void* o, int64_t o_stride, void* lse_or_null, const void* q, int64_t q_stride, int q_had_mode,                                 \
+                        const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data, const void* kv_param,                \
+                        const void* kv_indptr, const void* kv_indices, const void* last_page_offset, int64_t num_pages, int num_layers,               \
+                        int layer_idx, int num_heads, int page_size, int head_dim, int64_t batch_size, int64_t max_new_len, int64_t max_seq_len,      \
+                        int64_t window, int64_t sinks, const void* prefix_indptr, const void* prefix_indices, const void* prefix_last_page_offset,    \
+                        const void* prefix_sequences_or_null, int64_t prefixes, int64_t max_prefix_len, void* workspace, size_t workspace_bytes,      \
+                        void* stream) {                                                                                                               \
+        return batch_shared(FP16, ChunkCall{o, o_stride, q, q_stride, q_had_mode, seqlen_indptr_or_null, tokens, num_q_heads, kv_data, kv_param,       \
+                                            kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size,          \
+                                            head_dim, batch_size, max_new_len, max_seq_len, window, sinks, workspace, workspace_bytes, stream},       \
+                            Prefixes{prefix_indptr, prefix_indices, prefix_last_page_offset, prefix_sequences_or_null, prefixes, max_prefix_len},     \
+                            (float*)lse_or_null);                                                                                                     \
+    }
+QR_SHARED_ENTRY(qr_batch_shared_i4, false)
+QR_SHARED_ENTRY(qr_batch_shared_f16, true)

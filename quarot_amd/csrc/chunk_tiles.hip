@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 
     for (int r_tile = tile * kRows; r_tile < rows; r_tile += a.tiles * kRows) {
         const int r_end = r_tile + kRows < rows ? r_tile + kRows : rows;
-        const int tile_lowest = first_place + divided(r_tile, a.per_group), tile_highest = first_place + divided(r_end - 1, a.per_group);
+        const int tile_lowest = first_place + divided(r_tile, a.per_place), tile_highest = first_place + divided(r_end - 1, a.per_place);
         const Steps steps = steps_of<6>(a, tile_lowest, tile_highest);
         const int s_begin = divided(steps.all * split, a.per_split), s_end = divided(steps.all * (split + 1), a.per_split);      // (below 2^24 steps, 2^5 splits)
         const int last = s_end - 1;
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         const int r0 = r_tile + 64 * wave;
         const int r_last = r0 + 63 < rows ? r0 + 63 : rows - 1;
         // (a wave without rows hides nothing: its results go nowhere, and the others wait for it)
-        const int lowest = r0 < rows ? first_place + divided(r0, a.per_group) : 0x7fffffff, highest = r0 < rows ? first_place + divided(r_last, a.per_group) : -1;
+        const int lowest = r0 < rows ? first_place + divided(r0, a.per_place) : 0x7fffffff, highest = r0 < rows ? first_place + divided(r_last, a.per_place) : -1;
         auto row_of = [&](int cb) { return r0 + 32 * cb + n; };
         auto token_of = [&](int cb) { return divided(row_of(cb) < rows ? row_of(cb) : r_tile, a.per_group); };
         auto head_of = [&](int cb, int token) { return head * a.group + (row_of(cb) < rows ? row_of(cb) : r_tile) - token * a.group; };
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         for (int cb = 0; cb < 2; ++cb) {
             const bool in = row_of(cb) < rows;
             const int token = token_of(cb);
-            place[cb] = in ? first_place + token : -1;
+            place[cb] = in ? first_place + divided(row_of(cb), a.per_place) : -1;
             const u32x4* src = (const u32x4*)(a.q + (int64_t)(tokens.start + token) * a.q_stride + (int64_t)head_of(cb, token) * 128) + (F16 ? 4 * h : h);
 #pragma unroll
             for (int s = 0; s < 8; ++s) qf[cb][s] = src[F16 ? (s >> 1) + 8 * (s & 1) : 2 * s];       // (rows that are not there: another one's, whose results go nowhere)
@@ -750,8 +750,9 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             if (row_of(cb) >= rows) continue;
             const int token = token_of(cb), q_head = head_of(cb, token);
             // lane (n, h): dimensions 32 db + 16 i + 8 h + 4 k + j of row n in register 4 (i + 2 k) + j of block db
-            if (a.splits == 1) {
+            if (a.parts == 1) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum, less = -zero * inv;
+                if (a.lse && h == 0) a.lse[(int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head] = lse_of(limit[cb] < 0.f ? kEmpty : m[cb], sum);
                 u32x4* const dst = (u32x4*)(a.o + (int64_t)(tokens.start + token) * a.o_stride + (int64_t)q_head * 128) + h;
 #pragma unroll
                 for (int db = 0; db < 4; ++db)
@@ -766,7 +767,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
                         dst[4 * db + 2 * i] = w;
                     }
             } else {
-                float* const dst = a.part + (((int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head) * a.splits + split) * 132;
+                float* const dst = a.part + (((int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head) * a.parts + a.part_at + split) * 132;
                 if (h == 0) dst[0] = limit[cb] < 0.f ? kEmpty : m[cb], dst[1] = sum;
 #pragma unroll
                 for (int db = 0; db < 4; ++db)

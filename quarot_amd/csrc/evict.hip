@@ -1,0 +1,229 @@
+// Eviction from the paged cache: which positions of a (sequence, key head) stay, and their move to the front.
+#include "qr_paged.h"
+
+namespace {
+
+// ---- which stay ------------------------------------------------------------------------------------------------------------------------------
+// Of a sequence of more than `keep` positions the first `sinks`, the last `recent`, and of those between the ones of the largest sums, the lowest
+// positions first among equal ones.  The least sum that stays is found digit by digit (11, 11 and 10 bits of the sums' order as integers) from
+// histograms in LDS; then every wave goes through its own range of positions in order and writes those that stay behind what the waves before it have.
+struct Heavy {
+    const float* sums;
+    const int32_t* lengths;
+    int32_t *kept, *left;
+    int64_t capacity;
+    int heads, keep, sinks, recent;
+};
+// sums in the order of unsigned integers: NaN below all numbers, both zeros the same
+__device__ __forceinline__ u32 order_of(float v) {
+    const u32 u = __builtin_bit_cast(u32, v);
+    return v != v ? 0u : v == 0.f ? 0x80000000u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+constexpr int kBins = 2048, kHeavyWaves = 16;
+
+__global__ __launch_bounds__(64 * kHeavyWaves) void heavy_positions_kernel(Heavy a) {
+    __shared__ u32 bins[kBins];
+    __shared__ u32 found[3];                               // the digit, how many lie above it, how many have it
+    __shared__ int counts[kHeavyWaves][2];
+    const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t held = a.lengths[b];
+    const int len = (int)(held < 0 ? 0 : held > a.capacity ? a.capacity : held);
+    if (h == 0 && tid == 0) a.left[b] = len < a.keep ? len : a.keep;
+    int32_t* const kept = a.kept + (int64_t)blockIdx.x * a.keep;
+    if (len <= a.keep) {
+        for (int i = tid; i < a.keep; i += 64 * kHeavyWaves) kept[i] = i < len ? i : -1;
+        return;
+    }
+    for (int i = tid; i < a.sinks; i += 64 * kHeavyWaves) kept[i] = i;
+    for (int i = tid; i < a.recent; i += 64 * kHeavyWaves) kept[a.keep - a.recent + i] = len - a.recent + i;
+    const int need = a.keep - a.sinks - a.recent, count = len - a.sinks - a.recent;          // 0 <= need < count
+    if (need == 0) return;
+    const float* const sums = a.sums + (int64_t)blockIdx.x * a.capacity + a.sinks;
+    const int each = ((count + kHeavyWaves - 1) / kHeavyWaves + 63) & ~63, from = wave * each, to = from + each < count ? from + each : count;
+
+    u32 prefix = 0, above = 0;                             // the digits found so far; how many sums lie above all that have them
+    int shift = 32;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int bits = pass < 2 ? 11 : 10, below = shift;
+        shift -= bits;
+        for (int i = tid; i < kBins; i += 64 * kHeavyWaves) bins[i] = 0;
+        __syncthreads();
+        for (int i = from + lane; i < to; i += 64) {
+            const u32 k = order_of(sums[i]);
+            if (below == 32 || k >> below == prefix) atomicAdd(&bins[k >> shift & ((1u << bits) - 1)], 1u);
+        }
+        __syncthreads();
+        // thread t has the bins 2 t and 2 t + 1 from the top; how many sums lie in the bins before its own
+        const u32 b0 = bins[kBins - 1 - 2 * tid], b1 = bins[kBins - 2 - 2 * tid];
+        u32 upto = b0 + b1;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const u32 v = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 63) counts[wave][0] = (int)upto;
+        __syncthreads();
+        u32 before = above + upto - b0 - b1;
+        for (int w = 0; w < wave; ++w) before += (u32)counts[w][0];
+        const u32 want = (u32)need;
+        if (before < want && before + b0 >= want) found[0] = kBins - 1 - 2 * tid, found[1] = before, found[2] = b0;
+        if (before + b0 < want && before + b0 + b1 >= want) found[0] = kBins - 2 - 2 * tid, found[1] = before + b0, found[2] = b1;
+        __syncthreads();
+        prefix = prefix << bits | found[0];
+        above = found[1];
+        const u32 in = found[2];
+        __syncthreads();
+        if (above + in == want) break;                     // (all that share these digits stay)
+    }
+    const int equal = need - (int)above;                   // of those with these digits that many stay, the first ones
+
+    int greater = 0, same = 0;
+    for (int i = from + lane; i - lane < to; i += 64) {
+        const u32 k = i < to ? order_of(sums[i]) >> shift : 0u;
+        greater += __popcll(__builtin_amdgcn_ballot_w64(i < to && k > prefix));
+        same += __popcll(__builtin_amdgcn_ballot_w64(i < to && k == prefix));
+    }
+    if (lane == 0) counts[wave][0] = greater, counts[wave][1] = same;
+    __syncthreads();
+    int out = 0, seen = 0;                                 // of the waves before this one: how many stay, how many have these digits
+    for (int w = 0; w < wave; ++w) out += counts[w][0], seen += counts[w][1];
+    out += seen < equal ? seen : equal;
+    for (int i = from + lane; i - lane < to; i += 64) {
+        const u32 k = i < to ? order_of(sums[i]) >> shift : 0u;
+        const uint64_t eq = __builtin_amdgcn_ballot_w64(i < to && k == prefix);
+        const int rank = seen + __builtin_amdgcn_mbcnt_hi((u32)(eq >> 32), __builtin_amdgcn_mbcnt_lo((u32)eq, 0));
+        const bool stays = i < to && (k > prefix || (k == prefix && rank < equal));
+        const uint64_t all = __builtin_amdgcn_ballot_w64(stays);
+        if (stays) kept[a.sinks + out + __builtin_amdgcn_mbcnt_hi((u32)(all >> 32), __builtin_amdgcn_mbcnt_lo((u32)all, 0))] = a.sinks + i;
+        out += __popcll(all), seen += __popcll(eq);
+    }
+}
+
+// ---- their move --------------------------------------------------------------------------------------------------------------------------------
+// Entry i of the list of a (sequence, key head) goes to position i, in place.  The list ascends, so a position is never behind its entry's: a workgroup goes
+// through one side's vectors (keys or values) in batches, all of a batch in registers before the first is written, and what it writes lies before every entry of
+// the batches to come.
+struct Keep {
+    PagedKV c;
+    const int32_t* kept;
+    float* sums;                       // [sequence, key head, capacity]; may be nullptr
+    int64_t capacity;
+    int keep;
+};
+constexpr int kKeepThreads = 512;
+
+template <bool F16>
+__global__ __launch_bounds__(kKeepThreads) void keep_positions_kernel(Keep a) {
+    constexpr int LANES = F16 ? 16 : 4, EACH = kKeepThreads / LANES, TURNS = 8;              // lanes of a vector, vectors at a time
+    const PagedKV& c = a.c;
+    const int id = blockIdx.x >> 1, side = blockIdx.x & 1, b = id / c.num_heads, h = id - b * c.num_heads;
+    const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
+    const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
+    const int32_t* const kept = a.kept + (int64_t)id * a.keep;
+    const int l = threadIdx.x % LANES, mine = threadIdx.x / LANES;
+    auto slot_of = [&](int pos) -> int64_t {               // -1: there is none
+        if (pos < 0 || pos >= len) return -1;
+        const int it = pos / c.page_size, entry = pos - it * c.page_size;
+        if (it >= npages) return -1;
+        const int64_t page = c.indices[p0 + it];
+        return page >= 0 && page < c.num_pages ? paged_slot(c, page, side, h, entry) : -1;
+    };
+    const int end = a.keep < len ? a.keep : len;
+    for (int first = 0; first < end; first += EACH * TURNS) {
+        u32x4 v[TURNS];
+        u32 p[TURNS];
+        int64_t to[TURNS];
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u) {
+            const int i = first + u * EACH + mine, source = i < end ? kept[i] : -1;
+            const int64_t at = source > i ? slot_of(source) : -1;
+            to[u] = at >= 0 ? slot_of(i) : -1;
+            if (to[u] >= 0) {
+                v[u] = *((const u32x4*)c.data + at * LANES + l);
+                if (l == 0) p[u] = c.param[at];
+            }
+        }
+        // (a batch's loads are over before any of its stores begins)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < TURNS; ++u)
+            if (to[u] >= 0) {
+                *((u32x4*)c.data + to[u] * LANES + l) = v[u];
+                if (l == 0) c.param[to[u]] = p[u];
+            }
+    }
+    if (side == 1 || !a.sums) return;
+    float* const sums = a.sums + (int64_t)id * a.capacity;
+    const int have = (int)(len < a.capacity ? len : a.capacity);
+    constexpr int W = 4;
+    for (int first = 0; first < have; first += kKeepThreads * W) {
+        float w[W];
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+            const int i = first + u * kKeepThreads + (int)threadIdx.x, source = i < a.keep && i < have ? kept[i] : -1;
+            w[u] = source >= i && source < have ? sums[source] : 0.f;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < W; ++u) {
+            const int i = first + u * kKeepThreads + (int)threadIdx.x;
+            if (i < have) sums[i] = w[u];
+        }
+    }
+}
+
+int keep_positions(bool fp16, const void* kept, int64_t keep, void* kv_data, void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,
+                   int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim, int64_t batch_size, void* weights, int64_t capacity,
+                   void* stream) {
+    const int rc = qr_internal_check_paged_cache(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size,
+                                                 head_dim, batch_size);
+    if (rc != QR_OK) return rc;
+    if (keep < 0 || keep > 0x3fffffff || capacity < 0) return QR_E_SHAPE;
+    if (batch_size == 0) return QR_OK;
+    if (batch_size * num_heads > 0x3fffff) return QR_E_SHAPE;              // (a launch has fewer than 2^32 threads)
+    if (keep > 0 && !kept) return QR_E_NULL;
+    if (((uintptr_t)kept & 3) || ((uintptr_t)weights & 3)) return QR_E_ALIGN;
+    Keep a;
+    a.c = qr_internal_paged_kv(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size, batch_size);
+    a.kept = (const int32_t*)kept;
+    a.sums = (float*)weights;
+    a.capacity = capacity;
+    a.keep = (int)keep;
+    const dim3 grid((unsigned)(batch_size * num_heads * 2));
+    if (fp16) keep_positions_kernel<true><<<grid, dim3(kKeepThreads), 0, (hipStream_t)stream>>>(a);
+    else keep_positions_kernel<false><<<grid, dim3(kKeepThreads), 0, (hipStream_t)stream>>>(a);
+    return qr_launch_status();
+}
+
+}  // namespace
+
+extern "C" int qr_heavy_positions(const void* weights, int64_t capacity, const void* lengths, int64_t batch_size, int num_heads, int64_t keep, int64_t sinks,
+                                  int64_t recent, void* kept, void* new_lengths, void* stream) {
+    if (batch_size < 0 || num_heads <= 0 || capacity < 0 || capacity > 0x3fffffff || keep < 0 || keep > 0x3fffffff || sinks < 0 || recent < 0 || sinks > keep ||
+        recent > keep - sinks)
+        return QR_E_SHAPE;
+    if (batch_size == 0) return QR_OK;
+    if (batch_size > 0x3fffff || batch_size * num_heads > 0x3fffff) return QR_E_SHAPE;      // (a launch has fewer than 2^32 threads)
+    if ((!weights && capacity > 0) || !lengths || (!kept && keep > 0) || !new_lengths) return QR_E_NULL;
+    if (((uintptr_t)weights & 3) || ((uintptr_t)lengths & 3) || ((uintptr_t)kept & 3) || ((uintptr_t)new_lengths & 3)) return QR_E_ALIGN;
+    Heavy a;
+    a.sums = (const float*)weights, a.lengths = (const int32_t*)lengths;
+    a.kept = (int32_t*)kept, a.left = (int32_t*)new_lengths;
+    a.capacity = capacity;
+    a.heads = num_heads, a.keep = (int)keep, a.sinks = (int)sinks, a.recent = (int)recent;
+    heavy_positions_kernel<<<dim3((unsigned)(batch_size * num_heads)), dim3(64 * kHeavyWaves), 0, (hipStream_t)stream>>>(a);
+    return qr_launch_status();
+}
+
+#define QR_KEEP_ENTRY(NAME, FP16)                                                                                                                        \
+    extern "C" int NAME(const void* kept, int64_t keep, void* kv_data, void* kv_param, const void* kv_indptr, const void* kv_indices,                    \
+                        const void* last_page_offset, int64_t num_pages, int num_layers, int layer_idx, int num_heads, int page_size, int head_dim,      \
+                        int64_t batch_size, void* weights_or_null, int64_t capacity, void* stream) {                                                     \
+        return keep_positions(FP16, kept, keep, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads,  \
+                              page_size, head_dim, batch_size, weights_or_null, capacity, stream);                                                       \
+    }
+QR_KEEP_ENTRY(qr_keep_positions_i4, false)
+QR_KEEP_ENTRY(qr_keep_positions_f16, true)

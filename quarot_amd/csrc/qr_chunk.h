@@ -18,12 +18,22 @@ struct Chunk {
     const f16* q;
     f16* o;
     const int32_t* starts;            // nullptr: one new token per sequence
-    float* part;                      // splits > 1: 132 floats per row and split: maximum, sum, -, -, 128 outputs
+    float* part;                      // parts > 1: 132 floats per row and split: maximum, sum, -, -, 128 outputs
     int64_t q_stride, o_stride;       // halves from a token to the next
     int tokens, group, tiles, splits, window, sinks;      // window 0: none
     int q_had;
     Divisor per_group, per_split, per_head;     // of `group`, `splits`, the key heads
+    // A row's position is the first new token's + divided(row, per_place): per_group's token by token; kNoPlace where all rows see all positions, which is a prefix
+    // that several sequences share.  Its "sequences" are the prefixes then: the rows of number b are the tokens of sequences members[b] .. members[b + 1] - 1
+    // (nullptr: of all `sequences`).
+    Divisor per_place;
+    const int32_t* members;
+    int prefix, sequences;
+    int parts, part_at;                         // partial states per row, and where this launch's begin (one state in all: rows are finished)
+    float* lse;                                 // parts 1: where the rows' logarithms of the softmax's sum go, [token, head]; may be nullptr
 };
+constexpr Divisor kNoPlace{0, 0};
+constexpr float kLn2 = 0.6931471805599453f;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kScale = 0.08838834764831845f;             // 1 / sqrt(128)
@@ -55,6 +65,9 @@ __device__ __forceinline__ float quarters_max(float v) {
     const u32x2 b = both_halves<32>(as_u32(v));
     return __builtin_fmaxf(as_f32(b.x), as_f32(b.y));
 }
+
+// of a row's maximum and sum (base 2): the natural logarithm of its sum of exponentials, -inf where it has seen nothing
+__device__ __forceinline__ float lse_of(float m, float sum) { return (m + __builtin_amdgcn_logf(sum)) * kLn2; }
 
 // ---- int4 operands
 // The codes of a word as fp16 operands: pairs (0, 4), (1, 5), (2, 6), (3, 7).  A code in the lowest (next) four bits of a half is the subnormal number
@@ -139,6 +152,14 @@ struct Fresh {
     int start, count, all;
 };
 __device__ __forceinline__ Fresh fresh_of(const Chunk& a, int b) {
+    if (a.prefix) {
+        auto sequence = [&](int i) { const int s = a.members[i]; return s < 0 ? 0 : s > a.sequences ? a.sequences : s; };
+        const int from = a.members ? sequence(b) : 0, to = a.members ? sequence(b + 1) : a.sequences;
+        int start = a.starts ? a.starts[from] : from, stop = a.starts ? a.starts[to] : to;
+        start = start < 0 ? 0 : start;
+        stop = stop > a.tokens ? a.tokens : stop;
+        return Fresh{start, stop > start ? stop - start : 0, 1};               // (all rows at the prefix's last position)
+    }
     if (!a.starts) return Fresh{b, 1, 1};
     int start = a.starts[b];
     const int end = a.starts[b + 1];

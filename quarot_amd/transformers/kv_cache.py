@@ -289,48 +289,59 @@ def batch_decode_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
             None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev)))
 
 
-def _chunk(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
-           window, sinks, q_hadamard, workspace):
-    if _lib.host.chunk(f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
-                       window, sinks, q_hadamard, workspace):
-        return
-    pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
-    dev, batch = kv_data.device, last_page_offset.shape[0]
-    for name, t in (("o", o), ("q", q)):
+def _queries(fn, queries, seqlen_indptr, heads, head_dim, batch, others, dev):
+    """The checks that attention of new tokens and what goes with it share: `queries`, (name, tensor) of [tokens, q_heads, 128], the bounds of the new
+    tokens, and that `others` lie on the cache's device.  Returns (tokens, q_heads)."""
+    for name, t in queries:
         if not (t.is_cuda and t.dim() == 3 and t.dtype == torch.float16):
             raise RuntimeError(f"{fn}: {name} must be a 3D fp16 CUDA tensor")
         if not (t.shape[2] == head_dim and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == head_dim)):
             raise RuntimeError(f"{fn}: {name} must be [tokens, heads, {head_dim}] with contiguous heads")
         if t.shape[0] > 1 and not (t.stride(0) >= t.shape[1] * head_dim and t.stride(0) % 8 == 0):
             raise RuntimeError(f"{fn}: {name}'s tokens must not overlap and start at multiples of 8 elements")
-    if not (o.shape == q.shape):
+    if len(queries) == 2 and not (queries[0][1].shape == queries[1][1].shape):
         raise RuntimeError(f"{fn}: o.size() != q.size()")
-    tokens, q_heads = q.shape[0], q.shape[1]
+    tokens, q_heads = queries[-1][1].shape[0], queries[-1][1].shape[1]
     if not (q_heads > 0 and heads > 0 and q_heads % heads == 0):
         raise RuntimeError(f"{fn}: q's heads must be a multiple of the cache's {heads}")
-    if not (kv_indptr.shape[0] == batch + 1):
-        raise RuntimeError(f"{fn}: CHECK_EQ(kv_indptr.size(0), batch_size + 1) failed")
     if seqlen_indptr is None:
         if not (tokens == batch):
             raise RuntimeError(f"{fn}: one token per sequence expected")
     elif not (seqlen_indptr.is_cuda and seqlen_indptr.is_contiguous() and seqlen_indptr.dtype == torch.int32
               and tuple(seqlen_indptr.shape) == (batch + 1,)):
         raise RuntimeError(f"{fn}: seqlen_indptr must be int32 [batch_size + 1]")
-    for name, t in (("o", o), ("q", q), ("kv_param", kv_param), ("kv_indptr", kv_indptr), ("kv_indicies", kv_indices),
-                    ("last_page_offset", last_page_offset), ("seqlen_indptr", seqlen_indptr)):
+    for name, t in (*queries, *others, ("seqlen_indptr", seqlen_indptr)):
         if t is not None and t.device != dev:
             raise RuntimeError(f"{fn}: expected all tensors on {dev}, but {name} is on {t.device}")
+    return tokens, q_heads
+
+
+def _lse(fn, lse, tokens, q_heads):
+    if not (lse.is_cuda and lse.is_contiguous() and lse.dtype == torch.float32 and tuple(lse.shape) == (tokens, q_heads)):
+        raise RuntimeError(f"{fn}: lse must be a contiguous fp32 [{tokens}, {q_heads}] CUDA tensor")
+
+
+def _chunk(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
+           window, sinks, q_hadamard, workspace, lse=None):
+    if lse is not None:
+        return _shared(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, None, None, None, None, seqlen_indptr, max_new_len,
+                       max_seq_len, 0, window, sinks, q_hadamard, lse, workspace)
+    if _lib.host.chunk(f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
+                       window, sinks, q_hadamard, workspace):
+        return
+    pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
+    dev, batch = kv_data.device, last_page_offset.shape[0]
+    if not (kv_indptr.shape[0] == batch + 1):
+        raise RuntimeError(f"{fn}: CHECK_EQ(kv_indptr.size(0), batch_size + 1) failed")
+    tokens, q_heads = _queries(fn, (("o", o), ("q", q)), seqlen_indptr, heads, head_dim, batch,
+                               (("kv_param", kv_param), ("kv_indptr", kv_indptr), ("kv_indicies", kv_indices), ("last_page_offset", last_page_offset)), dev)
     window, sinks, max_new_len, max_seq_len = int(window), int(sinks), int(max_new_len), int(max_seq_len)
     if window < 0 or sinks < 0 or max_new_len < 0 or max_seq_len < 0:
         raise RuntimeError(f"{fn}: window, sinks and the lengths must not be negative")
     with _lib.on_device(dev):
         ws_bytes = _lib.lib().qr_batch_chunk_workspace_bytes(1 if f16 else 0, tokens, q_heads, heads, batch, 1 if seqlen_indptr is None else max_new_len,
                                                              max_seq_len, window, sinks)
-        ws = None
-        if ws_bytes:
-            fits = (workspace is not None and workspace.device == dev and workspace.dtype == torch.uint8
-                    and workspace.is_contiguous() and workspace.numel() >= ws_bytes)
-            ws = workspace if fits else torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+        ws = _scratch(workspace, ws_bytes, dev)
         entry = _lib.lib().qr_batch_chunk_f16 if f16 else _lib.lib().qr_batch_chunk_i4
         row = q_heads * head_dim
         _lib.check(entry(
@@ -341,8 +352,61 @@ def _chunk(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
             _lib.stream_ptr(dev)))
 
 
+def _scratch(workspace, ws_bytes, dev):
+    if not ws_bytes:
+        return None
+    fits = (workspace is not None and workspace.device == dev and workspace.dtype == torch.uint8
+            and workspace.is_contiguous() and workspace.numel() >= ws_bytes)
+    return workspace if fits else torch.empty((ws_bytes,), dtype=torch.uint8, device=dev)
+
+
+def _shared(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices, prefix_last_page_offset,
+            prefix_sequences, seqlen_indptr, max_new_len, max_seq_len, max_prefix_len, window, sinks, q_hadamard, lse, workspace):
+    pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
+    dev, batch = kv_data.device, last_page_offset.shape[0]
+    if not (kv_indptr.shape[0] == batch + 1):
+        raise RuntimeError(f"{fn}: CHECK_EQ(kv_indptr.size(0), batch_size + 1) failed")
+    tables = (("prefix_indptr", prefix_indptr), ("prefix_indices", prefix_indices), ("prefix_last_page_offset", prefix_last_page_offset))
+    prefixes = 0
+    if prefix_indptr is not None:
+        for name, t in tables:
+            if not (t is not None and t.is_cuda and t.is_contiguous() and t.dim() == 1 and t.dtype == torch.int32):
+                raise RuntimeError(f"{fn}: {name} must be a contiguous 1D int32 CUDA tensor")
+        prefixes = prefix_last_page_offset.shape[0]
+        if not (prefix_indptr.shape[0] == prefixes + 1):
+            raise RuntimeError(f"{fn}: prefix_indptr must have one entry more than prefix_last_page_offset")
+        if prefix_sequences is None:
+            if prefixes > 1:
+                raise RuntimeError(f"{fn}: several prefixes need prefix_sequences")
+        elif not (prefix_sequences.is_cuda and prefix_sequences.is_contiguous() and prefix_sequences.dtype == torch.int32
+                  and tuple(prefix_sequences.shape) == (prefixes + 1,)):
+            raise RuntimeError(f"{fn}: prefix_sequences must be int32 [{prefixes + 1}]")
+    tokens, q_heads = _queries(fn, (("o", o), ("q", q)), seqlen_indptr, heads, head_dim, batch,
+                               (("kv_param", kv_param), ("kv_indptr", kv_indptr), ("kv_indicies", kv_indices), ("last_page_offset", last_page_offset), *tables,
+                                ("prefix_sequences", prefix_sequences), ("lse", lse)), dev)
+    if lse is not None:
+        _lse(fn, lse, tokens, q_heads)
+    max_new_len, max_seq_len, max_prefix_len, window, sinks = int(max_new_len), int(max_seq_len), int(max_prefix_len), int(window), int(sinks)
+    if window < 0 or sinks < 0 or max_new_len < 0 or max_seq_len < 0 or max_prefix_len < 0:
+        raise RuntimeError(f"{fn}: window, sinks and the lengths must not be negative")
+    with _lib.on_device(dev):
+        if seqlen_indptr is None:
+            max_new_len = 1
+        ws_bytes = _lib.lib().qr_batch_shared_workspace_bytes(1 if f16 else 0, tokens, q_heads, heads, batch, max_new_len, max_seq_len, window, sinks, prefixes,
+                                                              max_prefix_len)
+        ws = _scratch(workspace, ws_bytes, dev)
+        entry = _lib.lib().qr_batch_shared_f16 if f16 else _lib.lib().qr_batch_shared_i4
+        row = q_heads * head_dim
+        ptr = lambda t: None if t is None else t.data_ptr()
+        _lib.check(entry(
+            o.data_ptr(), o.stride(0) if tokens > 1 else row, ptr(lse), q.data_ptr(), q.stride(0) if tokens > 1 else row, 1 if q_hadamard else 0,
+            ptr(seqlen_indptr), tokens, q_heads, kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), last_page_offset.data_ptr(),
+            pages, layers, int(layer_idx), heads, page_size, head_dim, batch, max_new_len, max_seq_len, window, sinks, ptr(prefix_indptr), ptr(prefix_indices),
+            ptr(prefix_last_page_offset), ptr(prefix_sequences), prefixes, max_prefix_len, ptr(ws), ws_bytes, _lib.stream_ptr(dev)))
+
+
 def batch_chunk_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
-                   max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None):
+                   max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None, lse=None):
     """Attention of several new tokens per sequence over the int4 cache: q, o fp16 [tokens, q_heads, 128], the tokens of sequence b
     being seqlen_indptr[b] .. seqlen_indptr[b + 1] - 1 (None: token b, one per sequence), its LAST positions, whose keys and values
     quantize_append_kv_i4 or init_kv_i4 has stored with the same bounds.
@@ -355,16 +419,154 @@ def batch_chunk_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_off
     may be slices of wider rows (a fused projection), each token's heads contiguous.  max_new_len, max_seq_len (optional): the largest
     counts of new tokens and of positions; they size the launch, may be wrong at the cost of time only, and the latter lets few rows be
     split along the positions.  q_hadamard: the kernel applies matmul_had_cuda(q, torch.float16) first.  workspace: as
-    batch_decode_i4's, with arbitrary contents (at most 1 GiB is asked for).  Writes into `o` and returns None."""
+    batch_decode_i4's, with arbitrary contents (at most 1 GiB is asked for).  lse: an fp32 [tokens, q_heads] tensor for the natural logarithm of
+    every row's sum of exponentials (of the weights as they were rounded to fp16: within 2^-11; -inf for a row that sees nothing), which
+    accumulate_weights_i4 takes.  Writes into `o` and returns None."""
     _chunk("batch_chunk_i4", False, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
-           max_seq_len, window, sinks, q_hadamard, workspace)
+           max_seq_len, window, sinks, q_hadamard, workspace, lse)
 
 
 def batch_chunk_f16(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
-                    max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None):
+                    max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None, lse=None):
     """batch_chunk_i4 for the cache with fp16 pages (kv_data fp16 [pages, layers, 2, heads, page_size, 128])."""
     _chunk("batch_chunk_f16", True, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
-           max_seq_len, window, sinks, q_hadamard, workspace)
+           max_seq_len, window, sinks, q_hadamard, workspace, lse)
+
+
+def batch_shared_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices, prefix_last_page_offset,
+                    prefix_sequences=None, seqlen_indptr=None, max_new_len=0, max_seq_len=0, max_prefix_len=0, q_hadamard=False, lse=None, workspace=None):
+    """batch_chunk_i4 for sequences that begin with the same text, whose pages the pool holds once and each of whose vectors is read once for
+    all of them: prefix p lies on the page list prefix_indices[prefix_indptr[p]] .. with prefix_last_page_offset[p] entries in its last page,
+    and is that of sequences prefix_sequences[p] .. prefix_sequences[p + 1] - 1 (int32 [prefixes + 1], not descending; None, for one prefix:
+    of all).  kv_indptr, kv_indices and last_page_offset hold what follows the prefix, the new tokens last.
+
+        o[t, h] = softmax(q[t, h] . K^T / sqrt(128)) . V   over the prefix and the sequence's own positions up to the token's own
+
+    A sequence outside prefix_sequences' bounds has no prefix.  max_prefix_len (optional): the largest number of positions of a prefix; sizes the
+    launch like max_seq_len, which counts the sequences' own positions.  There is no window.  The rest as batch_chunk_i4."""
+    _prefix_needed("batch_shared_i4", prefix_indptr)
+    _shared("batch_shared_i4", False, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices,
+            prefix_last_page_offset, prefix_sequences, seqlen_indptr, max_new_len, max_seq_len, max_prefix_len, 0, 0, q_hadamard, lse, workspace)
+
+
+def batch_shared_f16(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices, prefix_last_page_offset,
+                     prefix_sequences=None, seqlen_indptr=None, max_new_len=0, max_seq_len=0, max_prefix_len=0, q_hadamard=False, lse=None, workspace=None):
+    """batch_shared_i4 for the cache with fp16 pages."""
+    _prefix_needed("batch_shared_f16", prefix_indptr)
+    _shared("batch_shared_f16", True, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices,
+            prefix_last_page_offset, prefix_sequences, seqlen_indptr, max_new_len, max_seq_len, max_prefix_len, 0, 0, q_hadamard, lse, workspace)
+
+
+def _prefix_needed(fn, prefix_indptr):
+    if prefix_indptr is None:
+        raise RuntimeError(f"{fn}: prefix_indptr must be a contiguous 1D int32 CUDA tensor")
+
+
+def _accumulate(fn, f16, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
+                window, sinks, q_hadamard):
+    pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
+    dev, batch = kv_data.device, last_page_offset.shape[0]
+    if not (kv_indptr.shape[0] == batch + 1):
+        raise RuntimeError(f"{fn}: CHECK_EQ(kv_indptr.size(0), batch_size + 1) failed")
+    tokens, q_heads = _queries(fn, (("q", q),), seqlen_indptr, heads, head_dim, batch,
+                               (("weights", weights), ("lse", lse), ("kv_param", kv_param), ("kv_indptr", kv_indptr), ("kv_indicies", kv_indices),
+                                ("last_page_offset", last_page_offset)), dev)
+    _lse(fn, lse, tokens, q_heads)
+    _weights(fn, weights, batch, heads)
+    window, sinks, max_new_len, max_seq_len = int(window), int(sinks), int(max_new_len), int(max_seq_len)
+    if window < 0 or sinks < 0 or max_new_len < 0 or max_seq_len < 0:
+        raise RuntimeError(f"{fn}: window, sinks and the lengths must not be negative")
+    with _lib.on_device(dev):
+        entry = _lib.lib().qr_accumulate_weights_f16 if f16 else _lib.lib().qr_accumulate_weights_i4
+        _lib.check(entry(
+            weights.data_ptr(), weights.shape[2], q.data_ptr(), q.stride(0) if tokens > 1 else q_heads * head_dim, 1 if q_hadamard else 0, lse.data_ptr(),
+            None if seqlen_indptr is None else seqlen_indptr.data_ptr(), tokens, q_heads, kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), last_page_offset.data_ptr(), pages, layers, int(layer_idx), heads, page_size, head_dim, batch,
+            1 if seqlen_indptr is None else max_new_len, max_seq_len, window, sinks, _lib.stream_ptr(dev)))
+
+
+def _weights(fn, weights, batch=None, heads=None):
+    if not (weights.is_cuda and weights.is_contiguous() and weights.dtype == torch.float32 and weights.dim() == 3
+            and (batch is None or tuple(weights.shape[:2]) == (batch, heads))):
+        raise RuntimeError(f"{fn}: weights must be a contiguous fp32 [batch_size, heads, capacity] CUDA tensor")
+
+
+def accumulate_weights_i4(weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
+                          max_seq_len=0, window=0, sinks=0, q_hadamard=False):
+    """Adds to every cached position what the new tokens' attention gives to it: with q and the bounds of a batch_chunk_i4 (or batch_shared_i4, whose
+    own positions they are) call and the lse that it gave,
+
+        weights[b, h, j] += sum of exp(q[t, g] . k[j, h] / sqrt(128) - lse[t, g])   over the sequence's new tokens t, the query heads g of key head h
+
+    for the positions j that t sees.  weights fp32 [batch_size, heads, capacity], contiguous; positions beyond its capacity are left out.  A
+    row whose lse is -inf gives nothing.  max_new_len and max_seq_len size the launch; window, sinks and q_hadamard as in the
+    attention's call.  The same inputs give the same bits.  Adds to `weights` and returns None."""
+    _accumulate("accumulate_weights_i4", False, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
+                max_seq_len, window, sinks, q_hadamard)
+
+
+def accumulate_weights_f16(weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
+                           max_seq_len=0, window=0, sinks=0, q_hadamard=False):
+    """accumulate_weights_i4 for the cache with fp16 pages."""
+    _accumulate("accumulate_weights_f16", True, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
+                max_seq_len, window, sinks, q_hadamard)
+
+
+def heavy_positions(weights, lengths, keep, sinks=0, recent=0):
+    """Which `keep` positions of every sequence and key head stay in the cache: the first `sinks`, the last `recent`, and between them those of the
+    largest weights (of equal ones the lowest positions; NaN counts below all numbers).  weights fp32 [batch_size, heads, capacity], lengths
+    int32 [batch_size], the positions that every sequence holds (at most the capacity).  Returns (kept, new_lengths): int32 [batch_size, heads, keep],
+    ascending, and int32 [batch_size] = min(length, keep); of a sequence of no more than `keep` positions kept is all of them, then -1."""
+    fn = "heavy_positions"
+    keep, sinks, recent = int(keep), int(sinks), int(recent)
+    _weights(fn, weights)
+    batch, heads, capacity = weights.shape
+    if not (lengths.is_cuda and lengths.device == weights.device and lengths.is_contiguous() and lengths.dtype == torch.int32 and tuple(lengths.shape) == (batch,)):
+        raise RuntimeError(f"{fn}: lengths must be int32 [batch_size] on {weights.device}")
+    if not (keep >= 0 and sinks >= 0 and recent >= 0 and sinks + recent <= keep):
+        raise RuntimeError(f"{fn}: sinks and recent must not be negative, nor together more than keep")
+    dev = weights.device
+    kept = torch.empty((batch, heads, keep), dtype=torch.int32, device=dev)
+    new_lengths = torch.empty((batch,), dtype=torch.int32, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().qr_heavy_positions(weights.data_ptr(), capacity, lengths.data_ptr(), batch, heads, keep, sinks, recent, kept.data_ptr(),
+                                                 new_lengths.data_ptr(), _lib.stream_ptr(dev)))
+    return kept, new_lengths
+
+
+def _keep(fn, f16, kept, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, weights):
+    pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
+    dev, batch = kv_data.device, last_page_offset.shape[0]
+    if not (kv_indptr.shape[0] == batch + 1):
+        raise RuntimeError(f"{fn}: CHECK_EQ(kv_indptr.size(0), batch_size + 1) failed")
+    if not (kept.is_cuda and kept.is_contiguous() and kept.dtype == torch.int32 and kept.dim() == 3 and tuple(kept.shape[:2]) == (batch, heads)):
+        raise RuntimeError(f"{fn}: kept must be a contiguous int32 [{batch}, {heads}, keep] CUDA tensor")
+    if weights is not None:
+        _weights(fn, weights, batch, heads)
+    for name, t in (("kept", kept), ("kv_param", kv_param), ("kv_indptr", kv_indptr), ("kv_indicies", kv_indices), ("last_page_offset", last_page_offset),
+                    ("weights", weights)):
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"{fn}: expected all tensors on {dev}, but {name} is on {t.device}")
+    with _lib.on_device(dev):
+        entry = _lib.lib().qr_keep_positions_f16 if f16 else _lib.lib().qr_keep_positions_i4
+        _lib.check(entry(
+            kept.data_ptr(), kept.shape[2], kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), last_page_offset.data_ptr(), pages,
+            layers, int(layer_idx), heads, page_size, head_dim, batch, None if weights is None else weights.data_ptr(), 0 if weights is None else weights.shape[2],
+            _lib.stream_ptr(dev)))
+
+
+def keep_positions_i4(kept, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, weights=None):
+    """Moves the positions that stay to the front of their sequences' pages, in place, for one layer: entry i of kept int32 [batch_size, heads, keep]
+    (heavy_positions': ascending, then -1) becomes position i, its key, value and parameters, and its entry of weights fp32 [batch_size,
+    heads, capacity] if that is given; weights behind the last entry, up to the sequence's length, become zero.  The page tables are those from before;
+    build_page_tables makes the new ones from new_lengths once all layers have moved.  What lies behind the moved positions stays as it was.
+    Entries that are no positions of their sequence are skipped.  Pages that other sequences read too must not move."""
+    _keep("keep_positions_i4", False, kept, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, weights)
+
+
+def keep_positions_f16(kept, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, weights=None):
+    """keep_positions_i4 for the cache with fp16 pages."""
+    _keep("keep_positions_f16", True, kept, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, weights)
 
 
 def build_page_tables(lengths, page_size, max_pages=None, block_table=None, new_lengths=None, tokens=0):
