@@ -10,6 +10,8 @@
 // that no element of q is divided.  Logits, exponentials and sums are in 32 bits, nothing is rounded to fewer.
 #include "qr_chunk.h"
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
 namespace {
 
 struct Weights {
@@ -21,6 +23,8 @@ struct Weights {
     int64_t q_stride, capacity;
     int tokens, group, blocks, window, sinks, q_had;
     Divisor per_group, per_block, per_head;
+    uint8_t* units;                   // the queries as the kernel of many rows takes them: units of 32 rows, [key head, unit]
+    int64_t all_units;
 };
 
 __device__ __forceinline__ Fresh fresh_of(const Weights& a, int b) {
@@ -216,16 +220,283 @@ __global__ __launch_bounds__(64 * kWaves) void weights_rows_kernel(Weights a, Di
     }
 }
 
+// ---- many rows -----------------------------------------------------------------------------------------------------------------------------
+// Four waves of 64 positions each, whose keys stay in their registers; the rows come past in units of 32, which the waves share in LDS.  A first launch lays the
+// queries out as the matrix instructions take them, so that a unit goes from memory to LDS as it lies, without registers, and is read without
+// bank conflicts: eight operands of 1 KB (lane (n, h): dimensions 64 h + 8 i .. of row n) and a ninth, the line: what a logit has besides the codes' product,
+// zero sum(q) and the row's logarithm, as a product of bf16 pieces that hold 24 bits together.
+constexpr int kUnitBytes = 9 * 1024, kStageUnits = 4;
+constexpr float kNothing = -3e38f;                         // minus the logarithm of a row that gives nothing
+
+__device__ __forceinline__ u32 tops(float lo, float hi) { return __builtin_amdgcn_perm(as_u32(hi), as_u32(lo), 0x07060302u); }
+__device__ __forceinline__ float top(float v) { return as_f32(as_u32(v) & 0xFFFF0000u); }
+// where the units of a sequence begin: behind those of the sequences before it, whose last units may be filled in part
+__device__ __forceinline__ int64_t first_unit(const Weights& a, int start, int b) { return (int64_t)start * a.group / 32 + b; }
+
 template <bool F16>
-int launch_weights(const Weights& a, int64_t groups, hipStream_t st) {
-    weights_rows_kernel<F16><<<dim3((unsigned)groups), dim3(64 * kWaves), 0, st>>>(a, divisor_of(a.c.page_size));
+__global__ __launch_bounds__(256) void weights_queries_kernel(Weights a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
+    const int id = divided(blockIdx.x, a.per_block), first = blockIdx.x - id * a.blocks, b = divided(id, a.per_head), h = id - b * a.c.num_heads;
+    const Fresh mine = fresh_of(a, b);
+    const int rows = mine.count * a.group;
+    for (int unit = first * 4 + wave; unit * 32 < rows; unit += a.blocks * 4) {
+        const int row = unit * 32 + n, r = row < rows ? row : rows - 1;        // (the last unit is filled up with the last row, which gives nothing there)
+        const int t = divided(r, a.per_group), head = h * a.group + r - t * a.group;
+        const u32x4* const src = (const u32x4*)(a.q + (int64_t)(mine.start + t) * a.q_stride + (int64_t)head * 128) + 8 * hh;
+        const float lse = a.lse[(int64_t)(mine.start + t) * (a.c.num_heads * a.group) + head];
+        u32x4 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = src[i];
+        if (a.q_had) {
+            float v[64];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const f16x2 p = as_f16x2(w[i >> 2][i & 3]);
+                v[2 * i] = (float)p[0], v[2 * i + 1] = (float)p[1];
+            }
+#pragma unroll
+            for (int bit = 1; bit < 64; bit *= 2)
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (!(i & bit)) {
+                        const float x = v[i], y = v[i | bit];
+                        v[i] = x + y, v[i | bit] = x - y;
+                    }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) {
+                const u32x2 e = both_halves<32>(as_u32(v[i]));
+                v[i] = hh ? as_f32(e.x) - as_f32(e.y) : as_f32(e.x) + as_f32(e.y);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) w[i >> 2][i & 3] = narrow_f16x2(v[2 * i] * kScale, v[2 * i + 1] * kScale);
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const f16x2 p = as_f16x2(w[i >> 2][i & 3]);
+            sum += (float)p[0] + (float)p[1];
+        }
+        const u32x2 both = both_halves<32>(as_u32(sum));
+        const float s = (as_f32(both.x) + as_f32(both.y)) * -(kLog2e * kScale), s1 = top(s), s2 = top(s - s1), s3 = s - s1 - s2;
+        float m = lse * -kLog2e;
+        m = row >= rows || __builtin_fabsf(m) > 3e38f ? kNothing : m != m ? __builtin_nanf("") : m;
+        const float m1 = top(m), m2 = top(m - m1), m3 = m - m1 - m2;
+        uint8_t* const to = a.units + ((int64_t)h * a.all_units + first_unit(a, mine.start, b) + unit) * kUnitBytes + lane * 16;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *(u32x4*)(to + 1024 * i) = F16 ? w[i] : query_for_low_codes(w[i]);
+        *(u32x4*)(to + 8192) = hh ? u32x4{tops(m3, 0.f), 0, 0, 0} : u32x4{tops(s1, s2), tops(s3, s1), tops(s2, s3), tops(m1, m2)};
+    }
+}
+
+typedef __attribute__((address_space(1))) const void* GlobalPtr;
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+template <bool F16>
+__global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Divisor pages) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2][kStageUnits * kUnitBytes];
+    const PagedKV& c = a.c;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
+    // (a head's workgroups are on one XCD where 8 divides the heads; blocks that most rows see come first)
+    const int items = c.batch_size * c.num_heads;
+    const int first_block = blockIdx.x / items, id = blockIdx.x - first_block * items, b = divided(id, a.per_head), h = id - b * c.num_heads;
+    const Fresh mine = fresh_of(a, b);
+    const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
+    const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
+    const int rows = mine.count * a.group, first_place = len - mine.all;
+    if (rows == 0) return;
+    const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
+    const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
+    constexpr uint32_t VEC = F16 ? 256 : 64;
+    constexpr float kUnit = kLog2e * kScale * (F16 ? 1.f : kCodeUnit);
+    const int highest = first_place + divided(rows - 1, a.per_group);
+    Steps steps{0, 0, 0};                                  // blocks of 256 positions that some row sees
+    if (highest >= 0) {
+        int from = 0;
+        if (a.window > 0 && first_place - a.window + 1 > 0) {
+            from = first_place - a.window + 1;
+            const int sinks = a.sinks < from ? a.sinks : from;
+            steps.near = (sinks + 255) >> 8;
+        }
+        steps.far = from >> 8;
+        if (steps.far < steps.near) steps.far = steps.near;
+        const int end = (highest >> 8) + 1;
+        steps.all = steps.near + (end > steps.far ? end - steps.far : 0);
+    }
+    const uint8_t* const units = a.units + ((int64_t)h * a.all_units + first_unit(a, mine.start, b)) * kUnitBytes;
+    // Row r is of token r / group, so it sees the position `pos` if it is not before `seen_from` and before `seen_to`
+    auto seen_from = [&](int pos) {
+        const int t = pos - first_place;                   // the token at that position
+        return t <= 0 ? 0 : t >= mine.count ? rows : t * a.group;
+    };
+    auto seen_to = [&](int pos) {
+        if (a.window == 0 || pos < a.sinks) return rows + 32;              // (rows that only fill up give nothing by themselves)
+        const int64_t t = (int64_t)pos + a.window - first_place;
+        return t <= 0 ? 0 : t >= mine.count ? rows + 32 : (int)t * a.group;
+    };
+
+    for (int block = first_block; block < steps.all; block += a.blocks) {
+        const int block_at = steps.at(block) * 256, at = block_at + 64 * wave;
+        const int pos = at + lane, it = divided(pos, pages);
+        const u32 entry = (u32)(pos - it * c.page_size);
+        const bool in = pos < len && it < npages && entry < (u32)c.page_size;
+        const int page = c.indices[p0 + (in ? it : 0)];
+        const bool there = in && page >= 0 && page < c.num_pages;
+        const int64_t slot = there ? page * page_slots + head_slots + entry : head_slots;
+        const u32 param = F16 ? 0u : c.param[slot];
+        u32x4 k[2][8], line[2];
+        float slope[2];
+        int from[2], to[2];
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) {
+            const uint8_t* const kd = c.data + __shfl(slot, 32 * cb + n, 64) * VEC + hh * (VEC / 2);
+            if (F16) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) k[cb][i] = *(const u32x4*)(kd + 16 * i);
+            } else {
+                const u32x4 w0 = *(const u32x4*)kd, w1 = *(const u32x4*)(kd + 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) k[cb][i] = low_codes_of(w0[i]), k[cb][4 + i] = low_codes_of(w1[i]);
+            }
+            const f16x2 p = as_f16x2((u32)__shfl((int)param, 32 * cb + n, 64));
+            slope[cb] = F16 ? kUnit : (float)p[0] * kUnit;
+            const float zero = F16 ? 0.f : (float)p[1], z1 = top(zero), z2 = zero - z1;
+            line[cb] = hh ? u32x4{0x00003F80u, 0, 0, 0} : u32x4{tops(z1, z1), tops(z1, z2), tops(z2, z2), 0x3F803F80u};
+            from[cb] = seen_from(at + 32 * cb + n), to[cb] = seen_to(at + 32 * cb + n);
+        }
+        // rows that see one of the workgroup's positions; those that see all of the wave's, and those that see any
+        const int last_seen = a.window == 0 || block_at < a.sinks ? rows : seen_to(block_at + 255);
+        const int u_begin = seen_from(block_at) / 32, u_end = ((last_seen < rows ? last_seen : rows) + 31) / 32;
+        const int all_from = seen_from(at + 63), all_to = at + 63 < a.sinks ? rows + 32 : seen_to(at < a.sinks ? a.sinks : at);
+        const int any_from = seen_from(at), any_to = a.window == 0 || at < a.sinks ? rows + 32 : seen_to(at + 63);
+
+        auto fetch = [&](int stage, int buffer) {          // units u_begin + 4 stage .. into LDS; each wave takes a fourth of their pieces of 1 KB
+            const int u = u_begin + stage * kStageUnits;
+#pragma unroll
+            for (int i = 0; i < 9; ++i) {
+                const int piece = 4 * i + wave;
+                if (u + piece / 9 < u_end)
+                    __builtin_amdgcn_global_load_lds((GlobalPtr)(units + (int64_t)u * kUnitBytes + piece * 1024 + lane * 16), (LdsPtr)(&lds[buffer][piece * 1024]), 16, 0, 0);
+            }
+        };
+        float sum[2] = {0.f, 0.f}, total[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};
+        const int stages = (u_end - u_begin + kStageUnits - 1) / kStageUnits;
+        if (stages > 0) fetch(0, 0);
+        for (int stage = 0; stage < stages; ++stage) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();                               // this stage is in LDS, and nobody reads the last one's any more
+            if (stage + 1 < stages) fetch(stage + 1, stage + 1 & 1);
+            const uint8_t* const buffer = lds[stage & 1];
+#pragma unroll 1
+            for (int i = 0; i < kStageUnits; ++i) {
+                const int u = u_begin + stage * kStageUnits + i, r0 = u * 32;
+                if (u >= u_end || r0 + 31 < any_from || r0 >= any_to) continue;
+                const uint8_t* const from_lds = buffer + i * kUnitBytes + lane * 16;
+                f32x16 x[2], t[2];
+                const u32x4 q_line = *(const u32x4*)(from_lds + 8192);
+#pragma unroll
+                for (int cb = 0; cb < 2; ++cb) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[cb][j] = t[cb][j] = 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const f16x8 q = *(const f16x8*)(from_lds + 1024 * j);
+#pragma unroll
+                    for (int cb = 0; cb < 2; ++cb) x[cb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q, __builtin_bit_cast(f16x8, k[cb][j]), x[cb], 0, 0, 0);
+                }
+#pragma unroll
+                for (int cb = 0; cb < 2; ++cb) t[cb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, q_line), __builtin_bit_cast(bf16x8, line[cb]), t[cb], 0, 0, 0);
+                if (r0 >= all_from && r0 + 32 <= all_to) {
+#pragma unroll
+                    for (int cb = 0; cb < 2; ++cb) {
+                        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            s0 += __builtin_amdgcn_exp2f(__builtin_fmaf(x[cb][j], slope[cb], t[cb][j]));
+                            s1 += __builtin_amdgcn_exp2f(__builtin_fmaf(x[cb][j + 1], slope[cb], t[cb][j + 1]));
+                        }
+                        sum[cb] += s0 + s1;
+                    }
+                } else {
+#pragma unroll
+                    for (int cb = 0; cb < 2; ++cb) {
+                        float s0 = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int r = r0 + 8 * (j >> 2) + 4 * hh + (j & 3);
+                            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[cb][j], slope[cb], t[cb][j]));
+                            s0 += r >= from[cb] && r < to[cb] ? e : 0.f;
+                        }
+                        sum[cb] += s0;
+                    }
+                }
+            }
+            if ((stage & 3) == 3 || stage + 1 == stages) {
+                // (what is lost of a small sum added to a large one is kept for the next)
+#pragma unroll
+                for (int cb = 0; cb < 2; ++cb) {
+                    const float more = sum[cb] - lost[cb], now = total[cb] + more;
+                    lost[cb] = (now - total[cb]) - more, total[cb] = now, sum[cb] = 0.f;
+                }
+            }
+        }
+        float all[2];
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) {
+            const u32x2 both = both_halves<32>(as_u32(total[cb]));
+            all[cb] = as_f32(both.x) + as_f32(both.y);
+        }
+        if (there && pos < a.capacity) a.sums[((int64_t)b * c.num_heads + h) * a.capacity + pos] += hh ? all[1] : all[0];
+        __syncthreads();                                   // (the next block's first stage overwrites LDS)
+    }
+}
+
+// Which kernel, and workgroups per (sequence, key head)
+struct WeightsPlan {
+    bool tiles;
+    int64_t blocks, most;              // most: workgroups of a launch, which has fewer than 2^32 threads
+};
+WeightsPlan weights_plan(int64_t tokens, int group, int64_t num_heads, int64_t batch, int64_t max_new_len, int64_t seen) {
+    if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
+    WeightsPlan p;
+    p.tiles = max_new_len * group > 64;
+    p.most = 0xffffffffll / 256;
+    p.blocks = (seen + 255) / 256;
+    if (p.blocks > 0xffff) p.blocks = 0xffff;
+    if (batch * num_heads * p.blocks > p.most) p.blocks = batch * num_heads < p.most ? p.most / (batch * num_heads) : 1;
+    return p;
+}
+int64_t weights_units(int64_t tokens, int group, int64_t batch) { return tokens * group / 32 + batch + 2; }
+// positions that the launch is sized for (what is longer is gone through in turns)
+int64_t seen_positions(int64_t tokens, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks, int64_t capacity) {
+    int64_t seen = max_seq_len > 0 && max_seq_len < capacity ? max_seq_len : capacity;
+    const int64_t fresh = max_new_len > 0 && max_new_len < tokens ? max_new_len : tokens;
+    if (window > 0 && window < seen && sinks < seen && seen > window + fresh + sinks + 768) seen = window + fresh + sinks + 768;
+    return seen;
+}
+
+template <bool F16>
+int launch_weights(const WeightsPlan& plan, Weights a, hipStream_t st) {
+    const int64_t items = (int64_t)a.c.batch_size * a.c.num_heads;
+    const Divisor pages = divisor_of(a.c.page_size);
+    if (plan.tiles) {
+        // (a wave of the first launch takes the units of a (sequence, key head) in turns)
+        int64_t each = ((int64_t)a.tokens * a.group / 32 / a.c.batch_size + 4) / 4, most = plan.most / items;
+        each = each > most ? most : each;
+        Weights first = a;
+        first.blocks = (int)each, first.per_block = divisor_of(each);
+        weights_queries_kernel<F16><<<dim3((unsigned)(items * each)), dim3(256), 0, st>>>(first);
+        weights_tiles_kernel<F16><<<dim3((unsigned)(items * a.blocks)), dim3(256), 0, st>>>(a, pages);
+    } else {
+        weights_rows_kernel<F16><<<dim3((unsigned)(items * a.blocks)), dim3(64 * kWaves), 0, st>>>(a, pages);
+    }
     return qr_launch_status();
 }
 
 int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_t q_stride, int q_had_mode, const void* lse, const void* starts, int64_t tokens,
                int num_q_heads, const void* kv_data, const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset, int64_t num_pages,
                int num_layers, int layer_idx, int num_heads, int page_size, int head_dim, int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window,
-               int64_t sinks, void* stream) {
+               int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = qr_internal_check_paged_cache(kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size,
                                                  head_dim, batch_size);
     if (rc != QR_OK) return rc;
@@ -247,16 +518,13 @@ int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_
     a.sinks = (int)(sinks > 0x3fffffff ? 0x3fffffff : sinks);
     a.q_had = q_had_mode;
     a.per_group = divisor_of(a.group), a.per_head = divisor_of(num_heads);
-    // positions that the launch is sized for (what is longer is gone through in turns); a launch has fewer than 2^32 threads
-    int64_t seen = max_seq_len > 0 && max_seq_len < capacity ? max_seq_len : capacity;
-    const int64_t fresh = max_new_len > 0 && starts ? max_new_len : starts ? tokens : 1;
-    if (a.window > 0 && a.sinks < seen && seen > a.window + fresh + a.sinks + 192) seen = a.window + fresh + a.sinks + 192;
-    int64_t blocks = (seen + 64 * kWaves - 1) / (64 * kWaves);
-    if (blocks > 0xffff) blocks = 0xffff;
-    const int64_t most = 0xffffffffll / (64 * kWaves);
-    if (batch_size * num_heads * blocks > most) blocks = batch_size * num_heads < most ? most / (batch_size * num_heads) : 1;
-    a.blocks = (int)blocks, a.per_block = divisor_of(blocks);
-    const int64_t wide = num_heads * blocks, at_once = batch_size * wide <= most ? batch_size : most / wide;
+    const int64_t fresh = starts ? max_new_len : 1;
+    WeightsPlan plan = weights_plan(tokens, a.group, num_heads, batch_size, fresh, seen_positions(tokens, fresh, max_seq_len, a.window, a.sinks, capacity));
+    a.all_units = weights_units(tokens, a.group, batch_size);
+    if (plan.tiles && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < (size_t)a.all_units * num_heads * kUnitBytes)) plan.tiles = false;
+    a.units = (uint8_t*)workspace;
+    a.blocks = (int)plan.blocks, a.per_block = divisor_of(plan.blocks);
+    const int64_t wide = num_heads * plan.blocks, at_once = batch_size * wide <= plan.most ? batch_size : plan.most / wide;
     int lrc = QR_OK;
     for (int64_t first = 0; first < batch_size && lrc == QR_OK; first += at_once) {
         Weights some = a;
@@ -265,22 +533,30 @@ int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_
         some.sums += first * num_heads * capacity;
         if (a.starts) some.starts += first;
         else some.q += first * q_stride, some.lse += first * num_q_heads;
-        lrc = fp16 ? launch_weights<true>(some, some.c.batch_size * wide, (hipStream_t)stream) : launch_weights<false>(some, some.c.batch_size * wide, (hipStream_t)stream);
+        lrc = fp16 ? launch_weights<true>(plan, some, (hipStream_t)stream) : launch_weights<false>(plan, some, (hipStream_t)stream);
     }
     return lrc;
 }
 
 }  // namespace
 
+extern "C" size_t qr_accumulate_weights_workspace_bytes(int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len) {
+    if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0 || batch_size > 0x7fffffff || tokens > 0x3fffffff ||
+        tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > 65536)
+        return 0;                                          // (the call itself refuses them)
+    if (!weights_plan(tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, 1).tiles) return 0;
+    return (size_t)weights_units(tokens, num_q_heads / num_heads, batch_size) * num_heads * kUnitBytes;
+}
+
 #define QR_WEIGHTS_ENTRY(NAME, FP16)                                                                                                                     \
     extern "C" int NAME(void* weights, int64_t capacity, const void* q, int64_t q_stride, int q_had_mode, const void* lse,                               \
                         const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data, const void* kv_param,                   \
                         const void* kv_indptr, const void* kv_indices, const void* last_page_offset, int64_t num_pages, int num_layers, int layer_idx,   \
                         int num_heads, int page_size, int head_dim, int64_t batch_size, int64_t max_new_len, int64_t max_seq_len, int64_t window,        \
-                        int64_t sinks, void* stream) {                                                                                                   \
+                        int64_t sinks, void* workspace, size_t workspace_bytes, void* stream) {                                                                                                   \
         return accumulate(FP16, weights, capacity, q, q_stride, q_had_mode, lse, seqlen_indptr_or_null, tokens, num_q_heads, kv_data, kv_param, kv_indptr, \
                           kv_indices, last_page_offset, num_pages, num_layers, layer_idx, num_heads, page_size, head_dim, batch_size, max_new_len,       \
-                          max_seq_len, window, sinks, stream);                                                                                           \
+                          max_seq_len, window, sinks, workspace, workspace_bytes, stream);                                                                                           \
     }
 QR_WEIGHTS_ENTRY(qr_accumulate_weights_i4, false)
 QR_WEIGHTS_ENTRY(qr_accumulate_weights_f16, true)

@@ -463,7 +463,7 @@ def _prefix_needed(fn, prefix_indptr):
 
 
 def _accumulate(fn, f16, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
-                window, sinks, q_hadamard):
+                window, sinks, q_hadamard, workspace):
     pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
     dev, batch = kv_data.device, last_page_offset.shape[0]
     if not (kv_indptr.shape[0] == batch + 1):
@@ -477,12 +477,16 @@ def _accumulate(fn, f16, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indic
     if window < 0 or sinks < 0 or max_new_len < 0 or max_seq_len < 0:
         raise RuntimeError(f"{fn}: window, sinks and the lengths must not be negative")
     with _lib.on_device(dev):
+        if seqlen_indptr is None:
+            max_new_len = 1
+        ws_bytes = _lib.lib().qr_accumulate_weights_workspace_bytes(tokens, q_heads, heads, batch, max_new_len)
+        ws = _scratch(workspace, ws_bytes, dev)
         entry = _lib.lib().qr_accumulate_weights_f16 if f16 else _lib.lib().qr_accumulate_weights_i4
         _lib.check(entry(
             weights.data_ptr(), weights.shape[2], q.data_ptr(), q.stride(0) if tokens > 1 else q_heads * head_dim, 1 if q_hadamard else 0, lse.data_ptr(),
             None if seqlen_indptr is None else seqlen_indptr.data_ptr(), tokens, q_heads, kv_data.data_ptr(), kv_param.data_ptr(), kv_indptr.data_ptr(),
             kv_indices.data_ptr(), last_page_offset.data_ptr(), pages, layers, int(layer_idx), heads, page_size, head_dim, batch,
-            1 if seqlen_indptr is None else max_new_len, max_seq_len, window, sinks, _lib.stream_ptr(dev)))
+            max_new_len, max_seq_len, window, sinks, None if ws is None else ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev)))
 
 
 def _weights(fn, weights, batch=None, heads=None):
@@ -492,7 +496,7 @@ def _weights(fn, weights, batch=None, heads=None):
 
 
 def accumulate_weights_i4(weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
-                          max_seq_len=0, window=0, sinks=0, q_hadamard=False):
+                          max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None):
     """Adds to every cached position what the new tokens' attention gives to it: with q and the bounds of a batch_chunk_i4 (or batch_shared_i4, whose
     own positions they are) call and the lse that it gave,
 
@@ -500,16 +504,16 @@ def accumulate_weights_i4(weights, q, lse, kv_data, kv_param, kv_indptr, kv_indi
 
     for the positions j that t sees.  weights fp32 [batch_size, heads, capacity], contiguous; positions beyond its capacity are left out.  A
     row whose lse is -inf gives nothing.  max_new_len and max_seq_len size the launch; window, sinks and q_hadamard as in the
-    attention's call.  The same inputs give the same bits.  Adds to `weights` and returns None."""
+    attention's call.  workspace: as batch_chunk_i4's, used where there are many rows.  The same inputs give the same bits.  Adds to `weights` and returns None."""
     _accumulate("accumulate_weights_i4", False, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
-                max_seq_len, window, sinks, q_hadamard)
+                max_seq_len, window, sinks, q_hadamard, workspace)
 
 
 def accumulate_weights_f16(weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr=None, max_new_len=0,
-                           max_seq_len=0, window=0, sinks=0, q_hadamard=False):
+                           max_seq_len=0, window=0, sinks=0, q_hadamard=False, workspace=None):
     """accumulate_weights_i4 for the cache with fp16 pages."""
     _accumulate("accumulate_weights_f16", True, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len,
-                max_seq_len, window, sinks, q_hadamard)
+                max_seq_len, window, sinks, q_hadamard, workspace)
 
 
 def heavy_positions(weights, lengths, keep, sinks=0, recent=0):

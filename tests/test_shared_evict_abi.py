@@ -59,7 +59,7 @@ def test_shared_workspace_needs_no_gpu(lib):
 
 def weights_args(**changes):
     return changed(dict(weights=AT, capacity=100, q=AT, q_stride=1024, had=0, lse=AT, starts=AT, tokens=5, q_heads=8, data=AT, param=AT, indptr=AT, indices=AT, last=AT, pages=10,
-                        layers=2, layer=1, heads=2, page_size=16, head_dim=128, batch=3, new=0, seq=0, window=0, sinks=0, stream=None), changes)
+                        layers=2, layer=1, heads=2, page_size=16, head_dim=128, batch=3, new=0, seq=0, window=0, sinks=0, workspace=None, bytes=0, stream=None), changes)
 
 
 @pytest.mark.parametrize("entry", ["qr_accumulate_weights_i4", "qr_accumulate_weights_f16"])
