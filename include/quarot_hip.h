@@ -479,8 +479,8 @@ int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_strid
  *   -inf for a row that sees nothing; of the weights as they were rounded, so within 2^-11 of the exact one.  Rows that are left stay as they are.
  *   prefixes == 0: the sequences' own positions only (qr_batch_chunk with lse); window > 0 only then (QR_E_SHAPE).
  *   max_prefix_len: the largest number of a prefix's positions if the caller knows it, else 0.
- *   With prefixes a workspace of qr_batch_shared_workspace_bytes bytes is required (QR_E_WORKSPACE): a row's partial states, two at least, 528
- *   bytes each.
+ *   With prefixes a workspace of qr_batch_shared_workspace_bytes bytes is required (QR_E_WORKSPACE): a row's partial states, 528 bytes
+ *   each.
  */
 size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                        int64_t max_seq_len, int64_t window, int64_t sinks, int64_t prefixes, int64_t max_prefix_len);

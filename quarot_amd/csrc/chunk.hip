@@ -434,7 +434,35 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                         for (int j = 0; j < 4; ++j) O[i][j] = __builtin_fmaf(src[1 + PER * l + i][j], keep, O[i][j]);
                 }
                 const int t = divided(r, a.per_group), head = h * a.group + r - t * a.group;
-                if (a.parts == 1) {
+                if (!a.states) {
+                    if (a.join > 0 && (!a.members || (a.first + b >= a.members[0] && a.first + b < a.members[a.prefixes]))) {
+                        // the states of the prefix that the row's sequence shares
+                        const f32x4* const src = (const f32x4*)a.part + ((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.join * 33;
+                        for (int from = 0; from < a.join; from += 4) {
+                            f32x4 state[4], x[4][PER];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const f32x4* const at = src + (from + i < a.join ? from + i : a.join - 1) * 33;
+                                state[i] = at[0];
+#pragma unroll
+                                for (int j = 0; j < PER; ++j) x[i][j] = at[1 + PER * l + j];
+                            }
+                            float high = M;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) high = __builtin_fmaxf(high, state[i][0]);
+                            const float mine = __builtin_amdgcn_exp2f(M - high);
+                            M = high, D *= mine;
+#pragma unroll
+                            for (int j = 0; j < PER; ++j) O[j] *= mine;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float keep = from + i < a.join ? __builtin_amdgcn_exp2f(state[i][0] - high) : 0.f;
+                                D += from + i < a.join ? state[i][1] * keep : 0.f;
+#pragma unroll
+                                for (int j = 0; j < PER; ++j) O[j] += from + i < a.join ? x[i][j] * keep : f32x4{0.f, 0.f, 0.f, 0.f};
+                            }
+                        }
+                    }
                     const float inv = D == 0.f ? 0.f : 1.f / D;                 // (a row that sees nothing is zero)
                     if (a.lse && l == 0) a.lse[(int64_t)(start + t) * (c.num_heads * a.group) + head] = lse_of(M, D);
                     u32x2* const dst = (u32x2*)(a.o + (int64_t)(start + t) * a.o_stride + (int64_t)head * 128) + PER * l;
@@ -575,7 +603,8 @@ struct ChunkPlan {
 };
 constexpr size_t kMostParts = (size_t)1 << 30;
 constexpr int kMostHeads = 65536;                          // (with most splits a sequence's heads are a launch)
-size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? (size_t)tokens * q_heads * splits * 132 * sizeof(float) : 0; }
+size_t part_bytes(int64_t tokens, int64_t q_heads, int parts) { return (size_t)tokens * q_heads * parts * 132 * sizeof(float); }
+size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? part_bytes(tokens, q_heads, splits) : 0; }
 ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
                      bool causal = true) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
@@ -659,11 +688,12 @@ int launch_chunk(bool fp16, const ChunkPlan& plan, Chunk a, hipStream_t st) {
         Chunk some = a;
         some.c.batch_size = (int)(batch_size - first < at_once ? batch_size - first : at_once);
         some.c.indptr += first, some.c.last_page_offset += first;
+        some.first = (int)first;
         if (a.prefix) some.members += a.members ? first : 0;
         else if (a.starts) some.starts += first;
         else {
             some.q += first * a.q_stride, some.o += first * a.o_stride;
-            some.part += a.parts > 1 ? first * num_q_heads * a.parts * 132 : 0;
+            some.part += a.states ? first * num_q_heads * a.parts * 132 : first * num_q_heads * a.join * 132;
             some.lse += a.lse ? first * num_q_heads : 0;
         }
         const int64_t groups = some.c.batch_size * wide * a.tiles;
@@ -722,7 +752,7 @@ Chunk chunk_of(const ChunkCall& t) {
     a.sinks = (int)(t.sinks > 0x3fffffff ? 0x3fffffff : t.sinks);
     a.q_had = t.q_had_mode;
     a.members = nullptr;
-    a.prefix = 0, a.sequences = (int)t.batch_size;
+    a.prefix = 0, a.sequences = (int)t.batch_size, a.prefixes = 0, a.first = 0, a.join = 0;
     a.part = (float*)t.workspace;
     a.part_at = 0;
     a.lse = nullptr;
@@ -738,7 +768,7 @@ int batch_chunk(bool fp16, const ChunkCall& t) {
     ChunkPlan plan = plan_of(fp16, t);
     if (plan.splits > 1 && (!t.workspace || ((uintptr_t)t.workspace & 15) || t.workspace_bytes < chunk_part_bytes(t.tokens, t.num_q_heads, plan.splits))) plan.splits = 1;
     Chunk a = chunk_of(t);
-    a.parts = plan.splits;
+    a.parts = plan.splits, a.states = plan.splits > 1;
     hipStream_t st = (hipStream_t)t.stream;
     const int lrc = launch_chunk(fp16, plan, a, st);
     if (lrc != QR_OK || plan.splits == 1) return lrc;
@@ -757,12 +787,15 @@ struct Prefixes {
 struct SharedPlan {
     ChunkPlan own, prefix;
     int parts;                         // states per row; 1: none are written
+    bool joined;                       // the sequences' own launch takes the prefixes' states in, so that it has none and there is no third launch
 };
 SharedPlan shared_plan(bool fp16, const ChunkCall& t, int64_t prefixes, int64_t max_prefix_len, bool one_prefix) {
-    SharedPlan p{plan_of(fp16, t), ChunkPlan{0, 0, 0, 0}, 0};
-    if (prefixes > 0)
+    SharedPlan p{plan_of(fp16, t), ChunkPlan{0, 0, 0, 0}, 0, false};
+    if (prefixes > 0) {
         p.prefix = chunk_plan(fp16, t.tokens, t.num_q_heads / t.num_heads, t.num_heads, prefixes, one_prefix ? t.tokens : 0, max_prefix_len, 0, 0, false);
-    p.parts = p.own.splits + p.prefix.splits;
+        p.joined = p.own.splits == 1 && p.own.nb != 0;
+    }
+    p.parts = (p.joined ? 0 : p.own.splits) + p.prefix.splits;
     return p;
 }
 
@@ -774,26 +807,30 @@ int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
     if (t.tokens == 0 || t.batch_size == 0) return rc;
     if ((uintptr_t)lse & 3) return QR_E_ALIGN;
     SharedPlan plan = shared_plan(fp16, t, p.count, p.max_len, p.count == 1);
-    if (plan.parts > 1 && (!t.workspace || ((uintptr_t)t.workspace & 15) || t.workspace_bytes < chunk_part_bytes(t.tokens, t.num_q_heads, plan.parts))) {
-        if (p.count > 0) return QR_E_WORKSPACE;                // (its states are joined through memory)
+    const bool states = plan.parts > 1 || p.count > 0;
+    if (states && (!t.workspace || ((uintptr_t)t.workspace & 15) || t.workspace_bytes < part_bytes(t.tokens, t.num_q_heads, plan.parts))) {
+        if (p.count > 0) return QR_E_WORKSPACE;                // (the states are joined through memory)
         plan.own.splits = plan.parts = 1;
     }
     Chunk a = chunk_of(t);
     a.parts = plan.parts;
     a.lse = lse;
     hipStream_t st = (hipStream_t)t.stream;
-    rc = launch_chunk(fp16, plan.own, a, st);
-    if (rc != QR_OK || plan.parts == 1) return rc;
     if (p.count > 0) {
         Chunk b = a;
         b.c.indptr = (const int32_t*)p.indptr, b.c.indices = (const int32_t*)p.indices, b.c.last_page_offset = (const int32_t*)p.last_page_offset;
         b.c.batch_size = (int)p.count;
         b.members = (const int32_t*)p.members;
         b.prefix = 1, b.per_place = kNoPlace;
-        b.part_at = plan.own.splits;
+        b.states = 1;
+        b.part_at = plan.joined ? 0 : plan.own.splits;
         rc = launch_chunk(fp16, plan.prefix, b, st);
         if (rc != QR_OK) return rc;
+        if (plan.joined) a.parts = 1, a.join = plan.parts, a.members = b.members, a.prefixes = (int)p.count;
     }
+    a.states = a.parts > 1;
+    rc = launch_chunk(fp16, plan.own, a, st);
+    if (rc != QR_OK || a.parts == 1) return rc;
     Joined j;
     j.part = a.part, j.starts = a.starts, j.members = (const int32_t*)p.members;
     j.o = a.o, j.lse = lse, j.o_stride = t.o_stride;
@@ -834,7 +871,8 @@ extern "C" size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens
     t.starts = &t;                     // (the caller gives max_new_len 1 where there are no bounds)
     t.tokens = tokens, t.num_q_heads = num_q_heads, t.num_heads = num_heads, t.batch_size = batch_size;
     t.max_new_len = max_new_len, t.max_seq_len = max_seq_len, t.window = window, t.sinks = sinks;
-    return chunk_part_bytes(tokens, num_q_heads, shared_plan(fp16_pages != 0, t, prefixes, max_prefix_len, prefixes == 1).parts);
+    const int parts = shared_plan(fp16_pages != 0, t, prefixes, max_prefix_len, prefixes == 1).parts;
+    return prefixes > 0 ? part_bytes(tokens, num_q_heads, parts) : chunk_part_bytes(tokens, num_q_heads, parts);
 }
 
 #define QR_SHARED_ENTRY(NAME, FP16)                                                                                                                   \

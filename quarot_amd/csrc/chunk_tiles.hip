@@ -750,7 +750,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             if (row_of(cb) >= rows) continue;
             const int token = token_of(cb), q_head = head_of(cb, token);
             // lane (n, h): dimensions 32 db + 16 i + 8 h + 4 k + j of row n in register 4 (i + 2 k) + j of block db
-            if (a.parts == 1) {
+            if (!a.states) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum, less = -zero * inv;
                 if (a.lse && h == 0) a.lse[(int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head] = lse_of(limit[cb] < 0.f ? kEmpty : m[cb], sum);
                 u32x4* const dst = (u32x4*)(a.o + (int64_t)(tokens.start + token) * a.o_stride + (int64_t)q_head * 128) + h;

@@ -618,6 +618,137 @@ PyObject* chunk(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     QR_END
 }
 
+// shared(fp16 pages, o, q, kv_data, kv_param, indptr, indices, last, layer, prefix_indptr or None, prefix_indices, prefix_last, prefix_sequences or None,
+// seqlen_indptr or None, max_new_len, max_seq_len, max_prefix_len, window, sinks, q_hadamard, lse or None, workspace or None) -> True
+PyObject* shared(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    QR_ARGS(22)
+    const int device = device_of(tensor(a[3]));
+    long long layer, fresh_bound, bound, prefix_bound, window, sinks;
+    bool fp16_pages, q_had;
+    Cache c;
+    if (!arg_bool(a[0], &fp16_pages) || !arg_int(a[8], &layer) || !arg_int(a[14], &fresh_bound) || !arg_int(a[15], &bound) || !arg_int(a[16], &prefix_bound) ||
+        !arg_int(a[17], &window) || !arg_int(a[18], &sinks) || !arg_bool(a[19], &q_had) || !cache_args(a + 3, device, layer, &c, fp16_pages))
+        return none();
+    const at::Tensor *o = tensor(a[1]), *q = tensor(a[2]), *seq, *lse, *ws, *members, *table[3] = {nullptr, nullptr, nullptr};
+    int64_t o_stride, q_stride, prefixes = 0;
+    if (!token_rows(o, device, &o_stride) || !token_rows(q, device, &q_stride) || o->sizes() != q->sizes() || !plain_or_none(a[12], at::kInt, device, &members) ||
+        !plain_or_none(a[13], at::kInt, device, &seq) || !plain_or_none(a[20], at::kFloat, device, &lse) || !plain_or_none(a[21], kByte, device, &ws))
+        return none();
+    if (a[9] != Py_None) {
+        for (int i = 0; i < 3; ++i) {
+            table[i] = tensor(a[9 + i]);
+            if (!plain(table[i], at::kInt, device) || table[i]->dim() != 1) return none();
+        }
+        prefixes = table[2]->numel();
+        if (table[0]->numel() != prefixes + 1 || (members ? (members->dim() != 1 || members->numel() != prefixes + 1) : prefixes > 1)) return none();
+    }
+    const int64_t tokens = q->size(0), heads = q->size(1);
+    if (c.heads == 0 || heads % c.heads || heads > 0x7fffffff || (seq ? (seq->dim() != 1 || seq->numel() != c.batch + 1) : tokens != c.batch) || fresh_bound < 0 ||
+        bound < 0 || prefix_bound < 0 || window < 0 || sinks < 0 || (lse && (lse->dim() != 2 || lse->size(0) != tokens || lse->size(1) != heads)))
+        return none();
+    if (!seq) fresh_bound = 1;
+    const size_t need = qr_batch_shared_workspace_bytes(fp16_pages ? 1 : 0, tokens, (int)heads, c.heads, c.batch, fresh_bound, bound, window, sinks, prefixes, prefix_bound);
+    const bool kept = need && ws && (size_t)ws->numel() >= need;
+    at::Tensor own;
+    const auto call = [&] {
+        if (need && !kept) own = fresh({(int64_t)need}, kByte, device);
+        return (fp16_pages ? qr_batch_shared_f16 : qr_batch_shared_i4)(
+            o->data_ptr(), o_stride, ptr(lse), q->data_ptr(), q_stride, q_had ? 1 : 0, ptr(seq), tokens, (int)heads, c.data->data_ptr(), c.param->data_ptr(),
+            c.indptr->data_ptr(), c.indices->data_ptr(), c.last->data_ptr(), c.pages, c.layers, (int)layer, c.heads, c.page_size, 128, c.batch, fresh_bound, bound, window,
+            sinks, ptr(table[0]), ptr(table[1]), ptr(table[2]), ptr(members), prefixes, prefix_bound, kept ? ws->data_ptr() : need ? own.data_ptr() : nullptr, need,
+            stream(device));
+    };
+    if (!done(call)) return none();
+    Py_RETURN_TRUE;
+    QR_END
+}
+
+// sums of weights: fp32 [batch, key heads, capacity]
+bool sums_of(const at::Tensor* t, int device, const Cache& c) {
+    return plain(t, at::kFloat, device) && t->dim() == 3 && t->size(0) == c.batch && t->size(1) == c.heads;
+}
+
+// accumulate(fp16 pages, weights, q, lse, kv_data, kv_param, indptr, indices, last, layer, seqlen_indptr or None, max_new_len, max_seq_len, window, sinks, q_hadamard,
+// workspace or None) -> True
+PyObject* accumulate(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    QR_ARGS(17)
+    const int device = device_of(tensor(a[4]));
+    long long layer, fresh_bound, bound, window, sinks;
+    bool fp16_pages, q_had;
+    Cache c;
+    if (!arg_bool(a[0], &fp16_pages) || !arg_int(a[9], &layer) || !arg_int(a[11], &fresh_bound) || !arg_int(a[12], &bound) || !arg_int(a[13], &window) ||
+        !arg_int(a[14], &sinks) || !arg_bool(a[15], &q_had) || !cache_args(a + 4, device, layer, &c, fp16_pages))
+        return none();
+    const at::Tensor *weights = tensor(a[1]), *q = tensor(a[2]), *lse = tensor(a[3]), *seq, *ws;
+    int64_t q_stride;
+    if (!sums_of(weights, device, c) || !token_rows(q, device, &q_stride) || !plain(lse, at::kFloat, device) || !plain_or_none(a[10], at::kInt, device, &seq) ||
+        !plain_or_none(a[16], kByte, device, &ws))
+        return none();
+    const int64_t tokens = q->size(0), heads = q->size(1);
+    if (c.heads == 0 || heads % c.heads || heads > 0x7fffffff || (seq ? (seq->dim() != 1 || seq->numel() != c.batch + 1) : tokens != c.batch) || fresh_bound < 0 ||
+        bound < 0 || window < 0 || sinks < 0 || lse->dim() != 2 || lse->size(0) != tokens || lse->size(1) != heads)
+        return none();
+    if (!seq) fresh_bound = 1;
+    const size_t need = qr_accumulate_weights_workspace_bytes(tokens, (int)heads, c.heads, c.batch, fresh_bound);
+    const bool kept = need && ws && (size_t)ws->numel() >= need;
+    at::Tensor own;
+    const auto call = [&] {
+        if (need && !kept) own = fresh({(int64_t)need}, kByte, device);
+        return (fp16_pages ? qr_accumulate_weights_f16 : qr_accumulate_weights_i4)(
+            weights->data_ptr(), weights->size(2), q->data_ptr(), q_stride, q_had ? 1 : 0, lse->data_ptr(), ptr(seq), tokens, (int)heads, c.data->data_ptr(),
+            c.param->data_ptr(), c.indptr->data_ptr(), c.indices->data_ptr(), c.last->data_ptr(), c.pages, c.layers, (int)layer, c.heads, c.page_size, 128, c.batch,
+            fresh_bound, bound, window, sinks, kept ? ws->data_ptr() : need ? own.data_ptr() : nullptr, need, stream(device));
+    };
+    if (!done(call)) return none();
+    Py_RETURN_TRUE;
+    QR_END
+}
+
+// heavy_positions(weights, lengths, keep, sinks, recent) -> (kept, new lengths)
+PyObject* heavy_positions(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    QR_ARGS(5)
+    const at::Tensor *weights = tensor(a[0]), *lengths = tensor(a[1]);
+    const int device = device_of(weights);
+    long long keep, sinks, recent;
+    if (!plain(weights, at::kFloat, device) || weights->dim() != 3 || !plain(lengths, at::kInt, device) || lengths->dim() != 1 || lengths->numel() != weights->size(0) ||
+        lengths->numel() == 0 || !arg_int(a[2], &keep) || !arg_int(a[3], &sinks) || !arg_int(a[4], &recent) || keep <= 0 || keep > 0x3fffffff || sinks < 0 || recent < 0 ||
+        weights->size(1) <= 0 || weights->size(1) > 0x3fffff)
+        return none();
+    const int64_t batch = weights->size(0), heads = weights->size(1);
+    at::Tensor kept, left;
+    const auto call = [&] {
+        kept = fresh({batch, heads, keep}, at::kInt, device);
+        left = fresh({batch}, at::kInt, device);
+        return qr_heavy_positions(weights->data_ptr(), weights->size(2), lengths->data_ptr(), batch, (int)heads, keep, sinks, recent, kept.data_ptr(), left.data_ptr(),
+                                  stream(device));
+    };
+    if (!done(call)) return none();
+    return wrap2(std::move(kept), std::move(left));
+    QR_END
+}
+
+// keep_positions(fp16 pages, kept, kv_data, kv_param, indptr, indices, last, layer, weights or None) -> True
+PyObject* keep_positions(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    QR_ARGS(9)
+    const int device = device_of(tensor(a[2]));
+    long long layer;
+    bool fp16_pages;
+    Cache c;
+    if (!arg_bool(a[0], &fp16_pages) || !arg_int(a[7], &layer) || !cache_args(a + 2, device, layer, &c, fp16_pages)) return none();
+    const at::Tensor *kept = tensor(a[1]), *weights;
+    if (!plain(kept, at::kInt, device) || kept->dim() != 3 || kept->size(0) != c.batch || kept->size(1) != c.heads || !plain_or_none(a[8], at::kFloat, device, &weights) ||
+        (weights && !sums_of(weights, device, c)))
+        return none();
+    const auto call = [&] {
+        return (fp16_pages ? qr_keep_positions_f16 : qr_keep_positions_i4)(kept->data_ptr(), kept->size(2), c.data->data_ptr(), c.param->data_ptr(), c.indptr->data_ptr(),
+                                                                           c.indices->data_ptr(), c.last->data_ptr(), c.pages, c.layers, (int)layer, c.heads, c.page_size, 128,
+                                                                           c.batch, ptr(weights), weights ? weights->size(2) : 0, stream(device));
+    };
+    if (!done(call)) return none();
+    Py_RETURN_TRUE;
+    QR_END
+}
+
 // A vector that lies in part of another tensor's memory and keeps all of it (the six tables of a call: 5.9 us, with an allocation each 9.0)
 at::Tensor part_of(const at::Tensor& whole, int64_t byte, int64_t count, at::ScalarType dtype) {
     const auto meta = c10::scalarTypeToTypeMeta(dtype);
@@ -700,6 +831,10 @@ PyMethodDef methods[] = {QR_METHOD(quantize_rows),
                          QR_METHOD(quantize_append),
                          QR_METHOD(decode_step),
                          QR_METHOD(chunk),
+                         QR_METHOD(shared),
+                         QR_METHOD(accumulate),
+                         QR_METHOD(heavy_positions),
+                         QR_METHOD(keep_positions),
                          QR_METHOD(build_page_tables),
                          QR_METHOD(outcome),
                          {nullptr, nullptr, 0, nullptr}};

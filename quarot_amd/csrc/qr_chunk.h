@@ -18,7 +18,7 @@ struct Chunk {
     const f16* q;
     f16* o;
     const int32_t* starts;            // nullptr: one new token per sequence
-    float* part;                      // parts > 1: 132 floats per row and split: maximum, sum, -, -, 128 outputs
+    float* part;                      // 132 floats per row and state: maximum, sum, -, -, 128 outputs
     int64_t q_stride, o_stride;       // halves from a token to the next
     int tokens, group, tiles, splits, window, sinks;      // window 0: none
     int q_had;
@@ -28,9 +28,10 @@ struct Chunk {
     // (nullptr: of all `sequences`).
     Divisor per_place;
     const int32_t* members;
-    int prefix, sequences;
-    int parts, part_at;                         // partial states per row, and where this launch's begin (one state in all: rows are finished)
-    float* lse;                                 // parts 1: where the rows' logarithms of the softmax's sum go, [token, head]; may be nullptr
+    int prefix, sequences, prefixes, first;     // first: the launch's first sequence's number
+    int states, parts, part_at;                 // whether the launch writes partial states, states per row, and where this launch's begin; else rows are finished
+    int join;                                   // states 0: states per row at `part`, of the prefix of the row's sequence, that belong to it too
+    float* lse;                                 // states 0: where the rows' logarithms of the softmax's sum go, [token, head]; may be nullptr
 };
 constexpr Divisor kNoPlace{0, 0};
 constexpr float kLn2 = 0.6931471805599453f;

@@ -362,6 +362,9 @@ def _scratch(workspace, ws_bytes, dev):
 
 def _shared(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices, prefix_last_page_offset,
             prefix_sequences, seqlen_indptr, max_new_len, max_seq_len, max_prefix_len, window, sinks, q_hadamard, lse, workspace):
+    if _lib.host.shared(f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices, prefix_last_page_offset,
+                        prefix_sequences, seqlen_indptr, max_new_len, max_seq_len, max_prefix_len, window, sinks, q_hadamard, lse, workspace):
+        return
     pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
     dev, batch = kv_data.device, last_page_offset.shape[0]
     if not (kv_indptr.shape[0] == batch + 1):
@@ -464,6 +467,9 @@ def _prefix_needed(fn, prefix_indptr):
 
 def _accumulate(fn, f16, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
                 window, sinks, q_hadamard, workspace):
+    if _lib.host.accumulate(f16, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, seqlen_indptr, max_new_len, max_seq_len,
+                            window, sinks, q_hadamard, workspace):
+        return
     pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
     dev, batch = kv_data.device, last_page_offset.shape[0]
     if not (kv_indptr.shape[0] == batch + 1):
@@ -521,6 +527,9 @@ def heavy_positions(weights, lengths, keep, sinks=0, recent=0):
     largest weights (of equal ones the lowest positions; NaN counts below all numbers).  weights fp32 [batch_size, heads, capacity], lengths
     int32 [batch_size], the positions that every sequence holds (at most the capacity).  Returns (kept, new_lengths): int32 [batch_size, heads, keep],
     ascending, and int32 [batch_size] = min(length, keep); of a sequence of no more than `keep` positions kept is all of them, then -1."""
+    made = _lib.host.heavy_positions(weights, lengths, keep, sinks, recent)
+    if made is not None:
+        return made
     fn = "heavy_positions"
     keep, sinks, recent = int(keep), int(sinks), int(recent)
     _weights(fn, weights)
@@ -539,6 +548,8 @@ def heavy_positions(weights, lengths, keep, sinks=0, recent=0):
 
 
 def _keep(fn, f16, kept, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, weights):
+    if _lib.host.keep_positions(f16, kept, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, weights):
+        return
     pages, layers, heads, page_size, head_dim = _cache_args(fn, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, f16)
     dev, batch = kv_data.device, last_page_offset.shape[0]
     if not (kv_indptr.shape[0] == batch + 1):
