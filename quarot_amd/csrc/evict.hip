@@ -1,5 +1,5 @@
 // Eviction from the paged cache: which positions of a (sequence, key head) stay, and their move to the front.
-#include "qr_paged.h"
+#include "qr_chunk.h"
 
 namespace {
 
@@ -19,12 +19,25 @@ __device__ __forceinline__ u32 order_of(float v) {
     const u32 u = __builtin_bit_cast(u32, v);
     return v != v ? 0u : v == 0.f ? 0x80000000u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-constexpr int kBins = 2048, kHeavyWaves = 16;
+constexpr int kBins = 2048, kHeavyWaves = 16, kHeavyThreads = 64 * kHeavyWaves;
 
-__global__ __launch_bounds__(64 * kHeavyWaves) void heavy_positions_kernel(Heavy a) {
+// the sum of v over the lanes before this one, of 16 lanes
+__device__ __forceinline__ int before16(int v, int lane) {
+    int all = v;
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+        const int other = __shfl_up(all, d, 16);
+        if ((lane & 15) >= d) all += other;
+    }
+    return all - v;
+}
+
+// HOLD > 0: a lane keeps its sums, at most that many, in registers; 0: they are read for every digit
+template <int HOLD>
+__global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a) {
     __shared__ u32 bins[kBins];
     __shared__ u32 found[3];                               // the digit, how many lie above it, how many have it
-    __shared__ int counts[kHeavyWaves][2];
+    __shared__ int counts[3][kHeavyWaves], after[2][kHeavyWaves];
     const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t held = a.lengths[b];
@@ -32,27 +45,52 @@ __global__ __launch_bounds__(64 * kHeavyWaves) void heavy_positions_kernel(Heavy
     if (h == 0 && tid == 0) a.left[b] = len < a.keep ? len : a.keep;
     int32_t* const kept = a.kept + (int64_t)blockIdx.x * a.keep;
     if (len <= a.keep) {
-        for (int i = tid; i < a.keep; i += 64 * kHeavyWaves) kept[i] = i < len ? i : -1;
+        for (int i = tid; i < a.keep; i += kHeavyThreads) kept[i] = i < len ? i : -1;
         return;
     }
-    for (int i = tid; i < a.sinks; i += 64 * kHeavyWaves) kept[i] = i;
-    for (int i = tid; i < a.recent; i += 64 * kHeavyWaves) kept[a.keep - a.recent + i] = len - a.recent + i;
     const int need = a.keep - a.sinks - a.recent, count = len - a.sinks - a.recent;          // 0 <= need < count
-    if (need == 0) return;
     const float* const sums = a.sums + (int64_t)blockIdx.x * a.capacity + a.sinks;
     const int each = ((count + kHeavyWaves - 1) / kHeavyWaves + 63) & ~63, from = wave * each, to = from + each < count ? from + each : count;
+    // the wave's sums in the order of positions, 64 at a time
+    u32 mine[HOLD > 0 ? HOLD : 1];
+    if (HOLD > 0) {
+        float v[HOLD > 0 ? HOLD : 1];
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j) v[j] = from + 64 * j + lane < to ? sums[from + 64 * j + lane] : 0.f;
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j) mine[j] = order_of(v[j]);
+    }
+    for (int i = tid; i < a.sinks; i += kHeavyThreads) kept[i] = i;
+    for (int i = tid; i < a.recent; i += kHeavyThreads) kept[a.keep - a.recent + i] = len - a.recent + i;
+    if (need == 0) return;
+    auto go_through = [&](auto&& visit) {                  // visit(position, its sum's order, whether it is one); all lanes of a wave together
+        if (HOLD > 0) {
+#pragma unroll
+            for (int j = 0; j < HOLD; ++j)
+                if (from + 64 * j < to) visit(from + 64 * j + lane, mine[j], from + 64 * j + lane < to);
+        } else {
+            for (int at = from; at < to; at += 64 * 8) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = at + 64 * j + lane < to ? sums[at + 64 * j + lane] : 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (at + 64 * j < to) visit(at + 64 * j + lane, order_of(v[j]), at + 64 * j + lane < to);
+            }
+        }
+    };
 
     u32 prefix = 0, above = 0;                             // the digits found so far; how many sums lie above all that have them
     int shift = 32;
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
         const int bits = pass < 2 ? 11 : 10, below = shift;
         shift -= bits;
-        for (int i = tid; i < kBins; i += 64 * kHeavyWaves) bins[i] = 0;
+        bins[tid] = bins[kHeavyThreads + tid] = 0;
         __syncthreads();
-        for (int i = from + lane; i < to; i += 64) {
-            const u32 k = order_of(sums[i]);
-            if (below == 32 || k >> below == prefix) atomicAdd(&bins[k >> shift & ((1u << bits) - 1)], 1u);
-        }
+        go_through([&](int, u32 k, bool is) {
+            if (is && (pass == 0 || k >> (below & 31) == prefix)) atomicAdd(&bins[k >> shift & ((1u << bits) - 1)], 1u);
+        });
         __syncthreads();
         // thread t has the bins 2 t and 2 t + 1 from the top; how many sums lie in the bins before its own
         const u32 b0 = bins[kBins - 1 - 2 * tid], b1 = bins[kBins - 2 - 2 * tid];
@@ -62,42 +100,38 @@ __global__ __launch_bounds__(64 * kHeavyWaves) void heavy_positions_kernel(Heavy
             const u32 v = __shfl_up(upto, d, 64);
             if (lane >= d) upto += v;
         }
-        if (lane == 63) counts[wave][0] = (int)upto;
+        if (lane == 63) counts[pass][wave] = (int)upto;
         __syncthreads();
-        u32 before = above + upto - b0 - b1;
-        for (int w = 0; w < wave; ++w) before += (u32)counts[w][0];
-        const u32 want = (u32)need;
+        const int waves_before = __shfl(before16(counts[pass][lane & 15], lane), wave, 64);
+        const u32 before = above + (u32)waves_before + upto - b0 - b1, want = (u32)need;
         if (before < want && before + b0 >= want) found[0] = kBins - 1 - 2 * tid, found[1] = before, found[2] = b0;
         if (before + b0 < want && before + b0 + b1 >= want) found[0] = kBins - 2 - 2 * tid, found[1] = before + b0, found[2] = b1;
         __syncthreads();
         prefix = prefix << bits | found[0];
         above = found[1];
-        const u32 in = found[2];
-        __syncthreads();
-        if (above + in == want) break;                     // (all that share these digits stay)
+        if (above + found[2] == want) break;               // (all that share these digits stay)
     }
     const int equal = need - (int)above;                   // of those with these digits that many stay, the first ones
 
     int greater = 0, same = 0;
-    for (int i = from + lane; i - lane < to; i += 64) {
-        const u32 k = i < to ? order_of(sums[i]) >> shift : 0u;
-        greater += __popcll(__builtin_amdgcn_ballot_w64(i < to && k > prefix));
-        same += __popcll(__builtin_amdgcn_ballot_w64(i < to && k == prefix));
-    }
-    if (lane == 0) counts[wave][0] = greater, counts[wave][1] = same;
+    go_through([&](int, u32 k, bool is) {
+        greater += __popcll(__builtin_amdgcn_ballot_w64(is && k >> shift > prefix));
+        same += __popcll(__builtin_amdgcn_ballot_w64(is && k >> shift == prefix));
+    });
+    if (lane == 0) after[0][wave] = greater, after[1][wave] = same;
     __syncthreads();
-    int out = 0, seen = 0;                                 // of the waves before this one: how many stay, how many have these digits
-    for (int w = 0; w < wave; ++w) out += counts[w][0], seen += counts[w][1];
+    // of the waves before this one: how many stay, how many have these digits
+    int out = __shfl(before16(after[0][lane & 15], lane), wave, 64), seen = __shfl(before16(after[1][lane & 15], lane), wave, 64);
     out += seen < equal ? seen : equal;
-    for (int i = from + lane; i - lane < to; i += 64) {
-        const u32 k = i < to ? order_of(sums[i]) >> shift : 0u;
-        const uint64_t eq = __builtin_amdgcn_ballot_w64(i < to && k == prefix);
+    go_through([&](int i, u32 k, bool is) {
+        k >>= shift;
+        const uint64_t eq = __builtin_amdgcn_ballot_w64(is && k == prefix);
         const int rank = seen + __builtin_amdgcn_mbcnt_hi((u32)(eq >> 32), __builtin_amdgcn_mbcnt_lo((u32)eq, 0));
-        const bool stays = i < to && (k > prefix || (k == prefix && rank < equal));
+        const bool stays = is && (k > prefix || (k == prefix && rank < equal));
         const uint64_t all = __builtin_amdgcn_ballot_w64(stays);
         if (stays) kept[a.sinks + out + __builtin_amdgcn_mbcnt_hi((u32)(all >> 32), __builtin_amdgcn_mbcnt_lo((u32)all, 0))] = a.sinks + i;
         out += __popcll(all), seen += __popcll(eq);
-    }
+    });
 }
 
 // ---- their move --------------------------------------------------------------------------------------------------------------------------------
@@ -109,68 +143,87 @@ struct Keep {
     const int32_t* kept;
     float* sums;                       // [sequence, key head, capacity]; may be nullptr
     int64_t capacity;
-    int keep;
+    int keep, jobs;                    // workgroups per (sequence, key head): keys, values, sums
+    Divisor pages;                     // of the page size
 };
-constexpr int kKeepThreads = 512;
+constexpr int kKeepThreads = 512, kListed = 2048;
 
 template <bool F16>
-__global__ __launch_bounds__(kKeepThreads) void keep_positions_kernel(Keep a) {
+__global__ __launch_bounds__(kKeepThreads, 4) void keep_positions_kernel(Keep a) {
     constexpr int LANES = F16 ? 16 : 4, EACH = kKeepThreads / LANES, TURNS = 8;              // lanes of a vector, vectors at a time
+    __shared__ int64_t sources[kListed], targets[kListed];                                  // slots; a target of -1: nothing moves
     const PagedKV& c = a.c;
-    const int id = blockIdx.x >> 1, side = blockIdx.x & 1, b = id / c.num_heads, h = id - b * c.num_heads;
-    const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
+    const int id = blockIdx.x / a.jobs, side = blockIdx.x - id * a.jobs, b = id / c.num_heads, h = id - b * c.num_heads;
+    const int tid = threadIdx.x, p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
     const int32_t* const kept = a.kept + (int64_t)id * a.keep;
-    const int l = threadIdx.x % LANES, mine = threadIdx.x / LANES;
-    auto slot_of = [&](int pos) -> int64_t {               // -1: there is none
-        if (pos < 0 || pos >= len) return -1;
-        const int it = pos / c.page_size, entry = pos - it * c.page_size;
-        if (it >= npages) return -1;
-        const int64_t page = c.indices[p0 + it];
-        return page >= 0 && page < c.num_pages ? paged_slot(c, page, side, h, entry) : -1;
-    };
-    const int end = a.keep < len ? a.keep : len;
-    for (int first = 0; first < end; first += EACH * TURNS) {
-        u32x4 v[TURNS];
-        u32 p[TURNS];
-        int64_t to[TURNS];
+    if (side == 2) {
+        float* const sums = a.sums + (int64_t)id * a.capacity;
+        const int have = (int)(len < a.capacity ? len : a.capacity), end = a.keep < have ? a.keep : have;
+        constexpr int W = 8;
+        for (int first = 0; first < end; first += kKeepThreads * W) {
+            int from[W];
+            float w[W];
 #pragma unroll
-        for (int u = 0; u < TURNS; ++u) {
-            const int i = first + u * EACH + mine, source = i < end ? kept[i] : -1;
-            const int64_t at = source > i ? slot_of(source) : -1;
-            to[u] = at >= 0 ? slot_of(i) : -1;
-            if (to[u] >= 0) {
-                v[u] = *((const u32x4*)c.data + at * LANES + l);
-                if (l == 0) p[u] = c.param[at];
+            for (int u = 0; u < W; ++u) {
+                const int i = first + u * kKeepThreads + tid;
+                from[u] = i < end ? kept[i] : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < W; ++u) {
+                const int i = first + u * kKeepThreads + tid;
+                w[u] = from[u] >= i && from[u] < have ? sums[from[u]] : 0.f;
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < W; ++u) {
+                const int i = first + u * kKeepThreads + tid;
+                if (i < end) sums[i] = w[u];
             }
         }
-        // (a batch's loads are over before any of its stores begins)
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < TURNS; ++u)
-            if (to[u] >= 0) {
-                *((u32x4*)c.data + to[u] * LANES + l) = v[u];
-                if (l == 0) c.param[to[u]] = p[u];
-            }
+        for (int i = end + tid; i < have; i += kKeepThreads) sums[i] = 0.f;     // (every entry of the list has been read)
+        return;
     }
-    if (side == 1 || !a.sums) return;
-    float* const sums = a.sums + (int64_t)id * a.capacity;
-    const int have = (int)(len < a.capacity ? len : a.capacity);
-    constexpr int W = 4;
-    for (int first = 0; first < have; first += kKeepThreads * W) {
-        float w[W];
+    const int l = tid % LANES, mine = tid / LANES, end = a.keep < len ? a.keep : len;
+    for (int list = 0; list < end; list += kListed) {
+        const int listed = end - list < kListed ? end - list : kListed;
+        // (the last batch has left the list behind the barrier between its loads and stores but for its targets, which its threads hold)
 #pragma unroll
-        for (int u = 0; u < W; ++u) {
-            const int i = first + u * kKeepThreads + (int)threadIdx.x, source = i < a.keep && i < have ? kept[i] : -1;
-            w[u] = source >= i && source < have ? sums[source] : 0.f;
+        for (int u = 0; u < kListed / kKeepThreads; ++u) {
+            const int i = list + u * kKeepThreads + tid, source = i < end ? kept[i] : -1;
+            const bool moves = source > i && source < len;
+            const int from_page = divided(moves ? source : 0, a.pages), to_page = divided(moves ? i : 0, a.pages);
+            const bool listed_pages = from_page < npages;
+            const int64_t from = c.indices[p0 + (listed_pages ? from_page : 0)], to = c.indices[p0 + (listed_pages ? to_page : 0)];
+            const bool good = moves && listed_pages && from >= 0 && from < c.num_pages && to >= 0 && to < c.num_pages;
+            sources[u * kKeepThreads + tid] = good ? paged_slot(c, from, side, h, source - from_page * c.page_size) : -1;
+            targets[u * kKeepThreads + tid] = good ? paged_slot(c, to, side, h, i - to_page * c.page_size) : -1;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+        for (int first = 0; first < listed; first += EACH * TURNS) {
+            u32x4 v[TURNS];
+            u32 p[TURNS];
+            int64_t to[TURNS];
 #pragma unroll
-        for (int u = 0; u < W; ++u) {
-            const int i = first + u * kKeepThreads + (int)threadIdx.x;
-            if (i < have) sums[i] = w[u];
+            for (int u = 0; u < TURNS; ++u) {
+                const int i = first + u * EACH + mine;
+                to[u] = i < listed ? targets[i] : -1;
+                if (to[u] >= 0) {
+                    const int64_t at = sources[i];
+                    v[u] = *((const u32x4*)c.data + at * LANES + l);
+                    if (l == 0) p[u] = c.param[at];
+                }
+            }
+            // (a batch's loads are over before any of its stores begins)
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < TURNS; ++u)
+                if (to[u] >= 0) {
+                    *((u32x4*)c.data + to[u] * LANES + l) = v[u];
+                    if (l == 0) c.param[to[u]] = p[u];
+                }
         }
     }
 }
@@ -192,7 +245,9 @@ int keep_positions(bool fp16, const void* kept, int64_t keep, void* kv_data, voi
     a.sums = (float*)weights;
     a.capacity = capacity;
     a.keep = (int)keep;
-    const dim3 grid((unsigned)(batch_size * num_heads * 2));
+    a.jobs = weights && capacity > 0 ? 3 : 2;
+    a.pages = divisor_of(page_size);
+    const dim3 grid((unsigned)(batch_size * num_heads * a.jobs));
     if (fp16) keep_positions_kernel<true><<<grid, dim3(kKeepThreads), 0, (hipStream_t)stream>>>(a);
     else keep_positions_kernel<false><<<grid, dim3(kKeepThreads), 0, (hipStream_t)stream>>>(a);
     return qr_launch_status();
@@ -214,7 +269,11 @@ extern "C" int qr_heavy_positions(const void* weights, int64_t capacity, const v
     a.kept = (int32_t*)kept, a.left = (int32_t*)new_lengths;
     a.capacity = capacity;
     a.heads = num_heads, a.keep = (int)keep, a.sinks = (int)sinks, a.recent = (int)recent;
-    heavy_positions_kernel<<<dim3((unsigned)(batch_size * num_heads)), dim3(64 * kHeavyWaves), 0, (hipStream_t)stream>>>(a);
+    const dim3 grid((unsigned)(batch_size * num_heads)), threads(kHeavyThreads);
+    if (capacity <= 4 * kHeavyThreads) heavy_positions_kernel<4><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+    else if (capacity <= 16 * kHeavyThreads) heavy_positions_kernel<16><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+    else if (capacity <= 32 * kHeavyThreads) heavy_positions_kernel<32><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+    else heavy_positions_kernel<0><<<grid, threads, 0, (hipStream_t)stream>>>(a);
     return qr_launch_status();
 }
 
