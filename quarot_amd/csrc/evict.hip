@@ -21,21 +21,30 @@ __device__ __forceinline__ u32 order_of(float v) {
 }
 constexpr int kBins = 2048, kHeavyWaves = 16, kHeavyThreads = 64 * kHeavyWaves;
 
-// the sum of v over the lanes before this one, of 16 lanes
-__device__ __forceinline__ int before16(int v, int lane) {
-    int all = v;
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-        const int other = __shfl_up(all, d, 16);
-        if ((lane & 15) >= d) all += other;
-    }
-    return all - v;
+// running sums over a wave's lanes up to this one, and over each 16 of them
+__device__ __forceinline__ int upto16(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);       // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
 }
+__device__ __forceinline__ int upto64(int v) {
+    v = upto16(v);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);       // row_bcast 15, 31
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
+// of one number per wave: the sum of those of the waves before this one
+__device__ __forceinline__ int of_waves_before(const int* counts, int lane, int wave) {
+    const int v = counts[lane & 15];
+    return __builtin_amdgcn_readlane(upto16(v) - v, wave);
+}
+__device__ __forceinline__ int lanes_before(uint64_t mask) { return __builtin_amdgcn_mbcnt_hi((u32)(mask >> 32), __builtin_amdgcn_mbcnt_lo((u32)mask, 0)); }
 
 // HOLD > 0: a lane keeps its sums, at most that many, in registers; 0: they are read for every digit
 template <int HOLD>
 __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a) {
-    __shared__ u32 bins[kBins];
+    // four counters per bin, a lane's by its number: half of a wave's sums have one of a few dozen leading digits, and would wait for each other
+    __shared__ u32x4 bins[kBins];
     __shared__ u32 found[3];                               // the digit, how many lie above it, how many have it
     __shared__ int counts[3][kHeavyWaves], after[2][kHeavyWaves];
     const int b = blockIdx.x / a.heads, h = blockIdx.x - b * a.heads;
@@ -86,23 +95,19 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
     for (int pass = 0; pass < 3; ++pass) {
         const int bits = pass < 2 ? 11 : 10, below = shift;
         shift -= bits;
-        bins[tid] = bins[kHeavyThreads + tid] = 0;
+        bins[tid] = bins[kHeavyThreads + tid] = u32x4{0, 0, 0, 0};
         __syncthreads();
         go_through([&](int, u32 k, bool is) {
-            if (is && (pass == 0 || k >> (below & 31) == prefix)) atomicAdd(&bins[k >> shift & ((1u << bits) - 1)], 1u);
+            if (is && (pass == 0 || k >> (below & 31) == prefix)) atomicAdd((u32*)&bins[k >> shift & ((1u << bits) - 1)] + (lane & 3), 1u);
         });
         __syncthreads();
         // thread t has the bins 2 t and 2 t + 1 from the top; how many sums lie in the bins before its own
-        const u32 b0 = bins[kBins - 1 - 2 * tid], b1 = bins[kBins - 2 - 2 * tid];
-        u32 upto = b0 + b1;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const u32 v = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += v;
-        }
+        const u32x4 c0 = bins[kBins - 1 - 2 * tid], c1 = bins[kBins - 2 - 2 * tid];
+        const u32 b0 = c0[0] + c0[1] + c0[2] + c0[3], b1 = c1[0] + c1[1] + c1[2] + c1[3];
+        const u32 upto = (u32)upto64((int)(b0 + b1));
         if (lane == 63) counts[pass][wave] = (int)upto;
         __syncthreads();
-        const int waves_before = __shfl(before16(counts[pass][lane & 15], lane), wave, 64);
+        const int waves_before = of_waves_before(counts[pass], lane, wave);
         const u32 before = above + (u32)waves_before + upto - b0 - b1, want = (u32)need;
         if (before < want && before + b0 >= want) found[0] = kBins - 1 - 2 * tid, found[1] = before, found[2] = b0;
         if (before + b0 < want && before + b0 + b1 >= want) found[0] = kBins - 2 - 2 * tid, found[1] = before + b0, found[2] = b1;
@@ -112,7 +117,25 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
         if (above + found[2] == want) break;               // (all that share these digits stay)
     }
     const int equal = need - (int)above;                   // of those with these digits that many stay, the first ones
-
+    if (HOLD > 0 && HOLD <= 16 && (u32)equal == found[2]) {
+        // all of them: one comparison for each, kept in scalar registers between the count and the list
+        uint64_t stay[HOLD > 0 ? HOLD : 1];
+        int count_here = 0;
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j) {
+            stay[j] = __builtin_amdgcn_ballot_w64(from + 64 * j + lane < to && mine[j] >> shift >= prefix);
+            count_here += __popcll(stay[j]);
+        }
+        if (lane == 0) after[0][wave] = count_here;
+        __syncthreads();
+        int32_t* to_list = kept + a.sinks + of_waves_before(after[0], lane, wave);
+#pragma unroll
+        for (int j = 0; j < HOLD; ++j) {
+            if (stay[j] >> lane & 1) to_list[lanes_before(stay[j])] = a.sinks + from + 64 * j + lane;
+            to_list += __popcll(stay[j]);
+        }
+        return;
+    }
     int greater = 0, same = 0;
     go_through([&](int, u32 k, bool is) {
         greater += __popcll(__builtin_amdgcn_ballot_w64(is && k >> shift > prefix));
@@ -121,15 +144,14 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
     if (lane == 0) after[0][wave] = greater, after[1][wave] = same;
     __syncthreads();
     // of the waves before this one: how many stay, how many have these digits
-    int out = __shfl(before16(after[0][lane & 15], lane), wave, 64), seen = __shfl(before16(after[1][lane & 15], lane), wave, 64);
+    int out = of_waves_before(after[0], lane, wave), seen = of_waves_before(after[1], lane, wave);
     out += seen < equal ? seen : equal;
     go_through([&](int i, u32 k, bool is) {
         k >>= shift;
         const uint64_t eq = __builtin_amdgcn_ballot_w64(is && k == prefix);
-        const int rank = seen + __builtin_amdgcn_mbcnt_hi((u32)(eq >> 32), __builtin_amdgcn_mbcnt_lo((u32)eq, 0));
-        const bool stays = is && (k > prefix || (k == prefix && rank < equal));
+        const bool stays = is && (k > prefix || (k == prefix && seen + lanes_before(eq) < equal));
         const uint64_t all = __builtin_amdgcn_ballot_w64(stays);
-        if (stays) kept[a.sinks + out + __builtin_amdgcn_mbcnt_hi((u32)(all >> 32), __builtin_amdgcn_mbcnt_lo((u32)all, 0))] = a.sinks + i;
+        if (stays) kept[a.sinks + out + lanes_before(all)] = a.sinks + i;
         out += __popcll(all), seen += __popcll(eq);
     });
 }

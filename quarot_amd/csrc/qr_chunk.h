@@ -213,8 +213,8 @@ struct Steps {
     int near, far, all;
     __device__ int at(int s) const { return s < near ? s : s - near + far; }
 };
-template <int LOG>
-__device__ __forceinline__ Steps steps_of(const Chunk& a, int lowest, int highest) {        // positions of the tile's first and last row
+template <int LOG, class Launch>
+__device__ __forceinline__ Steps steps_of(const Launch& a, int lowest, int highest) {        // positions of the tile's first and last row
     Steps s{0, 0, 0};
     if (highest < 0) return s;
     int from = 0;

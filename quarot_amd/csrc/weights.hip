@@ -74,11 +74,73 @@ __device__ __forceinline__ void hadamard_row(u32x4 (&w)[4], int lane) {
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------------------------------------
-// A wave takes 64 positions of a (sequence, key head), lane by lane for their places, and all rows in tiles of 16: lane (n, g) holds quarter g of the
-// keys of positions n, 16 + n, 32 + n and 48 + n.
+// A wave takes 64 positions of a (sequence, key head) at a time, lane by lane for their places, and all rows in tiles of 16: lane (n, g) holds quarter g of the
+// keys of positions n, 16 + n, 32 + n and 48 + n.  While it works on them the next 64 positions' keys and sums are under way, and the page numbers of those behind.
+// Of 16 rows and fewer the queries stay in registers, of up to 64 in LDS, ready for the products (a wave makes one tile of them; more are made for every block).
 constexpr int kWaves = 4;
 template <bool F16>
-__global__ __launch_bounds__(64 * kWaves) void weights_rows_kernel(Weights a, Divisor pages) {
+struct RowTile {                       // 16 rows: queries as the products take them; slope, logarithm (base 2, negative) and the token of rows 4 g + i
+    u32x4 q[4];
+    float slope[4] = {0.f, 0.f, 0.f, 0.f}, less[4];
+    int place[4];
+};
+template <bool F16, bool HAD>
+__device__ __forceinline__ RowTile<F16> row_tile(const Weights& a, const Fresh& mine, int h, int r0, int rows, int first_place, int lane) {
+    const int n = lane & 15, g = lane >> 4;
+    RowTile<F16> t;
+    // lane (n, g) holds dimensions 32 g + 8 i .. (fp16 pages: 32 i + 8 g ..) of row n
+    const int r = r0 + n < rows ? r0 + n : r0, token = divided(r, a.per_group), head = h * a.group + r - token * a.group;
+    const u32x4* src = (const u32x4*)(a.q + (int64_t)(mine.start + token) * a.q_stride + (int64_t)head * 128);
+    u32x4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = src[F16 && !HAD ? 4 * i + g : 4 * g + i];
+    float lse[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = r0 + 4 * g + i, of = divided(row < rows ? row : r0, a.per_group);
+        lse[i] = a.lse[(int64_t)(mine.start + of) * (a.c.num_heads * a.group) + h * a.group + (row < rows ? row : r0) - of * a.group];
+        t.place[i] = row < rows && lse[i] != -__builtin_inff() ? first_place + of : -1;        // (a row that has seen nothing gives nothing)
+        t.less[i] = lse[i] * -kLog2e;
+    }
+    if (HAD) {
+        hadamard_row(w, lane);
+        if (F16) {                                         // (dimensions 32 g + 8 i to 32 i + 8 g: lanes (n, 0 .. 3) trade pieces)
+            u32x4 other[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    u32 pick = 0;
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const u32 v = (u32)__shfl((int)w[m][j], 16 * i + n, 64);
+                        pick = g == m ? v : pick;
+                    }
+                    other[i][j] = pick;
+                }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = other[i];
+        }
+    }
+    if (!F16) {
+        float all = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const f16x2 p = as_f16x2(w[i >> 2][i & 3]);
+            all += (float)p[0] + (float)p[1];
+        }
+        const float slope = quarters_sum(all) * -(kLog2e * kScale);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t.slope[i] = __shfl(slope, 4 * g + i, 64);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.q[i] = F16 ? w[i] : query_for_low_codes(w[i]);
+    return t;
+}
+
+// ALIGNED: pages of a multiple of 16 positions, so that every 16 positions lie in one page
+template <bool F16, bool ALIGNED, bool HAD>
+__global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(Weights a, Divisor pages) {
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -92,131 +154,146 @@ __global__ __launch_bounds__(64 * kWaves) void weights_rows_kernel(Weights a, Di
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
     constexpr uint32_t VEC = F16 ? 256 : 64;
     constexpr float kUnit = kLog2e * kScale * (F16 ? 1.f : kCodeUnit);
-
     const int highest = first_place + divided(rows - 1, a.per_group);
-    auto sees = [&](int place, int pos) { return pos <= place && (a.window == 0 || pos > place - a.window || pos < a.sinks); };
-    // blocks of 64 positions that some row sees
-    struct {
-        int near, far, all;
-    } steps{0, 0, 0};
-    if (highest >= 0) {
-        const Steps s = [&] {
-            Steps t{0, 0, 0};
-            int from = 0;
-            if (a.window > 0 && first_place - a.window + 1 > 0) {
-                from = first_place - a.window + 1;
-                const int sinks = a.sinks < from ? a.sinks : from;
-                t.near = (sinks + 63) >> 6;
-            }
-            t.far = from >> 6;
-            if (t.far < t.near) t.far = t.near;
-            const int end = (highest >> 6) + 1;
-            t.all = t.near + (end > t.far ? end - t.far : 0);
-            return t;
-        }();
-        steps.near = s.near, steps.far = s.far, steps.all = s.all;
-    }
-    for (int block = first_block * kWaves + wave; block < steps.all; block += a.blocks * kWaves) {
-        const int at = (block < steps.near ? block : block - steps.near + steps.far) * 64;
-        // the lane's own position: where its key is
-        const int pos = at + lane, it = divided(pos, pages);
-        const u32 entry = (u32)(pos - it * c.page_size);
-        const bool in = pos < len && it < npages && entry < (u32)c.page_size;
+    const Steps steps = steps_of<6>(a, first_place, highest);              // blocks of 64 positions that some row sees
+    const int stride = a.blocks * kWaves;
+    float* const sums = a.sums + ((int64_t)b * c.num_heads + h) * a.capacity;
+
+    struct Place {                     // of the lane's position
+        int pos, entry, page;
+    };
+    auto ask = [&](int block) {
+        const int at = steps.at(block < steps.all ? block : steps.all - 1) * 64, pos = at + lane, it = divided(pos, pages);
+        const int entry = pos - it * c.page_size;
+        const bool in = pos < len && it < npages && (u32)entry < (u32)c.page_size;
         const int page = c.indices[p0 + (in ? it : 0)];
-        const bool there = in && page >= 0 && page < c.num_pages;
-        const int64_t slot = there ? page * page_slots + head_slots + entry : head_slots;
-        const u32 param = F16 ? 0u : c.param[slot];
-        u32x4 k[4][4];
-        float scale[4], zero[4];
+        return Place{pos, entry, in ? page : -1};
+    };
+    struct Block {
+        u32x4 k[4][F16 ? 4 : 1];
+        u32 param[F16 ? 1 : 4];
+        float before;
+    };
+    auto there = [&](const Place& p) { return p.page >= 0 && p.page < c.num_pages; };
+    auto fetch = [&](Block& f, const Place& p) {           // (a position that is not there reads the first entries of page 0, for nothing)
+        const bool is = there(p);
+        const int64_t slot = is ? p.page * page_slots + head_slots + p.entry : head_slots;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const uint8_t* const kd = c.data + __shfl(slot, 16 * s + n, 64) * VEC + g * 16;
-            if (F16) {
+            if (ALIGNED) {
+                const int page = __builtin_amdgcn_readlane(is ? p.page : -1, 16 * s), entry = __builtin_amdgcn_readlane(p.entry, 16 * s);
+                const int64_t base = page >= 0 ? page * page_slots + head_slots + entry : head_slots;
+                uint32_t off = (uint32_t)n * VEC + (uint32_t)g * 16, p_off = (uint32_t)n * 4;
+                asm volatile("" : "+v"(off), "+v"(p_off));                         // (32-bit offsets behind wave-uniform addresses)
+                const uint8_t* const kd = c.data + base * VEC;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) k[s][i] = *(const u32x4*)(kd + 64 * i);
+                for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[s][i] = *(const u32x4*)(kd + off + 64 * i);
+                if (!F16) f.param[F16 ? 0 : s] = *(const u32*)((const uint8_t*)(c.param + base) + p_off);
             } else {
-                const u32x4 w = *(const u32x4*)kd;
+                const int64_t base = __shfl(slot, 16 * s + n, 64);
+                const uint8_t* const kd = c.data + base * VEC + g * 16;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) k[s][i] = low_codes_of(w[i]);
-                const f16x2 p = as_f16x2((u32)__shfl((int)param, 16 * s + n, 64));
-                scale[s] = (float)p[0] * kUnit, zero[s] = (float)p[1];
+                for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[s][i] = *(const u32x4*)(kd + 64 * i);
+                if (!F16) f.param[F16 ? 0 : s] = c.param[base];
             }
         }
-        // (sums of 16 tiles of rows, then of these: a long chain of additions would lose what is small)
-        float sum[4] = {0.f, 0.f, 0.f, 0.f}, all_before[4] = {0.f, 0.f, 0.f, 0.f};
+        f.before = is && p.pos < a.capacity ? sums[p.pos] : 0.f;
+    };
+    int block = first_block * kWaves + wave;
+    __shared__ u32x4 staged[4][7][64];
+    const bool in_lds = rows > 16 && rows <= 64;
+    if (in_lds) {
+        if (16 * wave < rows) {
+            const RowTile<F16> t = row_tile<F16, HAD>(a, mine, h, 16 * wave, rows, first_place, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) staged[wave][i][lane] = t.q[i];
+            staged[wave][4][lane] = u32x4{as_u32(t.slope[0]), as_u32(t.slope[1]), as_u32(t.slope[2]), as_u32(t.slope[3])};
+            staged[wave][5][lane] = u32x4{as_u32(t.less[0]), as_u32(t.less[1]), as_u32(t.less[2]), as_u32(t.less[3])};
+            staged[wave][6][lane] = u32x4{(u32)t.place[0], (u32)t.place[1], (u32)t.place[2], (u32)t.place[3]};
+        }
+        __syncthreads();
+    }
+    auto tile_of = [&](int r0) {
+        if (!in_lds) return row_tile<F16, HAD>(a, mine, h, r0, rows, first_place, lane);
+        RowTile<F16> t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t.q[i] = staged[r0 >> 4][i][lane];
+        const u32x4 slope = staged[r0 >> 4][4][lane], less = staged[r0 >> 4][5][lane], place = staged[r0 >> 4][6][lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t.slope[i] = as_f32(slope[i]), t.less[i] = as_f32(less[i]), t.place[i] = (int)place[i];
+        return t;
+    };
+    if (block >= steps.all) return;
+    Place here = ask(block), next = ask(block + stride);
+    Block f;
+    fetch(f, here);
+    RowTile<F16> tile = tile_of(0);
+    for (;;) {
+        const int at = __builtin_amdgcn_readfirstlane(here.pos);
+        u32x4 k[4][F16 ? 4 : 1];
+        float scale[4], zero[4], sum[4] = {0.f, 0.f, 0.f, 0.f}, before_tiles[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int i = 0; i < (F16 ? 4 : 1); ++i) k[s][i] = f.k[s][i];
+            const f16x2 p = as_f16x2(f.param[F16 ? 0 : s]);
+            scale[s] = F16 ? kUnit : (float)p[0] * kUnit, zero[s] = (float)p[1];
+        }
+        const float before = f.before;
+        const Place now = here;
+        const bool more = block + stride < steps.all;
+        if (more) {
+            here = next, next = ask(block + 2 * stride);
+            fetch(f, here);
+        }
         for (int r0 = 0; r0 < rows; r0 += 16) {
-            if ((r0 & 255) == 0) {
+            if (r0 > 0) {
+                tile = tile_of(r0);
+                if ((r0 & 255) == 0) {                     // (sums of 16 tiles, then of these: a long chain of additions would lose what is small)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) all_before[s] += sum[s], sum[s] = 0.f;
-            }
-            // queries: lane (n, g) holds dimensions 32 g + 8 i .. (fp16 pages: 32 i + 8 g ..) of row n
-            const int r = r0 + n < rows ? r0 + n : r0, t = divided(r, a.per_group), head = h * a.group + r - t * a.group;
-            const u32x4* src = (const u32x4*)(a.q + (int64_t)(mine.start + t) * a.q_stride + (int64_t)head * 128);
-            u32x4 w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = src[F16 && !a.q_had ? 4 * i + g : 4 * g + i];
-            float slope = 0.f;
-            if (!F16) {
-                if (a.q_had) hadamard_row(w, lane);
-                float all = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const f16x2 p = as_f16x2(w[i >> 2][i & 3]);
-                    all += (float)p[0] + (float)p[1];
+                    for (int s = 0; s < 4; ++s) before_tiles[s] += sum[s], sum[s] = 0.f;
                 }
-                slope = quarters_sum(all) * -(kLog2e * kScale);
-            } else if (a.q_had) {
-                hadamard_row(w, lane);
-                // (dimensions 32 g + 8 i to 32 i + 8 g: lanes (n, 0..3) trade pieces)
-                u32x4 other[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        u32 pick = 0;
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) {
-                            const u32 v = (u32)__shfl((int)w[m][j], 16 * i + n, 64);
-                            pick = g == m ? v : pick;
-                        }
-                        other[i][j] = pick;
-                    }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = other[i];
             }
             f32x4 x[4];
 #pragma unroll
             for (int s = 0; s < 4; ++s) x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const f16x8 q = __builtin_bit_cast(f16x8, F16 ? w[i] : query_for_low_codes(w[i]));
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int s = 0; s < 4; ++s) x[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q, __builtin_bit_cast(f16x8, k[s][i]), x[s], 0, 0, 0);
-            }
+                for (int s = 0; s < 4; ++s) {
+                    u32x4 key;
+                    if (F16) {
+                        key = k[s][F16 ? i : 0];
+                    } else {
+                        u32 w = k[s][0][i];
+                        asm volatile("" : "+v"(w));        // (unpacked here, tile by tile of rows: all of them are 64 registers)
+                        key = low_codes_of(w);
+                    }
+                    x[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, tile.q[i]), __builtin_bit_cast(f16x8, key), x[s], 0, 0, 0);
+                }
             // register i of lane (n, g): row 4 g + i, position n
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = r0 + 4 * g + i, token = divided(row < rows ? row : 0, a.per_group), place = row < rows ? first_place + token : -1;
-                const float lse = row < rows ? a.lse[(int64_t)(mine.start + token) * (c.num_heads * a.group) + h * a.group + row - token * a.group] : 0.f;
-                const float less = lse * -kLog2e, mine_slope = F16 ? 0.f : __shfl(slope, 4 * g + i, 64);
-                const bool any = lse != -__builtin_inff();         // (a row that has seen nothing gives nothing)
+                const int high = tile.place[i] - at, low = a.window == 0 ? -1 : high - a.window, sinks = a.sinks - at;
 #pragma unroll
                 for (int s = 0; s < 4; ++s) {
-                    const float y = F16 ? __builtin_fmaf(x[s][i], kUnit, less) : __builtin_fmaf(x[s][i], scale[s], __builtin_fmaf(zero[s], mine_slope, less));
-                    sum[s] += any && sees(place, at + 16 * s + n) ? __builtin_amdgcn_exp2f(y) : 0.f;
+                    const float y = F16 ? __builtin_fmaf(x[s][i], scale[s], tile.less[i]) : __builtin_fmaf(x[s][i], scale[s], __builtin_fmaf(zero[s], tile.slope[i], tile.less[i]));
+                    const int p = 16 * s + n;
+                    const bool sees = (p <= high) & ((a.window == 0) | (p > low) | (p < sinks));
+                    sum[s] += sees ? __builtin_amdgcn_exp2f(y) : 0.f;
                 }
             }
         }
         float total = 0.f;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const float all = quarters_sum(sum[s] + all_before[s]);
+            const float all = quarters_sum(sum[s] + before_tiles[s]);
             total = g == s ? all : total;
         }
-        if (there && pos < a.capacity) {
-            float* const to = a.sums + ((int64_t)b * c.num_heads + h) * a.capacity + pos;
-            *to += total;
-        }
+        if (there(now) && now.pos < a.capacity) sums[now.pos] = before + total;
+        if (!more) break;
+        block += stride;
+        if (rows > 16) tile = tile_of(0);
     }
 }
 
@@ -309,19 +386,7 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
     constexpr uint32_t VEC = F16 ? 256 : 64;
     constexpr float kUnit = kLog2e * kScale * (F16 ? 1.f : kCodeUnit);
     const int highest = first_place + divided(rows - 1, a.per_group);
-    Steps steps{0, 0, 0};                                  // blocks of 256 positions that some row sees
-    if (highest >= 0) {
-        int from = 0;
-        if (a.window > 0 && first_place - a.window + 1 > 0) {
-            from = first_place - a.window + 1;
-            const int sinks = a.sinks < from ? a.sinks : from;
-            steps.near = (sinks + 255) >> 8;
-        }
-        steps.far = from >> 8;
-        if (steps.far < steps.near) steps.far = steps.near;
-        const int end = (highest >> 8) + 1;
-        steps.all = steps.near + (end > steps.far ? end - steps.far : 0);
-    }
+    const Steps steps = steps_of<8>(a, first_place, highest);              // blocks of 256 positions that some row sees
     const uint8_t* const units = a.units + ((int64_t)h * a.all_units + first_unit(a, mine.start, b)) * kUnitBytes;
     // Row r is of token r / group, so it sees the position `pos` if it is not before `seen_from` and before `seen_to`
     auto seen_from = [&](int pos) {
@@ -456,12 +521,17 @@ struct WeightsPlan {
     bool tiles;
     int64_t blocks, most;              // most: workgroups of a launch, which has fewer than 2^32 threads
 };
-WeightsPlan weights_plan(int64_t tokens, int group, int64_t num_heads, int64_t batch, int64_t max_new_len, int64_t seen) {
+WeightsPlan weights_plan(bool fp16, int64_t tokens, int group, int64_t num_heads, int64_t batch, int64_t max_new_len, int64_t seen) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     WeightsPlan p;
     p.tiles = max_new_len * group > 64;
     p.most = 0xffffffffll / 256;
     p.blocks = (seen + 255) / 256;
+    if (!p.tiles) {                    // workgroups that are on the chip at once, of equal work
+        const int64_t room = (fp16 ? 2 : 3) * (int64_t)qr_device().cus / (batch * num_heads), all = (seen + 63) / 64;
+        const int64_t turns = room > 0 ? (all + 4 * room - 1) / (4 * room) : all;
+        if (turns > 1) p.blocks = (all + 4 * turns - 1) / (4 * turns);
+    }
     if (p.blocks > 0xffff) p.blocks = 0xffff;
     if (batch * num_heads * p.blocks > p.most) p.blocks = batch * num_heads < p.most ? p.most / (batch * num_heads) : 1;
     return p;
@@ -488,7 +558,11 @@ int launch_weights(const WeightsPlan& plan, Weights a, hipStream_t st) {
         weights_queries_kernel<F16><<<dim3((unsigned)(items * each)), dim3(256), 0, st>>>(first);
         weights_tiles_kernel<F16><<<dim3((unsigned)(items * a.blocks)), dim3(256), 0, st>>>(a, pages);
     } else {
-        weights_rows_kernel<F16><<<dim3((unsigned)(items * a.blocks)), dim3(64 * kWaves), 0, st>>>(a, pages);
+        const bool aligned = a.c.page_size % 16 == 0;
+        using Kernel = void (*)(Weights, Divisor);
+        const Kernel kernel = a.q_had ? (aligned ? weights_rows_kernel<F16, true, true> : weights_rows_kernel<F16, false, true>)
+                                      : (aligned ? weights_rows_kernel<F16, true, false> : weights_rows_kernel<F16, false, false>);
+        kernel<<<dim3((unsigned)(items * a.blocks)), dim3(64 * kWaves), 0, st>>>(a, pages);
     }
     return qr_launch_status();
 }
@@ -519,7 +593,7 @@ int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_
     a.q_had = q_had_mode;
     a.per_group = divisor_of(a.group), a.per_head = divisor_of(num_heads);
     const int64_t fresh = starts ? max_new_len : 1;
-    WeightsPlan plan = weights_plan(tokens, a.group, num_heads, batch_size, fresh, seen_positions(tokens, fresh, max_seq_len, a.window, a.sinks, capacity));
+    WeightsPlan plan = weights_plan(fp16, tokens, a.group, num_heads, batch_size, fresh, seen_positions(tokens, fresh, max_seq_len, a.window, a.sinks, capacity));
     a.all_units = weights_units(tokens, a.group, batch_size);
     if (plan.tiles && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < (size_t)a.all_units * num_heads * kUnitBytes)) plan.tiles = false;
     a.units = (uint8_t*)workspace;
@@ -544,7 +618,7 @@ extern "C" size_t qr_accumulate_weights_workspace_bytes(int64_t tokens, int num_
     if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0 || batch_size > 0x7fffffff || tokens > 0x3fffffff ||
         tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > 65536)
         return 0;                                          // (the call itself refuses them)
-    if (!weights_plan(tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, 1).tiles) return 0;
+    if (!weights_plan(false, tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, 1).tiles) return 0;
     return (size_t)weights_units(tokens, num_q_heads / num_heads, batch_size) * num_heads * kUnitBytes;
 }
 
