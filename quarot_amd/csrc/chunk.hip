@@ -605,8 +605,7 @@ constexpr size_t kMostParts = (size_t)1 << 30;
 constexpr int kMostHeads = 65536;                          // (with most splits a sequence's heads are a launch)
 size_t part_bytes(int64_t tokens, int64_t q_heads, int parts) { return (size_t)tokens * q_heads * parts * 132 * sizeof(float); }
 size_t chunk_part_bytes(int64_t tokens, int64_t q_heads, int splits) { return splits > 1 ? part_bytes(tokens, q_heads, splits) : 0; }
-ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks,
-                     bool causal = true) {
+ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t batch, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     if (max_new_len < (tokens + batch - 1) / batch) max_new_len = (tokens + batch - 1) / batch;        // (some sequence has as many)
     const bool even = max_new_len * batch == tokens;
@@ -643,7 +642,7 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
             if (some < groups) groups = some;
         }
         groups *= num_heads;
-        const int64_t late = causal ? max_new_len - per / group : 0;    // (what the first tile does not see of the last one's positions, at most)
+        const int64_t late = max_new_len - per / group;    // (what the first tile does not see of the last one's positions, at most)
         const float steps = (float)(seen - (late > 0 ? (late < seen ? late : seen) / 2 : 0)) / (float)step;
         for (int s = 1; s <= 32; ++s) {
             if (s > 1 && (steps < (float)(3 * s) || chunk_part_bytes(tokens, (int64_t)group * num_heads, s) > kMostParts)) break;
@@ -780,6 +779,46 @@ int batch_chunk(bool fp16, const ChunkCall& t) {
 // ---- prefixes that several sequences share ---------------------------------------------------------------------------------------------------
 // A prefix is a page list that is attended to by the rows of all its sequences' tokens, as if they were one sequence's that see all of it: its vectors are read (and
 // unpacked) once per tile of those rows instead of once per sequence.  States of both launches are joined by a third.
+//
+// How the prefixes' launch is cut: tiles of 16, 32 or 256 rows, and splits of the positions, whose states are written in any case.  The cut of the least sum is taken,
+// of the kernels' own times in microseconds: a step of a wave (32 positions by 16 or 32 rows, shorter where the chip is not full) or of a workgroup
+// (64 by 256), what goes around the steps, 0.16 a thousand states.  The numbers are those that lose least over 16 .. 1024 rows of 8 and 32 key heads after
+// 500 .. 24000 positions, 1 - 2 % on average against the best of 5 to 40 cuts (the rule above, which knows no tiles of 16 of more than 16 rows and counts a
+// third launch: 10 - 13 %).  Int4 pages, microseconds of a whole call with tiles of 16, 32 and 256, each at its best: 64 rows of 8 heads after 2000 17.2,
+// 19.7, 28.3; after 24000 36.6, 33.7, 54.2; 512 rows after 8000 -, 54.0, 53.3; after 24000 -, 121, 90.5.  Fp16 pages: 64 rows after 8000 26.2, 32.3, 36.7;
+// 256 rows -, 49.3, 44.7.
+ChunkPlan prefix_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_t prefixes, int64_t max_len) {
+    const int64_t rows = tokens * group, cus = qr_device().cus, seen = max_len < 0x3fffffff ? max_len : 0x3fffffff;
+    ChunkPlan p{1, 4, 1, 1};
+    float least = -1.f;
+    auto consider = [&](int nb, int nw, int64_t per, int64_t at_once, int64_t step, float each, float around, float part, float each_state) {
+        int64_t some = prefixes == 1 ? (rows + per - 1) / per : rows / per + prefixes / 2;
+        if (some < prefixes) some = prefixes;
+        const int64_t groups = some * num_heads, most = (rows + per - 1) / per, even = 3 * ((rows + prefixes * per - 1) / (prefixes * per)), steps = (seen + step - 1) / step;
+        for (int s = 1; s <= 32; ++s) {
+            if (s > 1 && (steps < s || chunk_part_bytes(tokens, (int64_t)group * num_heads, s) > kMostParts)) break;
+            const float turns = (float)((steps + s - 1) / s), full = (float)(groups * s) / (float)at_once;
+            const float time = (float)((groups * s + at_once - 1) / at_once) * (turns * each * (part + (1.f - part) * (full < 1.f ? full : 1.f)) + around) +
+                               (float)(rows * num_heads) * (float)s * each_state;
+            const int64_t tiles = most < even ? most : even;               // (a workgroup goes on to the next tile behind them)
+            if (least < 0.f || time < least) least = time, p = ChunkPlan{nb, nw, (int)(tiles > 4096 ? 4096 : tiles), s};
+        }
+    };
+    const bool few = rows <= 64 * prefixes;                // (the tiles of 16 were measured up to there)
+    if (fp16) {
+        if (few) consider(1, 4, 16, cus, 32 * 4, 0.87f, 4.7f, 0.6f, 1.75e-4f);
+        consider(2, 4, 32, 2 * cus, 32 * 4, 5.3f, 6.5f, 0.6f, 1.75e-4f);
+        consider(2, 8, 32, cus, 32 * 8, 5.3f, 7.3f, 0.6f, 1.75e-4f);
+        consider(0, 4, 256, cus, 64, 3.27f, 14.f, 0.6f, 1.75e-4f);
+    } else {
+        if (few) consider(1, 4, 16, 3 * cus, 32 * 4, 0.72f, 4.7f, 0.46f, 1.62e-4f);
+        consider(2, 4, 32, 2 * cus, 32 * 4, 2.4f, 6.5f, 0.46f, 1.62e-4f);
+        consider(2, 8, 32, cus, 32 * 8, 2.4f, 7.7f, 0.46f, 1.62e-4f);
+        consider(0, 4, 256, cus, 64, 2.9f, 8.1f, 0.46f, 1.62e-4f);
+    }
+    return p;
+}
+
 struct Prefixes {
     const void *indptr, *indices, *last_page_offset, *members;
     int64_t count, max_len;
@@ -789,10 +828,12 @@ struct SharedPlan {
     int parts;                         // states per row; 1: none are written
     bool joined;                       // the sequences' own launch takes the prefixes' states in, so that it has none and there is no third launch
 };
-SharedPlan shared_plan(bool fp16, const ChunkCall& t, int64_t prefixes, int64_t max_prefix_len, bool one_prefix) {
+SharedPlan shared_plan(bool fp16, const ChunkCall& t, int64_t prefixes, int64_t max_prefix_len) {
     SharedPlan p{plan_of(fp16, t), ChunkPlan{0, 0, 0, 0}, 0, false};
     if (prefixes > 0) {
-        p.prefix = chunk_plan(fp16, t.tokens, t.num_q_heads / t.num_heads, t.num_heads, prefixes, one_prefix ? t.tokens : 0, max_prefix_len, 0, 0, false);
+        p.prefix = prefix_plan(fp16, t.tokens, t.num_q_heads / t.num_heads, t.num_heads, prefixes, max_prefix_len);
+        // (int4 pages, 64 sequences of up to 700 positions of their own, 64 on 8 heads: 16.7 us, with twelve waves 22.5)
+        if (p.own.nb == 1 && p.own.nw == 12 && t.batch_size * t.num_heads >= 2 * qr_device().cus) p.own.nw = 4;
         p.joined = p.own.splits == 1 && p.own.nb != 0;
     }
     p.parts = (p.joined ? 0 : p.own.splits) + p.prefix.splits;
@@ -806,7 +847,7 @@ int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
     if (p.count > 0 && t.batch_size > 0 && (!p.indptr || !p.indices || !p.last_page_offset)) return QR_E_NULL;
     if (t.tokens == 0 || t.batch_size == 0) return rc;
     if ((uintptr_t)lse & 3) return QR_E_ALIGN;
-    SharedPlan plan = shared_plan(fp16, t, p.count, p.max_len, p.count == 1);
+    SharedPlan plan = shared_plan(fp16, t, p.count, p.max_len);
     const bool states = plan.parts > 1 || p.count > 0;
     if (states && (!t.workspace || ((uintptr_t)t.workspace & 15) || t.workspace_bytes < part_bytes(t.tokens, t.num_q_heads, plan.parts))) {
         if (p.count > 0) return QR_E_WORKSPACE;                // (the states are joined through memory)
@@ -871,7 +912,7 @@ extern "C" size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens
     t.starts = &t;                     // (the caller gives max_new_len 1 where there are no bounds)
     t.tokens = tokens, t.num_q_heads = num_q_heads, t.num_heads = num_heads, t.batch_size = batch_size;
     t.max_new_len = max_new_len, t.max_seq_len = max_seq_len, t.window = window, t.sinks = sinks;
-    const int parts = shared_plan(fp16_pages != 0, t, prefixes, max_prefix_len, prefixes == 1).parts;
+    const int parts = shared_plan(fp16_pages != 0, t, prefixes, max_prefix_len).parts;
     return prefixes > 0 ? part_bytes(tokens, num_q_heads, parts) : chunk_part_bytes(tokens, num_q_heads, parts);
 }
 
