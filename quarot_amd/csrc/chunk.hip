@@ -456,10 +456,12 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
                             for (int j = 0; j < PER; ++j) O[j] *= mine;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const float keep = from + i < a.join ? __builtin_amdgcn_exp2f(state[i][0] - high) : 0.f;
-                                D += from + i < a.join ? state[i][1] * keep : 0.f;
+                                // (an empty state may be its maximum and sum alone: what lies behind them is anything)
+                                const bool is = from + i < a.join && state[i][0] != kEmpty;
+                                const float keep = is ? __builtin_amdgcn_exp2f(state[i][0] - high) : 0.f;
+                                D += is ? state[i][1] * keep : 0.f;
 #pragma unroll
-                                for (int j = 0; j < PER; ++j) O[j] += from + i < a.join ? x[i][j] * keep : f32x4{0.f, 0.f, 0.f, 0.f};
+                                for (int j = 0; j < PER; ++j) O[j] += is ? x[i][j] * keep : f32x4{0.f, 0.f, 0.f, 0.f};
                             }
                         }
                     }
@@ -563,7 +565,7 @@ __global__ __launch_bounds__(64) void chunk_join_kernel(Joined a) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (from + i < states) {
+            if (from + i < states && head4[i][0] != kEmpty) {              // (an empty state may be its maximum and sum alone)
                 const float k = __builtin_amdgcn_exp2f(head4[i][0] - M);
                 D = __builtin_fmaf(head4[i][1], k, D);
 #pragma unroll
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(64) void chunk_join_kernel(Joined a) {
 // Partial states fill at most kMostParts bytes: a call of that many rows (16384 tokens of 64 heads in two splits) has 16 turns of tiles of 256 and more, and a split
 // gains no more than a part of the last one.
 struct ChunkPlan {
-    int nb, nw, tiles, splits;
+    int nb, nw, tiles, splits, dealt = 0;
 };
 constexpr size_t kMostParts = (size_t)1 << 30;
 constexpr int kMostHeads = 65536;                          // (with most splits a sequence's heads are a launch)
@@ -676,9 +678,10 @@ int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t gr
 int launch_chunk(bool fp16, const ChunkPlan& plan, Chunk a, hipStream_t st) {
     const int64_t batch_size = a.c.batch_size, num_q_heads = (int64_t)a.c.num_heads * a.group;
     a.tiles = plan.tiles;
-    a.splits = plan.splits, a.per_split = divisor_of(plan.splits);
+    a.splits = plan.dealt ? 1 : plan.splits, a.per_split = divisor_of(a.splits);
+    a.dealt = plan.dealt;
     const int64_t most = 0xffffffffll / (plan.nb == 0 ? 256 : 64 * plan.nw), wide = (int64_t)a.c.num_heads * a.splits;
-    if (batch_size * wide * plan.tiles > most) a.tiles = (int)(batch_size * wide < most ? most / (batch_size * wide) : 1);
+    if (!a.dealt && batch_size * wide * plan.tiles > most) a.tiles = (int)(batch_size * wide < most ? most / (batch_size * wide) : 1);
     const int64_t at_once = batch_size * wide <= most ? batch_size : most / wide;
     const Divisor pages = divisor_of(a.c.page_size);
     const bool aligned = a.c.page_size % 16 == 0;
@@ -695,7 +698,7 @@ int launch_chunk(bool fp16, const ChunkPlan& plan, Chunk a, hipStream_t st) {
             some.part += a.states ? first * num_q_heads * a.parts * 132 : first * num_q_heads * a.join * 132;
             some.lse += a.lse ? first * num_q_heads : 0;
         }
-        const int64_t groups = some.c.batch_size * wide * a.tiles;
+        const int64_t groups = a.dealt ? a.dealt : some.c.batch_size * wide * a.tiles;
         rc = plan.nb == 0 ? qr_internal_chunk_tiles(fp16, some, pages, groups, st)
              : fp16       ? (aligned ? launch_rows<true, true>(plan, some, pages, groups, st) : launch_rows<true, false>(plan, some, pages, groups, st))
                           : (aligned ? launch_rows<false, true>(plan, some, pages, groups, st) : launch_rows<false, false>(plan, some, pages, groups, st));
@@ -751,7 +754,7 @@ Chunk chunk_of(const ChunkCall& t) {
     a.sinks = (int)(t.sinks > 0x3fffffff ? 0x3fffffff : t.sinks);
     a.q_had = t.q_had_mode;
     a.members = nullptr;
-    a.prefix = 0, a.sequences = (int)t.batch_size, a.prefixes = 0, a.first = 0, a.join = 0;
+    a.dealt = 0, a.prefix = 0, a.sequences = (int)t.batch_size, a.prefixes = 0, a.first = 0, a.join = 0;
     a.part = (float*)t.workspace;
     a.part_at = 0;
     a.lse = nullptr;
@@ -804,17 +807,37 @@ ChunkPlan prefix_plan(bool fp16, int64_t tokens, int group, int num_heads, int64
             if (least < 0.f || time < least) least = time, p = ChunkPlan{nb, nw, (int)(tiles > 4096 ? 4096 : tiles), s};
         }
     };
+    // One prefix: the steps of all its tiles in equal shares, five steps at least, one to a CU at most.  A tile has the states of its shares, which is the same number for all
+    // of them where the shares' number is a multiple of the tiles' or the other way round, else one more than its shares' length makes at most.
+    auto deal = [&](float each, float around, float part, float each_state) {
+        int64_t tiles = (rows + 255) / 256;
+        tiles = tiles > 4096 ? 4096 : tiles;               // (rows are fewer than 2^30; what lies behind is left to the splits of whole tiles)
+        if (tiles * 256 < rows) return consider(0, 4, 256, cus, 64, each, around, part, each_state);
+        const int64_t all = tiles * num_heads, steps = (seen + 63) / 64 < 1 ? 1 : (seen + 63) / 64;
+        int64_t shares = seen > 0 && all * steps < 5 * cus ? all * steps / 5 : cus;
+        if (shares < 1) shares = 1;
+        if (shares < all && 8 * shares > 7 * all) shares = all;                // (a little more than one tile each)
+        int64_t states = shares % all == 0 ? shares / all : all % shares == 0 ? 1 : shares / all + 2;
+        if (states > 32) states = 32, shares = 32 * all < shares ? 32 * all : shares;
+        const float full = (float)shares / (float)cus;
+        const float time = (float)(all * steps + shares - 1) / (float)shares * each * (part + (1.f - part) * (full < 1.f ? full : 1.f)) +
+                           (float)((all + shares - 1) / shares + (all % shares && shares % all ? 1 : 0)) * around + (float)(rows * num_heads) * (float)states * each_state;
+        if (chunk_part_bytes(tokens, (int64_t)group * num_heads, (int)states) > kMostParts && states > 2) return consider(0, 4, 256, cus, 64, each, around, part, each_state);
+        if (least < 0.f || time < least) least = time, p = ChunkPlan{0, 4, (int)tiles, (int)states, (int)shares};
+    };
     const bool few = rows <= 64 * prefixes;                // (the tiles of 16 were measured up to there)
     if (fp16) {
         if (few) consider(1, 4, 16, cus, 32 * 4, 0.87f, 4.7f, 0.6f, 1.75e-4f);
         consider(2, 4, 32, 2 * cus, 32 * 4, 5.3f, 6.5f, 0.6f, 1.75e-4f);
         consider(2, 8, 32, cus, 32 * 8, 5.3f, 7.3f, 0.6f, 1.75e-4f);
-        consider(0, 4, 256, cus, 64, 3.27f, 14.f, 0.6f, 1.75e-4f);
+        if (prefixes > 1) consider(0, 4, 256, cus, 64, 3.27f, 14.f, 0.6f, 1.75e-4f);
+        else deal(3.27f, 14.f, 0.6f, 1.75e-4f);
     } else {
         if (few) consider(1, 4, 16, 3 * cus, 32 * 4, 0.72f, 4.7f, 0.46f, 1.62e-4f);
         consider(2, 4, 32, 2 * cus, 32 * 4, 2.4f, 6.5f, 0.46f, 1.62e-4f);
         consider(2, 8, 32, cus, 32 * 8, 2.4f, 7.7f, 0.46f, 1.62e-4f);
-        consider(0, 4, 256, cus, 64, 2.9f, 8.1f, 0.46f, 1.62e-4f);
+        if (prefixes > 1) consider(0, 4, 256, cus, 64, 2.9f, 8.1f, 0.46f, 1.62e-4f);
+        else deal(2.9f, 8.1f, 0.46f, 1.62e-4f);
     }
     return p;
 }

@@ -85,19 +85,32 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     const PagedKV& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
-    const int id = divided(blockIdx.x, a.per_split), split = blockIdx.x - id * a.splits, item = divided(id, a.per_head);
-    const int head = id - item * c.num_heads;              // neighbours are on different XCDs, a head's tiles on one where 8 divides the heads
-    int b, tile;
-    if (!item_of<kRows>(a, item, b, tile)) return;
+    const int id = divided(blockIdx.x, a.per_split), item = divided(id, a.per_head);
+    int split = blockIdx.x - id * a.splits, head = id - item * c.num_heads;    // neighbours are on different XCDs, a head's tiles on one where 8 divides the heads
+    int b = 0, tile = 0;
+    if (!a.dealt && !item_of<kRows>(a, item, b, tile)) return;
     const Fresh tokens = fresh_of(a, b);
     const int rows = tokens.count * a.group;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
     const int first_place = len - tokens.all;              // the first new token's position
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
-    const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;
+    int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;
     const int64_t kv_slots = (int64_t)c.num_heads * c.page_size;
     constexpr uint32_t VEC = F16 ? 256 : 64;               // bytes of a vector
+
+    // Dealt out: the steps of all heads' tiles, one behind the other, in equal shares (544 tiles on 256 CUs: 2.1 turns of a tile's steps, where whole tiles take 3 and
+    // fourths of them 2.25 and twice the states).  An XCD has shares that follow one another, of few heads.  A tile's shares are its states 0, 1, ..., and
+    // whoever has its last step marks those that there are not as empty.
+    int64_t share_at = 0, share_end = 0, dealt_steps = 0;
+    int share = 0, tile_steps = 1;
+    if (a.dealt) {
+        const int eighths = a.dealt / 8 * 8;
+        share = (int)blockIdx.x < eighths ? (int)(blockIdx.x & 7) * (a.dealt / 8) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
+        tile_steps = len > 0 ? ((len - 1) >> 6) + 1 : 1;   // (of an empty prefix: one that shows nothing)
+        dealt_steps = (int64_t)c.num_heads * a.tiles * tile_steps;
+        share_at = dealt_steps * share / a.dealt, share_end = dealt_steps * (share + 1) / a.dealt;
+    }
 
     // what never changes: the values' operand beyond row 131 (fp16 pages: beyond 127, with a row of ones for the weights' sum), the second half of the logits'
     // line, whose first factor is one
@@ -118,11 +131,27 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     const int v_row = 4 * (word & 1) + 8 * (word >> 1 & 1) + 32 * (word >> 2);              // row of dimension 8 word; 8 word + 4 is 16 rows on
     const uint32_t v_to = (uint32_t)(dim_row(v_row) + jj * 8 + piece * 16);
 
-    for (int r_tile = tile * kRows; r_tile < rows; r_tile += a.tiles * kRows) {
+    for (int r_tile = tile * kRows;; r_tile += a.tiles * kRows) {
+        int first_step = 0, end_step = 0;
+        if (a.dealt) {
+            if (share_at >= share_end) break;
+            const int64_t number = share_at / tile_steps;
+            first_step = (int)(share_at - number * tile_steps);
+            end_step = share_end - share_at < tile_steps - first_step ? first_step + (int)(share_end - share_at) : tile_steps;
+            // (the share that has the tile's first step)
+            split = share - (int)(((number * tile_steps + 1) * a.dealt - 1) / dealt_steps);
+            head = (int)(number / a.tiles), r_tile = ((int)number - head * a.tiles) * kRows;
+            head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;
+            share_at += end_step - first_step;
+            if (r_tile >= rows) continue;
+        } else if (r_tile >= rows) {
+            break;
+        }
         const int r_end = r_tile + kRows < rows ? r_tile + kRows : rows;
         const int tile_lowest = first_place + divided(r_tile, a.per_place), tile_highest = first_place + divided(r_end - 1, a.per_place);
         const Steps steps = steps_of<6>(a, tile_lowest, tile_highest);
-        const int s_begin = divided(steps.all * split, a.per_split), s_end = divided(steps.all * (split + 1), a.per_split);      // (below 2^24 steps, 2^5 splits)
+        const int s_begin = a.dealt ? first_step : divided(steps.all * split, a.per_split);      // (below 2^24 steps, 2^5 splits)
+        const int s_end = a.dealt ? (end_step < steps.all ? end_step : steps.all) : divided(steps.all * (split + 1), a.per_split);
         const int last = s_end - 1;
         auto position = [&](int s) INLINE { return steps.at(s < last ? s : last) * kStep; };        // (behind the last step the last again)
 
@@ -769,6 +798,8 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             } else {
                 float* const dst = a.part + (((int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head) * a.parts + a.part_at + split) * 132;
                 if (h == 0) dst[0] = limit[cb] < 0.f ? kEmpty : m[cb], dst[1] = sum;
+                if (h == 0 && end_step == tile_steps)
+                    for (int i = a.part_at + split + 1; a.dealt && i < a.parts; ++i) dst[132 * (i - a.part_at - split)] = kEmpty, dst[132 * (i - a.part_at - split) + 1] = 0.f;
 #pragma unroll
                 for (int db = 0; db < 4; ++db)
 #pragma unroll

@@ -29,6 +29,8 @@ struct Chunk {
     Divisor per_place;
     const int32_t* members;
     int prefix, sequences, prefixes, first;     // first: the launch's first sequence's number
+    int dealt;                                  // tiles of 256 rows of one prefix: the launch's workgroups, each with as many steps as the others, from any tile to
+                                                // any other; 0: a workgroup has its splits of whole tiles
     int states, parts, part_at;                 // whether the launch writes partial states, states per row, and where this launch's begin; else rows are finished
     int join;                                   // states 0: states per row at `part`, of the prefix of the row's sequence, that belong to it too
     float* lse;                                 // states 0: where the rows' logarithms of the softmax's sum go, [token, head]; may be nullptr
