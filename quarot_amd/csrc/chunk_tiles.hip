@@ -79,8 +79,9 @@ __device__ __forceinline__ bool strange(u32 w) { return (w & 0x7C00u) == 0x7C00u
 #define INLINE __attribute__((always_inline))        // (what a function that is not inlined captures lies in memory)
 
 // ALIGNED: pages of a multiple of 16 positions, so that the sixteen positions that a wave fetches lie in one page
-template <bool F16, bool ALIGNED>
-__global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pages) {
+// DEALT: one prefix's tiles, whose steps the workgroups share evenly
+template <bool F16, bool ALIGNED, bool DEALT>
+__device__ __forceinline__ void attend_tiles(const Chunk& a, const Divisor& pages) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const PagedKV& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     const int id = divided(blockIdx.x, a.per_split), item = divided(id, a.per_head);
     int split = blockIdx.x - id * a.splits, head = id - item * c.num_heads;    // neighbours are on different XCDs, a head's tiles on one where 8 divides the heads
     int b = 0, tile = 0;
-    if (!a.dealt && !item_of<kRows>(a, item, b, tile)) return;
+    if (!DEALT && !item_of<kRows>(a, item, b, tile)) return;
     const Fresh tokens = fresh_of(a, b);
     const int rows = tokens.count * a.group;
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
@@ -102,15 +103,7 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     // Dealt out: the steps of all heads' tiles, one behind the other, in equal shares (544 tiles on 256 CUs: 2.1 turns of a tile's steps, where whole tiles take 3 and
     // fourths of them 2.25 and twice the states).  An XCD has shares that follow one another, of few heads.  A tile's shares are its states 0, 1, ..., and
     // whoever has its last step marks those that there are not as empty.
-    int64_t share_at = 0, share_end = 0, dealt_steps = 0;
-    int share = 0, tile_steps = 1;
-    if (a.dealt) {
-        const int eighths = a.dealt / 8 * 8;
-        share = (int)blockIdx.x < eighths ? (int)(blockIdx.x & 7) * (a.dealt / 8) + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
-        tile_steps = len > 0 ? ((len - 1) >> 6) + 1 : 1;   // (of an empty prefix: one that shows nothing)
-        dealt_steps = (int64_t)c.num_heads * a.tiles * tile_steps;
-        share_at = dealt_steps * share / a.dealt, share_end = dealt_steps * (share + 1) / a.dealt;
-    }
+    int done = 0;                                          // of the workgroup's share
 
     // what never changes: the values' operand beyond row 131 (fp16 pages: beyond 127, with a row of ones for the weights' sum), the second half of the logits'
     // line, whose first factor is one
@@ -133,16 +126,18 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
 
     for (int r_tile = tile * kRows;; r_tile += a.tiles * kRows) {
         int first_step = 0, end_step = 0;
-        if (a.dealt) {
-            if (share_at >= share_end) break;
-            const int64_t number = share_at / tile_steps;
-            first_step = (int)(share_at - number * tile_steps);
-            end_step = share_end - share_at < tile_steps - first_step ? first_step + (int)(share_end - share_at) : tile_steps;
-            // (the share that has the tile's first step)
-            split = share - (int)(((number * tile_steps + 1) * a.dealt - 1) / dealt_steps);
+        if (DEALT) {
+            const int eighths = a.dealt >> 3, share = (int)blockIdx.x < eighths * 8 ? (int)(blockIdx.x & 7) * eighths + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
+            const int tile_steps = len > 0 ? ((len - 1) >> 6) + 1 : 1;         // (of an empty prefix: one that shows nothing)
+            const int64_t all = (int64_t)c.num_heads * a.tiles * tile_steps, at = all * share / a.dealt + done, end = all * (share + 1) / a.dealt;
+            if (at >= end) break;
+            const int64_t number = at / tile_steps;
+            first_step = (int)(at - number * tile_steps);
+            end_step = end - at < tile_steps - first_step ? first_step + (int)(end - at) : tile_steps;
+            split = share - (int)(((number * tile_steps + 1) * a.dealt - 1) / all);          // (the share that has the tile's first step is state 0)
             head = (int)(number / a.tiles), r_tile = ((int)number - head * a.tiles) * kRows;
             head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;
-            share_at += end_step - first_step;
+            done += end_step - first_step;
             if (r_tile >= rows) continue;
         } else if (r_tile >= rows) {
             break;
@@ -150,8 +145,8 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
         const int r_end = r_tile + kRows < rows ? r_tile + kRows : rows;
         const int tile_lowest = first_place + divided(r_tile, a.per_place), tile_highest = first_place + divided(r_end - 1, a.per_place);
         const Steps steps = steps_of<6>(a, tile_lowest, tile_highest);
-        const int s_begin = a.dealt ? first_step : divided(steps.all * split, a.per_split);      // (below 2^24 steps, 2^5 splits)
-        const int s_end = a.dealt ? (end_step < steps.all ? end_step : steps.all) : divided(steps.all * (split + 1), a.per_split);
+        const int s_begin = DEALT ? first_step : divided(steps.all * split, a.per_split);      // (below 2^24 steps, 2^5 splits)
+        const int s_end = DEALT ? (end_step < steps.all ? end_step : steps.all) : divided(steps.all * (split + 1), a.per_split);
         const int last = s_end - 1;
         auto position = [&](int s) INLINE { return steps.at(s < last ? s : last) * kStep; };        // (behind the last step the last again)
 
@@ -798,8 +793,8 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
             } else {
                 float* const dst = a.part + (((int64_t)(tokens.start + token) * (c.num_heads * a.group) + q_head) * a.parts + a.part_at + split) * 132;
                 if (h == 0) dst[0] = limit[cb] < 0.f ? kEmpty : m[cb], dst[1] = sum;
-                if (h == 0 && end_step == tile_steps)
-                    for (int i = a.part_at + split + 1; a.dealt && i < a.parts; ++i) dst[132 * (i - a.part_at - split)] = kEmpty, dst[132 * (i - a.part_at - split) + 1] = 0.f;
+                if (DEALT && h == 0 && s_end == steps.all)
+                    for (int i = a.part_at + split + 1; i < a.parts; ++i) dst[132 * (i - a.part_at - split)] = kEmpty, dst[132 * (i - a.part_at - split) + 1] = 0.f;
 #pragma unroll
                 for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -811,12 +806,20 @@ __global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pa
     }
 }
 
+template <bool F16, bool ALIGNED>
+__global__ __launch_bounds__(256, 1) void chunk_tiles_kernel(Chunk a, Divisor pages) { attend_tiles<F16, ALIGNED, false>(a, pages); }
+// (a kernel of its own: what the shares need costs the other one registers, 4 % of its time on fp16 pages)
+template <bool F16, bool ALIGNED>
+__global__ __launch_bounds__(256, 1) void prefix_tiles_kernel(Chunk a, Divisor pages) { attend_tiles<F16, ALIGNED, true>(a, pages); }
+
 }  // namespace
 
 int qr_internal_chunk_tiles(bool fp16, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st) {
     using Kernel = void (*)(Chunk, Divisor);
     const bool aligned = a.c.page_size % 16 == 0;
-    const Kernel kernel = fp16 ? (aligned ? chunk_tiles_kernel<true, true> : chunk_tiles_kernel<true, false>)
+    const Kernel kernel = a.dealt ? (fp16 ? (aligned ? prefix_tiles_kernel<true, true> : prefix_tiles_kernel<true, false>)
+                                          : (aligned ? prefix_tiles_kernel<false, true> : prefix_tiles_kernel<false, false>))
+                          : fp16 ? (aligned ? chunk_tiles_kernel<true, true> : chunk_tiles_kernel<true, false>)
                                : (aligned ? chunk_tiles_kernel<false, true> : chunk_tiles_kernel<false, false>);
     const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, kLds);
     if (e != hipSuccess) return (int)e;

@@ -148,6 +148,28 @@ def test_many_rows(page_size, prefixes, members, lens, news, heads, group, f16):
     check(specs, prefix, q, starts, prefixes, members, lens, news)
 
 
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("page_size,prefix_len,members,lens,news,heads,group", [
+    (16, 8000, None, [70] * 9, [70] * 9, 5, 2),              # five tiles a head: no number of shares goes into them, nor they into it
+    (16, 900, None, [130] * 20, [130] * 20, 3, 8),           # more tiles than shares
+    (64, 20000, None, [300], [300], 1, 1),                   # more shares than a tile has states
+    (16, 40, None, [300, 90], [300, 90], 2, 4),              # a step of the prefix for several tiles
+    (7, 3000, [0, 2], [200, 100, 300], [200, 100, 300], 2, 3),              # sequences behind the prefix's last: tiles without rows
+    (16, 2000, [1, 1], [200, 300], [200, 300], 2, 2),        # a prefix of no sequence
+    (16, 0, None, [300, 100], [300, 100], 2, 2)])            # and one without positions
+def test_one_prefix_and_many_rows(page_size, prefix_len, members, lens, news, heads, group, f16):
+    """The steps of a prefix's tiles dealt out evenly: shares that begin and end inside tiles, whatever is hinted."""
+    specs, prefix, q, starts = make_shared(prefix_len + heads, page_size, [prefix_len], members, lens, news, heads, group, f16)
+    outs = check(specs, prefix, q, starts, [prefix_len], members, lens, news)
+    (want, tol), _ = definition(specs, prefix, q, [prefix_len], members, lens, news, 1)
+    call = kv.batch_shared_f16 if f16 else kv.batch_shared_i4
+    for hint in (1, 500, 3 * prefix_len, 1 << 40):
+        o = torch.empty_like(outs[0])
+        call(o, q, **specs, layer_idx=1, **prefix, seqlen_indptr=starts, max_new_len=max(news), max_seq_len=max(lens), max_prefix_len=hint,
+             workspace=torch.full((1 << 28,), 255, dtype=torch.uint8, device=DEV))
+        assert bool(((o.double() - want).abs() <= tol).all()), hint
+
+
 @pytest.mark.parametrize("news", [[1, 1, 1, 1, 1], [3, 0, 200, 1, 9]])
 @pytest.mark.parametrize("f16", [False, True])
 def test_sequences_without_a_prefix_empty_prefixes_and_empty_sequences(f16, news):
