@@ -511,7 +511,8 @@ int qr_batch_shared_f16(void* o, int64_t o_stride, void* lse_or_null, const void
  *   lse fp32 [tokens, num_q_heads] (a row whose lse is -inf gives nothing).  Everything in 32 bits, int4 codes as they are; no atomics: the
  *   same inputs give the same bits.  A NaN or infinity of a key reaches that position alone, one of a query the positions that it sees.
  *   Positions on page numbers outside [0, num_pages) get nothing.  With a workspace of qr_accumulate_weights_workspace_bytes bytes (the same
- *   arguments, max_new_len 1 where seqlen_indptr is NULL; 16-byte aligned, contents arbitrary: the queries in another order) many rows are faster.
+ *   arguments, max_new_len 1 where seqlen_indptr is NULL; 16-byte aligned, contents arbitrary: the queries in another order, 9/8 of their size, and sums of
+ *   parts of the rows) many rows are faster.
  * qr_heavy_positions: of every sequence b and key head h that holds more than `keep` of lengths[b] positions the first `sinks`, the last
  *   `recent` (sinks + recent <= keep) and between them those of the largest weights, of equal ones the lowest positions (NaN counts below all
  *   numbers): kept int32 [batch_size, num_heads, keep], ascending; of shorter sequences all of them, then -1.  lengths int32 (below 0: 0,
@@ -521,7 +522,8 @@ int qr_batch_shared_f16(void* o, int64_t o_stride, void* lse_or_null, const void
  *   length (as the page tables have it, before) become zero.  Entries that are no position of the sequence, or lie on a page number outside
  *   [0, num_pages), are skipped.  Sequences of one prefix's pages must not be among those that move.
  */
-size_t qr_accumulate_weights_workspace_bytes(int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len);
+size_t qr_accumulate_weights_workspace_bytes(int fp16_pages, int64_t capacity, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size,
+                                             int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks);
 int qr_accumulate_weights_i4(void* weights, int64_t capacity, const void* q, int64_t q_stride, int q_had_mode, const void* lse,
                              const void* seqlen_indptr_or_null, int64_t tokens, int num_q_heads, const void* kv_data,
                              const void* kv_param, const void* kv_indptr, const void* kv_indices, const void* last_page_offset,

@@ -70,7 +70,7 @@ SIGNATURES = {
     "qr_batch_shared_workspace_bytes": (_c.c_size_t, (_int, _i64, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64)),
     "qr_batch_shared_i4": (_int, _SHARED),
     "qr_batch_shared_f16": (_int, _SHARED),
-    "qr_accumulate_weights_workspace_bytes": (_c.c_size_t, (_i64, _int, _int, _i64, _i64)),
+    "qr_accumulate_weights_workspace_bytes": (_c.c_size_t, (_int, _i64, _i64, _int, _int, _i64, _i64, _i64, _i64, _i64)),
     "qr_accumulate_weights_i4": (_int, _WEIGHTS),
     "qr_accumulate_weights_f16": (_int, _WEIGHTS),
     "qr_heavy_positions": (_int, (_ptr, _i64, _ptr, _i64, _int, _i64, _i64, _i64, _ptr, _ptr, _ptr)),

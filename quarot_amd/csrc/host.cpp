@@ -689,7 +689,7 @@ PyObject* accumulate(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         bound < 0 || window < 0 || sinks < 0 || lse->dim() != 2 || lse->size(0) != tokens || lse->size(1) != heads)
         return none();
     if (!seq) fresh_bound = 1;
-    const size_t need = qr_accumulate_weights_workspace_bytes(tokens, (int)heads, c.heads, c.batch, fresh_bound);
+    const size_t need = qr_accumulate_weights_workspace_bytes(fp16_pages ? 1 : 0, weights->size(2), tokens, (int)heads, c.heads, c.batch, fresh_bound, bound, window, sinks);
     const bool kept = need && ws && (size_t)ws->numel() >= need;
     at::Tensor own;
     const auto call = [&] {

@@ -6,8 +6,7 @@
 // its key to its sum: nothing is exchanged but the four partial sums of a column, no atomics, and the order of the additions is always the same.
 //
 // The logits are a product rows x positions, positions in the lanes: a position's scale and zero point are its lane's, sums over rows are sums of
-// registers.  Int4 keys enter as codes, which fp16 holds exactly (chunk.hip); every q too: a code is shifted into its half's lowest four bits, so
-// that no element of q is divided.  Logits, exponentials and sums are in 32 bits, nothing is rounded to fewer.
+// registers.  Int4 keys enter as codes, which fp16 holds exactly, q as it is.  Logits, exponentials and sums are in 32 bits, nothing is rounded to fewer.
 #include "qr_chunk.h"
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -23,6 +22,8 @@ struct Weights {
     int64_t q_stride, capacity;
     int tokens, group, blocks, window, sinks, q_had;
     Divisor per_group, per_block, per_head;
+    float* part;                      // splits > 1: sums of every split of the rows, [split, item, block, 256]
+    int splits;
     uint8_t* units;                   // the queries as the kernel of many rows takes them: units of 32 rows, [key head, unit]
     int64_t all_units;
 };
@@ -36,12 +37,17 @@ __device__ __forceinline__ Fresh fresh_of(const Weights& a, int b) {
     return Fresh{start, stop > start ? stop - start : 0, end > start ? end - start : 0};
 }
 
-// the codes of a word as in codes_of, all of them in a half's lowest four bits
-__device__ __forceinline__ u32x4 low_codes_of(u32 w) {
-    return u32x4{w & 0x000F000Fu, (w >> 4) & 0x000F000Fu, (w >> 8) & 0x000F000Fu, (w >> 12) & 0x000F000Fu};
+// The codes of a word as fp16 numbers, in the order of codes_of: (1024 + code) - 1024, (64 + code) - 64.  (As subnormal numbers, which codes_of makes without
+// the subtraction, they lose bits on the way: a sum of 128 products is off by 27 steps of 2^-24 of itself then, root mean square, and by 0.6 like this, and
+// the sums of 16384 rows by 2.4e-5 instead of 5e-7.)
+__device__ __forceinline__ u32x4 numbers_of(u32 w, CodeMasks m) {
+    const u32 w8 = w >> 8;
+    const f16x2 a = {(f16)-1024.f, (f16)-1024.f}, b = {(f16)-64.f, (f16)-64.f};
+    return u32x4{__builtin_bit_cast(u32, as_f16x2(and_or(w, m.low, 0x64006400u)) + a), __builtin_bit_cast(u32, as_f16x2(and_or(w, m.high, 0x54005400u)) + b),
+                 __builtin_bit_cast(u32, as_f16x2(and_or(w8, m.low, 0x64006400u)) + a), __builtin_bit_cast(u32, as_f16x2(and_or(w8, m.high, 0x54005400u)) + b)};
 }
 // eight elements of q in the order of a word's codes: (0, 4), (1, 5), (2, 6), (3, 7)
-__device__ __forceinline__ u32x4 query_for_low_codes(u32x4 w) {
+__device__ __forceinline__ u32x4 query_for_numbers(u32x4 w) {
     return u32x4{__builtin_amdgcn_perm(w[2], w[0], 0x05040100u), __builtin_amdgcn_perm(w[2], w[0], 0x07060302u),
                  __builtin_amdgcn_perm(w[3], w[1], 0x05040100u), __builtin_amdgcn_perm(w[3], w[1], 0x07060302u)};
 }
@@ -134,7 +140,7 @@ __device__ __forceinline__ RowTile<F16> row_tile(const Weights& a, const Fresh& 
         for (int i = 0; i < 4; ++i) t.slope[i] = __shfl(slope, 4 * g + i, 64);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) t.q[i] = F16 ? w[i] : query_for_low_codes(w[i]);
+    for (int i = 0; i < 4; ++i) t.q[i] = F16 ? w[i] : query_for_numbers(w[i]);
     return t;
 }
 
@@ -153,7 +159,7 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
     constexpr uint32_t VEC = F16 ? 256 : 64;
-    constexpr float kUnit = kLog2e * kScale * (F16 ? 1.f : kCodeUnit);
+    constexpr float kUnit = kLog2e * kScale;
     const int highest = first_place + divided(rows - 1, a.per_group);
     const Steps steps = steps_of<6>(a, first_place, highest);              // blocks of 64 positions that some row sees
     const int stride = a.blocks * kWaves;
@@ -224,6 +230,7 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
         return t;
     };
     if (block >= steps.all) return;
+    const CodeMasks masks = code_masks();
     Place here = ask(block), next = ask(block + stride);
     Block f;
     fetch(f, here);
@@ -267,7 +274,7 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
                     } else {
                         u32 w = k[s][0][i];
                         asm volatile("" : "+v"(w));        // (unpacked here, tile by tile of rows: all of them are 64 registers)
-                        key = low_codes_of(w);
+                        key = numbers_of(w, masks);
                     }
                     x[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, tile.q[i]), __builtin_bit_cast(f16x8, key), x[s], 0, 0, 0);
                 }
@@ -360,7 +367,7 @@ __global__ __launch_bounds__(256) void weights_queries_kernel(Weights a) {
         const float m1 = top(m), m2 = top(m - m1), m3 = m - m1 - m2;
         uint8_t* const to = a.units + ((int64_t)h * a.all_units + first_unit(a, mine.start, b) + unit) * kUnitBytes + lane * 16;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) *(u32x4*)(to + 1024 * i) = F16 ? w[i] : query_for_low_codes(w[i]);
+        for (int i = 0; i < 8; ++i) *(u32x4*)(to + 1024 * i) = F16 ? w[i] : query_for_numbers(w[i]);
         *(u32x4*)(to + 8192) = hh ? u32x4{tops(m3, 0.f), 0, 0, 0} : u32x4{tops(s1, s2), tops(s3, s1), tops(s2, s3), tops(m1, m2)};
     }
 }
@@ -375,7 +382,8 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hh = lane >> 5;
     // (a head's workgroups are on one XCD where 8 divides the heads; blocks that most rows see come first)
     const int items = c.batch_size * c.num_heads;
-    const int first_block = blockIdx.x / items, id = blockIdx.x - first_block * items, b = divided(id, a.per_head), h = id - b * c.num_heads;
+    const int turn = blockIdx.x / items, id = blockIdx.x - turn * items, b = divided(id, a.per_head), h = id - b * c.num_heads;
+    const int first_block = turn / a.splits, split = turn - first_block * a.splits;
     const Fresh mine = fresh_of(a, b);
     const int p0 = c.indptr[b], npages = c.indptr[b + 1] - p0;
     const int len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
@@ -384,7 +392,7 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
     const int64_t page_slots = (int64_t)c.num_layers * 2 * c.num_heads * c.page_size;
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
     constexpr uint32_t VEC = F16 ? 256 : 64;
-    constexpr float kUnit = kLog2e * kScale * (F16 ? 1.f : kCodeUnit);
+    constexpr float kUnit = kLog2e * kScale;
     const int highest = first_place + divided(rows - 1, a.per_group);
     const Steps steps = steps_of<8>(a, first_place, highest);              // blocks of 256 positions that some row sees
     const uint8_t* const units = a.units + ((int64_t)h * a.all_units + first_unit(a, mine.start, b)) * kUnitBytes;
@@ -400,6 +408,8 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
     };
 
     for (int block = first_block; block < steps.all; block += a.blocks) {
+        const bool whole = a.splits == 1 || block >= a.blocks;             // (blocks that the launch was not sized for are not split)
+        if (whole && split > 0) break;
         const int block_at = steps.at(block) * 256, at = block_at + 64 * wave;
         const int pos = at + lane, it = divided(pos, pages);
         const u32 entry = (u32)(pos - it * c.page_size);
@@ -408,6 +418,7 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
         const bool there = in && page >= 0 && page < c.num_pages;
         const int64_t slot = there ? page * page_slots + head_slots + entry : head_slots;
         const u32 param = F16 ? 0u : c.param[slot];
+        const CodeMasks masks = code_masks();
         u32x4 k[2][8], line[2];
         float slope[2];
         int from[2], to[2];
@@ -420,7 +431,7 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
             } else {
                 const u32x4 w0 = *(const u32x4*)kd, w1 = *(const u32x4*)(kd + 16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) k[cb][i] = low_codes_of(w0[i]), k[cb][4 + i] = low_codes_of(w1[i]);
+                for (int i = 0; i < 4; ++i) k[cb][i] = numbers_of(w0[i], masks), k[cb][4 + i] = numbers_of(w1[i], masks);
             }
             const f16x2 p = as_f16x2((u32)__shfl((int)param, 32 * cb + n, 64));
             slope[cb] = F16 ? kUnit : (float)p[0] * kUnit;
@@ -430,7 +441,11 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
         }
         // rows that see one of the workgroup's positions; those that see all of the wave's, and those that see any
         const int last_seen = a.window == 0 || block_at < a.sinks ? rows : seen_to(block_at + 255);
-        const int u_begin = seen_from(block_at) / 32, u_end = ((last_seen < rows ? last_seen : rows) + 31) / 32;
+        int u_begin = seen_from(block_at) / 32, u_end = ((last_seen < rows ? last_seen : rows) + 31) / 32;
+        if (!whole) {
+            const int all = u_end > u_begin ? u_end - u_begin : 0, first = u_begin;
+            u_begin = first + (int)((int64_t)all * split / a.splits), u_end = first + (int)((int64_t)all * (split + 1) / a.splits);
+        }
         const int all_from = seen_from(at + 63), all_to = at + 63 < a.sinks ? rows + 32 : seen_to(at < a.sinks ? a.sinks : at);
         const int any_from = seen_from(at), any_to = a.window == 0 || at < a.sinks ? rows + 32 : seen_to(at + 63);
 
@@ -511,32 +526,74 @@ __global__ __launch_bounds__(256, 2) void weights_tiles_kernel(Weights a, Diviso
             const u32x2 both = both_halves<32>(as_u32(total[cb]));
             all[cb] = as_f32(both.x) + as_f32(both.y);
         }
-        if (there && pos < a.capacity) a.sums[((int64_t)b * c.num_heads + h) * a.capacity + pos] += hh ? all[1] : all[0];
+        if (!whole) a.part[(((int64_t)split * items + id) * a.blocks + block) * 256 + 64 * wave + lane] = there ? (hh ? all[1] : all[0]) : 0.f;
+        else if (there && pos < a.capacity) a.sums[((int64_t)b * c.num_heads + h) * a.capacity + pos] += hh ? all[1] : all[0];
         __syncthreads();                                   // (the next block's first stage overwrites LDS)
     }
 }
 
-// Which kernel, and workgroups per (sequence, key head)
+// The sums of the rows' splits -> the positions' sums, in the splits' order
+__global__ __launch_bounds__(256) void weights_join_kernel(Weights a) {
+    const PagedKV& c = a.c;
+    const int items = c.batch_size * c.num_heads, block = blockIdx.x / items, id = blockIdx.x - block * items, b = divided(id, a.per_head);
+    const Fresh mine = fresh_of(a, b);
+    const int npages = c.indptr[b + 1] - c.indptr[b], len = npages > 0 ? (npages - 1) * c.page_size + c.last_page_offset[b] : 0;
+    const int rows = mine.count * a.group, first_place = len - mine.all;
+    if (rows == 0) return;
+    const Steps steps = steps_of<8>(a, first_place, first_place + divided(rows - 1, a.per_group));
+    const int pos = steps.at(block) * 256 + (int)threadIdx.x;
+    if (block >= steps.all || pos >= len || pos >= a.capacity) return;
+    const float* const src = a.part + ((int64_t)id * a.blocks + block) * 256 + threadIdx.x;
+    float sum = 0.f;
+    for (int s = 0; s < a.splits; ++s) sum += src[(int64_t)s * items * a.blocks * 256];
+    a.sums[(int64_t)id * a.capacity + pos] += sum;
+}
+
+// Which kernel, workgroups per (sequence, key head), and among how many of them the rows are split
 struct WeightsPlan {
     bool tiles;
+    int splits;
     int64_t blocks, most;              // most: workgroups of a launch, which has fewer than 2^32 threads
 };
 WeightsPlan weights_plan(bool fp16, int64_t tokens, int group, int64_t num_heads, int64_t batch, int64_t max_new_len, int64_t seen) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     WeightsPlan p;
     p.tiles = max_new_len * group > 64;
+    p.splits = 1;
     p.most = 0xffffffffll / 256;
     p.blocks = (seen + 255) / 256;
+    const int64_t cus = qr_device().cus, items = batch * num_heads;
     if (!p.tiles) {                    // workgroups that are on the chip at once, of equal work
-        const int64_t room = (fp16 ? 2 : 3) * (int64_t)qr_device().cus / (batch * num_heads), all = (seen + 63) / 64;
+        const int64_t room = (fp16 ? 2 : 3) * cus / items, all = (seen + 63) / 64;
         const int64_t turns = room > 0 ? (all + 4 * room - 1) / (4 * room) : all;
         if (turns > 1) p.blocks = (all + 4 * turns - 1) / (4 * turns);
     }
     if (p.blocks > 0xffff) p.blocks = 0xffff;
-    if (batch * num_heads * p.blocks > p.most) p.blocks = batch * num_heads < p.most ? p.most / (batch * num_heads) : 1;
+    if (items * p.blocks > p.most) p.blocks = items < p.most ? p.most / items : 1;
+    if (p.tiles) {
+        // Parts of the rows: microseconds of a workgroup's unit of 32 rows, alone on its CU 0.74, with another one 0.98, what goes around its units 6, the join 4 and
+        // 0.0003 for a part of a block.  (8192 rows of one key head, one block: 193 us whole, 112, 72, 48, 32 and 27 in 2, 4, 8, 16 and 32 parts; 536 blocks of
+        // 8192 rows, two rounds of which the second is nearly empty: 403 whole, 328 in four parts; 512 rows of a block 24.5, in eight parts 13.7.)
+        const int64_t units = (max_new_len * group + 31) / 32, all = items * p.blocks;
+        float least = -1.f;
+        for (int splits = 1; splits <= 32 && (splits == 1 || (2 * splits <= units && all * splits <= p.most)); ++splits) {
+            const float each = all * splits <= cus ? 0.74f : 0.98f;
+            const float time = (float)((all * splits + 2 * cus - 1) / (2 * cus)) * ((float)((units + splits - 1) / splits) * each + 6.f) +
+                               (splits > 1 ? 4.f + 0.0003f * (float)(all * splits) : 0.f);
+            // (parts for a tenth at least: blocks that few rows see fill rounds up by themselves)
+            if (least < 0.f || time < (p.splits == 1 ? 0.9f : 1.f) * least) least = time, p.splits = splits;
+        }
+    }
     return p;
 }
+int bounded_window(int64_t window) { return (int)(window > 0x3fffffff ? 0 : window); }       // (longer than any sequence)
+int bounded_sinks(int64_t sinks) { return (int)(sinks > 0x3fffffff ? 0x3fffffff : sinks); }
 int64_t weights_units(int64_t tokens, int group, int64_t batch) { return tokens * group / 32 + batch + 2; }
+// workspace: the queries' units, then the splits' sums
+size_t weights_bytes(const WeightsPlan& p, int64_t tokens, int group, int64_t num_heads, int64_t batch) {
+    if (!p.tiles) return 0;
+    return (size_t)weights_units(tokens, group, batch) * num_heads * kUnitBytes + (p.splits > 1 ? (size_t)p.splits * batch * num_heads * p.blocks * 1024 : 0);
+}
 // positions that the launch is sized for (what is longer is gone through in turns)
 int64_t seen_positions(int64_t tokens, int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks, int64_t capacity) {
     int64_t seen = max_seq_len > 0 && max_seq_len < capacity ? max_seq_len : capacity;
@@ -556,7 +613,8 @@ int launch_weights(const WeightsPlan& plan, Weights a, hipStream_t st) {
         Weights first = a;
         first.blocks = (int)each, first.per_block = divisor_of(each);
         weights_queries_kernel<F16><<<dim3((unsigned)(items * each)), dim3(256), 0, st>>>(first);
-        weights_tiles_kernel<F16><<<dim3((unsigned)(items * a.blocks)), dim3(256), 0, st>>>(a, pages);
+        weights_tiles_kernel<F16><<<dim3((unsigned)(items * a.blocks * a.splits)), dim3(256), 0, st>>>(a, pages);
+        if (a.splits > 1) weights_join_kernel<<<dim3((unsigned)(items * a.blocks)), dim3(256), 0, st>>>(a);
     } else {
         const bool aligned = a.c.page_size % 16 == 0;
         using Kernel = void (*)(Weights, Divisor);
@@ -588,17 +646,18 @@ int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_
     a.starts = (const int32_t*)starts;
     a.q_stride = q_stride, a.capacity = capacity;
     a.tokens = (int)tokens, a.group = num_q_heads / num_heads;
-    a.window = (int)(window > 0x3fffffff ? 0 : window);
-    a.sinks = (int)(sinks > 0x3fffffff ? 0x3fffffff : sinks);
+    a.window = bounded_window(window), a.sinks = bounded_sinks(sinks);
     a.q_had = q_had_mode;
     a.per_group = divisor_of(a.group), a.per_head = divisor_of(num_heads);
     const int64_t fresh = starts ? max_new_len : 1;
     WeightsPlan plan = weights_plan(fp16, tokens, a.group, num_heads, batch_size, fresh, seen_positions(tokens, fresh, max_seq_len, a.window, a.sinks, capacity));
     a.all_units = weights_units(tokens, a.group, batch_size);
-    if (plan.tiles && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < (size_t)a.all_units * num_heads * kUnitBytes)) plan.tiles = false;
+    if (plan.tiles && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < weights_bytes(plan, tokens, a.group, num_heads, batch_size))) plan.tiles = false, plan.splits = 1;
     a.units = (uint8_t*)workspace;
+    a.part = (float*)((uint8_t*)workspace + (size_t)a.all_units * num_heads * kUnitBytes);
+    a.splits = plan.splits;
     a.blocks = (int)plan.blocks, a.per_block = divisor_of(plan.blocks);
-    const int64_t wide = num_heads * plan.blocks, at_once = batch_size * wide <= plan.most ? batch_size : plan.most / wide;
+    const int64_t wide = num_heads * plan.blocks * plan.splits, at_once = batch_size * wide <= plan.most ? batch_size : plan.most / wide;
     int lrc = QR_OK;
     for (int64_t first = 0; first < batch_size && lrc == QR_OK; first += at_once) {
         Weights some = a;
@@ -614,12 +673,15 @@ int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_
 
 }  // namespace
 
-extern "C" size_t qr_accumulate_weights_workspace_bytes(int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len) {
+extern "C" size_t qr_accumulate_weights_workspace_bytes(int fp16_pages, int64_t capacity, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size,
+                                                        int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks) {
     if (tokens <= 0 || num_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_heads || batch_size <= 0 || batch_size > 0x7fffffff || tokens > 0x3fffffff ||
-        tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > 65536)
-        return 0;                                          // (the call itself refuses them)
-    if (!weights_plan(false, tokens, num_q_heads / num_heads, num_heads, batch_size, max_new_len, 1).tiles) return 0;
-    return (size_t)weights_units(tokens, num_q_heads / num_heads, batch_size) * num_heads * kUnitBytes;
+        tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > 65536 || capacity <= 0)
+        return 0;                                          // (the call itself refuses them, or has nothing to do)
+    const int group = num_q_heads / num_heads;
+    return weights_bytes(weights_plan(fp16_pages != 0, tokens, group, num_heads, batch_size, max_new_len,
+                                      seen_positions(tokens, max_new_len, max_seq_len, bounded_window(window), bounded_sinks(sinks), capacity)),
+                         tokens, group, num_heads, batch_size);
 }
 
 #define QR_WEIGHTS_ENTRY(NAME, FP16)                                                                                                                     \

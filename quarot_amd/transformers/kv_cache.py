@@ -485,7 +485,7 @@ def _accumulate(fn, f16, weights, q, lse, kv_data, kv_param, kv_indptr, kv_indic
     with _lib.on_device(dev):
         if seqlen_indptr is None:
             max_new_len = 1
-        ws_bytes = _lib.lib().qr_accumulate_weights_workspace_bytes(tokens, q_heads, heads, batch, max_new_len)
+        ws_bytes = _lib.lib().qr_accumulate_weights_workspace_bytes(1 if f16 else 0, weights.shape[2], tokens, q_heads, heads, batch, max_new_len, max_seq_len, window, sinks)
         ws = _scratch(workspace, ws_bytes, dev)
         entry = _lib.lib().qr_accumulate_weights_f16 if f16 else _lib.lib().qr_accumulate_weights_i4
         _lib.check(entry(

@@ -139,6 +139,23 @@ def test_weights_of_many_rows(page_size, lens, news, heads, group, window, sinks
 
 
 @pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("lens,news,group,window,sinks", [([1500], [1400], 8, 0, 0), ([300, 1100], [300, 1000], 6, 0, 0), ([2600], [1200], 8, 300, 20), ([700, 0, 90], [600, 0, 90], 20, 0, 0)])
+def test_weights_of_rows_in_parts(lens, news, group, window, sinks, f16):
+    """Few blocks of positions and many rows, which several workgroups share; hints that are too small leave blocks to one workgroup, too large ones leave workgroups without a block."""
+    specs, q, starts = make(sum(lens), 16, lens, news, 1, group, f16)
+    lse = logarithms(specs, q, lens, news, window=window, sinks=sinks)
+    check(specs, q, starts, lens, news, window=window, sinks=sinks, lse=lse)
+    start = torch.rand(len(lens), 1, max(lens), device=DEV)
+    want, tol = definition(specs, q, lse, start, lens, news, window=window, sinks=sinks)
+    call = kv.accumulate_weights_f16 if f16 else kv.accumulate_weights_i4
+    for new, length in ((0, 1), (max(news), 200), (0, 40000), (1, 0), (100000, 1 << 40)):
+        got = start.clone()
+        call(got, q, lse, **specs, layer_idx=1, seqlen_indptr=starts, max_new_len=new, max_seq_len=length, window=window, sinks=sinks,
+             workspace=torch.full((1 << 26,), 255, dtype=torch.uint8, device=DEV))
+        assert bool(((got.double() - want).abs() <= tol).all()), (new, length)
+
+
+@pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("news", [[40, 90], [1, 1], [300, 20]])
 def test_weights_of_large_logits(f16, news):
     lens = [600, 90]
