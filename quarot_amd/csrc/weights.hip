@@ -21,6 +21,7 @@ struct Weights {
     const int32_t* starts;            // nullptr: one new token per sequence
     int64_t q_stride, capacity;
     int tokens, group, blocks, window, sinks, q_had;
+    int64_t rows;                     // no sequence has more of a key head
     Divisor per_group, per_block, per_head;
     float* part;                      // splits > 1: sums of every split of the rows, [split, item, block, 256]
     int splits;
@@ -85,14 +86,14 @@ __device__ __forceinline__ void hadamard_row(u32x4 (&w)[4], int lane) {
 // Of 16 rows and fewer the queries stay in registers, of up to 64 in LDS, ready for the products (a wave makes one tile of them; more are made for every block).
 constexpr int kWaves = 4;
 template <bool F16>
-struct RowTile {                       // 16 rows: queries as the products take them; slope, logarithm (base 2, negative) and the token of rows 4 g + i
+struct RowTile {                       // 16 rows: queries as the products take them; slope, logarithm (base 2, negative) and position of four of them
     u32x4 q[4];
     float slope[4] = {0.f, 0.f, 0.f, 0.f}, less[4];
     int place[4];
 };
 template <bool F16, bool HAD>
-__device__ __forceinline__ RowTile<F16> row_tile(const Weights& a, const Fresh& mine, int h, int r0, int rows, int first_place, int lane) {
-    const int n = lane & 15, g = lane >> 4;
+__device__ __forceinline__ RowTile<F16> row_tile(const Weights& a, const Fresh& mine, int h, int r0, int rows, int first_place, int lane, int quarter) {
+    const int n = lane & 15, g = lane >> 4;                // quarter: which four rows' numbers the lane holds
     RowTile<F16> t;
     // lane (n, g) holds dimensions 32 g + 8 i .. (fp16 pages: 32 i + 8 g ..) of row n
     const int r = r0 + n < rows ? r0 + n : r0, token = divided(r, a.per_group), head = h * a.group + r - token * a.group;
@@ -103,7 +104,7 @@ __device__ __forceinline__ RowTile<F16> row_tile(const Weights& a, const Fresh& 
     float lse[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int row = r0 + 4 * g + i, of = divided(row < rows ? row : r0, a.per_group);
+        const int row = r0 + 4 * quarter + i, of = divided(row < rows ? row : r0, a.per_group);
         lse[i] = a.lse[(int64_t)(mine.start + of) * (a.c.num_heads * a.group) + h * a.group + (row < rows ? row : r0) - of * a.group];
         t.place[i] = row < rows && lse[i] != -__builtin_inff() ? first_place + of : -1;        // (a row that has seen nothing gives nothing)
         t.less[i] = lse[i] * -kLog2e;
@@ -137,7 +138,7 @@ __device__ __forceinline__ RowTile<F16> row_tile(const Weights& a, const Fresh& 
         }
         const float slope = quarters_sum(all) * -(kLog2e * kScale);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t.slope[i] = __shfl(slope, 4 * g + i, 64);
+        for (int i = 0; i < 4; ++i) t.slope[i] = __shfl(slope, 4 * quarter + i, 64);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) t.q[i] = F16 ? w[i] : query_for_numbers(w[i]);
@@ -145,8 +146,9 @@ __device__ __forceinline__ RowTile<F16> row_tile(const Weights& a, const Fresh& 
 }
 
 // ALIGNED: pages of a multiple of 16 positions, so that every 16 positions lie in one page
-template <bool F16, bool ALIGNED, bool HAD>
-__global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(Weights a, Divisor pages) {
+// ROWS: 4, 8: no more than that many; 16: any number.
+template <bool F16, bool ALIGNED, bool HAD, int ROWS>
+__global__ __launch_bounds__(64 * kWaves, F16 ? (ROWS == 4 ? 3 : 2) : (ROWS < 16 ? 4 : 3)) void weights_rows_kernel(Weights a, Divisor pages) {
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
     };
     struct Block {
         u32x4 k[4][F16 ? 4 : 1];
-        u32 param[F16 ? 1 : 4];
+        u32 param;                     // of the lane's own position
         float before;
     };
     auto there = [&](const Place& p) { return p.page >= 0 && p.page < c.num_pages; };
@@ -189,42 +191,41 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
             if (ALIGNED) {
                 const int page = __builtin_amdgcn_readlane(is ? p.page : -1, 16 * s), entry = __builtin_amdgcn_readlane(p.entry, 16 * s);
                 const int64_t base = page >= 0 ? page * page_slots + head_slots + entry : head_slots;
-                uint32_t off = (uint32_t)n * VEC + (uint32_t)g * 16, p_off = (uint32_t)n * 4;
-                asm volatile("" : "+v"(off), "+v"(p_off));                         // (32-bit offsets behind wave-uniform addresses)
+                uint32_t off = (uint32_t)n * VEC + (uint32_t)g * 16;
+                asm volatile("" : "+v"(off));                                      // (a 32-bit offset behind wave-uniform addresses)
                 const uint8_t* const kd = c.data + base * VEC;
 #pragma unroll
                 for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[s][i] = *(const u32x4*)(kd + off + 64 * i);
-                if (!F16) f.param[F16 ? 0 : s] = *(const u32*)((const uint8_t*)(c.param + base) + p_off);
             } else {
                 const int64_t base = __shfl(slot, 16 * s + n, 64);
                 const uint8_t* const kd = c.data + base * VEC + g * 16;
 #pragma unroll
                 for (int i = 0; i < (F16 ? 4 : 1); ++i) f.k[s][i] = *(const u32x4*)(kd + 64 * i);
-                if (!F16) f.param[F16 ? 0 : s] = c.param[base];
             }
         }
+        f.param = F16 ? 0u : c.param[slot];
         f.before = is && p.pos < a.capacity ? sums[p.pos] : 0.f;
     };
     int block = first_block * kWaves + wave;
-    __shared__ u32x4 staged[4][7][64];
-    const bool in_lds = rows > 16 && rows <= 64;
+    __shared__ u32x4 staged[ROWS == 16 ? 4 : 1][7][64];
+    const bool in_lds = ROWS == 16 && rows > 16 && rows <= 64;
     if (in_lds) {
         if (16 * wave < rows) {
-            const RowTile<F16> t = row_tile<F16, HAD>(a, mine, h, 16 * wave, rows, first_place, lane);
+            const RowTile<F16> t = row_tile<F16, HAD>(a, mine, h, 16 * wave, rows, first_place, lane, g);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) staged[wave][i][lane] = t.q[i];
-            staged[wave][4][lane] = u32x4{as_u32(t.slope[0]), as_u32(t.slope[1]), as_u32(t.slope[2]), as_u32(t.slope[3])};
-            staged[wave][5][lane] = u32x4{as_u32(t.less[0]), as_u32(t.less[1]), as_u32(t.less[2]), as_u32(t.less[3])};
-            staged[wave][6][lane] = u32x4{(u32)t.place[0], (u32)t.place[1], (u32)t.place[2], (u32)t.place[3]};
+            for (int i = 0; i < 4; ++i) staged[wave % (ROWS == 16 ? 4 : 1)][i][lane] = t.q[i];
+            staged[wave % (ROWS == 16 ? 4 : 1)][4][lane] = u32x4{as_u32(t.slope[0]), as_u32(t.slope[1]), as_u32(t.slope[2]), as_u32(t.slope[3])};
+            staged[wave % (ROWS == 16 ? 4 : 1)][5][lane] = u32x4{as_u32(t.less[0]), as_u32(t.less[1]), as_u32(t.less[2]), as_u32(t.less[3])};
+            staged[wave % (ROWS == 16 ? 4 : 1)][6][lane] = u32x4{(u32)t.place[0], (u32)t.place[1], (u32)t.place[2], (u32)t.place[3]};
         }
         __syncthreads();
     }
     auto tile_of = [&](int r0) {
-        if (!in_lds) return row_tile<F16, HAD>(a, mine, h, r0, rows, first_place, lane);
+        if (!in_lds) return row_tile<F16, HAD>(a, mine, h, r0, rows, first_place, lane, ROWS == 4 ? 0 : ROWS == 8 ? g & 1 : g);
         RowTile<F16> t;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t.q[i] = staged[r0 >> 4][i][lane];
-        const u32x4 slope = staged[r0 >> 4][4][lane], less = staged[r0 >> 4][5][lane], place = staged[r0 >> 4][6][lane];
+        for (int i = 0; i < 4; ++i) t.q[i] = staged[(r0 >> 4) % (ROWS == 16 ? 4 : 1)][i][lane];
+        const u32x4 slope = staged[(r0 >> 4) % (ROWS == 16 ? 4 : 1)][4][lane], less = staged[(r0 >> 4) % (ROWS == 16 ? 4 : 1)][5][lane], place = staged[(r0 >> 4) % (ROWS == 16 ? 4 : 1)][6][lane];
 #pragma unroll
         for (int i = 0; i < 4; ++i) t.slope[i] = as_f32(slope[i]), t.less[i] = as_f32(less[i]), t.place[i] = (int)place[i];
         return t;
@@ -238,14 +239,11 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
     for (;;) {
         const int at = __builtin_amdgcn_readfirstlane(here.pos);
         u32x4 k[4][F16 ? 4 : 1];
-        float scale[4], zero[4], sum[4] = {0.f, 0.f, 0.f, 0.f}, before_tiles[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
             for (int i = 0; i < (F16 ? 4 : 1); ++i) k[s][i] = f.k[s][i];
-            const f16x2 p = as_f16x2(f.param[F16 ? 0 : s]);
-            scale[s] = F16 ? kUnit : (float)p[0] * kUnit, zero[s] = (float)p[1];
-        }
+        const u32 param = f.param;
         const float before = f.before;
         const Place now = here;
         const bool more = block + stride < steps.all;
@@ -253,15 +251,7 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
             here = next, next = ask(block + 2 * stride);
             fetch(f, here);
         }
-        for (int r0 = 0; r0 < rows; r0 += 16) {
-            if (r0 > 0) {
-                tile = tile_of(r0);
-                if ((r0 & 255) == 0) {                     // (sums of 16 tiles, then of these: a long chain of additions would lose what is small)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) before_tiles[s] += sum[s], sum[s] = 0.f;
-                }
-            }
-            f32x4 x[4];
+        auto products = [&](f32x4 (&x)[4]) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) x[s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -278,29 +268,78 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? 2 : 3) void weights_rows_kernel(
                     }
                     x[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, tile.q[i]), __builtin_bit_cast(f16x8, key), x[s], 0, 0, 0);
                 }
-            // register i of lane (n, g): row 4 g + i, position n
+        };
+        // the weights of four rows at the positions p of the lanes, whose keys' parameters are given: added up
+        auto weigh = [&](const f32x4& x, u32 key_param, int p, int r0) {
+            const f16x2 kp = as_f16x2(key_param);
+            const float scale = F16 ? kUnit : (float)kp[0] * kUnit, zero = (float)kp[1];
+            const int lowest = first_place + divided(r0, a.per_group), last = first_place + divided((r0 + 15 < rows ? r0 + 16 : rows) - 1, a.per_group);
+            const bool all_see = at + 63 <= lowest && (a.window == 0 || at > last - a.window || at + 63 < a.sinks);
+            float y[4], sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int high = tile.place[i] - at, low = a.window == 0 ? -1 : high - a.window, sinks = a.sinks - at;
+            for (int i = 0; i < 4; ++i)
+                y[i] = F16 ? __builtin_fmaf(x[i], scale, tile.less[i]) : __builtin_fmaf(x[i], scale, __builtin_fmaf(zero, tile.slope[i], tile.less[i]));
+            if (all_see) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
-                    const float y = F16 ? __builtin_fmaf(x[s][i], scale[s], tile.less[i]) : __builtin_fmaf(x[s][i], scale[s], __builtin_fmaf(zero[s], tile.slope[i], tile.less[i]));
-                    const int p = 16 * s + n;
-                    const bool sees = (p <= high) & ((a.window == 0) | (p > low) | (p < sinks));
-                    sum[s] += sees ? __builtin_amdgcn_exp2f(y) : 0.f;
+                for (int i = 0; i < 4; ++i) sum += tile.place[i] >= 0 ? __builtin_amdgcn_exp2f(y[i]) : 0.f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int high = tile.place[i] - at;
+                    const bool sees = (p <= high) & ((a.window == 0) | (p > high - a.window) | (p < a.sinks - at));
+                    sum += sees ? __builtin_amdgcn_exp2f(y[i]) : 0.f;
                 }
             }
-        }
+            return sum;
+        };
         float total = 0.f;
+        if constexpr (ROWS < 16) {
+            // Register i of lane (n, g) is row 4 g + i: half of the lanes, or three quarters, would have nothing to weigh.  They take the rows of other positions.
+            f32x4 x[4];
+            products(x);
+            auto swapped32 = [](float u, float v) { return as_f32(__builtin_amdgcn_permlane32_swap(as_u32(u), as_u32(v), false, false)[0]); };      // lower halves of both
+            auto swapped16 = [](float u, float v) { return as_f32(__builtin_amdgcn_permlane16_swap(as_u32(u), as_u32(v), false, false)[0]); };      // even quarters of both
+            f32x4 even, odd;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const float all = quarters_sum(sum[s] + before_tiles[s]);
-            total = g == s ? all : total;
+            for (int i = 0; i < 4; ++i) even[i] = swapped32(x[0][i], x[2][i]), odd[i] = swapped32(x[1][i], x[3][i]);
+            if (ROWS == 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) even[i] = swapped16(even[i], odd[i]);              // quarter g: rows 0 .. 3 of its own positions
+                total = weigh(even, param, lane, 0);
+            } else {
+                const int p = 32 * (lane >> 5) + n;        // quarters 0 and 1: positions 0 .., 16 .. (odd); 2 and 3: 32 .., 48 ..
+                const u32x2 s0 = both_halves<16>(as_u32(weigh(even, (u32)__shfl((int)param, p, 64), p, 0)));
+                const u32x2 s1 = both_halves<16>(as_u32(weigh(odd, (u32)__shfl((int)param, p + 16, 64), p + 16, 0)));
+                total = g & 1 ? as_f32(s1.x) + as_f32(s1.y) : as_f32(s0.x) + as_f32(s0.y);
+            }
+        } else {
+            float sum[4] = {0.f, 0.f, 0.f, 0.f}, before_tiles[4] = {0.f, 0.f, 0.f, 0.f};
+            u32 params[4];
+#pragma unroll
+            for (int s = 0; s < 4; ++s) params[s] = F16 ? 0u : (u32)__shfl((int)param, 16 * s + n, 64);
+            for (int r0 = 0; r0 < rows; r0 += 16) {
+                if (r0 > 0) {
+                    tile = tile_of(r0);
+                    if ((r0 & 255) == 0) {                 // (sums of 16 tiles, then of these: a long chain of additions would lose what is small)
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) before_tiles[s] += sum[s], sum[s] = 0.f;
+                    }
+                }
+                f32x4 x[4];
+                products(x);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) sum[s] += weigh(x[s], params[s], 16 * s + n, r0);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const float all = quarters_sum(sum[s] + before_tiles[s]);
+                total = g == s ? all : total;
+            }
         }
         if (there(now) && now.pos < a.capacity) sums[now.pos] = before + total;
         if (!more) break;
         block += stride;
-        if (rows > 16) tile = tile_of(0);
+        if (ROWS == 16 && rows > 16) tile = tile_of(0);
     }
 }
 
@@ -555,7 +594,7 @@ struct WeightsPlan {
     int splits;
     int64_t blocks, most;              // most: workgroups of a launch, which has fewer than 2^32 threads
 };
-WeightsPlan weights_plan(bool fp16, int64_t tokens, int group, int64_t num_heads, int64_t batch, int64_t max_new_len, int64_t seen) {
+WeightsPlan weights_plan(bool fp16, int64_t rows, int64_t tokens, int group, int64_t num_heads, int64_t batch, int64_t max_new_len, int64_t seen) {
     if (max_new_len <= 0 || max_new_len > tokens) max_new_len = tokens;
     WeightsPlan p;
     p.tiles = max_new_len * group > 64;
@@ -564,7 +603,7 @@ WeightsPlan weights_plan(bool fp16, int64_t tokens, int group, int64_t num_heads
     p.blocks = (seen + 255) / 256;
     const int64_t cus = qr_device().cus, items = batch * num_heads;
     if (!p.tiles) {                    // workgroups that are on the chip at once, of equal work
-        const int64_t room = (fp16 ? 2 : 3) * cus / items, all = (seen + 63) / 64;
+        const int64_t room = (fp16 ? (rows <= 4 ? 3 : 2) : (rows <= 8 ? 4 : 3)) * cus / items, all = (seen + 63) / 64;
         const int64_t turns = room > 0 ? (all + 4 * room - 1) / (4 * room) : all;
         if (turns > 1) p.blocks = (all + 4 * turns - 1) / (4 * turns);
     }
@@ -602,6 +641,13 @@ int64_t seen_positions(int64_t tokens, int64_t max_new_len, int64_t max_seq_len,
     return seen;
 }
 
+using Kernel = void (*)(Weights, Divisor);
+template <bool F16, int ROWS>
+Kernel rows_kernel(bool aligned, bool had) {
+    return had ? (aligned ? weights_rows_kernel<F16, true, true, ROWS> : weights_rows_kernel<F16, false, true, ROWS>)
+               : (aligned ? weights_rows_kernel<F16, true, false, ROWS> : weights_rows_kernel<F16, false, false, ROWS>);
+}
+
 template <bool F16>
 int launch_weights(const WeightsPlan& plan, Weights a, hipStream_t st) {
     const int64_t items = (int64_t)a.c.batch_size * a.c.num_heads;
@@ -617,9 +663,7 @@ int launch_weights(const WeightsPlan& plan, Weights a, hipStream_t st) {
         if (a.splits > 1) weights_join_kernel<<<dim3((unsigned)(items * a.blocks)), dim3(256), 0, st>>>(a);
     } else {
         const bool aligned = a.c.page_size % 16 == 0;
-        using Kernel = void (*)(Weights, Divisor);
-        const Kernel kernel = a.q_had ? (aligned ? weights_rows_kernel<F16, true, true> : weights_rows_kernel<F16, false, true>)
-                                      : (aligned ? weights_rows_kernel<F16, true, false> : weights_rows_kernel<F16, false, false>);
+        const Kernel kernel = a.rows <= 4 ? rows_kernel<F16, 4>(aligned, a.q_had) : a.rows <= 8 ? rows_kernel<F16, 8>(aligned, a.q_had) : rows_kernel<F16, 16>(aligned, a.q_had);
         kernel<<<dim3((unsigned)(items * a.blocks)), dim3(64 * kWaves), 0, st>>>(a, pages);
     }
     return qr_launch_status();
@@ -648,9 +692,10 @@ int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_
     a.tokens = (int)tokens, a.group = num_q_heads / num_heads;
     a.window = bounded_window(window), a.sinks = bounded_sinks(sinks);
     a.q_had = q_had_mode;
+    a.rows = starts ? tokens * a.group : a.group;
     a.per_group = divisor_of(a.group), a.per_head = divisor_of(num_heads);
     const int64_t fresh = starts ? max_new_len : 1;
-    WeightsPlan plan = weights_plan(fp16, tokens, a.group, num_heads, batch_size, fresh, seen_positions(tokens, fresh, max_seq_len, a.window, a.sinks, capacity));
+    WeightsPlan plan = weights_plan(fp16, a.rows, tokens, a.group, num_heads, batch_size, fresh, seen_positions(tokens, fresh, max_seq_len, a.window, a.sinks, capacity));
     a.all_units = weights_units(tokens, a.group, batch_size);
     if (plan.tiles && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < weights_bytes(plan, tokens, a.group, num_heads, batch_size))) plan.tiles = false, plan.splits = 1;
     a.units = (uint8_t*)workspace;
@@ -679,7 +724,7 @@ extern "C" size_t qr_accumulate_weights_workspace_bytes(int fp16_pages, int64_t 
         tokens * num_q_heads > 0x3fffffff || num_q_heads / num_heads > 1024 || num_heads > 65536 || capacity <= 0)
         return 0;                                          // (the call itself refuses them, or has nothing to do)
     const int group = num_q_heads / num_heads;
-    return weights_bytes(weights_plan(fp16_pages != 0, tokens, group, num_heads, batch_size, max_new_len,
+    return weights_bytes(weights_plan(fp16_pages != 0, tokens * group, tokens, group, num_heads, batch_size, max_new_len,
                                       seen_positions(tokens, max_new_len, max_seq_len, bounded_window(window), bounded_sinks(sinks), capacity)),
                          tokens, group, num_heads, batch_size);
 }
