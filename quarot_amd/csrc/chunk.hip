@@ -37,12 +37,12 @@ struct There {
 
 // ALIGNED: pages of a multiple of 16 positions, so that each half of a step lies in one page.
 template <int NB, int NW, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) {
+__device__ __forceinline__ void attend_rows(const Chunk& a, const Divisor& pages, const int group_number) {
     extern __shared__ __attribute__((aligned(16))) f32x4 st4[];            // per wave and row: maximum, sum, -, -, 128 outputs
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int id = divided(blockIdx.x, a.per_split), split = blockIdx.x - id * a.splits, item = divided(id, a.per_head), h = id - item * c.num_heads;
+    const int id = divided(group_number, a.per_split), split = group_number - id * a.splits, item = divided(id, a.per_head), h = id - item * c.num_heads;
     int b, first_tile;
     if (!item_of<16 * NB>(a, item, b, first_tile)) return;
     const Fresh mine_tokens = fresh_of(a, b);
@@ -481,6 +481,15 @@ __global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_ke
     }
 }
 
+template <int NB, int NW, bool F16, bool ALIGNED>
+__global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) { attend_rows<NB, NW, F16, ALIGNED>(a, pages, blockIdx.x); }
+// Two launches in one: the first `groups` workgroups are a's, the others b's
+template <bool F16, bool ALIGNED>
+__global__ __launch_bounds__(256, F16 ? 2 : 3) void chunk_rows_pair_kernel(Chunk a, Chunk b, Divisor pages, int groups) {
+    const bool first = (int)blockIdx.x < groups;
+    attend_rows<1, 4, F16, ALIGNED>(first ? a : b, pages, first ? blockIdx.x : blockIdx.x - groups);
+}
+
 // The partial states of every row -> its output: sixteen lanes per row, eight dimensions each.  The states' maxima and sums are read by a lane each (at most 32),
 // so that all loads are on their way at once: with few rows this launch is their latency (64 rows of 32 states: 5.6 us; with the states read one after the other 20.3).
 __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict__ part, const int32_t* __restrict__ starts, int batch, int tokens,
@@ -524,7 +533,7 @@ __global__ __launch_bounds__(64) void chunk_merge_kernel(const float* __restrict
 }
 
 // The same where a row's states are of two launches, `own` of its sequence's positions and then those of the prefix that its sequence shares (a row of a sequence
-// outside members[0] .. members[prefixes] has none of these), and where the logarithms of the sums are asked for: sixteen lanes per row, eight dimensions each.
+// outside members[0] .. members[prefixes] has none of these), and where the logarithms of the sums are asked for.
 struct Joined {
     const float* part;
     const int32_t *starts, *members;
@@ -534,11 +543,13 @@ struct Joined {
     int batch, tokens, heads, prefixes, own, parts;
     Divisor per_head;
 };
-__global__ __launch_bounds__(64) void chunk_join_kernel(Joined a) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 4);
-    const int l = threadIdx.x & 15;
-    const int64_t token = divided((int)row, a.per_head);
-    const int head = (int)(row - token * a.heads);
+// QUARTERS 4: a wave per row, whose quarters take every fourth state, so that the states of a row that has many are on their way at once (two launches of 256 rows
+// with 34 states 27.0 -> 23.1 us); 1: four rows per wave, for many rows (139264 of three states: 41 us, with a wave each 86).
+template <int QUARTERS>
+__global__ __launch_bounds__(256) void chunk_join_kernel(Joined a) {
+    const int64_t row = (int64_t)blockIdx.x * (16 / QUARTERS) + (threadIdx.x / (16 * QUARTERS));
+    const int l = threadIdx.x & 15, quarter = QUARTERS == 4 ? threadIdx.x >> 4 & 3 : 0;
+    const int token = divided((int)row, a.per_head), head = (int)row - token * a.heads;
     if (token >= a.tokens || (a.starts && (token < a.starts[0] || token >= a.starts[a.batch]))) return;
     int from_token = 0, to_token = 0x7fffffff;             // tokens of sequences that have a prefix
     if (a.members) {
@@ -549,33 +560,44 @@ __global__ __launch_bounds__(64) void chunk_join_kernel(Joined a) {
         from_token = bound(0), to_token = bound(a.prefixes);
     }
     const int states = token >= from_token && token < to_token ? a.parts : a.own;
-    const f32x4* src = (const f32x4*)(a.part + row * a.parts * 132);
-    float M = kEmpty;
-    for (int s = l; s < states; s += 16) M = __builtin_fmaxf(M, src[s * 33][0]);
-#pragma unroll
-    for (int bit = 1; bit < 16; bit *= 2) M = __builtin_fmaxf(M, __shfl_xor(M, bit, 16));
-    float D = 0.f;
+    const f32x4* const src = (const f32x4*)(a.part + row * a.parts * 132);
+    constexpr int EACH = 4;                                // states of a quarter at a time
+    float M = kEmpty, D = 0.f;
     f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
-    for (int from = 0; from < states; from += 4) {
-        f32x4 head4[4], x4[4], y4[4];
+    for (int from = 0; from < states; from += QUARTERS * EACH) {
+        f32x4 head4[EACH], x4[EACH], y4[EACH];
+        float high = M;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f32x4* const at = src + (from + i < states ? from + i : states - 1) * 33;
+        for (int i = 0; i < EACH; ++i) {
+            const int s = from + QUARTERS * i + quarter;
+            const f32x4* const at = src + (s < states ? s : states - 1) * 33;
             head4[i] = at[0], x4[i] = at[1 + 2 * l], y4[i] = at[2 + 2 * l];
+            if (s >= states) head4[i][0] = kEmpty;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (from + i < states && head4[i][0] != kEmpty) {              // (an empty state may be its maximum and sum alone)
-                const float k = __builtin_amdgcn_exp2f(head4[i][0] - M);
-                D = __builtin_fmaf(head4[i][1], k, D);
+        for (int i = 0; i < EACH; ++i) high = __builtin_fmaxf(high, head4[i][0]);
+        const float mine = __builtin_amdgcn_exp2f(M - high);
+        M = high, D *= mine;
+        x *= mine, y *= mine;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = __builtin_fmaf(x4[i][j], k, x[j]), y[j] = __builtin_fmaf(y4[i][j], k, y[j]);
-            }
+        for (int i = 0; i < EACH; ++i) {
+            const bool is = head4[i][0] != kEmpty;         // (an empty state may be its maximum and sum alone: what lies behind them is anything)
+            const float keep = is ? __builtin_amdgcn_exp2f(head4[i][0] - high) : 0.f;
+            D += is ? head4[i][1] * keep : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] += is ? x4[i][j] * keep : 0.f, y[j] += is ? y4[i][j] * keep : 0.f;
         }
+    }
+    if (QUARTERS == 4) {
+        const float all = quarters_max(M), mine = __builtin_amdgcn_exp2f(M - all);
+        M = all, D = quarters_sum(D * mine);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = quarters_sum(x[j] * mine), y[j] = quarters_sum(y[j] * mine);
+        if (quarter) return;
     }
     const float inv = D == 0.f ? 0.f : 1.f / D;
     if (a.lse && l == 0) a.lse[row] = lse_of(M, D);
-    *((u32x4*)(a.o + token * a.o_stride + (int64_t)head * 128) + l) =
+    *((u32x4*)(a.o + (int64_t)token * a.o_stride + (int64_t)head * 128) + l) =
         u32x4{cvt_f16x2(x[0] * inv, x[1] * inv), cvt_f16x2(x[2] * inv, x[3] * inv), cvt_f16x2(y[0] * inv, y[1] * inv), cvt_f16x2(y[2] * inv, y[3] * inv)};
 }
 
@@ -849,18 +871,53 @@ struct Prefixes {
 struct SharedPlan {
     ChunkPlan own, prefix;
     int parts;                         // states per row; 1: none are written
+    bool paired;                       // both are tiles of 16 rows and one launch
     bool joined;                       // the sequences' own launch takes the prefixes' states in, so that it has none and there is no third launch
 };
 SharedPlan shared_plan(bool fp16, const ChunkCall& t, int64_t prefixes, int64_t max_prefix_len) {
-    SharedPlan p{plan_of(fp16, t), ChunkPlan{0, 0, 0, 0}, 0, false};
+    SharedPlan p{plan_of(fp16, t), ChunkPlan{0, 0, 0, 0}, 0, false, false};
     if (prefixes > 0) {
         p.prefix = prefix_plan(fp16, t.tokens, t.num_q_heads / t.num_heads, t.num_heads, prefixes, max_prefix_len);
         // (int4 pages, 64 sequences of up to 700 positions of their own, 64 on 8 heads: 16.7 us, with twelve waves 22.5)
         if (p.own.nb == 1 && p.own.nw == 12 && t.batch_size * t.num_heads >= 2 * qr_device().cus) p.own.nw = 4;
-        p.joined = p.own.splits == 1 && p.own.nb != 0;
+        p.paired = p.own.nb == 1 && p.prefix.nb == 1;
+        if (p.paired) {
+            // Each has a workgroup to a CU where two turns of its four waves' steps make as many.  (Prefix and own splits, microseconds cold: 8 sequences of 300 after 4000, 64 on
+            // 8 heads 8 and 2 15.2, 12 and 2 16.4, 3 and 1 18.0; one of 3000 after 300, 32 heads 2 and 8 14.2, 2 and 4 16.4, 2 and 16 15.3.  One launch instead of two:
+            // 4 of 100 after 1200, 32 heads 15.7 -> 12.5; fp16 pages, 30 of up to 333 behind three prefixes 85 -> 68.)
+            const int64_t cus = qr_device().cus, heads = t.num_heads, group = t.num_q_heads / t.num_heads;
+            auto cut = [&](int64_t groups, int64_t positions) {
+                const int64_t steps = (positions + 31) / 32, turns = (steps + 7) / 8;
+                int64_t s = groups < cus ? cus / groups : 1;
+                s = s < turns ? s : turns;
+                return (int)(s < 1 ? 1 : s > 32 ? 32 : s);
+            };
+            const int64_t tiles = prefixes == 1 ? (t.tokens * group + 15) / 16 : t.tokens * group / 16 + prefixes / 2;
+            p.own.nw = 4, p.own.splits = cut(t.batch_size * heads, t.max_seq_len < 0x3fffffff ? t.max_seq_len : 0x3fffffff);
+            p.prefix.splits = cut((tiles < prefixes ? prefixes : tiles) * heads, max_prefix_len < 0x3fffffff ? max_prefix_len : 0x3fffffff);
+            const int64_t most = (int64_t)(0xffffffffll / 256);                // (one launch)
+            if (t.batch_size * heads * p.own.splits + prefixes * heads * p.prefix.splits * p.prefix.tiles > most) p.paired = false;
+        }
+        p.joined = !p.paired && p.own.splits == 1 && p.own.nb != 0;
     }
     p.parts = (p.joined ? 0 : p.own.splits) + p.prefix.splits;
     return p;
+}
+
+int launch_pair(bool fp16, const SharedPlan& plan, Chunk prefix, Chunk own, hipStream_t st) {
+    prefix.tiles = plan.prefix.tiles, prefix.splits = plan.prefix.splits, prefix.per_split = divisor_of(plan.prefix.splits);
+    own.tiles = plan.own.tiles, own.splits = plan.own.splits, own.per_split = divisor_of(plan.own.splits), own.states = 1;
+    const int64_t first = (int64_t)prefix.c.batch_size * prefix.c.num_heads * prefix.splits * prefix.tiles;
+    const int64_t second = (int64_t)own.c.batch_size * own.c.num_heads * own.splits * own.tiles;
+    using Kernel = void (*)(Chunk, Chunk, Divisor, int);
+    const bool aligned = own.c.page_size % 16 == 0;
+    const Kernel kernel = fp16 ? (aligned ? chunk_rows_pair_kernel<true, true> : chunk_rows_pair_kernel<true, false>)
+                               : (aligned ? chunk_rows_pair_kernel<false, true> : chunk_rows_pair_kernel<false, false>);
+    const size_t lds = (size_t)4 * 16 * 33 * sizeof(f32x4);
+    const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, lds);
+    if (e != hipSuccess) return (int)e;
+    kernel<<<dim3((unsigned)(first + second)), dim3(256), lds, st>>>(prefix, own, divisor_of(own.c.page_size), (int)first);
+    return qr_launch_status();
 }
 
 int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
@@ -888,19 +945,21 @@ int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
         b.prefix = 1, b.per_place = kNoPlace;
         b.states = 1;
         b.part_at = plan.joined ? 0 : plan.own.splits;
-        rc = launch_chunk(fp16, plan.prefix, b, st);
+        rc = plan.paired ? launch_pair(fp16, plan, b, a, st) : launch_chunk(fp16, plan.prefix, b, st);
         if (rc != QR_OK) return rc;
         if (plan.joined) a.parts = 1, a.join = plan.parts, a.members = b.members, a.prefixes = (int)p.count;
     }
     a.states = a.parts > 1;
-    rc = launch_chunk(fp16, plan.own, a, st);
+    if (!plan.paired) rc = launch_chunk(fp16, plan.own, a, st);
     if (rc != QR_OK || a.parts == 1) return rc;
     Joined j;
     j.part = a.part, j.starts = a.starts, j.members = (const int32_t*)p.members;
     j.o = a.o, j.lse = lse, j.o_stride = t.o_stride;
     j.batch = (int)t.batch_size, j.tokens = (int)t.tokens, j.heads = t.num_q_heads, j.prefixes = (int)p.count, j.own = plan.own.splits, j.parts = plan.parts;
     j.per_head = divisor_of(t.num_q_heads);
-    chunk_join_kernel<<<dim3((unsigned)((t.tokens * t.num_q_heads + 3) / 4)), dim3(64), 0, st>>>(j);
+    const int64_t rows = t.tokens * t.num_q_heads;
+    if (rows <= 32 * (int64_t)qr_device().cus) chunk_join_kernel<4><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st>>>(j);
+    else chunk_join_kernel<1><<<dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st>>>(j);
     return qr_launch_status();
 }
 
