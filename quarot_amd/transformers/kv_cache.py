@@ -660,14 +660,14 @@ class _AttentionStub(object):
         self.disable_quant = disable_quant
         self.hadamard_dtype = hadamard_dtype
 
-    def forward(self, q, num_kv_heads, attention_kwargs, layer_idx, max_seq_len=0, cache=None, token=None, added=1, window=0, sinks=0):
+    def forward(self, q, num_kv_heads, attention_kwargs, layer_idx, max_seq_len=0, cache=None, token=None, added=1, window=0, sinks=0, weights=None):
         _, q_len, num_qo_heads, _ = q.shape
         assert q_len == added
-        if added > 1 or window or num_qo_heads != num_kv_heads:
+        if added > 1 or window or num_qo_heads != num_kv_heads or weights is not None:
             held = cache._pending.get(layer_idx) if cache is not None else None
             if held is not None and held[0] is token:
                 cache._flush(layer_idx)
-            return self._attend_chunk(q, attention_kwargs, layer_idx, max_seq_len, window, sinks)
+            return self._attend_chunk(q, attention_kwargs, layer_idx, max_seq_len, window, sinks, weights)
         o = workspace = held = None
         if cache is not None:
             # the step's new token, if the cache still holds it back for this call (see MultiLayerPagedKVCache4Bit.update; otherwise it
@@ -690,7 +690,7 @@ class _AttentionStub(object):
             cache._pending.pop(layer_idx, None)
         return o
 
-    def _attend_chunk(self, q, attention_kwargs, layer_idx, max_seq_len, window, sinks):
+    def _attend_chunk(self, q, attention_kwargs, layer_idx, max_seq_len, window, sinks, weights=None):
         batch_size, q_len, num_qo_heads, head_dim = q.shape
         q = q.reshape(batch_size * q_len, num_qo_heads, head_dim)
         fused = self.hadamard_dtype == torch.float16 and q.dtype == torch.float16
@@ -699,8 +699,12 @@ class _AttentionStub(object):
         attn_output = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         starts = torch.arange(batch_size + 1, device=q.device, dtype=torch.int32) * q_len if q_len > 1 else None
         attend = batch_chunk_f16 if self.disable_quant else batch_chunk_i4
-        attend(attn_output, q, **attention_kwargs, layer_idx=layer_idx, seqlen_indptr=starts, max_new_len=q_len, max_seq_len=max_seq_len,
-               window=window, sinks=sinks, q_hadamard=fused)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if weights is not None else None
+        how = {**attention_kwargs, "layer_idx": layer_idx, "seqlen_indptr": starts, "max_new_len": q_len, "max_seq_len": max_seq_len, "window": window, "sinks": sinks,
+               "q_hadamard": fused}
+        attend(attn_output, q, **how, lse=lse)
+        if weights is not None:
+            (accumulate_weights_f16 if self.disable_quant else accumulate_weights_i4)(weights, q, lse, **how)
         return attn_output.view(batch_size, q_len, num_qo_heads, head_dim)
 
     def _attend(self, q, attention_kwargs, layer_idx, max_seq_len, workspace, held):
@@ -737,12 +741,14 @@ class MultiLayerPagedKVCache4Bit:
     (hadamard_dtype, None to skip).  The callable takes any multiple of num_heads as query heads.  window > 0: it lets a token see the
     last `window` positions, its own among them, and the first `sinks`.  After a padded prompt (cache_kwargs["attention_mask"], as the
     reference takes it) turns of several tokens, or with a window, need the mask of all tokens so far, none of the new ones left out.
+    track_weights adds up what the callables' attention gives to every position (`weights`, fp32 [layers, batch, heads, positions]; `observe` does so for
+    queries of the prompt, whose attention is the caller's), and `evict` leaves the positions of the largest sums.
     The reference derives the class from transformers' Cache for the methods that base supplied in the
     version it pins (get_usable_length); they are defined here instead, so the class does not depend on the
     installed transformers version."""
 
     def __init__(self, batch_size, page_size, max_seq_len, device, n_layers, num_heads, head_dim, disable_quant=False,
-                 hadamard_dtype=torch.float16, window=0, sinks=0):
+                 hadamard_dtype=torch.float16, window=0, sinks=0, track_weights=False):
         if window < 0 or sinks < 0:
             raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
         self.window, self.sinks = int(window), int(sinks)
@@ -755,6 +761,7 @@ class MultiLayerPagedKVCache4Bit:
                                   dtype=torch.float16 if disable_quant else torch.uint8, device=device)
         self._scales = torch.empty((max_page_cnt * batch_size, n_layers, 2, num_heads, page_size, 2), dtype=torch.float16,
                                    device=device)
+        self.weights = torch.zeros((n_layers, batch_size, num_heads, max_page_cnt * page_size), dtype=torch.float32, device=device) if track_weights else None
         self._pending = {}      # layer -> (token, k, v, specs, hadamard): a decode step's new token, held for the attention call
         self._workspaces = {}           # _where() -> (heads, length, workspace), see _decode_workspace
         self._decode_ws = None          # the one made last, captures aside
@@ -904,13 +911,13 @@ class MultiLayerPagedKVCache4Bit:
                                       v=value_states.reshape(-1, num_heads, head_dim).contiguous(), seqlen_indptr=seqlens,
                                       layer_idx=layer_idx, hadamard=fused_had)
             return key_states, value_states
-        if added_length > 1 or self.window:
+        if added_length > 1 or self.window or self.weights is not None:
             starts = torch.arange(b_sz + 1, device=self.device, dtype=torch.int32) * added_length if added_length > 1 else None
             quantize_append_kv_i4(**specs, k=k_in.reshape(-1, num_heads, head_dim).contiguous(),
                                   v=value_states.reshape(-1, num_heads, head_dim).contiguous(), seqlen_indptr=starts, layer_idx=layer_idx,
                                   hadamard=fused_had)
             return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
-                                     max_seq_len=self.length, added=added_length, window=self.window, sinks=self.sinks)
+                                     max_seq_len=self.length, added=added_length, window=self.window, sinks=self.sinks, weights=self._layer_weights(layer_idx))
         k1, v1 = k_in.contiguous(), value_states.contiguous()
         if k1.dtype == torch.float16 and v1.dtype == torch.float16 and head_dim == 128:
             # held for the attention call, which quantises and stores the token itself
@@ -951,7 +958,47 @@ class MultiLayerPagedKVCache4Bit:
         else:
             append_kv_f16(**specs, k=k, v=v, k_param=param, v_param=param, layer_idx=layer_idx)
         return functools.partial(self._stub.forward, num_kv_heads=num_heads, attention_kwargs=specs, layer_idx=layer_idx,
-                                 max_seq_len=self.length, added=added_length, window=self.window, sinks=self.sinks)
+                                 max_seq_len=self.length, added=added_length, window=self.window, sinks=self.sinks, weights=self._layer_weights(layer_idx))
+
+    def _layer_weights(self, layer_idx):
+        return None if self.weights is None else self.weights[layer_idx]
+
+    def observe(self, query_states, layer_idx):
+        """Adds what the last tokens' attention gives to every position of a layer to `weights`: query_states [batch, n, heads, head_dim] of the last n tokens that
+        the layer holds, as the callables take them.  For the prompt, whose attention the caller runs (a callable adds its own tokens' by itself).
+        Returns the attention's outputs, shaped like query_states."""
+        self._check_tracked("observe", [layer_idx])
+        batch_size, n, _, head_dim = query_states.shape
+        if not (batch_size == self.batch_size and 1 <= n <= self.length):
+            raise ValueError(f"query_states must be of {self.batch_size} sequences and 1 to {self.length} tokens, got {list(query_states.shape)}")
+        return self._stub._attend_chunk(query_states, self.get_cache_specs_for_flash_infer(None), layer_idx, self.length, self.window, self.sinks,
+                                        self.weights[layer_idx])
+
+    def evict(self, keep, sinks=0, recent=0):
+        """Leaves `keep` positions of every layer, sequence and key head, which may differ between them: the first `sinks`, the last `recent`, and those of the largest
+        sums of weights between them (heavy_positions), moved to the front in their order (keep_positions_i4).  The cache then holds and
+        counts min(length, keep) tokens; keys keep the positions that they were rotated for.  To be called between turns, when all layers have the same tokens."""
+        self._check_tracked("evict", range(len(self._needs_init)))
+        keep, sinks, recent = int(keep), int(sinks), int(recent)
+        if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"keep must be positive, sinks and recent not negative and together no more than keep, got {keep}, {sinks} and {recent}")
+        if self.length <= keep:
+            return
+        specs = self.get_cache_specs_for_flash_infer(None)
+        lengths = torch.full((self.batch_size,), self.length, dtype=torch.int32, device=self._pages.device)
+        move = keep_positions_f16 if self.disable_quant else keep_positions_i4
+        for layer_idx, weights in enumerate(self.weights):
+            kept, _ = heavy_positions(weights, lengths, keep, sinks=sinks, recent=recent)
+            move(kept, **specs, layer_idx=layer_idx, weights=weights)
+        self.length = keep
+
+    def _check_tracked(self, what, layers):
+        if self.weights is None:
+            raise RuntimeError(f"{what}: the cache was made without track_weights")
+        if self._padded:
+            raise NotImplementedError("Current implementation does not support weights of padded prompts")
+        if any(self._needs_init[layer] for layer in layers):
+            raise RuntimeError(f"{what}: a layer has no tokens yet")
 
     def get_cache_specs_for_flash_infer(self, attention_mask):
         """Page tables of the current state (kv_cache.py:253-275): page i of sequence b is page number
