@@ -469,18 +469,19 @@ int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_strid
 
 /*
  * Attention of new tokens of sequences that begin with the same text, whose pages are held once (no counterpart in the reference):
- *   the first prefixes of positions lie on page lists of their own, prefix_indptr int32 [prefixes + 1], prefix_indices,
- *   prefix_last_page_offset int32 [prefixes], in the same pool of pages; prefix p is that of the sequences prefix_sequences[p] ..
- *   prefix_sequences[p + 1] - 1 (int32 [prefixes + 1], not descending; NULL, with one prefix: of all sequences).  The page tables of the
- *   sequences hold what follows.  Every new token sees all of its sequence's prefix and, as qr_batch_chunk_i4, its own positions up to its own.
- *   A sequence of no prefix (before the first bound, behind the last) sees its own positions only.
+ *   these prefixes lie on page lists of their own, prefix_indptr int32 [prefixes + 1], prefix_indices, prefix_last_page_offset int32
+ *   [prefixes], in the same pool of pages; prefix p is that of the sequences prefix_sequences[p] .. prefix_sequences[p + 1] - 1 (int32
+ *   [prefixes + 1], not descending; NULL, with one prefix: of all sequences).  The sequences' page tables hold what follows.  A new token sees all
+ *   of its sequence's prefix and, as in qr_batch_chunk_i4, the sequence's own positions up to its own; a sequence of no prefix (before the
+ *   first bound, behind the last) its own positions only.
  * Everything else as qr_batch_chunk_i4 / qr_batch_chunk_f16, except:
- *   lse_or_null fp32 [tokens, num_q_heads]: the natural logarithm of every row's sum of exponentials of its logits (over 1 / sqrt(128) included),
- *   -inf for a row that sees nothing; of the weights as they were rounded, so within 2^-11 of the exact one.  Rows that are left stay as they are.
+ *   lse_or_null fp32 [tokens, num_q_heads]: the natural logarithm of every row's sum of exponentials of its logits (the factor 1 / sqrt(128)
+ *   included), -inf for a row that sees nothing; of the weights as they were rounded, so within 2^-11 of the exact one.  Rows that o leaves
+ *   as they are are left here too.
  *   prefixes == 0: the sequences' own positions only (qr_batch_chunk with lse); window > 0 only then (QR_E_SHAPE).
  *   max_prefix_len: the largest number of a prefix's positions if the caller knows it, else 0.
- *   With prefixes a workspace of qr_batch_shared_workspace_bytes bytes is required (QR_E_WORKSPACE): a row's partial states, 528 bytes
- *   each.
+ *   With prefixes tokens * num_q_heads is below 2^28, and a workspace of qr_batch_shared_workspace_bytes bytes (the same arguments, max_new_len 1 where
+ *   seqlen_indptr is NULL) is required (QR_E_WORKSPACE): a row's partial states, 528 bytes each.
  */
 size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                        int64_t max_seq_len, int64_t window, int64_t sinks, int64_t prefixes, int64_t max_prefix_len);
@@ -516,11 +517,13 @@ int qr_batch_shared_f16(void* o, int64_t o_stride, void* lse_or_null, const void
  * qr_heavy_positions: of every sequence b and key head h that holds more than `keep` of lengths[b] positions the first `sinks`, the last
  *   `recent` (sinks + recent <= keep) and between them those of the largest weights, of equal ones the lowest positions (NaN counts below all
  *   numbers): kept int32 [batch_size, num_heads, keep], ascending; of shorter sequences all of them, then -1.  lengths int32 (below 0: 0,
- *   above `capacity`: capacity), new_lengths int32 [batch_size] = min(length, keep).  batch_size * num_heads below 2^22, capacity and keep below 2^30.
+ *   above `capacity`: capacity), new_lengths int32 [batch_size] = min(length, keep).  batch_size * num_heads below 2^22, capacity and keep below 2^30.  Up to
+ *   32768 positions of `capacity` a list is kept in registers; longer ones are read five times.
  * qr_keep_positions_i4 / _f16: entry i of kept int32 [batch_size, num_heads, keep] (ascending where it is not negative) goes to position i of its
  *   sequence, in place, for one layer: keys, values, their parameters, and weights if they are given, whose other entries up to the sequence's
  *   length (as the page tables have it, before) become zero.  Entries that are no position of the sequence, or lie on a page number outside
- *   [0, num_pages), are skipped.  Sequences of one prefix's pages must not be among those that move.
+ *   [0, num_pages), are skipped; what lies behind the moved entries stays as it was.  Pages that other sequences read too (a prefix's) must not be among
+ *   those that move.  batch_size * num_heads below 2^21.
  */
 size_t qr_accumulate_weights_workspace_bytes(int fp16_pages, int64_t capacity, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size,
                                              int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks);

@@ -543,8 +543,8 @@ struct Joined {
     int batch, tokens, heads, prefixes, own, parts;
     Divisor per_head;
 };
-// QUARTERS 4: a wave per row, whose quarters take every fourth state, so that the states of a row that has many are on their way at once (two launches of 256 rows
-// with 34 states 27.0 -> 23.1 us); 1: four rows per wave, for many rows (139264 of three states: 41 us, with a wave each 86).
+// QUARTERS 4: a wave per row, whose quarters take every fourth state, so that the states of a row that has many are on their way at once (256 rows
+// of 34 states: a call of 27.0 us takes 23.1); 1: four rows per wave, for many rows (139264 of three states: 41 us, with a wave each 86).
 template <int QUARTERS>
 __global__ __launch_bounds__(256) void chunk_join_kernel(Joined a) {
     const int64_t row = (int64_t)blockIdx.x * (16 / QUARTERS) + (threadIdx.x / (16 * QUARTERS));
@@ -926,6 +926,7 @@ int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
     if (p.count < 0 || p.count > 0x7fffffff || p.max_len < 0 || (p.count > 0 && t.window > 0) || (p.count > 1 && !p.members)) return QR_E_SHAPE;
     if (p.count > 0 && t.batch_size > 0 && (!p.indptr || !p.indices || !p.last_page_offset)) return QR_E_NULL;
     if (t.tokens == 0 || t.batch_size == 0) return rc;
+    if (p.count > 0 && t.tokens * t.num_q_heads > 0xfffffff) return QR_E_SHAPE;            // (rows that one launch joins; their states are 142 GB)
     if ((uintptr_t)lse & 3) return QR_E_ALIGN;
     SharedPlan plan = shared_plan(fp16, t, p.count, p.max_len);
     const bool states = plan.parts > 1 || p.count > 0;

@@ -258,7 +258,7 @@ int keep_positions(bool fp16, const void* kept, int64_t keep, void* kv_data, voi
     if (rc != QR_OK) return rc;
     if (keep < 0 || keep > 0x3fffffff || capacity < 0) return QR_E_SHAPE;
     if (batch_size == 0) return QR_OK;
-    if (batch_size * num_heads > 0x3fffff) return QR_E_SHAPE;              // (a launch has fewer than 2^32 threads)
+    if (batch_size > 0x1fffff || batch_size * num_heads > 0x1fffff) return QR_E_SHAPE;      // (a launch has fewer than 2^32 threads)
     if (keep > 0 && !kept) return QR_E_NULL;
     if (((uintptr_t)kept & 3) || ((uintptr_t)weights & 3)) return QR_E_ALIGN;
     Keep a;

@@ -30,7 +30,7 @@ def shared_args(**changes):
     (NULL, {"o": None}), (NULL, {"q": None}), (NULL, {"data": None}), (NULL, {"indptr": None}), (NULL, {"p_indptr": None}), (NULL, {"p_indices": None}), (NULL, {"p_last": None}),
     (DTYPE, {"had": 2}), (SHAPE, {"tokens": -1}), (SHAPE, {"q_heads": 7}), (SHAPE, {"window": -1}), (SHAPE, {"window": 5}), (SHAPE, {"new": -1}), (SHAPE, {"prefix": -1}),
     (SHAPE, {"prefixes": -1}), (SHAPE, {"prefixes": 2}), (SHAPE, {"prefixes": 1 << 31, "members": AT}), (SHAPE, {"starts": None}), (SHAPE, {"q_stride": 1016}), (SHAPE, {"layer": 2}),
-    (SHAPE, {"tokens": 1 << 27}), (ALIGN, {"q": ctypes.c_void_p(4104)}), (ALIGN, {"o_stride": 1026}), (ALIGN, {"lse": ctypes.c_void_p(4098)}), (WORKSPACE, {}),
+    (SHAPE, {"tokens": 1 << 27}), (SHAPE, {"tokens": 1 << 25}), (ALIGN, {"q": ctypes.c_void_p(4104)}), (ALIGN, {"o_stride": 1026}), (ALIGN, {"lse": ctypes.c_void_p(4098)}), (WORKSPACE, {}),
     (WORKSPACE, {"workspace": ctypes.c_void_p(4104), "bytes": 1 << 30}), (WORKSPACE, {"workspace": AT, "bytes": 1000})])
 def test_shared_argument_errors(lib, entry, code, change):
     assert getattr(lib, entry)(*shared_args(**change)) == code
@@ -85,7 +85,7 @@ def heavy_args(**changes):
 @pytest.mark.parametrize("code,change", [
     (NULL, {"weights": None}), (NULL, {"lengths": None}), (NULL, {"kept": None}), (NULL, {"left": None}), (SHAPE, {"batch": -1}), (SHAPE, {"heads": 0}), (SHAPE, {"capacity": -1}),
     (SHAPE, {"capacity": 1 << 40}), (SHAPE, {"keep": -1}), (SHAPE, {"keep": 1 << 40}), (SHAPE, {"sinks": -1}), (SHAPE, {"recent": -1}), (SHAPE, {"sinks": 41}), (SHAPE, {"recent": (1 << 63) - 1}),
-    (SHAPE, {"batch": 1 << 22}), (ALIGN, {"weights": ctypes.c_void_p(4098)}), (ALIGN, {"kept": ctypes.c_void_p(4098)})])
+    (SHAPE, {"batch": 1 << 22}), (SHAPE, {"batch": 1 << 21}), (ALIGN, {"weights": ctypes.c_void_p(4098)}), (ALIGN, {"kept": ctypes.c_void_p(4098)})])
 def test_heavy_argument_errors(lib, code, change):
     assert lib.qr_heavy_positions(*heavy_args(**change)) == code
 
@@ -98,7 +98,7 @@ def keep_args(**changes):
 @pytest.mark.parametrize("entry", ["qr_keep_positions_i4", "qr_keep_positions_f16"])
 @pytest.mark.parametrize("code,change", [
     (NULL, {"kept": None}), (NULL, {"data": None}), (NULL, {"param": None}), (NULL, {"indices": None}), (SHAPE, {"keep": -1}), (SHAPE, {"keep": 1 << 31}), (SHAPE, {"capacity": -1}),
-    (SHAPE, {"layer": 2}), (SHAPE, {"batch": 1 << 22}), (ALIGN, {"kept": ctypes.c_void_p(4098)}), (ALIGN, {"weights": ctypes.c_void_p(4098)})])
+    (SHAPE, {"layer": 2}), (SHAPE, {"batch": 1 << 20}), (SHAPE, {"batch": 1 << 30, "heads": 1 << 30}), (ALIGN, {"kept": ctypes.c_void_p(4098)}), (ALIGN, {"weights": ctypes.c_void_p(4098)})])
 def test_keep_argument_errors(lib, entry, code, change):
     assert getattr(lib, entry)(*keep_args(**change)) == code
 
