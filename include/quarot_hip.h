@@ -509,7 +509,7 @@ int qr_batch_shared_f16(void* o, int64_t o_stride, void* lse_or_null, const void
  *   exp( q[t, g, :] . k[j, h] / sqrt(128) - lse[t, g] ), over the positions j that t sees: what the attention of qr_batch_chunk_* or
  *   qr_batch_shared_* with that lse gives to position j.  weights fp32 [batch_size, num_heads, capacity]; positions from `capacity` on are left
  *   out.  q, q_stride, q_had_mode, seqlen_indptr_or_null, tokens, the cache, max_new_len, max_seq_len, window and sinks as qr_batch_chunk_i4;
- *   lse fp32 [tokens, num_q_heads] (a row whose lse is -inf gives nothing).  Everything in 32 bits, int4 codes as they are; no atomics: the
+ *   lse fp32 [tokens, num_q_heads] (a row whose lse is -inf gives nothing, whatever its q holds).  Everything in 32 bits, int4 codes as they are; no atomics: the
  *   same inputs give the same bits.  A NaN or infinity of a key reaches that position alone, one of a query the positions that it sees.
  *   Positions on page numbers outside [0, num_pages) get nothing.  With a workspace of qr_accumulate_weights_workspace_bytes bytes (the same
  *   arguments, max_new_len 1 where seqlen_indptr is NULL; 16-byte aligned, contents arbitrary: the queries in another order, 9/8 of their size, and sums of
@@ -517,13 +517,14 @@ int qr_batch_shared_f16(void* o, int64_t o_stride, void* lse_or_null, const void
  * qr_heavy_positions: of every sequence b and key head h that holds more than `keep` of lengths[b] positions the first `sinks`, the last
  *   `recent` (sinks + recent <= keep) and between them those of the largest weights, of equal ones the lowest positions (NaN counts below all
  *   numbers): kept int32 [batch_size, num_heads, keep], ascending; of shorter sequences all of them, then -1.  lengths int32 (below 0: 0,
- *   above `capacity`: capacity), new_lengths int32 [batch_size] = min(length, keep).  batch_size * num_heads below 2^22, capacity and keep below 2^30.  Up to
+ *   above `capacity`: capacity), new_lengths int32 [batch_size] = min(length, keep), not where lengths is
+ *   (QR_E_UNSUPPORTED).  batch_size * num_heads below 2^22, capacity and keep below 2^30.  Up to
  *   32768 positions of `capacity` a list is kept in registers; longer ones are read five times.
  * qr_keep_positions_i4 / _f16: entry i of kept int32 [batch_size, num_heads, keep] (ascending where it is not negative) goes to position i of its
  *   sequence, in place, for one layer: keys, values, their parameters, and weights if they are given, whose other entries up to the sequence's
  *   length (as the page tables have it, before) become zero.  Entries that are no position of the sequence, or lie on a page number outside
- *   [0, num_pages), are skipped; what lies behind the moved entries stays as it was.  Pages that other sequences read too (a prefix's) must not be among
- *   those that move.  batch_size * num_heads below 2^21.
+ *   [0, num_pages), are skipped; what lies behind the moved entries stays as it was.  Pages that other sequences read too (a prefix's), or that
+ *   a sequence lists twice, must not be among those that move.  batch_size * num_heads below 2^21.
  */
 size_t qr_accumulate_weights_workspace_bytes(int fp16_pages, int64_t capacity, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size,
                                              int64_t max_new_len, int64_t max_seq_len, int64_t window, int64_t sinks);

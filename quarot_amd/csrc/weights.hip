@@ -400,9 +400,14 @@ __global__ __launch_bounds__(256) void weights_queries_kernel(Weights a) {
             sum += (float)p[0] + (float)p[1];
         }
         const u32x2 both = both_halves<32>(as_u32(sum));
-        const float s = (as_f32(both.x) + as_f32(both.y)) * -(kLog2e * kScale), s1 = top(s), s2 = top(s - s1), s3 = s - s1 - s2;
+        const float all = as_f32(both.x) + as_f32(both.y);
         float m = lse * -kLog2e;
         m = row >= rows || __builtin_fabsf(m) > 3e38f ? kNothing : m != m ? __builtin_nanf("") : m;
+        // (a row that gives nothing may hold anything; its infinities and NaN would get into the sums)
+        const bool nothing = m == kNothing && !(__builtin_fabsf(all) < 3e38f);
+        const float s = nothing ? 0.f : all * -(kLog2e * kScale), s1 = top(s), s2 = top(s - s1), s3 = s - s1 - s2;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = nothing ? u32x4{0, 0, 0, 0} : w[i];
         const float m1 = top(m), m2 = top(m - m1), m3 = m - m1 - m2;
         uint8_t* const to = a.units + ((int64_t)h * a.all_units + first_unit(a, mine.start, b) + unit) * kUnitBytes + lane * 16;
 #pragma unroll

@@ -535,3 +535,88 @@ def test_refusals():
             move(**kw)
     empty, left = kv.heavy_positions(w[:0], n[:0], 4)
     assert tuple(empty.shape) == (0, 2, 4) and tuple(left.shape) == (0,)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("news", [[3, 9], [1, 1], [2, 8], [70, 200], [33, 400]])
+def test_rows_that_give_nothing_may_hold_anything(news, f16):
+    """A row whose logarithm is -inf gives nothing, whatever its queries are (rows that a caller leaves out): the bits of a call with zeros there."""
+    lens = [90, 500]
+    specs, q, starts = make(15, 16, lens, news, 2, 8, f16)
+    lse = logarithms(specs, q, lens, news)
+    out = [0, news[0], sum(news) - 1]
+    call = kv.accumulate_weights_f16 if f16 else kv.accumulate_weights_i4
+    sums = []
+    for value in (0.0, math.nan, math.inf):
+        row, of = q.clone(), lse.clone()
+        row[out, 3:11], of[out, 3:11] = value, -math.inf
+        row[out, 3:11, ::2] *= -1
+        got = torch.zeros(2, 2, 510, device=DEV)
+        call(got, row, of, **specs, layer_idx=1, seqlen_indptr=starts)
+        sums.append(got)
+    assert bool((sums[0] != 0).any()) and torch.equal(sums[1], sums[0]) and torch.equal(sums[2], sums[0])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_turn_with_eviction_captured_and_replayed(new, f16):
+    """Attention, its weights, which stay and their move in one graph, replayed with eager work between: the bits of as many eager turns.  The lengths and page tables are
+    those from before every turn, so each moves what the last has left."""
+    lens, news = [700, 300], [new, new]
+    specs, q, starts = make(16, 16, lens, news, 2, 4, f16)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    suffix = "_f16" if f16 else "_i4"
+    chunk, accumulate, move = (getattr(kv, name + suffix) for name in ("batch_chunk", "accumulate_weights", "keep_positions"))
+
+    def state():
+        return {**specs, "kv_data": specs["kv_data"].clone(), "kv_param": specs["kv_param"].clone()}, torch.zeros(2, 2, 700, device=DEV), torch.zeros_like(q), torch.zeros(q.shape[:2], device=DEV)
+
+    def turn(specs, sums, o, lse):
+        how = dict(**specs, layer_idx=1, seqlen_indptr=starts, max_new_len=new, max_seq_len=700)
+        chunk(o, q, **how, lse=lse)
+        accumulate(sums, q, lse, **how)
+        kept, _ = kv.heavy_positions(sums, lengths, 200, sinks=4, recent=50)
+        move(kept, **specs, layer_idx=1, weights=sums)
+
+    eager, captured, warm = state(), state(), state()
+    turn(*warm)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        turn(*captured)
+    for _ in range(4):
+        graph.replay()
+        turn(*eager)
+        torch.cuda.synchronize()
+        for have, want in zip((captured[0]["kv_data"], captured[0]["kv_param"], *captured[1:]), (eager[0]["kv_data"], eager[0]["kv_param"], *eager[1:])):
+            assert torch.equal(bits(have), bits(want))
+
+
+def test_evictions_on_two_streams_at_once():
+    """Two caches' turns under way together, each on a stream of its own: the bits of one after the other."""
+    lens, news = [2000, 900], [30, 5]
+    cases = []
+    for seed in (17, 18):
+        specs, q, starts = make(seed, 16, lens, news, 2, 4)
+        cases.append((specs, q, starts, logarithms(specs, q, lens, news)))
+    lengths = torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+    def turn(specs, q, starts, lse):
+        specs = {**specs, "kv_data": specs["kv_data"].clone(), "kv_param": specs["kv_param"].clone()}
+        sums = torch.zeros(2, 2, 2000, device=DEV)
+        kv.accumulate_weights_i4(sums, q, lse, **specs, layer_idx=1, seqlen_indptr=starts)
+        kept, left = kv.heavy_positions(sums, lengths, 500, sinks=4, recent=50)
+        kv.keep_positions_i4(kept, **specs, layer_idx=1, weights=sums)
+        return specs["kv_data"], specs["kv_param"], sums, kept, left
+
+    alone = [turn(*case) for case in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        together = []
+        for stream, case in zip(streams, cases):
+            with torch.cuda.stream(stream):
+                together.append(turn(*case))
+        torch.cuda.synchronize()
+        for got, want in zip(together, alone):
+            assert all(torch.equal(bits(a), bits(b)) for a, b in zip(got, want))
