@@ -286,6 +286,9 @@ extern "C" int qr_heavy_positions(const void* weights, int64_t capacity, const v
     if (batch_size > 0x3fffff || batch_size * num_heads > 0x3fffff) return QR_E_SHAPE;      // (a launch has fewer than 2^32 threads)
     if ((!weights && capacity > 0) || !lengths || (!kept && keep > 0) || !new_lengths) return QR_E_NULL;
     if (((uintptr_t)weights & 3) || ((uintptr_t)lengths & 3) || ((uintptr_t)kept & 3) || ((uintptr_t)new_lengths & 3)) return QR_E_ALIGN;
+    // (a workgroup per key head reads a sequence's length, and one of them writes the new one)
+    const uintptr_t from = (uintptr_t)lengths, to = (uintptr_t)new_lengths, bytes = (uintptr_t)batch_size * 4;
+    if (from < to + bytes && to < from + bytes) return QR_E_UNSUPPORTED;
     Heavy a;
     a.sums = (const float*)weights, a.lengths = (const int32_t*)lengths;
     a.kept = (int32_t*)kept, a.left = (int32_t*)new_lengths;

@@ -5,7 +5,7 @@ import pytest
 
 from quarot_amd import _lib
 
-NULL, SHAPE, ALIGN, DTYPE, WORKSPACE = -1, -2, -4, -5, -6
+NULL, SHAPE, UNSUPPORTED, ALIGN, DTYPE, WORKSPACE = -1, -2, -3, -4, -5, -6
 AT = ctypes.c_void_p(4096)              # never dereferenced
 
 
@@ -107,3 +107,10 @@ def test_nothing_stays_of_nothing(lib):
     assert lib.qr_heavy_positions(*heavy_args(batch=0)) == 0
     for entry in ("qr_keep_positions_i4", "qr_keep_positions_f16"):
         assert getattr(lib, entry)(*keep_args(batch=0)) == 0
+
+
+def test_new_lengths_apart_from_the_lengths(lib):
+    """A workgroup per key head reads a sequence's length, and one of them writes its new one."""
+    assert lib.qr_heavy_positions(*heavy_args()) == UNSUPPORTED
+    assert lib.qr_heavy_positions(*heavy_args(left=ctypes.c_void_p(AT.value + 8))) == UNSUPPORTED
+    assert lib.qr_heavy_positions(*heavy_args(lengths=ctypes.c_void_p(AT.value + 8))) == UNSUPPORTED
