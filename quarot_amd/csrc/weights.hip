@@ -84,6 +84,9 @@ __device__ __forceinline__ void hadamard_row(u32x4 (&w)[4], int lane) {
 // A wave takes 64 positions of a (sequence, key head) at a time, lane by lane for their places, and all rows in tiles of 16: lane (n, g) holds quarter g of the
 // keys of positions n, 16 + n, 32 + n and 48 + n.  While it works on them the next 64 positions' keys and sums are under way, and the page numbers of those behind.
 // Of 16 rows and fewer the queries stay in registers, of up to 64 in LDS, ready for the products (a wave makes one tile of them; more are made for every block).
+// One row and 32 heads after 3000: 5.0 us, a launch and one wave's chain of tables, pages, keys; 32 x one of 4001, 64 on 8 heads: 18.0 us, 4.4 TB/s of a copy's 5.2
+// (every lane's loads of two blocks under way; half of the lanes without rows: 22.0); fp16 pages, 5 x up to 37 in a window of 1500, 40 heads: 15.6 us, 3.5 TB/s, 200 chains
+// of unequal length.
 constexpr int kWaves = 4;
 template <bool F16>
 struct RowTile {                       // 16 rows: queries as the products take them; slope, logarithm (base 2, negative) and position of four of them
@@ -348,6 +351,10 @@ __global__ __launch_bounds__(64 * kWaves, F16 ? (ROWS == 4 ? 3 : 2) : (ROWS < 16
 // queries out as the matrix instructions take them, so that a unit goes from memory to LDS as it lies, without registers, and is read without
 // bank conflicts: eight operands of 1 KB (lane (n, h): dimensions 64 h + 8 i .. of row n) and a ninth, the line: what a logit has besides the codes' product,
 // zero sum(q) and the row's logarithm, as a product of bf16 pieces that hold 24 bits together.
+// 2048 after 14336, 64 on 8 heads: 522 - 557 us on several cards, 925 - 990 TFLOP/s, with the line's products a ninth more, of a large library product's 1185; 14 of them the
+// first launch.  The matrix unit is busy for half of the cycles, the vector unit (a product's exponentials, 32 rows by 64 positions) for the other half, and the clock is down to
+// 2.0 GHz.  Slower: three workgroups to a CU with stages half as large (599 against 522), products and exponentials of two units laid between each other (581), a wave's
+// products or its exponentials at a higher priority (3 %).
 constexpr int kUnitBytes = 9 * 1024, kStageUnits = 4;
 constexpr float kNothing = -3e38f;                         // minus the logarithm of a row that gives nothing
 
