@@ -44,6 +44,8 @@ __device__ __forceinline__ int of_waves_before(const int* counts, int lane, int 
 __device__ __forceinline__ int lanes_before(uint64_t mask) { return __builtin_amdgcn_mbcnt_hi((u32)(mask >> 32), __builtin_amdgcn_mbcnt_lo((u32)mask, 0)); }
 
 // HOLD > 0: a lane keeps its sums, at most that many, in registers; 0: they are read for every digit
+// (They are left behind eight at a time where the list ends: to pass over the rest one by one cost 14 us instead of 7.8 at 4000 positions of a capacity of 32768, a branch at every
+// one 12 - 20 % where all are there.)
 template <int HOLD>
 __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a) {
     // four counters per bin, a lane's by its number: half of a wave's sums have one of a few dozen leading digits, and would wait for each other
@@ -68,7 +70,10 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
     if (HOLD > 0) {
         float v[HOLD > 0 ? HOLD : 1];
 #pragma unroll
-        for (int j = 0; j < HOLD; ++j) v[j] = from + 64 * j + lane < to ? sums[from + 64 * j + lane] : 0.f;
+        for (int j = 0; j < HOLD; ++j) {
+            if (j % 8 == 0 && from + 64 * j >= to) break;
+            v[j] = from + 64 * j + lane < to ? sums[from + 64 * j + lane] : 0.f;
+        }
 #pragma unroll
         for (int j = 0; j < HOLD; ++j) mine[j] = order_of(v[j]);
     }
@@ -78,8 +83,10 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
     auto go_through = [&](auto&& visit) {                  // visit(position, its sum's order, whether it is one); all lanes of a wave together
         if (HOLD > 0) {
 #pragma unroll
-            for (int j = 0; j < HOLD; ++j)
-                if (from + 64 * j < to) visit(from + 64 * j + lane, mine[j], from + 64 * j + lane < to);
+            for (int j = 0; j < HOLD; ++j) {
+                if (j % 8 == 0 && from + 64 * j >= to) break;
+                visit(from + 64 * j + lane, mine[j], from + 64 * j + lane < to);         // (of a part of eight the others are none)
+            }
         } else {
             for (int at = from; at < to; at += 64 * 8) {
                 float v[8];
@@ -120,12 +127,13 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
         if (above + found[2] == want) break;               // (all that share these digits stay)
     }
     const int equal = need - (int)above;                   // of those with these digits that many stay, the first ones
-    if (HOLD > 0 && HOLD <= 16 && (u32)equal == found[2]) {
+    if (HOLD > 0 && (u32)equal == found[2]) {
         // all of them: one comparison for each, kept in scalar registers between the count and the list
         uint64_t stay[HOLD > 0 ? HOLD : 1];
         int count_here = 0;
 #pragma unroll
         for (int j = 0; j < HOLD; ++j) {
+            if (j % 8 == 0 && from + 64 * j >= to) break;
             stay[j] = __builtin_amdgcn_ballot_w64(from + 64 * j + lane < to && mine[j] >> shift >= prefix);
             count_here += __popcll(stay[j]);
         }
@@ -134,6 +142,7 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
         int32_t* to_list = kept + a.sinks + of_waves_before(after[0], lane, wave);
 #pragma unroll
         for (int j = 0; j < HOLD; ++j) {
+            if (j % 8 == 0 && from + 64 * j >= to) break;
             if (stay[j] >> lane & 1) to_list[lanes_before(stay[j])] = a.sinks + from + 64 * j + lane;
             to_list += __popcll(stay[j]);
         }
@@ -301,7 +310,10 @@ extern "C" int qr_heavy_positions(const void* weights, int64_t capacity, const v
     a.capacity = capacity;
     a.heads = num_heads, a.keep = (int)keep, a.sinks = (int)sinks, a.recent = (int)recent;
     const dim3 grid((unsigned)(batch_size * num_heads)), threads(kHeavyThreads);
+    // As few registers as the lists can need (microseconds of 8 lists of 4000 5.2, with eight 6.1, with sixteen 6.7; of 8000 6.5, with sixteen 7.1; of 16000 10.2, with 32 10.1 - 12 where there
+    // are more lists); longer ones are read from memory for every digit (60000 52, in 64 registers of which some spill 40, but 1024 lists 174 and 202).
     if (capacity <= 4 * kHeavyThreads) heavy_positions_kernel<4><<<grid, threads, 0, (hipStream_t)stream>>>(a);
+    else if (capacity <= 8 * kHeavyThreads) heavy_positions_kernel<8><<<grid, threads, 0, (hipStream_t)stream>>>(a);
     else if (capacity <= 16 * kHeavyThreads) heavy_positions_kernel<16><<<grid, threads, 0, (hipStream_t)stream>>>(a);
     else if (capacity <= 32 * kHeavyThreads) heavy_positions_kernel<32><<<grid, threads, 0, (hipStream_t)stream>>>(a);
     else heavy_positions_kernel<0><<<grid, threads, 0, (hipStream_t)stream>>>(a);
