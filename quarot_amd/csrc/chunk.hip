@@ -12,6 +12,8 @@
 // Only p_j f_j is rounded to fp16, the matrix instruction's type; f_j lies in [1, 2), so weights of large and of tiny scales have the same range.
 // The rounded number over f_j is the weight in every sum, so a rounding (2^-11 at most) changes a weight and nothing else.  Maxima, sums and
 // outputs are held in 32 bits.
+#include <type_traits>
+
 #include "qr_chunk.h"
 
 namespace {
@@ -35,9 +37,13 @@ struct There {
     bool all;                          // all of them are, in every lane
 };
 
+// SHARED: a Chunk, else ChunkRows alone (what a Chunk's rows need before the first load and behind the last step is 0.45 of the 7.4 us of a launch of a few steps, its arguments alone
+// 0.15).
+template <bool SHARED>
+using Launch = std::conditional_t<SHARED, Chunk, ChunkRows>;
 // ALIGNED: pages of a multiple of 16 positions, so that each half of a step lies in one page.
-template <int NB, int NW, bool F16, bool ALIGNED>
-__device__ __forceinline__ void attend_rows(const Chunk& a, const Divisor& pages, const int group_number) {
+template <int NB, int NW, bool F16, bool ALIGNED, bool SHARED>
+__device__ __forceinline__ void attend_rows(const Launch<SHARED>& a, const Divisor& pages, const int group_number) {
     extern __shared__ __attribute__((aligned(16))) f32x4 st4[];            // per wave and row: maximum, sum, -, -, 128 outputs
     const PagedKV& c = a.c;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -54,10 +60,12 @@ __device__ __forceinline__ void attend_rows(const Chunk& a, const Divisor& pages
     const int64_t head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + h) * c.page_size;
     const int64_t kv_slots = (int64_t)c.num_heads * c.page_size;
     constexpr uint32_t VEC = F16 ? 256 : 64;               // bytes of a vector
+    Divisor per_place = a.per_group;
+    if constexpr (SHARED) per_place = a.per_place;
 
     for (int tile = first_tile; tile * 16 * NB < rows; tile += a.tiles) {
         const int r0 = tile * 16 * NB, r1 = r0 + 16 * NB < rows ? r0 + 16 * NB : rows;
-        const int lowest = first_place + divided(r0, a.per_place), highest = first_place + divided(r1 - 1, a.per_place);
+        const int lowest = first_place + divided(r0, per_place), highest = first_place + divided(r1 - 1, per_place);
         const Steps steps = steps_of<5>(a, lowest, highest);
         const int stride = NW * a.splits;
 
@@ -158,7 +166,7 @@ __device__ __forceinline__ void attend_rows(const Chunk& a, const Divisor& pages
             const int r = r0 + 16 * nb + n;
             const bool in = r < rows;
             const int t = divided(in ? r : r0, a.per_group), head = h * a.group + (in ? r : r0) - t * a.group;
-            place[nb] = in ? first_place + divided(r, a.per_place) : -1;
+            place[nb] = in ? first_place + divided(r, per_place) : -1;
             const u32x4* src = (const u32x4*)(a.q + (int64_t)(start + t) * a.q_stride + (int64_t)head * 128) + (F16 ? g : 4 * g);
             u32x4 w[4];
 #pragma unroll
@@ -434,44 +442,51 @@ __device__ __forceinline__ void attend_rows(const Chunk& a, const Divisor& pages
                         for (int j = 0; j < 4; ++j) O[i][j] = __builtin_fmaf(src[1 + PER * l + i][j], keep, O[i][j]);
                 }
                 const int t = divided(r, a.per_group), head = h * a.group + r - t * a.group;
-                if (!a.states) {
-                    if (a.join > 0 && (!a.members || (a.first + b >= a.members[0] && a.first + b < a.members[a.prefixes]))) {
-                        // the states of the prefix that the row's sequence shares
-                        const f32x4* const src = (const f32x4*)a.part + ((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.join * 33;
-                        for (int from = 0; from < a.join; from += 4) {
-                            f32x4 state[4], x[4][PER];
+                bool finished = a.splits == 1;
+                if constexpr (SHARED) finished = !a.states;
+                if (finished) {
+                    if constexpr (SHARED) {
+                        if (a.join > 0 && (!a.members || (a.first + b >= a.members[0] && a.first + b < a.members[a.prefixes]))) {
+                            // the states of the prefix that the row's sequence shares
+                            const f32x4* const src = (const f32x4*)a.part + ((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.join * 33;
+                            for (int from = 0; from < a.join; from += 4) {
+                                f32x4 state[4], x[4][PER];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const f32x4* const at = src + (from + i < a.join ? from + i : a.join - 1) * 33;
-                                state[i] = at[0];
+                                for (int i = 0; i < 4; ++i) {
+                                    const f32x4* const at = src + (from + i < a.join ? from + i : a.join - 1) * 33;
+                                    state[i] = at[0];
 #pragma unroll
-                                for (int j = 0; j < PER; ++j) x[i][j] = at[1 + PER * l + j];
-                            }
-                            float high = M;
+                                    for (int j = 0; j < PER; ++j) x[i][j] = at[1 + PER * l + j];
+                                }
+                                float high = M;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) high = __builtin_fmaxf(high, state[i][0]);
-                            const float mine = __builtin_amdgcn_exp2f(M - high);
-                            M = high, D *= mine;
+                                for (int i = 0; i < 4; ++i) high = __builtin_fmaxf(high, state[i][0]);
+                                const float mine = __builtin_amdgcn_exp2f(M - high);
+                                M = high, D *= mine;
 #pragma unroll
-                            for (int j = 0; j < PER; ++j) O[j] *= mine;
+                                for (int j = 0; j < PER; ++j) O[j] *= mine;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                // (an empty state may be its maximum and sum alone: what lies behind them is anything)
-                                const bool is = from + i < a.join && state[i][0] != kEmpty;
-                                const float keep = is ? __builtin_amdgcn_exp2f(state[i][0] - high) : 0.f;
-                                D += is ? state[i][1] * keep : 0.f;
+                                for (int i = 0; i < 4; ++i) {
+                                    // (an empty state may be its maximum and sum alone: what lies behind them is anything)
+                                    const bool is = from + i < a.join && state[i][0] != kEmpty;
+                                    const float keep = is ? __builtin_amdgcn_exp2f(state[i][0] - high) : 0.f;
+                                    D += is ? state[i][1] * keep : 0.f;
 #pragma unroll
-                                for (int j = 0; j < PER; ++j) O[j] += is ? x[i][j] * keep : f32x4{0.f, 0.f, 0.f, 0.f};
+                                    for (int j = 0; j < PER; ++j) O[j] += is ? x[i][j] * keep : f32x4{0.f, 0.f, 0.f, 0.f};
+                                }
                             }
                         }
                     }
                     const float inv = D == 0.f ? 0.f : 1.f / D;                 // (a row that sees nothing is zero)
-                    if (a.lse && l == 0) a.lse[(int64_t)(start + t) * (c.num_heads * a.group) + head] = lse_of(M, D);
+                    if constexpr (SHARED)
+                        if (a.lse && l == 0) a.lse[(int64_t)(start + t) * (c.num_heads * a.group) + head] = lse_of(M, D);
                     u32x2* const dst = (u32x2*)(a.o + (int64_t)(start + t) * a.o_stride + (int64_t)head * 128) + PER * l;
 #pragma unroll
                     for (int i = 0; i < PER; ++i) dst[i] = u32x2{cvt_f16x2(O[i][0] * inv, O[i][1] * inv), cvt_f16x2(O[i][2] * inv, O[i][3] * inv)};
                 } else {
-                    float* dst = a.part + (((int64_t)(start + t) * (c.num_heads * a.group) + head) * a.parts + a.part_at + split) * 132;
+                    int parts = a.splits, at = split;
+                    if constexpr (SHARED) parts = a.parts, at = a.part_at + split;
+                    float* dst = a.part + (((int64_t)(start + t) * (c.num_heads * a.group) + head) * parts + at) * 132;
                     if (l == 0) dst[0] = M, dst[1] = D;
 #pragma unroll
                     for (int i = 0; i < PER; ++i) *((f32x4*)dst + 1 + PER * l + i) = O[i];
@@ -481,13 +496,13 @@ __device__ __forceinline__ void attend_rows(const Chunk& a, const Divisor& pages
     }
 }
 
-template <int NB, int NW, bool F16, bool ALIGNED>
-__global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_kernel(Chunk a, Divisor pages) { attend_rows<NB, NW, F16, ALIGNED>(a, pages, blockIdx.x); }
+template <int NB, int NW, bool F16, bool ALIGNED, bool SHARED>
+__global__ __launch_bounds__(64 * NW, NB == 2 || F16 ? 2 : 3) void chunk_rows_kernel(Launch<SHARED> a, Divisor pages) { attend_rows<NB, NW, F16, ALIGNED, SHARED>(a, pages, blockIdx.x); }
 // Two launches in one: the first `groups` workgroups are a's, the others b's
 template <bool F16, bool ALIGNED>
 __global__ __launch_bounds__(256, F16 ? 2 : 3) void chunk_rows_pair_kernel(Chunk a, Chunk b, Divisor pages, int groups) {
     const bool first = (int)blockIdx.x < groups;
-    attend_rows<1, 4, F16, ALIGNED>(first ? a : b, pages, first ? blockIdx.x : blockIdx.x - groups);
+    attend_rows<1, 4, F16, ALIGNED, true>(first ? a : b, pages, first ? blockIdx.x : blockIdx.x - groups);
 }
 
 // The partial states of every row -> its output: sixteen lanes per row, eight dimensions each.  The states' maxima and sums are read by a lane each (at most 32),
@@ -683,11 +698,11 @@ ChunkPlan chunk_plan(bool fp16, int64_t tokens, int group, int num_heads, int64_
     return p;
 }
 
-template <bool F16, bool ALIGNED>
+template <bool F16, bool ALIGNED, bool SHARED>
 int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t groups, hipStream_t st) {
-    using Kernel = void (*)(Chunk, Divisor);
-    const Kernel kernel = plan.nb == 2 ? (plan.nw == 8 ? chunk_rows_kernel<2, 8, F16, ALIGNED> : chunk_rows_kernel<2, 4, F16, ALIGNED>)
-                                       : (F16 || plan.nw == 4 ? chunk_rows_kernel<1, 4, F16, ALIGNED> : chunk_rows_kernel<1, F16 ? 4 : 12, F16, ALIGNED>);
+    using Kernel = void (*)(Launch<SHARED>, Divisor);
+    const Kernel kernel = plan.nb == 2 ? (plan.nw == 8 ? chunk_rows_kernel<2, 8, F16, ALIGNED, SHARED> : chunk_rows_kernel<2, 4, F16, ALIGNED, SHARED>)
+                                       : (F16 || plan.nw == 4 ? chunk_rows_kernel<1, 4, F16, ALIGNED, SHARED> : chunk_rows_kernel<1, F16 ? 4 : 12, F16, ALIGNED, SHARED>);
     const size_t lds = (size_t)plan.nw * 16 * 33 * sizeof(f32x4);
     const hipError_t e = qr_allow_dynamic_lds((const void*)kernel, lds);
     if (e != hipSuccess) return (int)e;
@@ -697,6 +712,7 @@ int launch_rows(const ChunkPlan& plan, const Chunk& a, Divisor pages, int64_t gr
 
 // The launches of one set of page tables: a's sequences (or prefixes) as the plan cuts them.  A launch has fewer than 2^32 threads: fewer tiles at a time where hints
 // are missing (a workgroup goes on to the next one behind them), then fewer sequences.
+template <bool SHARED>
 int launch_chunk(bool fp16, const ChunkPlan& plan, Chunk a, hipStream_t st) {
     const int64_t batch_size = a.c.batch_size, num_q_heads = (int64_t)a.c.num_heads * a.group;
     a.tiles = plan.tiles;
@@ -722,8 +738,8 @@ int launch_chunk(bool fp16, const ChunkPlan& plan, Chunk a, hipStream_t st) {
         }
         const int64_t groups = a.dealt ? a.dealt : some.c.batch_size * wide * a.tiles;
         rc = plan.nb == 0 ? qr_internal_chunk_tiles(fp16, some, pages, groups, st)
-             : fp16       ? (aligned ? launch_rows<true, true>(plan, some, pages, groups, st) : launch_rows<true, false>(plan, some, pages, groups, st))
-                          : (aligned ? launch_rows<false, true>(plan, some, pages, groups, st) : launch_rows<false, false>(plan, some, pages, groups, st));
+             : fp16       ? (aligned ? launch_rows<true, true, SHARED>(plan, some, pages, groups, st) : launch_rows<true, false, SHARED>(plan, some, pages, groups, st))
+                          : (aligned ? launch_rows<false, true, SHARED>(plan, some, pages, groups, st) : launch_rows<false, false, SHARED>(plan, some, pages, groups, st));
     }
     return rc;
 }
@@ -794,7 +810,7 @@ int batch_chunk(bool fp16, const ChunkCall& t) {
     Chunk a = chunk_of(t);
     a.parts = plan.splits, a.states = plan.splits > 1;
     hipStream_t st = (hipStream_t)t.stream;
-    const int lrc = launch_chunk(fp16, plan, a, st);
+    const int lrc = launch_chunk<false>(fp16, plan, a, st);
     if (lrc != QR_OK || plan.splits == 1) return lrc;
     chunk_merge_kernel<<<dim3((unsigned)((t.tokens * t.num_q_heads + 3) / 4)), dim3(64), 0, st>>>(a.part, a.starts, (int)t.batch_size, (int)t.tokens, t.num_q_heads,
                                                                                                   divisor_of(t.num_q_heads), plan.splits, a.o, t.o_stride);
@@ -950,12 +966,12 @@ int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
         b.prefix = 1, b.per_place = kNoPlace;
         b.states = 1;
         b.part_at = plan.joined ? 0 : plan.own.splits;
-        rc = plan.paired ? launch_pair(fp16, plan, b, a, st) : launch_chunk(fp16, plan.prefix, b, st);
+        rc = plan.paired ? launch_pair(fp16, plan, b, a, st) : launch_chunk<true>(fp16, plan.prefix, b, st);
         if (rc != QR_OK) return rc;
         if (plan.joined) a.parts = 1, a.join = plan.parts, a.members = b.members, a.prefixes = (int)p.count;
     }
     a.states = a.parts > 1;
-    if (!plan.paired) rc = launch_chunk(fp16, plan.own, a, st);
+    if (!plan.paired) rc = launch_chunk<true>(fp16, plan.own, a, st);
     if (rc != QR_OK || a.parts == 1) return rc;
     Joined j;
     j.part = a.part, j.starts = a.starts, j.members = (const int32_t*)p.members;

@@ -13,7 +13,7 @@ static inline Divisor divisor_of(int64_t d) {
 }
 
 // What a launch works on.  Rows of a (sequence, key head): row r is new token r / group, query head kv_head * group + r % group.
-struct Chunk {
+struct ChunkRows {
     PagedKV c;
     const f16* q;
     f16* o;
@@ -23,6 +23,9 @@ struct Chunk {
     int tokens, group, tiles, splits, window, sinks;      // window 0: none
     int q_had;
     Divisor per_group, per_split, per_head;     // of `group`, `splits`, the key heads
+};
+// The same of a prefix that several sequences share, or of sequences that have one, or where the logarithms of the sums are asked for.
+struct Chunk : ChunkRows {
     // A row's position is the first new token's + divided(row, per_place): per_group's token by token; kNoPlace where all rows see all positions, which is a prefix
     // that several sequences share.  Its "sequences" are the prefixes then: the rows of number b are the tokens of sequences members[b] .. members[b + 1] - 1
     // (nullptr: of all `sequences`).
@@ -154,6 +157,14 @@ __device__ __forceinline__ u32x4 scaled_codes_slow(u32 w, u32 w0, u32 w1) {
 struct Fresh {
     int start, count, all;
 };
+__device__ __forceinline__ Fresh fresh_of(const ChunkRows& a, int b) {
+    if (!a.starts) return Fresh{b, 1, 1};
+    int start = a.starts[b];
+    const int end = a.starts[b + 1];
+    start = start < 0 ? 0 : start;
+    const int stop = end > a.tokens ? a.tokens : end;
+    return Fresh{start, stop > start ? stop - start : 0, end > start ? end - start : 0};
+}
 __device__ __forceinline__ Fresh fresh_of(const Chunk& a, int b) {
     if (a.prefix) {
         auto sequence = [&](int i) { const int s = a.members[i]; return s < 0 ? 0 : s > a.sequences ? a.sequences : s; };
@@ -163,12 +174,7 @@ __device__ __forceinline__ Fresh fresh_of(const Chunk& a, int b) {
         stop = stop > a.tokens ? a.tokens : stop;
         return Fresh{start, stop > start ? stop - start : 0, 1};               // (all rows at the prefix's last position)
     }
-    if (!a.starts) return Fresh{b, 1, 1};
-    int start = a.starts[b];
-    const int end = a.starts[b + 1];
-    start = start < 0 ? 0 : start;
-    const int stop = end > a.tokens ? a.tokens : end;
-    return Fresh{start, stop > start ? stop - start : 0, end > start ? end - start : 0};
+    return fresh_of((const ChunkRows&)a, b);
 }
 
 __device__ __forceinline__ int lanes_sum(int v) {          // over the wave
@@ -183,8 +189,8 @@ __device__ __forceinline__ int lanes_sum(int v) {          // over the wave
 // Work item `number` of a head: a sequence and one of its tiles of PER rows, last tiles (most positions) first; false: there is none.  Items without rows come
 // last: between others they leave whole shader engines idle, since workgroups are handed out to them in turn (8 sequences of 2048, 1792 .. 256 tokens, 64 on 8
 // heads: 528 us with them, 369 without).  Of more than 64 sequences the tiles are not counted.
-template <int PER>
-__device__ __forceinline__ bool item_of(const Chunk& a, int number, int& b, int& tile) {
+template <int PER, class Launch>
+__device__ __forceinline__ bool item_of(const Launch& a, int number, int& b, int& tile) {
     const int batch = a.c.batch_size;
     if (a.tiles == 1 || batch > 64) {
         tile = a.tiles == 1 ? 0 : a.tiles - 1 - number / batch;
