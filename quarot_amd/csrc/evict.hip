@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kHeavyThreads) void heavy_positions_kernel(Heavy a)
 // the batches to come.
 // Eight vectors' pieces a thread are under way at a time, page numbers and slots come from a list in LDS made for 2048 entries at once (looked up by every thread
 // between its loads: 196 us where it takes 132).  1024 of 2048, 32 heads, int4: 7.0 us; fp16 pages, 32 x 2000 of up to 8001, 8 heads: 132 us, 4.1 TB/s read and written of a copy's
-// 5.2: loads and stores take turns in a workgroup, two of which share a CU.
+// 5.2: loads and stores take turns in a workgroup, three of which share a CU (two, with 94 registers for the next part of the list: 163).
 struct Keep {
     PagedKV c;
     const int32_t* kept;
