@@ -480,8 +480,9 @@ int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_strid
  *   as they are are left here too.
  *   prefixes == 0: the sequences' own positions only (qr_batch_chunk with lse); window > 0 only then (QR_E_SHAPE).
  *   max_prefix_len: the largest number of a prefix's positions if the caller knows it, else 0.
- *   With prefixes tokens * num_q_heads is below 2^28, and a workspace of qr_batch_shared_workspace_bytes bytes (the same arguments, max_new_len 1 where
+ *   With prefixes tokens * num_q_heads is at most 2^28 - 16, and a workspace of qr_batch_shared_workspace_bytes bytes (the same arguments, max_new_len 1 where
  *   seqlen_indptr is NULL) is required (QR_E_WORKSPACE): a row's partial states, 528 bytes each.
+ *   Calls that share a workspace must not overlap.
  */
 size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,
                                        int64_t max_seq_len, int64_t window, int64_t sinks, int64_t prefixes, int64_t max_prefix_len);
@@ -513,7 +514,7 @@ int qr_batch_shared_f16(void* o, int64_t o_stride, void* lse_or_null, const void
  *   same inputs give the same bits.  A NaN or infinity of a key reaches that position alone, one of a query the positions that it sees.
  *   Positions on page numbers outside [0, num_pages) get nothing.  With a workspace of qr_accumulate_weights_workspace_bytes bytes (the same
  *   arguments, max_new_len 1 where seqlen_indptr is NULL; 16-byte aligned, contents arbitrary: the queries in another order, 9/8 of their size, and sums of
- *   parts of the rows) many rows are faster.
+ *   parts of the rows) many rows are faster.  Calls that share a workspace, or add to the same weights, must not overlap.
  * qr_heavy_positions: of every sequence b and key head h that holds more than `keep` of lengths[b] positions the first `sinks`, the last
  *   `recent` (sinks + recent <= keep) and between them those of the largest weights, of equal ones the lowest positions (NaN counts below all
  *   numbers): kept int32 [batch_size, num_heads, keep], ascending; of shorter sequences all of them, then -1.  lengths int32 (below 0: 0,

@@ -946,7 +946,7 @@ int batch_shared(bool fp16, const ChunkCall& t, const Prefixes& p, float* lse) {
     if (p.count < 0 || p.count > 0x7fffffff || p.max_len < 0 || (p.count > 0 && t.window > 0) || (p.count > 1 && !p.members)) return QR_E_SHAPE;
     if (p.count > 0 && t.batch_size > 0 && (!p.indptr || !p.indices || !p.last_page_offset)) return QR_E_NULL;
     if (t.tokens == 0 || t.batch_size == 0) return rc;
-    if (p.count > 0 && t.tokens * t.num_q_heads > 0xfffffff) return QR_E_SHAPE;            // (rows that one launch joins; their states are 142 GB)
+    if (p.count > 0 && t.tokens * t.num_q_heads > 0xffffff0) return QR_E_SHAPE;            // (rows that one launch joins, 16 in 256 threads; their states are 142 GB)
     if ((uintptr_t)lse & 3) return QR_E_ALIGN;
     SharedPlan plan = shared_plan(fp16, t, p.count, p.max_len);
     const bool states = plan.parts > 1 || p.count > 0;

@@ -114,3 +114,11 @@ def test_new_lengths_apart_from_the_lengths(lib):
     assert lib.qr_heavy_positions(*heavy_args()) == UNSUPPORTED
     assert lib.qr_heavy_positions(*heavy_args(left=ctypes.c_void_p(AT.value + 8))) == UNSUPPORTED
     assert lib.qr_heavy_positions(*heavy_args(lengths=ctypes.c_void_p(AT.value + 8))) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("entry", ["qr_batch_shared_i4", "qr_batch_shared_f16"])
+def test_rows_that_one_launch_joins(lib, entry):
+    """16 rows take 256 threads of the launch that joins, which has fewer than 2^32."""
+    many = dict(q_heads=1, heads=1, o_stride=128, q_stride=128)
+    assert getattr(lib, entry)(*shared_args(tokens=(1 << 28) - 15, **many)) == SHAPE
+    assert getattr(lib, entry)(*shared_args(tokens=(1 << 28) - 16, **many)) == WORKSPACE           # (none was given)
