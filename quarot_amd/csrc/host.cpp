@@ -647,6 +647,7 @@ PyObject* shared(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         bound < 0 || prefix_bound < 0 || window < 0 || sinks < 0 || (lse && (lse->dim() != 2 || lse->size(0) != tokens || lse->size(1) != heads)))
         return none();
     if (!seq) fresh_bound = 1;
+    if (prefixes > 0 && prefix_bound == 0) prefix_bound = table[1]->numel() * c.page_size / prefixes;      // (what the page list has room for)
     const size_t need = qr_batch_shared_workspace_bytes(fp16_pages ? 1 : 0, tokens, (int)heads, c.heads, c.batch, fresh_bound, bound, window, sinks, prefixes, prefix_bound);
     const bool kept = need && ws && (size_t)ws->numel() >= need;
     at::Tensor own;

@@ -395,6 +395,8 @@ def _shared(fn, f16, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_o
     with _lib.on_device(dev):
         if seqlen_indptr is None:
             max_new_len = 1
+        if prefixes and not max_prefix_len:
+            max_prefix_len = prefix_indices.shape[0] * page_size // prefixes
         ws_bytes = _lib.lib().qr_batch_shared_workspace_bytes(1 if f16 else 0, tokens, q_heads, heads, batch, max_new_len, max_seq_len, window, sinks, prefixes,
                                                               max_prefix_len)
         ws = _scratch(workspace, ws_bytes, dev)
@@ -445,8 +447,8 @@ def batch_shared_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
 
         o[t, h] = softmax(q[t, h] . K^T / sqrt(128)) . V   over the prefix and the sequence's own positions up to the token's own
 
-    A sequence outside prefix_sequences' bounds has no prefix.  max_prefix_len (optional): the largest number of positions of a prefix; sizes the
-    launch like max_seq_len, which counts the sequences' own positions.  There is no window.  The rest as batch_chunk_i4."""
+    A sequence outside prefix_sequences' bounds has no prefix.  max_prefix_len: the largest number of positions of a prefix (0: what
+    prefix_indices has room for, on average); sizes the launch like max_seq_len, which counts the sequences' own positions.  There is no window.  The rest as batch_chunk_i4."""
     _prefix_needed("batch_shared_i4", prefix_indptr)
     _shared("batch_shared_i4", False, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices,
             prefix_last_page_offset, prefix_sequences, seqlen_indptr, max_new_len, max_seq_len, max_prefix_len, 0, 0, q_hadamard, lse, workspace)

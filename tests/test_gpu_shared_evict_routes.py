@@ -78,3 +78,19 @@ def test_on_another_stream_than_the_current_one(route):
     stream.synchronize()
     for a, b in zip(first, everything(False, False)):
         assert torch.equal(a, b)
+
+
+def test_a_prefix_of_unknown_length_is_cut_by_its_page_list(monkeypatch):
+    """Without a largest length the launch is sized for what the page list has room for, on both routes: the bits of a call that gives that number."""
+    specs, prefix, q, starts = make_shared(2, 16, [3000], None, [90, 33], [1, 1], 2, 4)
+    room = prefix["prefix_indices"].shape[0] * 16
+
+    def run(**hint):
+        o = torch.empty(q.shape, dtype=torch.float16, device=DEV)
+        kv.batch_shared_i4(o, q, **specs, layer_idx=1, **prefix, seqlen_indptr=starts, **hint)
+        return o
+
+    native = run()
+    assert torch.equal(native, run(max_prefix_len=room))
+    monkeypatch.setattr(_lib.host, "shared", lambda *a: None)
+    assert torch.equal(native, run()) and torch.equal(native, run(max_prefix_len=room))
