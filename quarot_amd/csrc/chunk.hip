@@ -849,18 +849,14 @@ ChunkPlan prefix_plan(bool fp16, int64_t tokens, int group, int num_heads, int64
             if (least < 0.f || time < least) least = time, p = ChunkPlan{nb, nw, (int)(tiles > 4096 ? 4096 : tiles), s};
         }
     };
-    // One prefix: the steps of all its tiles in equal shares, five steps at least, one to a CU at most.  A tile has the states of its shares, which is the same number for all
-    // of them where the shares' number is a multiple of the tiles' or the other way round, else one more than its shares' length makes at most.
+    // One prefix: the steps of all its tiles in equal shares (qr_deal.h).
     auto deal = [&](float each, float around, float part, float each_state) {
         int64_t tiles = (rows + 255) / 256;
         tiles = tiles > 4096 ? 4096 : tiles;               // (rows are fewer than 2^30; what lies behind is left to the splits of whole tiles)
         if (tiles * 256 < rows) return consider(0, 4, 256, cus, 64, each, around, part, each_state);
         const int64_t all = tiles * num_heads, steps = (seen + 63) / 64 < 1 ? 1 : (seen + 63) / 64;
-        int64_t shares = seen > 0 && all * steps < 5 * cus ? all * steps / 5 : cus;
-        if (shares < 1) shares = 1;
-        if (shares < all && 8 * shares > 7 * all) shares = all;                // (a little more than one tile each)
-        int64_t states = shares % all == 0 ? shares / all : all % shares == 0 ? 1 : shares / all + 2;
-        if (states > 32) states = 32, shares = 32 * all < shares ? 32 * all : shares;
+        const DealtCut cut = dealt_cut(all, seen > 0 ? steps : 0, cus);
+        const int64_t shares = cut.shares, states = cut.states;
         const float full = (float)shares / (float)cus;
         const float time = (float)(all * steps + shares - 1) / (float)shares * each * (part + (1.f - part) * (full < 1.f ? full : 1.f)) +
                            (float)((all + shares - 1) / shares + (all % shares && shares % all ? 1 : 0)) * around + (float)(rows * num_heads) * (float)states * each_state;

@@ -129,13 +129,10 @@ __device__ __forceinline__ void attend_tiles(const Chunk& a, const Divisor& page
         if (DEALT) {
             const int eighths = a.dealt >> 3, share = (int)blockIdx.x < eighths * 8 ? (int)(blockIdx.x & 7) * eighths + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
             const int tile_steps = len > 0 ? ((len - 1) >> 6) + 1 : 1;         // (of an empty prefix: one that shows nothing)
-            const int64_t all = (int64_t)c.num_heads * a.tiles * tile_steps, at = all * share / a.dealt + done, end = all * (share + 1) / a.dealt;
-            if (at >= end) break;
-            const int64_t number = at / tile_steps;
-            first_step = (int)(at - number * tile_steps);
-            end_step = end - at < tile_steps - first_step ? first_step + (int)(end - at) : tile_steps;
-            split = share - (int)(((number * tile_steps + 1) * a.dealt - 1) / all);          // (the share that has the tile's first step is state 0)
-            head = (int)(number / a.tiles), r_tile = ((int)number - head * a.tiles) * kRows;
+            DealtPiece piece;
+            if (!dealt_piece((int64_t)c.num_heads * a.tiles, tile_steps, a.dealt, share, done, piece)) break;
+            first_step = piece.first, end_step = piece.end, split = piece.state;
+            head = piece.tile / a.tiles, r_tile = (piece.tile - head * a.tiles) * kRows;
             head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;
             done += end_step - first_step;
             if (r_tile >= rows) continue;

@@ -1,6 +1,7 @@
 // Shared by the kernels of attention of new tokens over the paged cache (chunk.hip: few rows, chunk_tiles.hip: many).
 #pragma once
 #include "qr_paged.h"
+#include "qr_deal.h"
 
 // n / d for n below 2^30: umulhi(4 n, inverse) >> shift
 struct Divisor {
