@@ -127,10 +127,12 @@ __device__ __forceinline__ void attend_tiles(const Chunk& a, const Divisor& page
     for (int r_tile = tile * kRows;; r_tile += a.tiles * kRows) {
         int first_step = 0, end_step = 0;
         if (DEALT) {
-            const int eighths = a.dealt >> 3, share = (int)blockIdx.x < eighths * 8 ? (int)(blockIdx.x & 7) * eighths + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
             const int tile_steps = len > 0 ? ((len - 1) >> 6) + 1 : 1;         // (of an empty prefix: one that shows nothing)
+            const int64_t tiles = (int64_t)c.num_heads * a.tiles;
+            const int shares = dealt_shares(tiles, tile_steps, a.dealt), eighths = shares >> 3;
+            const int share = (int)blockIdx.x < eighths * 8 ? (int)(blockIdx.x & 7) * eighths + (int)(blockIdx.x >> 3) : (int)blockIdx.x;
             DealtPiece piece;
-            if (!dealt_piece((int64_t)c.num_heads * a.tiles, tile_steps, a.dealt, share, done, piece)) break;
+            if (!dealt_piece(tiles, tile_steps, shares, share, done, piece)) break;
             first_step = piece.first, end_step = piece.end, split = piece.state;
             head = piece.tile / a.tiles, r_tile = (piece.tile - head * a.tiles) * kRows;
             head_slots = ((int64_t)c.layer_idx * 2 * c.num_heads + head) * c.page_size;

@@ -25,14 +25,21 @@ __host__ __device__ __forceinline__ DealtCut dealt_cut(int64_t tiles, int64_t st
     return DealtCut{shares, states};
 }
 
+// The shares that tiles of `tile_steps` steps are cut into by workgroups for `cut` of them: none is empty, so that a tile's states are 0, 1, ... without a gap whatever length the
+// launch was cut for.  (One to a step where there are fewer steps than workgroups; a tile has that many states then, fewer than the cut's.)
+__host__ __device__ __forceinline__ int dealt_shares(int64_t tiles, int tile_steps, int cut) {
+    const int64_t all = tiles * tile_steps;
+    return all < cut ? (int)all : cut;
+}
+
 // The piece of share number `share` that begins `done` steps behind its first one: steps first .. end - 1 of a tile, whose state `state` they are; false: the share ends
-// there.
+// there.  A workgroup whose number is not below `shares` has none.
 struct DealtPiece {
     int tile, first, end, state;
 };
 __host__ __device__ __forceinline__ bool dealt_piece(int64_t tiles, int tile_steps, int shares, int share, int done, DealtPiece& p) {
     const int64_t all = tiles * tile_steps, at = all * share / shares + done, end = all * (share + 1) / shares;
-    if (at >= end) return false;
+    if (share >= shares || at >= end) return false;
     const int64_t tile = at / tile_steps;
     p.tile = (int)tile;
     p.first = (int)(at - tile * tile_steps);

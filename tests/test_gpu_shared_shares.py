@@ -48,3 +48,24 @@ def check_hints(f16, page_size, prefix_len, lens, news, heads, group, hints):
 def test_31_shares_and_a_fraction_to_a_tile(prefix_len, tokens, heads, group):
     """Fp16 pages, eight tiles: 251 to 254 shares of five steps would touch 33 states of a tile."""
     check_hints(True, 16, prefix_len, [1 + i % 5 for i in range(tokens)], [1] * tokens, heads, group, [prefix_len, 0])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("page_size,prefix_len,hints,tokens,new,heads,group", [
+    (16, 1000, [16384, 1 << 40], 32, 1, 8, 8), (16, 640, [8000, 100000], 64, 1, 8, 8), (7, 70, [1500, 20000], 300, 1, 1, 2), (64, 129, [30000], 20, 40, 2, 8),
+    (128, 64, [16384], 40, 1, 8, 8), (16, 1, [5000], 40, 1, 8, 8)])
+def test_prefixes_far_shorter_than_their_hint(page_size, prefix_len, hints, tokens, new, heads, group, f16):
+    """Fewer steps than the launch has workgroups: a tile's states have no gaps, which the workspace's contents would fill."""
+    check_hints(f16, page_size, prefix_len, [new + i % 5 for i in range(tokens)], [new] * tokens, heads, group, [*hints, prefix_len, 0])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_a_page_list_with_room_for_more(f16):
+    """Without a hint the launch is cut for what the page list has room for, here eight times the prefix."""
+    prefix_len, lens, news = 700, [3] * 40, [1] * 40
+    specs, prefix, q, _ = make_shared(4, 16, [prefix_len], None, lens, news, 8, 8, f16)
+    (want, tol), _ = definition(specs, prefix, q, [prefix_len], None, lens, news, 1)
+    more = {**prefix, "prefix_indices": torch.cat([prefix["prefix_indices"], prefix["prefix_indices"][:1].repeat(8 * 44)])}
+    o = torch.empty(q.shape, dtype=torch.float16, device=DEV)
+    (kv.batch_shared_f16 if f16 else kv.batch_shared_i4)(o, q, **specs, layer_idx=1, **more, workspace=torch.full((1 << 28,), 255, dtype=torch.uint8, device=DEV))
+    assert bool(((o.double() - want).abs() <= tol).all())

@@ -20,9 +20,10 @@ extern "C" int walk(int64_t tiles, int64_t hinted, int steps, int64_t cus, int* 
     if (cut.states < 1 || cut.states > kMostStates || cut.shares < 1) return 1;
     std::vector<int64_t> next(tiles, 0);                   // steps that have been done, from the tile's first on
     std::vector<uint64_t> written(tiles, 0);
+    const int shares = dealt_shares(tiles, steps, (int)cut.shares);
     for (int share = 0; share < cut.shares; ++share) {
         DealtPiece p;
-        for (int done = 0; dealt_piece(tiles, steps, (int)cut.shares, share, done, p); done += p.end - p.first) {
+        for (int done = 0; dealt_piece(tiles, steps, shares, share, done, p); done += p.end - p.first) {
             if (p.tile < 0 || p.tile >= tiles || p.first < 0 || p.end <= p.first || p.end > steps) return 2;
             if (p.first != next[p.tile]) return 3;
             next[p.tile] = p.end;
@@ -31,8 +32,10 @@ extern "C" int walk(int64_t tiles, int64_t hinted, int steps, int64_t cus, int* 
             written[p.tile] |= (uint64_t)1 << p.state;
         }
     }
-    for (int64_t t = 0; t < tiles; ++t)
+    for (int64_t t = 0; t < tiles; ++t) {
         if (next[t] != steps) return 6;
+        if (written[t] & (written[t] + 1)) return 7;       // (those behind the last one are marked empty, a state between them would be what the workspace held)
+    }
     return 0;
 }
 // the first fault over all tiles and hinted steps up to those given and prefixes as long as hinted, and shorter and longer: {fault, tiles, hinted, steps}
@@ -72,6 +75,13 @@ def test_a_tile_has_no_more_states_than_its_rows(shares, tiles, hinted):
     states = ctypes.c_int()
     for steps in (hinted, 100, 1000, 2 * hinted):
         assert shares.walk(tiles, hinted, steps, 256, ctypes.byref(states)) == 0 and states.value <= 32, steps
+
+
+@pytest.mark.parametrize("tiles,hinted,steps", [(8, 256, 16), (16, 125, 10), (1, 20, 2), (8, 0, 3), (64, 0, 2), (3, 1 << 20, 5)])
+def test_a_prefix_shorter_than_its_hint_leaves_no_state_out(shares, tiles, hinted, steps):
+    """More workgroups than steps: those without any may not have states between a tile's others."""
+    states = ctypes.c_int()
+    assert shares.walk(tiles, hinted, steps, 256, ctypes.byref(states)) == 0
 
 
 @pytest.mark.parametrize("cus,most_tiles,most_steps", [(256, 66, 260), (256, 300, 24), (304, 24, 260), (64, 70, 170), (1, 20, 200)])
