@@ -744,7 +744,9 @@ class MultiLayerPagedKVCache4Bit:
     last `window` positions, its own among them, and the first `sinks`.  After a padded prompt (cache_kwargs["attention_mask"], as the
     reference takes it) turns of several tokens, or with a window, need the mask of all tokens so far, none of the new ones left out.
     track_weights adds up what the callables' attention gives to every position (`weights`, fp32 [layers, batch, heads, positions]; `observe` does so for
-    queries of the prompt, whose attention is the caller's), and `evict` leaves the positions of the largest sums.
+    queries of the prompt, whose attention is the caller's), and `evict` leaves the positions of the largest sums.  From then on the cache counts what it holds:
+    seen_tokens and the getters, masks (which must be of that width, with nothing left out) and `window`, whose positions are the held ones.  Every sequence has had
+    seen_tokens + evicted_tokens tokens, which is what new ones are rotated by.  A mask of a cache that tracks weights is checked for turns of one token too.
     The reference derives the class from transformers' Cache for the methods that base supplied in the
     version it pins (get_usable_length); they are defined here instead, so the class does not depend on the
     installed transformers version."""
@@ -773,6 +775,7 @@ class MultiLayerPagedKVCache4Bit:
         self._needs_init = [True] * n_layers
         self._padded = False            # the prompt's mask left tokens out
         self.length = 0
+        self.evicted_tokens = 0         # of every sequence, by evict
         self.device = device
         self.hadamard_dtype = hadamard_dtype
         self._stub = _AttentionStub(self.page_size, device, n_layers, disable_quant=self.disable_quant,
@@ -854,14 +857,18 @@ class MultiLayerPagedKVCache4Bit:
 
     def _check_turn(self, attention_mask, added_length, length):
         """A turn behind the prompt appends and attends with the last `added_length` tokens of every sequence: the mask has to cover all tokens so far
-        and keep the new ones, and a prompt with padding needs it again, for the sequences' own lengths."""
+        and keep the new ones, and a prompt with padding needs it again, for the sequences' own lengths.  After an eviction the tokens so far are those that the cache
+        holds: which of a longer mask's columns they are differs between heads."""
         if attention_mask is None:
             if self._padded:
                 raise ValueError("the prompt was padded: later turns need its attention_mask, with the tokens since")
         elif tuple(attention_mask.shape) != (self.batch_size, length):
-            raise ValueError(f"attention_mask must be [{self.batch_size}, {length}], all tokens so far, got {list(attention_mask.shape)}")
+            gone = f" but the {self.evicted_tokens} that evict has let go" if self.evicted_tokens else ""
+            raise ValueError(f"attention_mask must be [{self.batch_size}, {length}], all tokens so far{gone}, got {list(attention_mask.shape)}")
         elif not attention_mask[:, length - added_length:].all():
             raise NotImplementedError("Current implementation does not support padding among the new tokens of a later turn")
+        elif self.evicted_tokens and not attention_mask.all():
+            raise NotImplementedError("Current implementation does not support masks that leave tokens out after evict")
 
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None):
         b_sz, added_length, num_heads, head_dim = key_states.shape
@@ -869,7 +876,7 @@ class MultiLayerPagedKVCache4Bit:
         attention_mask = cache_kwargs.get("attention_mask") if cache_kwargs else None
         first = self._needs_init[layer_idx]
         assert first or added_length >= 1
-        if not first and (added_length > 1 or self.window):
+        if not first and (added_length > 1 or self.window or self.weights is not None):
             self._check_turn(attention_mask, added_length, self.length + (added_length if layer_idx == 0 else 0))
         if self._pending:
             self._flush()
@@ -979,7 +986,8 @@ class MultiLayerPagedKVCache4Bit:
     def evict(self, keep, sinks=0, recent=0):
         """Leaves `keep` positions of every layer, sequence and key head, which may differ between them: the first `sinks`, the last `recent`, and those of the largest
         sums of weights between them (heavy_positions), moved to the front in their order (keep_positions_i4).  The cache then holds and
-        counts min(length, keep) tokens; keys keep the positions that they were rotated for.  To be called between turns, when all layers have the same tokens."""
+        counts min(length, keep) tokens, and evicted_tokens those that went; keys keep the positions that they were rotated for.  To be called between turns, when all layers
+        have the same tokens."""
         self._check_tracked("evict", range(len(self._needs_init)))
         keep, sinks, recent = int(keep), int(sinks), int(recent)
         if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
@@ -992,6 +1000,7 @@ class MultiLayerPagedKVCache4Bit:
         for layer_idx, weights in enumerate(self.weights):
             kept, _ = heavy_positions(weights, lengths, keep, sinks=sinks, recent=recent)
             move(kept, **specs, layer_idx=layer_idx, weights=weights)
+        self.evicted_tokens += self.length - keep
         self.length = keep
 
     def _check_tracked(self, what, layers):
