@@ -776,6 +776,7 @@ class MultiLayerPagedKVCache4Bit:
         self._padded = False            # the prompt's mask left tokens out
         self.length = 0
         self.evicted_tokens = 0         # of every sequence, by evict
+        self._held = [0] * n_layers     # with track_weights: what every layer has been given, which between a turn's layers differs
         self.device = device
         self.hadamard_dtype = hadamard_dtype
         self._stub = _AttentionStub(self.page_size, device, n_layers, disable_quant=self.disable_quant,
@@ -894,6 +895,8 @@ class MultiLayerPagedKVCache4Bit:
             except NotImplementedError:          # a mask of unequal page counts: nothing has been stored
                 self.length = length
                 raise
+        if self.weights is not None:
+            self._held[layer_idx] = self.length
         if self.disable_quant:
             return self._update_f16(key_states, value_states, layer_idx, attention_mask, first, specs)
         k_in, fused_had = key_states, self.hadamard_dtype is not None
@@ -1001,7 +1004,7 @@ class MultiLayerPagedKVCache4Bit:
             kept, _ = heavy_positions(weights, lengths, keep, sinks=sinks, recent=recent)
             move(kept, **specs, layer_idx=layer_idx, weights=weights)
         self.evicted_tokens += self.length - keep
-        self.length = keep
+        self.length, self._held = keep, [keep] * len(self._held)
 
     def _check_tracked(self, what, layers):
         if self.weights is None:
@@ -1010,6 +1013,8 @@ class MultiLayerPagedKVCache4Bit:
             raise NotImplementedError("Current implementation does not support weights of padded prompts")
         if any(self._needs_init[layer] for layer in layers):
             raise RuntimeError(f"{what}: a layer has no tokens yet")
+        if any(self._held[layer] != self.length for layer in layers):
+            raise RuntimeError(f"{what}: a layer has not had the tokens of this turn yet")
 
     def get_cache_specs_for_flash_infer(self, attention_mask):
         """Page tables of the current state (kv_cache.py:253-275): page i of sequence b is page number
