@@ -481,7 +481,7 @@ int qr_batch_chunk_f16(void* o, int64_t o_stride, const void* q, int64_t q_strid
  *   prefixes == 0: the sequences' own positions only (qr_batch_chunk with lse); window > 0 only then (QR_E_SHAPE).
  *   max_prefix_len: the largest number of a prefix's positions if the caller knows it, else 0.
  *   With prefixes tokens * num_q_heads is at most 2^28 - 16, and a workspace of qr_batch_shared_workspace_bytes bytes (the same arguments, max_new_len 1 where
- *   seqlen_indptr is NULL) is required (QR_E_WORKSPACE): a row's partial states, 528 bytes each.
+ *   seqlen_indptr is NULL) is required (QR_E_WORKSPACE): a row's partial states, 528 bytes each, at least one, two where the sequences' own rows are many (no bound in all).
  *   Calls that share a workspace must not overlap.
  */
 size_t qr_batch_shared_workspace_bytes(int fp16_pages, int64_t tokens, int num_q_heads, int num_heads, int64_t batch_size, int64_t max_new_len,

@@ -85,8 +85,8 @@ __device__ __forceinline__ void hadamard_row(u32x4 (&w)[4], int lane) {
 // keys of positions n, 16 + n, 32 + n and 48 + n.  While it works on them the next 64 positions' keys and sums are under way, and the page numbers of those behind.
 // Of 16 rows and fewer the queries stay in registers, of up to 64 in LDS, ready for the products (a wave makes one tile of them; more are made for every block).
 // One row and 32 heads after 3000: 5.0 us, a launch and one wave's chain of tables, pages, keys; 32 x one of 4001, 64 on 8 heads: 18.0 us, 4.4 TB/s of a copy's 5.2
-// (every lane's loads of two blocks under way; half of the lanes without rows: 22.0); fp16 pages, 5 x up to 37 in a window of 1500, 40 heads: 15.6 us, 3.5 TB/s, 200 chains
-// of unequal length.
+// (every lane's loads of two blocks under way; half of the lanes without rows: 22.0); fp16 pages, 5 x up to 37 in a window of 1500, 40 heads: 15.6 us, 3.5 TB/s: 200 lists
+// of unequal length, with as many workgroups each.
 constexpr int kWaves = 4;
 template <bool F16>
 struct RowTile {                       // 16 rows: queries as the products take them; slope, logarithm (base 2, negative) and position of four of them
@@ -704,7 +704,7 @@ int accumulate(bool fp16, void* weights, int64_t capacity, const void* q, int64_
     a.tokens = (int)tokens, a.group = num_q_heads / num_heads;
     a.window = bounded_window(window), a.sinks = bounded_sinks(sinks);
     a.q_had = q_had_mode;
-    a.rows = starts ? tokens * a.group : a.group;
+    a.rows = starts ? tokens * a.group : a.group;          // (by bounds, which are on the device, one sequence may have all of them)
     a.per_group = divisor_of(a.group), a.per_head = divisor_of(num_heads);
     const int64_t fresh = starts ? max_new_len : 1;
     WeightsPlan plan = weights_plan(fp16, a.rows, tokens, a.group, num_heads, batch_size, fresh, seen_positions(tokens, fresh, max_seq_len, a.window, a.sinks, capacity));

@@ -448,7 +448,9 @@ def batch_shared_i4(o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_of
         o[t, h] = softmax(q[t, h] . K^T / sqrt(128)) . V   over the prefix and the sequence's own positions up to the token's own
 
     A sequence outside prefix_sequences' bounds has no prefix.  max_prefix_len: the largest number of positions of a prefix (0: what
-    prefix_indices has room for, on average); sizes the launch like max_seq_len, which counts the sequences' own positions.  There is no window.  The rest as batch_chunk_i4."""
+    prefix_indices has room for, on average); sizes the launch like max_seq_len, which counts the sequences' own positions.  There is no window.  workspace: as
+    batch_chunk_i4's, but it holds partial states of every row in any case, 528 bytes per token, query head and state: 1 to 32 of the prefix, and the sequences' own, one at least
+    where they have many rows.  (16 x 2048 tokens of 64 heads ask for 2.2 GB; the 1 GiB bounds further splits only.)  The rest as batch_chunk_i4."""
     _prefix_needed("batch_shared_i4", prefix_indptr)
     _shared("batch_shared_i4", False, o, q, kv_data, kv_param, kv_indptr, kv_indices, last_page_offset, layer_idx, prefix_indptr, prefix_indices,
             prefix_last_page_offset, prefix_sequences, seqlen_indptr, max_new_len, max_seq_len, max_prefix_len, 0, 0, q_hadamard, lse, workspace)
